@@ -332,6 +332,101 @@ qvh_status qvh_pq_adc(qvh_pq* pq, const float* table, const uint8_t* codes, uint
 qvh_status qvh_nearest_centroid(const float* x, uint64_t n, const float* centroids, uint32_t k,
                                 uint32_t dim, uint32_t* out);
 
+/* ------------------------------------------------------------------------------------------ *
+ * The encoder in front of an index (no counterpart in the reference, whose callers bring finished
+ * vectors): embedding lookup, linear layers, their gradients, and orthogonalised updates. All buffers
+ * are device memory; every call enqueues on `stream` (NULL = the legacy null stream here) without
+ * synchronizing and allocates nothing. Workspaces are the caller's: *_workspace gives the bytes (0:
+ * none needed, NULL may be passed), 16-byte aligned, in use until the call's work on the stream is
+ * done. Element types are QVH_FP32, QVH_FP16 and QVH_BF16, the same for all of a call's matrices;
+ * sums are fp32, rounded once where they are stored. Strides count elements between rows; elements of
+ * a row are contiguous. Every result depends on the inputs alone, bit for bit.
+ * ------------------------------------------------------------------------------------------ */
+#define QVH_FP32 0
+#define QVH_FP16 1
+#define QVH_BF16 2
+
+#define QVH_ACT_NONE 0
+#define QVH_ACT_RELU 1
+#define QVH_ACT_GELU 2 /* z Phi(z), with the error function */
+#define QVH_ACT_SILU 3 /* z / (1 + exp(-z)) */
+
+/* out[count][dim] = scale * table[token], rows of zeros for tokens outside [0, rows): -1 is padding (and
+ * an empty slot of a search's labels). index_bytes is 4 (int32 tokens) or 8 (int64); dim is at most
+ * 32768, count below 2^31, rows below 2^32 - 1. */
+qvh_status qvh_embed_device(const void* d_table, uint64_t rows, uint32_t dim, uint64_t row_stride, int dtype,
+                            const void* d_tokens, int index_bytes, uint64_t count, float scale, void* d_out,
+                            void* stream);
+
+/* The table's gradient out[rows][dim]: scale * the sum of grad[t] over the tokens t that name the row, in
+ * order of t; zero for rows that no token names. Tokens outside the table add nothing. */
+qvh_status qvh_embed_grad_workspace(uint64_t rows, uint32_t dim, uint64_t count, uint64_t* bytes);
+qvh_status qvh_embed_grad_device(const void* d_grad, uint64_t row_stride, const void* d_tokens, int index_bytes,
+                                 uint64_t count, uint64_t rows, uint32_t dim, int dtype, float scale, void* d_out,
+                                 void* d_workspace, uint64_t workspace_bytes, void* stream);
+
+/* A linear layer: z = x w^T + bias, out = act(z) + residual, with x [m][k], w [n][k], bias [n] (nullable),
+ * residual [m][n] (nullable), out [m][n]; z is also stored to `preactivation` (nullable), which the
+ * backward pass of an activation takes. out may be the residual's own buffer, and no other overlap is
+ * allowed. m is below 2^31, k and n at most 2^20, strides at most 2^22. fp32 products run as sums of
+ * three bf16 parts of each operand (24 bits; what is dropped is below fp32's own rounding). */
+typedef struct qvh_linear_args {
+  uint64_t m;
+  uint32_t k, n;
+  int dtype, activation;
+  const void* x;
+  uint64_t x_stride;
+  const void* weight;
+  uint64_t weight_stride;
+  const void* bias;
+  const void* residual;
+  uint64_t residual_stride;
+  void* out;
+  uint64_t out_stride;
+  void* preactivation;
+  uint64_t preactivation_stride;
+} qvh_linear_args;
+qvh_status qvh_linear_workspace(const qvh_linear_args* args, uint64_t* bytes);
+qvh_status qvh_linear_device(const qvh_linear_args* args, void* d_workspace, uint64_t workspace_bytes, void* stream);
+
+/* Gradients of that layer from out's gradient grad [m][n]: with dz = grad * act'(preactivation),
+ * grad_x [m][k] = dz w, grad_weight [n][k] = dz^T x, grad_bias [n] = the sum of dz over m (each nullable;
+ * the residual's gradient is grad itself). preactivation is required with an activation. For 16-bit types
+ * dz enters the two products rounded to the type, as any operand of the matrix unit; grad_bias does not
+ * use the rounded values. */
+typedef struct qvh_linear_grad_args {
+  uint64_t m;
+  uint32_t k, n;
+  int dtype, activation;
+  const void* grad;
+  uint64_t grad_stride;
+  const void* preactivation;
+  uint64_t preactivation_stride;
+  const void* x;
+  uint64_t x_stride;
+  const void* weight;
+  uint64_t weight_stride;
+  void* grad_x;
+  uint64_t grad_x_stride;
+  void* grad_weight;
+  uint64_t grad_weight_stride;
+  void* grad_bias;
+} qvh_linear_grad_args;
+qvh_status qvh_linear_grad_workspace(const qvh_linear_grad_args* args, uint64_t* bytes);
+qvh_status qvh_linear_grad_device(const qvh_linear_grad_args* args, void* d_workspace, uint64_t workspace_bytes,
+                                  void* stream);
+
+/* Newton-Schulz steps on each of `batch` matrices [m][n] (contiguous): X = G / |G|_F (zero for a zero G),
+ * then `steps` times X <- a X + (b A + c A A) X with A = X X^T, or the same from the right where m > n;
+ * out holds X. The singular values s of X each go through s <- a s + b s^3 + c s^5, the singular vectors
+ * stay. m and n are at most 65536; coefficients that could drive a singular value above 3.5, or the
+ * polynomial a + b s^2 + c s^4 above 15, are refused (QVH_EINVAL). A matrix with a non-finite element comes
+ * out as NaN. */
+qvh_status qvh_orthogonalize_workspace(uint64_t batch, uint32_t m, uint32_t n, uint64_t* bytes);
+qvh_status qvh_orthogonalize_device(const void* d_update, uint64_t batch, uint32_t m, uint32_t n, int dtype,
+                                    uint32_t steps, float a, float b, float c, void* d_out, void* d_workspace,
+                                    uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

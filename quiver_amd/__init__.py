@@ -41,7 +41,10 @@ def _load_extension():
 _quiver = _load_extension()
 simd_isa = _quiver.simd_isa
 
-__all__ = ["FlatIndex", "IvfPqIndex", "kmeans", "simd_isa"]
+from .encoder import embed, embed_grad, linear, linear_grad, orthogonalize  # noqa: E402
+
+__all__ = ["FlatIndex", "IvfPqIndex", "embed", "embed_grad", "kmeans", "linear", "linear_grad", "orthogonalize",
+           "simd_isa"]
 __version__ = "0.1.0"
 
 ArrayLike = Union[np.ndarray, Iterable]

@@ -1,0 +1,629 @@
+// Embedding lookup with scaling and its gradient by sorted tokens.
+//
+// Lookup: y[t] = scale * table[token[t]], a row of zeros where the token is outside the table. One
+// pass that reads each named row and writes each output row; memory traffic is the whole cost.
+//
+// Gradient: dE[v] = scale * sum of dy[t] over the t with token[t] = v, in order of t, in fp32. The
+// tokens are sorted (stable, least significant digit first), so equal tokens are neighbours; waves
+// then sum fixed pieces of the sorted list, and runs that cross a piece are joined in order by a
+// second launch. Which partial sums are formed depends on the tokens alone, never on timing, so a
+// call repeats bit for bit, and a token that fills half of the batch is spread over many waves.
+// A small batch takes one launch instead: every wave owns a few rows of the table and looks through
+// all tokens for them.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.hpp"
+#include "types16.hpp"
+
+namespace qvh {
+namespace {
+
+constexpr uint32_t kMaxDim = 32768;
+
+// ---- lookup -----------------------------------------------------------------------------------
+
+/// Chunk c of the output is V elements; U chunks per thread, 256 apart, so that each thread has U
+/// independent row reads in flight.
+template <class T, int V, class I, int U>
+__global__ void __launch_bounds__(256) embed_kernel(const T* __restrict__ table, uint64_t rows, uint64_t stride,
+                                                    const I* __restrict__ tokens, uint64_t count, uint32_t cpr,
+                                                    uint32_t magic, float scale, T* __restrict__ out) {
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * (256 * U);
+  const uint64_t t0 = first / cpr;
+  const uint32_t lead = static_cast<uint32_t>(first - t0 * cpr);
+  const uint64_t total = count * cpr;
+  uint64_t at[U];
+  uint32_t col[U];
+  int64_t tok[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    // (lead + index) / cpr by a multiplication: exact below 2^32 / cpr.
+    const uint32_t i = lead + u * 256 + threadIdx.x;
+    const uint32_t q = cpr == 1 ? i : __umulhi(i, magic);
+    at[u] = first + u * 256 + threadIdx.x;
+    col[u] = (i - q * cpr) * V;
+    tok[u] = at[u] < total ? static_cast<int64_t>(tokens[t0 + q]) : -1;
+  }
+  float x[U][V];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (tok[u] >= 0 && static_cast<uint64_t>(tok[u]) < rows) {
+      load_floats<T, V>(table + static_cast<uint64_t>(tok[u]) * stride + col[u], x[u]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[u][i] *= scale;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[u][i] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (at[u] < total) store_floats<T, V>(out + at[u] * V, x[u]);
+  }
+}
+
+template <class T, class I>
+void launch_embed(const void* table, uint64_t rows, uint32_t dim, uint64_t stride, const void* tokens, uint64_t count,
+                  float scale, void* out, hipStream_t s) {
+  with_width<T>(vector_width(sizeof(T), {dim, stride}, {table, out}), [&](auto width) {
+    constexpr int V = decltype(width)::value;
+    const uint32_t cpr = dim / V;
+    const uint32_t magic = cpr == 1 ? 0u : static_cast<uint32_t>((uint64_t{1} << 32) / cpr + 1);
+    const uint64_t total = count * cpr;
+    const auto go = [&](auto unroll) {
+      constexpr int U = decltype(unroll)::value;
+      const uint64_t blocks = ceil_div(total, 256 * U);
+      QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "qvh_embed_device: too many tokens");
+      hipLaunchKernelGGL((embed_kernel<T, V, I, U>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s,
+                         static_cast<const T*>(table), rows, stride, static_cast<const I*>(tokens), count, cpr, magic,
+                         scale, static_cast<T*>(out));
+    };
+    if (total < 256 * 1024) {
+      go(std::integral_constant<int, 1>{});
+    } else {
+      go(std::integral_constant<int, 4>{});
+    }
+  });
+  QVH_HIP(hipGetLastError());
+}
+
+// ---- gradient of a small batch: rows look for their tokens ------------------------------------
+
+constexpr uint32_t kOwnTokens = 2048;
+
+/// Adds N gradient rows, in order: the loads first, so that they are in flight together.
+template <class T, int V, int N>
+__device__ __forceinline__ void add_rows(const T* __restrict__ grad, uint64_t stride, uint32_t col, bool in,
+                                         uint32_t entries, uint64_t& mask, float (&acc)[V]) {
+  float g[N][V];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int bit = __builtin_ctzll(mask);
+    mask &= mask - 1;
+    const uint32_t pos = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(entries), bit)) & 0xFFFFu;
+    if (in) {
+      load_floats<T, V>(grad + static_cast<uint64_t>(pos) * stride + col, g[j]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) g[j][k] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] += g[j][k];
+  }
+}
+
+/// One wave per `own` rows (at most 64): lists the batch's tokens that fall into its rows, then per row
+/// adds their gradient rows in order of position.
+template <class T, int V, class I>
+__global__ void __launch_bounds__(256) embed_grad_own_kernel(const T* __restrict__ grad, uint64_t stride,
+                                                             const I* __restrict__ tokens, uint32_t count, uint32_t rows,
+                                                             uint32_t dim, uint32_t own, float scale,
+                                                             T* __restrict__ out) {
+  __shared__ uint32_t s_list[4][kOwnTokens];  // (row - first) << 16 | position
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t first = (static_cast<uint64_t>(blockIdx.x) * 4 + wave) * own;
+  const uint32_t held = first < rows ? (rows - first < own ? static_cast<uint32_t>(rows - first) : own) : 0u;
+  uint32_t* list = s_list[wave];
+  uint32_t found = 0;
+  const uint64_t below = (uint64_t{1} << lane) - 1;
+#pragma unroll 4
+  for (uint32_t b = 0; b < count; b += 64) {
+    const uint32_t t = b + lane;
+    const int64_t tok = t < count ? static_cast<int64_t>(tokens[t]) : -1;
+    const uint64_t r = static_cast<uint64_t>(tok) - first;  // wraps to a large value below the first row
+    const bool mine = tok >= 0 && r < held;
+    const uint64_t mask = __builtin_amdgcn_ballot_w64(mine);
+    if (mine) list[found + __popcll(mask & below)] = static_cast<uint32_t>(r) << 16 | t;
+    found += static_cast<uint32_t>(__popcll(mask));
+  }
+  __syncthreads();
+  for (uint32_t r = 0; r < held; ++r) {
+    for (uint32_t c0 = 0; c0 < dim; c0 += 64 * V) {
+      const uint32_t c = c0 + lane * V;
+      const bool in = c < dim;
+      float acc[V] = {};
+      for (uint32_t b = 0; b < found; b += 64) {
+        const uint32_t e = b + lane < found ? list[b + lane] : 0xFFFFFFFFu;
+        uint64_t mask = __builtin_amdgcn_ballot_w64(e >> 16 == r);
+        while (__popcll(mask) >= 8) add_rows<T, V, 8>(grad, stride, c, in, e, mask, acc);
+        if (__popcll(mask) >= 4) add_rows<T, V, 4>(grad, stride, c, in, e, mask, acc);
+        while (mask) add_rows<T, V, 1>(grad, stride, c, in, e, mask, acc);
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] *= scale;
+      if (in) store_floats<T, V>(out + (first + r) * dim + c, acc);
+    }
+  }
+}
+
+// ---- sorting (key, position) pairs ------------------------------------------------------------
+//
+// Stable counting passes of at most 8 bits. Each of `parts` work-groups has a contiguous part of the
+// list; count[part][digit] gives every part its place per digit. The first pass's counts are taken by a
+// launch of their own, a later pass's by the scatter of the pass before it, which knows where its
+// pairs land (integer additions: their order changes nothing).
+
+constexpr uint32_t kParts = 128, kBins = 256;
+constexpr uint32_t kSortWaves = 8;
+
+/// The token as a key: its row, or `rows` (sorted behind all of them) outside the table.
+template <class I>
+__device__ __forceinline__ uint32_t token_key(const I* tokens, uint64_t t, uint32_t rows) {
+  const int64_t tok = static_cast<int64_t>(tokens[t]);
+  return tok >= 0 && static_cast<uint64_t>(tok) < rows ? static_cast<uint32_t>(tok) : rows;
+}
+
+template <class I>
+__global__ void __launch_bounds__(256) count_kernel(const I* __restrict__ tokens, uint32_t count, uint32_t part,
+                                                    uint32_t rows, uint32_t digit_mask, uint32_t* __restrict__ counts,
+                                                    uint32_t* __restrict__ next_counts) {
+  __shared__ uint32_t s_bins[kBins];
+  s_bins[threadIdx.x] = 0;
+  next_counts[blockIdx.x * kBins + threadIdx.x] = 0;  // a second and a third pass's
+  next_counts[(gridDim.x + blockIdx.x) * kBins + threadIdx.x] = 0;
+  next_counts[(2 * gridDim.x + blockIdx.x) * kBins + threadIdx.x] = 0;
+  __syncthreads();
+  const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * part;
+  const uint64_t end = begin + part < count ? begin + part : count;
+  for (uint64_t t = begin + threadIdx.x; t < end; t += 256) {
+    atomicAdd(&s_bins[token_key(tokens, t, rows) & digit_mask], 1u);
+  }
+  __syncthreads();
+  counts[blockIdx.x * kBins + threadIdx.x] = s_bins[threadIdx.x];
+}
+
+/// One pass. FIRST reads the tokens themselves (positions are the list's order).
+template <class I, bool FIRST>
+__global__ void __launch_bounds__(kSortWaves * 64) scatter_kernel(
+    const I* __restrict__ tokens, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ positions,
+    uint32_t count, uint32_t part, uint32_t rows, uint32_t shift, uint32_t bits, const uint32_t* __restrict__ counts,
+    uint32_t* __restrict__ next_counts, uint32_t next_shift, uint32_t next_mask, uint32_t* __restrict__ out_keys,
+    uint32_t* __restrict__ out_positions) {
+  __shared__ uint32_t s_at[kSortWaves][kBins];
+  __shared__ uint32_t s_scan[kBins];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t digit_mask = (1u << bits) - 1;
+  for (uint32_t i = tid; i < kSortWaves * kBins; i += kSortWaves * 64) (&s_at[0][0])[i] = 0;
+  __syncthreads();
+
+  // A wave's share of the part is contiguous: the pairs' order is the waves' order.
+  const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * part;
+  const uint64_t end = begin + part < count ? begin + part : count;
+  const uint32_t share = static_cast<uint32_t>(ceil_div(part, kSortWaves * 64)) * 64;
+  const uint64_t w0 = begin + static_cast<uint64_t>(wave) * share;
+  const uint64_t w1 = w0 + share < end ? w0 + share : end;
+  for (uint64_t i = w0 + lane; i < w1; i += 64) {
+    const uint32_t key = FIRST ? token_key(tokens, i, rows) : keys[i];
+    atomicAdd(&s_at[wave][key >> shift & digit_mask], 1u);
+  }
+  // This part's place per digit: all pairs of smaller digits, and this digit's in earlier parts.
+  uint32_t before = 0, all = 0;
+  if (tid < kBins) {
+#pragma unroll 8
+    for (uint32_t p = 0; p < gridDim.x; ++p) {
+      const uint32_t n = counts[p * kBins + tid];
+      before += p < blockIdx.x ? n : 0u;
+      all += n;
+    }
+    s_scan[tid] = all;
+  }
+  __syncthreads();
+  for (uint32_t d = 1; d < kBins; d <<= 1) {
+    const uint32_t add = tid < kBins && tid >= d ? s_scan[tid - d] : 0u;
+    __syncthreads();
+    if (tid < kBins) s_scan[tid] += add;
+    __syncthreads();
+  }
+  if (tid < kBins) {
+    uint32_t at = s_scan[tid] - all + before;
+#pragma unroll
+    for (uint32_t w = 0; w < kSortWaves; ++w) {
+      const uint32_t n = s_at[w][tid];
+      s_at[w][tid] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  const uint64_t below = (uint64_t{1} << lane) - 1;
+  for (uint64_t b = w0; b < w1; b += 64) {
+    const uint64_t i = b + lane;
+    const bool in = i < w1;
+    const uint32_t key = in ? (FIRST ? token_key(tokens, i, rows) : keys[i]) : 0u;
+    const uint32_t pos = in ? (FIRST ? static_cast<uint32_t>(i) : positions[i]) : 0u;
+    const uint32_t digit = key >> shift & digit_mask;
+    // Lanes with this lane's digit.
+    uint64_t same = __builtin_amdgcn_ballot_w64(in);
+    for (uint32_t k = 0; k < bits; ++k) {
+      const uint64_t ones = __builtin_amdgcn_ballot_w64((digit >> k & 1u) != 0);
+      same &= (digit >> k & 1u) ? ones : ~ones;
+    }
+    const uint32_t rank = static_cast<uint32_t>(__popcll(same & below));
+    uint32_t base = 0;
+    if (in && rank == 0) base = atomicAdd(&s_at[wave][digit], static_cast<uint32_t>(__popcll(same)));
+    base = static_cast<uint32_t>(__shfl(static_cast<int>(base), in ? __builtin_ctzll(same) : 0, 64));
+    if (in) {
+      const uint32_t to = base + rank;
+      out_keys[to] = key;
+      out_positions[to] = pos;
+      if (next_counts) atomicAdd(&next_counts[to / part * kBins + (key >> next_shift & next_mask)], 1u);
+    }
+  }
+}
+
+// ---- sums over the sorted list ----------------------------------------------------------------
+
+constexpr uint32_t kPiece = 64;     // sorted entries that one group of lanes adds
+constexpr uint32_t kZeroRows = 64;  // table rows that one work-group checks for having no token
+
+struct SumArgs {
+  const void* grad;
+  uint64_t stride;
+  const uint32_t* keys;
+  const uint32_t* positions;
+  uint32_t count, rows, dim;
+  float scale;
+  void* out;
+  float* partial;  // [piece][2][dim]: the run that came from the piece before, the one that goes on
+  uint32_t pieces, sum_blocks, slabs;
+  uint32_t cpr;
+};
+
+/// First index of [0, n) whose key is not below `key`.
+__device__ __forceinline__ uint32_t lower_bound(const uint32_t* keys, uint32_t n, uint32_t key) {
+  uint32_t lo = 0;
+  while (n > 0) {
+    const uint32_t half = n >> 1;
+    const bool right = keys[lo + half] < key;
+    lo = right ? lo + half + 1 : lo;
+    n = right ? n - half - 1 : half;
+  }
+  return lo;
+}
+
+/// Rows without a token become zero (work-groups past the sums').
+template <class T, int V>
+__device__ __forceinline__ void zero_rows(const SumArgs& a, uint32_t block, uint32_t* s_flag) {
+  const uint64_t r0 = static_cast<uint64_t>(block) * kZeroRows;
+  if (threadIdx.x < kZeroRows) {
+    const uint64_t r = r0 + threadIdx.x;
+    uint32_t touched = 1;
+    if (r < a.rows) {
+      const uint32_t i = lower_bound(a.keys, a.count, static_cast<uint32_t>(r));
+      touched = i < a.count && a.keys[i] == r ? 1u : 0u;
+    }
+    s_flag[threadIdx.x] = touched;
+  }
+  __syncthreads();
+  const float zero[V] = {};
+  T* out = static_cast<T*>(a.out) + r0 * a.dim;
+  for (uint32_t i = threadIdx.x; i < kZeroRows * a.cpr; i += 256) {
+    const uint32_t row = i / a.cpr;
+    if (!s_flag[row]) store_floats<T, V>(out + static_cast<uint64_t>(i) * V, zero);
+  }
+}
+
+/// Groups of G lanes, each adding one piece of the list over G * V columns (slab blockIdx.y).
+template <class T, int V, int G>
+__global__ void __launch_bounds__(256) embed_grad_sum_kernel(SumArgs a) {
+  constexpr uint32_t kGroups = 256 / G;
+  constexpr int kAhead = 8;
+  __shared__ uint32_t s_key[kGroups * kPiece];
+  __shared__ uint32_t s_pos[kGroups * kPiece];
+  if (blockIdx.x >= a.sum_blocks) {
+    if (blockIdx.y == 0) zero_rows<T, V>(a, blockIdx.x - a.sum_blocks, s_key);
+    return;
+  }
+  const uint64_t block0 = static_cast<uint64_t>(blockIdx.x) * (kGroups * kPiece);
+  for (uint32_t i = threadIdx.x; i < kGroups * kPiece; i += 256) {
+    const uint64_t e = block0 + i;
+    s_key[i] = e < a.count ? a.keys[e] : a.rows;
+    s_pos[i] = e < a.count ? a.positions[e] : 0u;
+  }
+  __syncthreads();
+  const uint32_t group = threadIdx.x / G;
+  const uint64_t piece = static_cast<uint64_t>(blockIdx.x) * kGroups + group;
+  const uint64_t e0 = piece * kPiece;
+  const uint32_t col = (blockIdx.y * G + threadIdx.x % G) * V;
+  if (e0 >= a.count || col >= a.dim) return;
+  const uint32_t n = a.count - e0 < kPiece ? static_cast<uint32_t>(a.count - e0) : kPiece;
+  const uint32_t* key = s_key + group * kPiece;
+  const uint32_t* pos = s_pos + group * kPiece;
+  const uint32_t from = e0 > 0 ? a.keys[e0 - 1] : a.rows;                // the run that came in, if any
+  const uint32_t onto = e0 + n < a.count ? a.keys[e0 + n] : a.rows;      // the run that goes on, if any
+  const T* grad = static_cast<const T*>(a.grad) + col;
+  T* out = static_cast<T*>(a.out) + col;
+  float* partial = a.partial + piece * 2 * a.dim + col;
+
+  float acc[V] = {};
+  uint32_t cur = key[0], began = 0;
+  const auto flush = [&](uint32_t end) {
+    if (cur == a.rows) return;
+    const bool came = began == 0 && from == cur, goes = end == n && onto == cur;
+    if (came || goes) {
+      float* p = partial + (came ? 0u : a.dim);
+#pragma unroll
+      for (int k = 0; k < V; ++k) p[k] = acc[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] *= a.scale;
+      store_floats<T, V>(out + static_cast<uint64_t>(cur) * a.dim, acc);
+    }
+  };
+  for (uint32_t j = 0; j < n; j += kAhead) {
+    float x[kAhead][V];
+    uint32_t kk[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      kk[u] = j + u < n ? key[j + u] : a.rows;
+      if (kk[u] != a.rows) {
+        load_floats<T, V>(grad + static_cast<uint64_t>(pos[j + u]) * a.stride, x[u]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[u][k] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (j + u < n && kk[u] != cur) {
+        flush(j + u);
+        cur = kk[u];
+        began = j + u;
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] += x[u][k];
+    }
+  }
+  flush(n);
+}
+
+/// Work-group per piece: where a run begins in this piece and goes on, its partial sums are added in
+/// order (four waves take contiguous shares of them) and the row is written.
+template <class T>
+__global__ void __launch_bounds__(256) embed_grad_join_kernel(SumArgs a) {
+  __shared__ float s_sum[4][64];
+  const uint64_t e0 = static_cast<uint64_t>(blockIdx.x) * kPiece, e1 = e0 + kPiece;
+  if (e1 >= a.count) return;  // nothing goes on from the last piece
+  const uint32_t cur = a.keys[e1 - 1];
+  if (cur == a.rows || a.keys[e1] != cur) return;
+  if (e0 > 0 && a.keys[e0] == cur && a.keys[e0 - 1] == cur) return;  // began earlier
+  const uint32_t end = static_cast<uint32_t>(e1) +
+                       lower_bound(a.keys + e1, a.count - static_cast<uint32_t>(e1), cur + 1);
+  const uint32_t last = (end - 1) / kPiece;             // pieces blockIdx.x .. last hold the run
+  const uint32_t n = last - blockIdx.x + 1;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t share = (n + 3) / 4;
+  const uint32_t p0 = wave * share < n ? wave * share : n, p1 = p0 + share < n ? p0 + share : n;
+  for (uint32_t c0 = blockIdx.y * 64; c0 < a.dim; c0 += gridDim.y * 64) {
+    const uint32_t c = c0 + lane;
+    float acc = 0.0f;
+    if (c < a.dim) {
+#pragma unroll 8
+      for (uint32_t p = p0; p < p1; ++p) {
+        acc += a.partial[((static_cast<uint64_t>(blockIdx.x) + p) * 2 + (p == 0 ? 1 : 0)) * a.dim + c];
+      }
+    }
+    __syncthreads();
+    s_sum[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0 && c < a.dim) {
+      const float sum = ((s_sum[0][lane] + s_sum[1][lane]) + s_sum[2][lane]) + s_sum[3][lane];
+      static_cast<T*>(a.out)[static_cast<uint64_t>(cur) * a.dim + c] = static_cast<T>(sum * a.scale);
+    }
+  }
+}
+
+/// Where the parts of the workspace lie, in bytes.
+struct GradLayout {
+  uint32_t parts, part, passes;
+  size_t counts, keys[2], positions[2], partial, total;
+};
+
+GradLayout grad_layout(uint64_t rows, uint32_t dim, uint64_t count) {
+  GradLayout l{};
+  if (count <= kOwnTokens) return l;
+  const auto round = [](size_t b) { return (b + 255) / 256 * 256; };
+  l.part = static_cast<uint32_t>(std::max<uint64_t>(ceil_div(count, kParts), 1024));
+  l.parts = static_cast<uint32_t>(ceil_div(count, l.part));
+  uint32_t bits = 0;
+  while (bits < 32 && (rows >> bits) != 0) ++bits;
+  l.passes = std::max(1u, (bits + 7) / 8);
+  size_t at = round(4 * static_cast<size_t>(l.parts) * kBins * 4);
+  for (int i = 0; i < 2; ++i) {
+    l.keys[i] = at;
+    at += round(count * 4);
+    l.positions[i] = at;
+    at += round(count * 4);
+  }
+  l.partial = at;
+  l.total = at + round(ceil_div(count, kPiece) * 2 * dim * 4);
+  return l;
+}
+
+template <class T, class I>
+void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, uint64_t count, uint64_t rows,
+                       uint32_t dim, float scale, void* out, char* ws, hipStream_t s) {
+  const int width = vector_width(sizeof(T), {dim, stride}, {grad, out});
+  if (count <= kOwnTokens) {
+    // At least about eight waves per SIMD of rows, where there are as many.
+    const uint32_t own = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(rows / 8192, 4), 64));
+    with_width<T>(width, [&](auto v) {
+      constexpr int V = decltype(v)::value;
+      hipLaunchKernelGGL((embed_grad_own_kernel<T, V, I>), dim3(static_cast<unsigned>(ceil_div(rows, 4 * own))),
+                         dim3(256), 0, s, static_cast<const T*>(grad), stride, static_cast<const I*>(tokens),
+                         static_cast<uint32_t>(count), static_cast<uint32_t>(rows), dim, own, scale,
+                         static_cast<T*>(out));
+    });
+    QVH_HIP(hipGetLastError());
+    return;
+  }
+  const GradLayout l = grad_layout(rows, dim, count);
+  const uint32_t n = static_cast<uint32_t>(count), r = static_cast<uint32_t>(rows);
+  uint32_t bits = 0;
+  while (bits < 32 && (rows >> bits) != 0) ++bits;
+  const uint32_t digit = (bits + l.passes - 1) / l.passes;
+  uint32_t* counts = reinterpret_cast<uint32_t*>(ws + l.counts);
+  const size_t counts_step = static_cast<size_t>(l.parts) * kBins;
+  uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(ws + l.keys[0]), reinterpret_cast<uint32_t*>(ws + l.keys[1])};
+  uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + l.positions[0]), reinterpret_cast<uint32_t*>(ws + l.positions[1])};
+  hipLaunchKernelGGL((count_kernel<I>), dim3(l.parts), dim3(256), 0, s, static_cast<const I*>(tokens), n, l.part, r,
+                     (1u << digit) - 1, counts, counts + counts_step);
+  QVH_HIP(hipGetLastError());
+  for (uint32_t p = 0; p < l.passes; ++p) {
+    uint32_t* next = p + 1 < l.passes ? counts + (p + 1) * counts_step : nullptr;
+    const uint32_t next_mask = (1u << digit) - 1;
+    uint32_t* ok = keys[p & 1];
+    uint32_t* op = pos[p & 1];
+    const auto pass = [&](auto first) {
+      constexpr bool F = decltype(first)::value;
+      hipLaunchKernelGGL((scatter_kernel<I, F>), dim3(l.parts), dim3(kSortWaves * 64), 0, s,
+                         static_cast<const I*>(tokens), keys[(p & 1) ^ 1], pos[(p & 1) ^ 1], n, l.part, r, p * digit,
+                         digit, counts + p * counts_step, next, (p + 1) * digit, next_mask, ok, op);
+    };
+    if (p == 0) {
+      pass(std::true_type{});
+    } else {
+      pass(std::false_type{});
+    }
+    QVH_HIP(hipGetLastError());
+  }
+  with_width<T>(width, [&](auto v) {
+    constexpr int V = decltype(v)::value;
+    SumArgs a{};
+    a.grad = grad;
+    a.stride = stride;
+    a.keys = keys[(l.passes - 1) & 1];
+    a.positions = pos[(l.passes - 1) & 1];
+    a.count = n;
+    a.rows = r;
+    a.dim = dim;
+    a.scale = scale;
+    a.out = out;
+    a.partial = reinterpret_cast<float*>(ws + l.partial);
+    a.pieces = static_cast<uint32_t>(ceil_div(count, kPiece));
+    a.cpr = dim / V;
+    const uint32_t zero_blocks = static_cast<uint32_t>(ceil_div(rows, kZeroRows));
+    const auto sum = [&](auto group) {
+      constexpr int G = decltype(group)::value;
+      a.sum_blocks = static_cast<uint32_t>(ceil_div(a.pieces, 256 / G));
+      a.slabs = static_cast<uint32_t>(ceil_div(a.cpr, G));
+      hipLaunchKernelGGL((embed_grad_sum_kernel<T, V, G>), dim3(a.sum_blocks + zero_blocks, a.slabs), dim3(256), 0, s, a);
+    };
+    if (a.cpr <= 8) {
+      sum(std::integral_constant<int, 8>{});
+    } else if (a.cpr <= 16) {
+      sum(std::integral_constant<int, 16>{});
+    } else if (a.cpr <= 32) {
+      sum(std::integral_constant<int, 32>{});
+    } else {
+      sum(std::integral_constant<int, 64>{});
+    }
+    QVH_HIP(hipGetLastError());
+    if (a.pieces > 1) {
+      hipLaunchKernelGGL((embed_grad_join_kernel<T>), dim3(a.pieces, std::min<uint32_t>(ceil_div(dim, 64), 16)), dim3(256),
+                         0, s, a);
+      QVH_HIP(hipGetLastError());
+    }
+  });
+}
+
+void check_embed(const char* who, uint64_t rows, uint32_t dim, int dtype, int index_bytes, uint64_t count) {
+  const std::string w(who);
+  require_dtype(who, dtype);
+  QVH_REQUIRE(index_bytes == 4 || index_bytes == 8, w + ": tokens must be int32 or int64");
+  QVH_REQUIRE(dim >= 1 && dim <= kMaxDim, w + ": dim must be in [1, 32768]");
+  QVH_REQUIRE(rows < 0xFFFFFFFFu, w + ": rows must be below 2^32 - 1");
+  QVH_REQUIRE(count < (uint64_t{1} << 31), w + ": the number of tokens must be below 2^31");
+}
+
+}  // namespace
+}  // namespace qvh
+
+extern "C" {
+
+qvh_status qvh_embed_device(const void* d_table, uint64_t rows, uint32_t dim, uint64_t row_stride, int dtype,
+                            const void* d_tokens, int index_bytes, uint64_t count, float scale, void* d_out,
+                            void* stream) {
+  return qvh::guarded([&] {
+    using namespace qvh;
+    check_embed("qvh_embed_device", rows, dim, dtype, index_bytes, count);
+    QVH_REQUIRE(row_stride >= dim || rows <= 1, "qvh_embed_device: the row stride must be at least dim");
+    if (count == 0) return;
+    QVH_REQUIRE((d_table || rows == 0) && d_tokens && d_out, "qvh_embed_device: null buffer");
+    current_device();
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    with_dtype(dtype, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      if (index_bytes == 8) {
+        launch_embed<T, int64_t>(d_table, rows, dim, row_stride, d_tokens, count, scale, d_out, s);
+      } else {
+        launch_embed<T, int32_t>(d_table, rows, dim, row_stride, d_tokens, count, scale, d_out, s);
+      }
+    });
+  });
+}
+
+qvh_status qvh_embed_grad_workspace(uint64_t rows, uint32_t dim, uint64_t count, uint64_t* bytes) {
+  return qvh::guarded([&] {
+    using namespace qvh;
+    QVH_REQUIRE(bytes != nullptr, "qvh_embed_grad_workspace: null output");
+    check_embed("qvh_embed_grad_workspace", rows, dim, QVH_FP32, 8, count);
+    *bytes = grad_layout(rows, dim, count).total;
+  });
+}
+
+qvh_status qvh_embed_grad_device(const void* d_grad, uint64_t row_stride, const void* d_tokens, int index_bytes,
+                                 uint64_t count, uint64_t rows, uint32_t dim, int dtype, float scale, void* d_out,
+                                 void* d_workspace, uint64_t workspace_bytes, void* stream) {
+  return qvh::guarded([&] {
+    using namespace qvh;
+    check_embed("qvh_embed_grad_device", rows, dim, dtype, index_bytes, count);
+    QVH_REQUIRE(row_stride >= dim || count <= 1, "qvh_embed_grad_device: the row stride must be at least dim");
+    if (rows == 0) return;
+    QVH_REQUIRE(((d_grad && d_tokens) || count == 0) && d_out, "qvh_embed_grad_device: null buffer");
+    const size_t need = grad_layout(rows, dim, count).total;
+    QVH_REQUIRE(need == 0 || (d_workspace != nullptr && workspace_bytes >= need),
+                "qvh_embed_grad_device: the workspace is too small");
+    QVH_REQUIRE(reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0,
+                "qvh_embed_grad_device: the workspace must be 16-byte aligned");
+    current_device();
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    with_dtype(dtype, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      if (index_bytes == 8) {
+        launch_embed_grad<T, int64_t>(d_grad, row_stride, d_tokens, count, rows, dim, scale, d_out,
+                                      static_cast<char*>(d_workspace), s);
+      } else {
+        launch_embed_grad<T, int32_t>(d_grad, row_stride, d_tokens, count, rows, dim, scale, d_out,
+                                      static_cast<char*>(d_workspace), s);
+      }
+    });
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,524 @@
+// Matrix product of the encoder operators on the 16-bit matrix unit: C[m][n] = sum_k A(m, k) B(n, k),
+// accumulated in fp32, with an epilogue.
+//
+// Operands. Each is a 16-bit matrix, stored either by rows ([row][k], k contiguous) or by k ([k][row],
+// row contiguous): a layer's forward pass reads both by rows, its input gradient the weight by k, its
+// weight gradient both by k, so no pass ever transposes a matrix in memory. fp32 operands come as a
+// sum of 16-bit planes; the product then runs over the listed pairs of planes as if they followed each
+// other along k.
+//
+// A work-group takes a BM x BN tile in 64-deep steps. The steps go from memory straight into LDS
+// (16 bytes per lane, no registers), the next one while the present one is multiplied; LDS holds
+// each row's (or each k's) 16-byte pieces permuted so that the fragments of the matrix unit are read
+// without bank conflicts, and because such loads fill LDS in lane order the permutation is in the
+// addresses that the lanes load from. Nothing is read outside the operands: rows and k past the end
+// are clamped to the last one, the results of clamped rows are not stored, and elements past the last
+// k are replaced by zeros in registers, in the last step only.
+#pragma once
+
+#include "types16.hpp"
+
+namespace qvh {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+
+template <class T>
+struct Frag;
+template <>
+struct Frag<half_t> {
+  typedef half_t x8 __attribute__((ext_vector_type(8)));
+  typedef half_t x4 __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ f32x16_t mfma(x8 a, x8 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Frag<bhalf_t> {
+  typedef bhalf_t x8 __attribute__((ext_vector_type(8)));
+  typedef bhalf_t x4 __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ f32x16_t mfma(x8 a, x8 b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+/// One operand: element (row, k) of plane p at base[p * plane + row * ld + k], or [.. k * ld + row] where
+/// it is stored by k. 16-byte aligned, ld % 8 == 0, and the contiguous extent rounded up to 8 is readable.
+struct GemmOperand {
+  const void* base = nullptr;
+  uint64_t ld = 0, plane = 0, batch = 0;  // in elements
+};
+
+constexpr int kMaxPairs = 6;
+
+struct GemmArgs {
+  GemmOperand a, b;
+  uint32_t m = 0, n = 0, k = 0;
+  uint32_t pairs = 1;  // plane pairs
+  uint8_t pa[kMaxPairs] = {0}, pb[kMaxPairs] = {0};
+  uint32_t tiles_m = 0, tiles_n = 0, splits = 1, batches = 1;
+  float* partial = nullptr;  // [split][batch][m][n rounded up to 8] when splits > 1
+};
+
+enum class Activation : int { kNone = QVH_ACT_NONE, kRelu = QVH_ACT_RELU, kGelu = QVH_ACT_GELU, kSilu = QVH_ACT_SILU };
+
+__device__ __forceinline__ float activate(float z, int act) {
+  if (act == QVH_ACT_RELU) return z > 0.0f || z != z ? z : 0.0f;
+  if (act == QVH_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  if (act == QVH_ACT_SILU) return z / (1.0f + __expf(-z));
+  return z;
+}
+
+/// d activate / dz.
+__device__ __forceinline__ float activate_slope(float z, int act) {
+  if (act == QVH_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  if (act == QVH_ACT_GELU) {
+    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+  }
+  if (act == QVH_ACT_SILU) {
+    const float s = 1.0f / (1.0f + __expf(-z));
+    return s * (1.0f + z * (1.0f - s));
+  }
+  return 1.0f;
+}
+
+/// Eight values as vector stores where the row is aligned and whole, else one by one.
+template <class T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8], uint32_t left, bool vec) {
+  if (vec && left >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      store_floats<T, 8>(p, v);
+    } else {
+      const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+      store_floats<T, 4>(p, lo);
+      store_floats<T, 4>(p + 4, hi);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (static_cast<uint32_t>(i) < left) p[i] = static_cast<T>(v[i]);
+    }
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8], uint32_t left, bool vec) {
+  if (vec && left >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      load_floats<T, 8>(p, v);
+    } else {
+      float lo[4], hi[4];
+      load_floats<T, 4>(p, lo);
+      load_floats<T, 4>(p + 4, hi);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = lo[i];
+        v[4 + i] = hi[i];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = static_cast<uint32_t>(i) < left ? static_cast<float>(p[i]) : 0.0f;
+  }
+}
+
+/// One element of a product whose operands are planes, in fp32. An infinity meets the zeros and the opposite
+/// signs of the other operand's lower planes and turns into NaN; with the planes added first it does not.
+/// Stops at the first NaN.
+__device__ __forceinline__ float direct_element(const GemmArgs& g, bool a_by_k, bool b_by_k, int planes, uint64_t m, uint64_t n) {
+  const bhalf_t* a = static_cast<const bhalf_t*>(g.a.base);
+  const bhalf_t* b = static_cast<const bhalf_t*>(g.b.base);
+  float sum = 0.0f;
+  for (uint64_t k = 0; k < g.k && sum == sum; ++k) {
+    const uint64_t ia = a_by_k ? k * g.a.ld + m : m * g.a.ld + k, ib = b_by_k ? k * g.b.ld + n : n * g.b.ld + k;
+    float x = 0.0f, y = 0.0f;
+    for (int p = planes - 1; p >= 0; --p) {
+      x += static_cast<float>(a[p * g.a.plane + ia]);
+      y += static_cast<float>(b[p * g.b.plane + ib]);
+    }
+    sum = fmaf(x, y, sum);
+  }
+  return sum;
+}
+
+/// y = act(acc + bias) + residual, the sum in front of the activation kept where it is asked for.
+template <class T>
+struct LinearEpilogue {
+  const T* bias = nullptr;
+  const T* residual = nullptr;
+  T* out = nullptr;
+  T* keep = nullptr;
+  uint64_t ld_residual = 0, ld_out = 0, ld_keep = 0;
+  int act = QVH_ACT_NONE;
+  int vec_bias = 0, vec_residual = 0, vec_out = 0, vec_keep = 0;
+  GemmArgs direct;  // fp32: the product itself, for elements that come out as NaN
+  int a_by_k = 0, b_by_k = 0;
+
+  /// The same for one element.
+  __device__ __forceinline__ void one(uint32_t m, uint32_t n, float v) const {
+    if (bias) v += static_cast<float>(bias[n]);
+    if (keep) keep[m * ld_keep + n] = static_cast<T>(v);
+    v = activate(v, act);
+    if (residual) v += static_cast<float>(residual[m * ld_residual + n]);
+    out[m * ld_out + n] = static_cast<T>(v);
+  }
+
+  __device__ __forceinline__ void operator()(uint32_t, uint32_t m, uint32_t n, uint32_t left, float (&v)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        if (v[i] != v[i] && static_cast<uint32_t>(i) < left) v[i] = direct_element(direct, a_by_k, b_by_k, 3, m, n + i);
+      }
+    }
+    if (bias) {
+      float b[8];
+      load8(bias + n, b, left, vec_bias);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += b[i];
+    }
+    if (keep) store8(keep + m * ld_keep + n, v, left, vec_keep);
+    if (act == QVH_ACT_RELU) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = activate(v[i], QVH_ACT_RELU);
+    } else if (act == QVH_ACT_GELU) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = activate(v[i], QVH_ACT_GELU);
+    } else if (act == QVH_ACT_SILU) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = activate(v[i], QVH_ACT_SILU);
+    }
+    if (residual) {
+      float r[8];
+      load8(residual + m * ld_residual + n, r, left, vec_residual);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] += r[i];
+    }
+    store8(out + m * ld_out + n, v, left, vec_out);
+  }
+};
+
+/// The partial sums of one split of k.
+struct PartialEpilogue {
+  float* out;
+  uint64_t ld, batch;
+  __device__ __forceinline__ void operator()(uint32_t z, uint32_t m, uint32_t n, uint32_t, float (&v)[8]) const {
+    const uint32_t whole = 8;
+    store8(out + z * batch + m * ld + n, v, whole, true);
+  }
+};
+
+// ---- the kernel -------------------------------------------------------------------------------
+
+constexpr int kStep = 64;  // k per step
+
+/// The 16-byte pieces of one operand's R x 64 step: addresses for the loads into LDS, and fragments.
+template <class T, bool BY_K, int R, int WAVES>
+struct Stage {
+  static constexpr int kBytes = R * kStep * 2;
+  static constexpr int kLoads = kBytes / 1024 / WAVES;
+  static constexpr int kChunks = R / 8;              // 16-byte pieces per k, stored by k
+  static constexpr int kLines = 64 / kChunks;        // k per load, stored by k
+  static_assert(kLoads >= 1 && kBytes % (1024 * WAVES) == 0, "every wave loads whole kilobytes");
+
+  /// Byte offset (from the tile's first row and the step's first k) of what this lane loads in load i; the
+  /// lanes fill LDS in order. `rows` and `depth`: how many of each there are from the tile's start on.
+  static __device__ __forceinline__ uint32_t offset(int i, int wave, int lane, uint32_t ld, uint32_t rows, uint32_t depth) {
+    const int block = i * WAVES + wave;
+    if constexpr (BY_K) {
+      uint32_t k = static_cast<uint32_t>(block * kLines + lane / kChunks);
+      uint32_t c = static_cast<uint32_t>(lane % kChunks) ^ flip(k);
+      k = k < depth ? k : depth - 1;
+      const uint32_t last = (rows + 7) / 8 - 1;
+      c = c < last ? c : last;
+      return k * ld * 2 + c * 16;
+    } else {
+      uint32_t r = static_cast<uint32_t>(block * 8 + (lane >> 3));
+      uint32_t c = static_cast<uint32_t>((lane & 7) ^ (lane >> 3));
+      r = r < rows ? r : rows - 1;
+      const uint32_t last = (depth + 7) / 8 - 1;
+      c = c < last ? c : last;
+      return r * ld * 2 + c * 16;
+    }
+  }
+
+  /// Stored by k, piece c of line k lies at c ^ flip(k): the four k that a transposing read takes at once
+  /// fall on different banks.
+  static __device__ __forceinline__ uint32_t flip(uint32_t k) { return (k & (R / 32 - 1)) * 4; }
+
+  /// Fragment of rows row0 .. row0 + 31 (a multiple of 32) and k kk * 16 .. + 15.
+  static __device__ __forceinline__ typename Frag<T>::x8 fragment(const char* lds, int row0, int kk, int lane) {
+    if constexpr (BY_K) {
+      typedef typename Frag<T>::x4 x4;
+      x4 part[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int p = lane & 15, j = p >> 2;
+        const int k = kk * 16 + 8 * (lane >> 5) + 4 * q + j;
+        const uint32_t chunk = static_cast<uint32_t>(row0 / 8 + 2 * (lane >> 4 & 1) + (p >> 1 & 1));
+        const char* at = lds + k * (R * 2) + ((chunk ^ flip(static_cast<uint32_t>(4 * q + j))) * 16 + (p & 1) * 8);
+        const s16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4_t*)(at));
+        part[q] = __builtin_bit_cast(x4, v);
+      }
+      return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      const int row = row0 + (lane & 31);
+      return *reinterpret_cast<const typename Frag<T>::x8*>(lds + row * 128 + (((kk * 2 + (lane >> 5)) ^ (lane & 7)) * 16));
+    }
+  }
+};
+
+/// 64 lanes x 16 bytes from rsrc + offset + scalar into LDS at lds (wave-uniform), in lane order. Nothing
+/// waits for it but s_waitcnt vmcnt.
+__device__ __forceinline__ void load_to_lds(uint32_t lds, uint32_t offset, u32x4_t rsrc, uint32_t scalar) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               :
+               : "s"(lds), "v"(offset), "s"(rsrc), "s"(scalar)
+               : "memory");
+}
+
+__device__ __forceinline__ u32x4_t buffer_resource(const void* base) {
+  const uint64_t p = reinterpret_cast<uint64_t>(base);
+  u32x4_t r;
+  r[0] = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(p)));
+  r[1] = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(p >> 32))) & 0xFFFFu;
+  r[2] = 0xFFFFFFFFu;
+  r[3] = 0x00027000u;
+  return r;
+}
+
+/// Elements of a fragment at or past `depth` (k counted from the fragment's step) become zero.
+template <class X8>
+__device__ __forceinline__ X8 clip(X8 f, int kk, int lane, uint32_t depth) {
+  const int first = kk * 16 + 8 * (lane >> 5);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (static_cast<uint32_t>(first + e) >= depth) f[e] = 0;
+  }
+  return f;
+}
+
+template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN, class Epi>
+__global__ void __launch_bounds__(WM* WN * 64, 2)
+    gemm_kernel(GemmArgs g, Epi epi) {
+  constexpr int kWaves = WM * WN;
+  using SA = Stage<T, AK, BM, kWaves>;
+  using SB = Stage<T, BK, BN, kWaves>;
+  constexpr int kStageBytes = SA::kBytes + SB::kBytes;
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 blocks per wave
+  constexpr int kSlabLd = BN / WN + 8;
+  constexpr int kSlabBytes = 32 * kSlabLd * 4 * kWaves;
+  constexpr int kLds = 2 * kStageBytes > kSlabBytes ? 2 * kStageBytes : kSlabBytes;
+  __shared__ __attribute__((aligned(1024))) char s_mem[kLds];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+
+  // Work-groups go round the XCDs in order of their number; each XCD takes a contiguous run of tiles,
+  // walked in bands of eight tile rows, so that its L2 serves the rows and columns they share.
+  const uint32_t per = g.tiles_m * g.tiles_n;
+  const uint32_t total = per * g.splits;
+  uint32_t id = blockIdx.x;
+  {
+    const uint32_t x = id % 8, q = total / 8, r = total % 8;
+    id = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + id / 8;
+  }
+  const uint32_t split = id / per;
+  const uint32_t tile = id % per;
+  const uint32_t band = 8 * g.tiles_n, b0 = tile / band * 8;
+  const uint32_t high = g.tiles_m - b0 < 8 ? g.tiles_m - b0 : 8;
+  const uint32_t tm = b0 + tile % band % high, tn = tile % band / high;
+  const uint32_t z = blockIdx.y;
+
+  const uint32_t row0 = tm * BM, col0 = tn * BN;
+  const uint32_t rows = g.m - row0, cols = g.n - col0;
+  const uint32_t ksteps = (g.k + kStep - 1) / kStep;
+  const uint32_t steps = ksteps * g.pairs;
+  const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(steps) * split / g.splits);
+  const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(steps) * (split + 1) / g.splits);
+
+  const T* const a0 = static_cast<const T*>(g.a.base) + z * g.a.batch + (AK ? uint64_t{row0} : row0 * g.a.ld);
+  const T* const b0p = static_cast<const T*>(g.b.base) + z * g.b.batch + (BK ? uint64_t{col0} : col0 * g.b.ld);
+  const uint32_t lda = static_cast<uint32_t>(g.a.ld), ldb = static_cast<uint32_t>(g.b.ld);
+  uint32_t oa[SA::kLoads], ob[SB::kLoads];
+#pragma unroll
+  for (int i = 0; i < SA::kLoads; ++i) oa[i] = SA::offset(i, wave, lane, lda, rows, kStep);
+#pragma unroll
+  for (int i = 0; i < SB::kLoads; ++i) ob[i] = SB::offset(i, wave, lane, ldb, cols, kStep);
+  const uint32_t lds0 = static_cast<uint32_t>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(s_mem)));
+
+  // Loads step `step` into half `buf`.
+  const auto load = [&](uint32_t step, int buf) {
+    const uint32_t pair = step / ksteps, ks = step - pair * ksteps;
+    const uint32_t k0 = ks * kStep;
+    const T* pa = a0 + g.pa[pair] * g.a.plane + (AK ? k0 * g.a.ld : uint64_t{k0});
+    const T* pb = b0p + g.pb[pair] * g.b.plane + (BK ? k0 * g.b.ld : uint64_t{k0});
+    const u32x4_t ra = buffer_resource(pa), rb = buffer_resource(pb);
+    const uint32_t la = lds0 + static_cast<uint32_t>(buf) * kStageBytes, lb = la + SA::kBytes;
+    const uint32_t depth = g.k - k0;
+    if (depth >= kStep) {
+#pragma unroll
+      for (int i = 0; i < SA::kLoads; ++i) load_to_lds(la + (i * kWaves + wave) * 1024, oa[i], ra, 0);
+#pragma unroll
+      for (int i = 0; i < SB::kLoads; ++i) load_to_lds(lb + (i * kWaves + wave) * 1024, ob[i], rb, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < SA::kLoads; ++i) {
+        load_to_lds(la + (i * kWaves + wave) * 1024, SA::offset(i, wave, lane, lda, rows, depth), ra, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < SB::kLoads; ++i) {
+        load_to_lds(lb + (i * kWaves + wave) * 1024, SB::offset(i, wave, lane, ldb, cols, depth), rb, 0);
+      }
+    }
+  };
+
+  f32x16_t acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x16_t{};
+  }
+
+  const int ra0 = wm * (BM / WM), rb0 = wn * (BN / WN);
+  const auto multiply = [&](int buf, uint32_t depth, auto whole) {
+    const char* la = s_mem + buf * kStageBytes;
+    const char* lb = la + SA::kBytes;
+#pragma unroll
+    for (int kk = 0; kk < kStep / 16; ++kk) {
+      if (!decltype(whole)::value && static_cast<uint32_t>(kk * 16) >= depth) break;
+      typename Frag<T>::x8 fa[TM], fb[TN];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fa[i] = SA::fragment(la, ra0 + 32 * i, kk, lane);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fb[j] = SB::fragment(lb, rb0 + 32 * j, kk, lane);
+      if constexpr (!decltype(whole)::value) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) fa[i] = clip(fa[i], kk, lane, depth);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) fb[j] = clip(fb[j], kk, lane, depth);
+      }
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = Frag<T>::mfma(fa[i], fb[j], acc[i][j]);
+      }
+    }
+  };
+
+  if (first < end) load(first, 0);
+  for (uint32_t s = first; s < end; ++s) {
+    const int buf = static_cast<int>((s - first) & 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of step s are in LDS
+    __syncthreads();                                  // everyone's are, and step s - 1 has been read
+    if (s + 1 < end) load(s + 1, buf ^ 1);
+    const uint32_t depth = g.k - s % ksteps * kStep;
+    if (depth >= kStep) {
+      multiply(buf, kStep, std::true_type{});
+    } else {
+      multiply(buf, depth, std::false_type{});
+    }
+  }
+  __syncthreads();
+
+  // The accumulators of 32 rows at a time through the wave's own piece of LDS, so that a lane gets eight
+  // neighbouring columns of one row: whole lines for the residual and the stores.
+  float* slab = reinterpret_cast<float*>(s_mem) + wave * (32 * kSlabLd);
+  constexpr int kPerRow = BN / WN / 8;      // lanes per row
+  constexpr int kRowsAtOnce = 64 / kPerRow;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        slab[(8 * (r / 4) + 4 * (lane >> 5) + r % 4) * kSlabLd + 32 * j + (lane & 31)] = acc[i][j][r];
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const uint32_t n = col0 + static_cast<uint32_t>(rb0 + lane % kPerRow * 8);
+#pragma unroll
+    for (int q = 0; q < 32 / kRowsAtOnce; ++q) {
+      const int r = q * kRowsAtOnce + lane / kPerRow;
+      const uint32_t m = row0 + static_cast<uint32_t>(ra0 + 32 * i + r);
+      const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(slab + r * kSlabLd + lane % kPerRow * 8);
+      const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(slab + r * kSlabLd + lane % kPerRow * 8 + 4);
+      float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      if (m < g.m && n < g.n) epi(g.splits > 1 ? split * g.batches + z : z, m, n, g.n - n, v);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+}
+
+/// Adds the splits' partial sums in order and runs the epilogue.
+template <class Epi>
+__global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs g, Epi epi) {
+  const uint32_t ld = (g.n + 7) / 8 * 8;
+  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const uint32_t per_row = ld / 8;
+  const uint64_t m = i / per_row;
+  if (m >= g.m) return;
+  const uint32_t n = static_cast<uint32_t>(i % per_row) * 8;
+  const uint64_t batch = static_cast<uint64_t>(g.m) * ld;
+  float v[8] = {};
+  for (uint32_t s = 0; s < g.splits; ++s) {
+    const float* p = g.partial + (static_cast<uint64_t>(s) * g.batches + blockIdx.y) * batch + m * ld + n;
+    float x[8];
+    load8(p, x, 8, true);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += x[e];
+  }
+  epi(blockIdx.y, static_cast<uint32_t>(m), n, g.n - n, v);
+}
+
+// ---- launching --------------------------------------------------------------------------------
+
+/// Tile shape and number of splits for a product; the same for the workspace's size and for the launch.
+struct GemmPlan {
+  int tile = 0;  // 0: 64 x 64, 1: 128 x 128, 2: 256 x 256
+  uint32_t bm = 64, bn = 64, splits = 1;
+  size_t partial_bytes = 0;
+};
+
+GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t pairs, uint32_t batches);
+
+template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN, class Epi>
+void launch_tile(GemmArgs g, const Epi& epi, hipStream_t s) {
+  g.tiles_m = static_cast<uint32_t>(ceil_div(g.m, BM));
+  g.tiles_n = static_cast<uint32_t>(ceil_div(g.n, BN));
+  const uint64_t blocks = static_cast<uint64_t>(g.tiles_m) * g.tiles_n * g.splits;
+  QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "the matrix product is too large");
+  const dim3 grid(static_cast<unsigned>(blocks), g.batches);
+  if (g.splits > 1) {
+    const uint64_t ld = ceil_div(g.n, 8) * 8;
+    const PartialEpilogue pe{g.partial, ld, ld * g.m};
+    hipLaunchKernelGGL((gemm_kernel<T, AK, BK, BM, BN, WM, WN, PartialEpilogue>), grid, dim3(WM * WN * 64), 0, s, g, pe);
+    QVH_HIP(hipGetLastError());
+    hipLaunchKernelGGL((gemm_join_kernel<Epi>), dim3(static_cast<unsigned>(ceil_div(ld / 8 * g.m, 256)), g.batches),
+                       dim3(256), 0, s, g, epi);
+  } else {
+    hipLaunchKernelGGL((gemm_kernel<T, AK, BK, BM, BN, WM, WN, Epi>), grid, dim3(WM * WN * 64), 0, s, g, epi);
+  }
+  QVH_HIP(hipGetLastError());
+}
+
+template <class T, bool AK, bool BK, class Epi>
+void launch_gemm(GemmArgs g, const Epi& epi, const GemmPlan& plan, void* partial, hipStream_t s) {
+  if (g.m == 0 || g.n == 0 || g.batches == 0) return;
+  g.splits = plan.splits;
+  g.partial = static_cast<float*>(partial);
+  if (plan.tile == 2) {
+    launch_tile<T, AK, BK, 256, 256, 2, 4>(g, epi, s);
+  } else if (plan.tile == 1) {
+    launch_tile<T, AK, BK, 128, 128, 2, 2>(g, epi, s);
+  } else {
+    launch_tile<T, AK, BK, 64, 64, 2, 2>(g, epi, s);
+  }
+}
+
+}  // namespace qvh

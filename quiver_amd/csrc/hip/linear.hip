@@ -1,0 +1,639 @@
+// The linear layer y = act(x w^T + b) + residual and its gradients: operand preparation, the few-row
+// kernel, and the choice between them and the tiled products (gemm.hpp).
+#include <algorithm>
+
+#include "linear.hpp"
+
+namespace qvh {
+
+// ---- plan -------------------------------------------------------------------------------------
+
+GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t pairs, uint32_t batches) {
+  GemmPlan p;
+  const auto tiles = [&](uint64_t t) { return ceil_div(m, t) * ceil_div(n, t) * batches; };
+  if (tiles(256) >= 192) {
+    p.tile = 2;
+    p.bm = p.bn = 256;
+  } else if (tiles(128) >= 128) {
+    p.tile = 1;
+    p.bm = p.bn = 128;
+  }
+  const uint64_t t = tiles(p.bm), steps = ceil_div(k, kStep) * pairs;
+  if (t > 0 && t < 192 && steps >= 16) {
+    p.splits = static_cast<uint32_t>(std::min<uint64_t>({ceil_div(384, t), steps / 8, 64}));
+  }
+  if (p.splits > 1) p.partial_bytes = static_cast<size_t>(p.splits) * batches * m * (ceil_div(n, 8) * 8) * 4;
+  return p;
+}
+
+namespace {
+
+constexpr uint64_t kMaxRows = uint64_t{1} << 31, kMaxStride = uint64_t{1} << 22;
+constexpr uint32_t kMaxWidth = 1u << 20;
+constexpr uint64_t kFewRows = 64;  // x rows that the few-row kernel takes
+constexpr uint32_t kPlanes = 3;    // bf16 parts of an fp32 value
+
+// ---- operand preparation ----------------------------------------------------------------------
+
+struct PrepareArgs {
+  const void* src = nullptr;
+  uint64_t rows = 0, stride = 0;
+  uint32_t cols = 0;
+  void* dst = nullptr;  // [planes][rows][ld], ld = cols rounded up to 8, zeros behind the columns
+  uint64_t ld = 0, plane = 0;
+  uint32_t blocks = 0;
+  int vec = 0;
+};
+
+/// The three bf16 parts of an fp32 value, each the rounding of what the ones before it leave: their sum is
+/// the value, and the products of parts that the pairs leave out are below 2^-24 of the product (with parts
+/// cut off instead of rounded 2^-21, all of one sign). A first part that would round up to infinity is cut
+/// off. Of an infinity or NaN the first part is all.
+__device__ __forceinline__ void split3(float x, bhalf_t (&out)[3]) {
+  out[0] = static_cast<bhalf_t>(x);
+  const bool finite = fabsf(x) < __builtin_huge_valf();
+  if (finite && fabsf(static_cast<float>(out[0])) == __builtin_huge_valf()) {
+    out[0] = __builtin_bit_cast(bhalf_t, static_cast<uint16_t>(__float_as_uint(x) >> 16));
+  }
+  const float r1 = finite ? x - static_cast<float>(out[0]) : 0.0f;
+  out[1] = static_cast<bhalf_t>(r1);
+  out[2] = static_cast<bhalf_t>(r1 - static_cast<float>(out[1]));
+}
+
+template <class T>
+__device__ __forceinline__ void store_prepared(void* dst, uint64_t at, uint64_t plane, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    Pack<bhalf_t, 8> part[3];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      bhalf_t s[3];
+      split3(v[i], s);
+      part[0].v[i] = s[0];
+      part[1].v[i] = s[1];
+      part[2].v[i] = s[2];
+    }
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<Pack<bhalf_t, 8>*>(static_cast<bhalf_t*>(dst) + p * plane + at) = part[p];
+  } else {
+    store_floats<T, 8>(static_cast<T*>(dst) + at, v);
+  }
+}
+
+/// Copies up to two matrices into rows that the tiled product can read: aligned, padded with zeros, fp32 in
+/// its three parts.
+template <class T>
+__global__ void __launch_bounds__(256) prepare_kernel(PrepareArgs a, PrepareArgs b) {
+  const bool second = blockIdx.x >= a.blocks;
+  const PrepareArgs& p = second ? b : a;
+  const uint64_t i = static_cast<uint64_t>(second ? blockIdx.x - a.blocks : blockIdx.x) * 256 + threadIdx.x;
+  const uint32_t per_row = static_cast<uint32_t>(p.ld / 8);
+  const uint64_t r = i / per_row;
+  if (r >= p.rows) return;
+  const uint32_t c = static_cast<uint32_t>(i - r * per_row) * 8;
+  float v[8];
+  load8(static_cast<const T*>(p.src) + r * p.stride + c, v, p.cols - c, p.vec);
+  store_prepared<T>(p.dst, r * p.ld + c, p.plane, v);
+}
+
+/// dz = grad * act'(z) (stored if asked for) and its column sums over this work-group's rows. A thread
+/// has eight columns; eight threads share them, each taking every eighth row.
+struct SlopeArgs {
+  const void* grad;
+  const void* pre;
+  uint64_t rows, ld_grad, ld_pre;
+  uint32_t cols;
+  int act, vec_grad, vec_pre;
+  void* dz;  // as PrepareArgs::dst, or null
+  uint64_t ld, plane;
+  float* sums;  // [work-group][cols rounded up to 8], or null
+  uint32_t rows_each;
+};
+
+template <class T>
+__global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
+  __shared__ float s_sum[8][32 * 8 + 4];
+  const uint32_t lane = threadIdx.x % 32, part = threadIdx.x / 32;
+  const uint32_t c = (blockIdx.y * 32 + lane) * 8;
+  const uint64_t r0 = static_cast<uint64_t>(blockIdx.x) * a.rows_each;
+  const uint64_t r1 = r0 + a.rows_each < a.rows ? r0 + a.rows_each : a.rows;
+  float sum[8] = {};
+  if (c < a.cols) {
+    const uint32_t left = a.cols - c;
+#pragma unroll 2
+    for (uint64_t r = r0 + part; r < r1; r += 8) {
+      float g[8];
+      load8(static_cast<const T*>(a.grad) + r * a.ld_grad + c, g, left, a.vec_grad);
+      if (a.act != QVH_ACT_NONE) {
+        float z[8];
+        load8(static_cast<const T*>(a.pre) + r * a.ld_pre + c, z, left, a.vec_pre);
+        if (a.act == QVH_ACT_RELU) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[i] *= activate_slope(z[i], QVH_ACT_RELU);
+        } else if (a.act == QVH_ACT_GELU) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[i] *= activate_slope(z[i], QVH_ACT_GELU);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[i] *= activate_slope(z[i], QVH_ACT_SILU);
+        }
+      }
+      if (a.dz) store_prepared<T>(a.dz, r * a.ld + c, a.plane, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += g[i];
+    }
+  }
+  if (!a.sums) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s_sum[part][lane * 8 + i] = sum[i];
+  __syncthreads();
+  const uint32_t ld = (a.cols + 7) / 8 * 8;
+  const uint32_t col = blockIdx.y * 256 + threadIdx.x;
+  if (col < ld) {
+    float t = 0.0f;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) t += s_sum[p][threadIdx.x];
+    a.sums[static_cast<uint64_t>(blockIdx.x) * ld + col] = t;
+  }
+}
+
+/// Adds the work-groups' column sums in order: four waves take contiguous shares of them.
+template <class T>
+__global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ sums, uint32_t parts, uint32_t cols,
+                                                         T* __restrict__ out) {
+  __shared__ float s_sum[4][64];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ld = (cols + 7) / 8 * 8;
+  const uint32_t c = blockIdx.x * 64 + lane, share = (parts + 3) / 4;
+  const uint32_t p0 = wave * share < parts ? wave * share : parts, p1 = p0 + share < parts ? p0 + share : parts;
+  float t = 0.0f;
+  if (c < cols) {
+#pragma unroll 8
+    for (uint32_t p = p0; p < p1; ++p) t += sums[static_cast<uint64_t>(p) * ld + c];
+  }
+  s_sum[wave][lane] = t;
+  __syncthreads();
+  if (wave == 0 && c < cols) out[c] = static_cast<T>(((s_sum[0][lane] + s_sum[1][lane]) + s_sum[2][lane]) + s_sum[3][lane]);
+}
+
+// ---- few rows ---------------------------------------------------------------------------------
+//
+// For a handful of rows of x the weight is the traffic: every work-group reads 16 of its rows once,
+// straight into the fragments of the matrix unit, its eight waves taking every eighth step of k, and
+// adds the waves' sums in LDS.
+
+constexpr int kFewWaves = 8;
+
+template <class T>
+__device__ __forceinline__ void load_k(const T* row, uint32_t k, uint32_t depth, bool vec, typename Frag<T>::x8& f) {
+  if (vec && k + 8 <= depth) {
+    f = *reinterpret_cast<const typename Frag<T>::x8*>(row + k);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = k + e < depth ? row[k + e] : static_cast<T>(0.0f);
+  }
+}
+
+__device__ __forceinline__ void load_k(const float* row, uint32_t k, uint32_t depth, bool vec, f32x4_t& f) {
+  if (vec && k + 4 <= depth) {
+    f = *reinterpret_cast<const f32x4_t*>(row + k);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = k + e < depth ? row[k + e] : 0.0f;
+  }
+}
+
+__device__ __forceinline__ f32x4_t mfma16(Frag<half_t>::x8 a, Frag<half_t>::x8 b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mfma16(Frag<bhalf_t>::x8 a, Frag<bhalf_t>::x8 b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4_t mfma16(f32x4_t a, f32x4_t b, f32x4_t c) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+template <class T>
+struct FewFrag {
+  using type = typename Frag<T>::x8;
+};
+template <>
+struct FewFrag<float> {
+  using type = f32x4_t;
+};
+
+template <class T, int MT>
+__global__ void __launch_bounds__(kFewWaves * 64) few_rows_kernel(const T* __restrict__ x, uint64_t ldx,
+                                                                  const T* __restrict__ w, uint64_t ldw, uint32_t m,
+                                                                  uint32_t n, uint32_t k, int vec_x, int vec_w,
+                                                                  LinearEpilogue<T> epi) {
+  using F = typename FewFrag<T>::type;
+  constexpr uint32_t kEach = sizeof(F) / sizeof(T);  // k per lane and step
+  constexpr uint32_t kDepth = kEach * 4;
+  __shared__ float s_sum[kFewWaves][16 * MT][17];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, h = lane >> 4;
+  const uint32_t n0 = blockIdx.x * 16;
+  const T* wr = w + static_cast<uint64_t>(n0 + i < n ? n0 + i : n - 1) * ldw;
+  const T* xr[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) xr[t] = x + static_cast<uint64_t>(16 * t + i < m ? 16 * t + i : m - 1) * ldx;
+  f32x4_t acc[MT] = {};
+#pragma unroll 4
+  for (uint32_t k0 = wave * kDepth; k0 < k; k0 += kFewWaves * kDepth) {
+    F fw, fx[MT];
+    load_k(wr, k0 + h * kEach, k, vec_w, fw);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) load_k(xr[t], k0 + h * kEach, k, vec_x, fx[t]);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = mfma16(fw, fx[t], acc[t]);
+  }
+  // Lane (i, h) holds rows 4 h .. + 3 of w against row i of x.
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s_sum[wave][16 * t + i][4 * h + r] = acc[t][r];
+  }
+  __syncthreads();
+  for (uint32_t o = threadIdx.x; o < 256 * MT; o += kFewWaves * 64) {
+    const uint32_t row = o / 16, col = o % 16;
+    float sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kFewWaves; ++v) sum += s_sum[v][row][col];
+    if (row < m && n0 + col < n) epi.one(row, n0 + col, sum);
+  }
+}
+
+// ---- host side --------------------------------------------------------------------------------
+
+bool aligned_rows(const void* p, uint64_t stride, uint64_t cols, size_t elem) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * elem % 16 == 0 && cols * elem % 16 == 0;
+}
+
+/// 8 elements at a time: base and stride allow 16-byte accesses.
+int vec8(const void* p, uint64_t stride, size_t elem) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * elem % 16 == 0;
+}
+
+struct Space {
+  size_t at = 0;
+  char* base = nullptr;
+  void* take(size_t bytes) {
+    void* p = base ? base + at : nullptr;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  }
+};
+
+/// A matrix as an operand of the tiled product: itself where it can be read as it is, else a copy to be made.
+struct Prepared {
+  GemmOperand op;
+  PrepareArgs job;
+  bool copy = false;
+};
+
+Prepared prepare_operand(const void* src, uint64_t rows, uint64_t stride, uint32_t cols, int dtype, Space& ws) {
+  Prepared p;
+  if (dtype != QVH_FP32 && aligned_rows(src, stride, cols, 2)) {
+    p.op.base = src;
+    p.op.ld = stride;
+    return p;
+  }
+  p.copy = true;
+  p.job.src = src;
+  p.job.rows = rows;
+  p.job.stride = stride;
+  p.job.cols = cols;
+  p.job.ld = ceil_div(cols, 8) * 8;
+  p.job.plane = p.job.ld * rows;
+  p.job.dst = ws.take(p.job.plane * (dtype == QVH_FP32 ? kPlanes : 1) * 2);
+  p.job.vec = vec8(src, stride, dtype_size(dtype));
+  p.job.blocks = static_cast<uint32_t>(ceil_div(p.job.ld / 8 * rows, 256));
+  p.op.base = p.job.dst;
+  p.op.ld = p.job.ld;
+  p.op.plane = p.job.plane;
+  return p;
+}
+
+void launch_prepare(int dtype, const Prepared& a, const Prepared& b, hipStream_t s) {
+  const PrepareArgs none;
+  const PrepareArgs& first = a.copy ? a.job : b.copy ? b.job : none;
+  const PrepareArgs& second = a.copy && b.copy ? b.job : none;
+  const uint64_t blocks = static_cast<uint64_t>(first.blocks) + second.blocks;
+  if (blocks == 0) return;
+  QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "the matrix product is too large");
+  with_dtype(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    hipLaunchKernelGGL((prepare_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, first, second);
+  });
+  QVH_HIP(hipGetLastError());
+}
+
+/// The pairs of parts whose products make up fp32's, the smallest first.
+void set_pairs(GemmArgs& g, int dtype) {
+  g.pairs = 1;
+  if (dtype != QVH_FP32) return;
+  const uint8_t pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
+  g.pairs = 6;
+  std::copy(pa, pa + 6, g.pa);
+  std::copy(pb, pb + 6, g.pb);
+}
+
+void run_product(Form form, int dtype, GemmArgs g, const void* bias, const void* residual, uint64_t ld_residual,
+                 void* out, uint64_t ld_out, void* keep, uint64_t ld_keep, int act, const GemmPlan& plan, void* partial,
+                 hipStream_t s) {
+  with_dtype(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    LinearEpilogue<T> e;
+    e.bias = static_cast<const T*>(bias);
+    e.residual = static_cast<const T*>(residual);
+    e.out = static_cast<T*>(out);
+    e.keep = static_cast<T*>(keep);
+    e.ld_residual = ld_residual;
+    e.ld_out = ld_out;
+    e.ld_keep = ld_keep;
+    e.act = act;
+    e.vec_bias = vec8(bias, 8, sizeof(T));
+    e.vec_residual = vec8(residual, ld_residual, sizeof(T));
+    e.vec_out = vec8(out, ld_out, sizeof(T));
+    e.vec_keep = vec8(keep, ld_keep, sizeof(T));
+    e.direct = g;
+    e.a_by_k = form == Form::kKK;
+    e.b_by_k = form != Form::kRowsRows;
+    if constexpr (std::is_same_v<T, float>) {
+      gemm_fp32(form, g, e, plan, partial, s);
+    } else if constexpr (std::is_same_v<T, half_t>) {
+      gemm_fp16(form, g, e, plan, partial, s);
+    } else {
+      gemm_bf16(form, g, e, plan, partial, s);
+    }
+  });
+}
+
+void check_shape(const std::string& w, uint64_t m, uint32_t k, uint32_t n, int dtype, int act) {
+  require_dtype(w.c_str(), dtype);
+  QVH_REQUIRE(act >= QVH_ACT_NONE && act <= QVH_ACT_SILU, w + ": unknown activation");
+  QVH_REQUIRE(m < kMaxRows, w + ": m must be below 2^31");
+  QVH_REQUIRE(k <= kMaxWidth && n <= kMaxWidth, w + ": k and n must be at most 2^20");
+}
+
+void check_matrix(const std::string& w, const char* name, const void* p, uint64_t rows, uint64_t cols, uint64_t stride,
+                  size_t elem) {
+  QVH_REQUIRE(p != nullptr || rows == 0 || cols == 0, w + ": " + name + " is null");
+  QVH_REQUIRE(reinterpret_cast<uintptr_t>(p) % elem == 0, w + ": " + name + " is not aligned to its element type");
+  QVH_REQUIRE((stride >= cols || rows <= 1) && stride <= kMaxStride, w + ": " + name + "'s stride must be in [row length, 2^22]");
+}
+
+struct LinearRun {
+  bool few = false;
+  Prepared x, w;
+  GemmPlan plan;
+  void* partial = nullptr;
+  size_t bytes = 0;
+};
+
+LinearRun plan_linear(const qvh_linear_args& a, void* ws) {
+  LinearRun r;
+  if (a.m == 0 || a.n == 0) return r;
+  r.few = a.m <= kFewRows;
+  if (r.few) return r;
+  Space sp;
+  sp.base = static_cast<char*>(ws);
+  r.x = prepare_operand(a.x, a.m, a.x_stride, a.k, a.dtype, sp);
+  r.w = prepare_operand(a.weight, a.n, a.weight_stride, a.k, a.dtype, sp);
+  r.plan = gemm_plan(a.m, a.n, a.k, a.dtype == QVH_FP32 ? 6 : 1, 1);
+  r.partial = sp.take(r.plan.partial_bytes);
+  r.bytes = sp.at;
+  return r;
+}
+
+void check_linear(const char* who, const qvh_linear_args* a) {
+  const std::string w(who);
+  QVH_REQUIRE(a != nullptr, w + ": null arguments");
+  check_shape(w, a->m, a->k, a->n, a->dtype, a->activation);
+  const size_t e = dtype_size(a->dtype);
+  check_matrix(w, "x", a->x, a->m, a->k, a->x_stride, e);
+  check_matrix(w, "weight", a->weight, a->n, a->k, a->weight_stride, e);
+  check_matrix(w, "out", a->out, a->m, a->n, a->out_stride, e);
+  if (a->residual) check_matrix(w, "residual", a->residual, a->m, a->n, a->residual_stride, e);
+  if (a->preactivation) check_matrix(w, "preactivation", a->preactivation, a->m, a->n, a->preactivation_stride, e);
+  QVH_REQUIRE(reinterpret_cast<uintptr_t>(a->bias) % e == 0, w + ": bias is not aligned to its element type");
+}
+
+template <class T>
+void launch_few(const qvh_linear_args& a, hipStream_t s) {
+  LinearEpilogue<T> e;
+  e.bias = static_cast<const T*>(a.bias);
+  e.residual = static_cast<const T*>(a.residual);
+  e.out = static_cast<T*>(a.out);
+  e.keep = static_cast<T*>(a.preactivation);
+  e.ld_residual = a.residual_stride;
+  e.ld_out = a.out_stride;
+  e.ld_keep = a.preactivation_stride;
+  e.act = a.activation;
+  const auto go = [&](auto tiles) {
+    hipLaunchKernelGGL((few_rows_kernel<T, decltype(tiles)::value>), dim3(static_cast<unsigned>(ceil_div(a.n, 16))),
+                       dim3(kFewWaves * 64), 0, s, static_cast<const T*>(a.x), a.x_stride,
+                       static_cast<const T*>(a.weight), a.weight_stride, static_cast<uint32_t>(a.m), a.n, a.k,
+                       vec8(a.x, a.x_stride, sizeof(T)), vec8(a.weight, a.weight_stride, sizeof(T)), e);
+  };
+  if (a.m <= 16) {
+    go(std::integral_constant<int, 1>{});
+  } else if (a.m <= 32) {
+    go(std::integral_constant<int, 2>{});
+  } else {
+    go(std::integral_constant<int, 4>{});
+  }
+  QVH_HIP(hipGetLastError());
+}
+
+struct GradRun {
+  bool slope = false;  // dz is written or summed
+  SlopeArgs job{};
+  uint32_t sum_parts = 0;
+  GemmOperand dz;
+  Prepared x, w;
+  GemmPlan plan_x, plan_w;
+  void *partial_x = nullptr, *partial_w = nullptr;
+  size_t bytes = 0;
+};
+
+GradRun plan_grad(const qvh_linear_grad_args& a, void* ws) {
+  GradRun r;
+  if (a.n == 0 || (a.m == 0 && a.k == 0)) return r;
+  const size_t e = dtype_size(a.dtype);
+  const uint32_t pairs = a.dtype == QVH_FP32 ? 6 : 1;
+  Space sp;
+  sp.base = static_cast<char*>(ws);
+  const bool products = (a.grad_x || a.grad_weight) && a.k > 0;
+  const bool as_is = a.activation == QVH_ACT_NONE && a.dtype != QVH_FP32 && aligned_rows(a.grad, a.grad_stride, a.n, 2);
+  r.slope = (products && !as_is) || a.grad_bias;
+  if (r.slope) {
+    SlopeArgs& j = r.job;
+    j.grad = a.grad;
+    j.pre = a.preactivation;
+    j.rows = a.m;
+    j.ld_grad = a.grad_stride;
+    j.ld_pre = a.preactivation_stride;
+    j.cols = a.n;
+    j.act = a.activation;
+    j.vec_grad = vec8(a.grad, a.grad_stride, e);
+    j.vec_pre = vec8(a.preactivation, a.preactivation_stride, e);
+    j.ld = ceil_div(a.n, 8) * 8;
+    j.plane = j.ld * a.m;
+    if (products && !as_is) j.dz = sp.take(j.plane * (a.dtype == QVH_FP32 ? kPlanes : 1) * 2);
+    // Work-groups of 256 columns; rows spread over about a thousand of them, at least 16 rows each.
+    const uint64_t across = ceil_div(a.n, 256);
+    j.rows_each = static_cast<uint32_t>(std::max<uint64_t>(16, ceil_div(ceil_div(a.m, 8), ceil_div(1024, across)) * 8));
+    r.sum_parts = static_cast<uint32_t>(ceil_div(a.m, j.rows_each));
+    if (a.grad_bias) j.sums = static_cast<float*>(sp.take(static_cast<size_t>(r.sum_parts) * j.ld * 4));
+    r.dz.base = j.dz;
+    r.dz.ld = j.ld;
+    r.dz.plane = j.plane;
+  }
+  if (as_is) {
+    r.dz.base = a.grad;
+    r.dz.ld = a.grad_stride;
+    r.dz.plane = 0;
+  }
+  if (products) {
+    if (a.grad_x) {
+      r.w = prepare_operand(a.weight, a.n, a.weight_stride, a.k, a.dtype, sp);
+      r.plan_x = gemm_plan(a.m, a.k, a.n, pairs, 1);
+      r.partial_x = sp.take(r.plan_x.partial_bytes);
+    }
+    if (a.grad_weight) {
+      r.x = prepare_operand(a.x, a.m, a.x_stride, a.k, a.dtype, sp);
+      r.plan_w = gemm_plan(a.n, a.k, a.m, pairs, 1);
+      r.partial_w = sp.take(r.plan_w.partial_bytes);
+    }
+  }
+  r.bytes = sp.at;
+  return r;
+}
+
+void check_grad(const char* who, const qvh_linear_grad_args* a) {
+  const std::string w(who);
+  QVH_REQUIRE(a != nullptr, w + ": null arguments");
+  check_shape(w, a->m, a->k, a->n, a->dtype, a->activation);
+  const size_t e = dtype_size(a->dtype);
+  check_matrix(w, "grad", a->grad, a->m, a->n, a->grad_stride, e);
+  if (a->activation != QVH_ACT_NONE) {
+    QVH_REQUIRE(a->preactivation != nullptr || a->m == 0 || a->n == 0, w + ": an activation's gradient needs the pre-activation");
+    check_matrix(w, "preactivation", a->preactivation, a->m, a->n, a->preactivation_stride, e);
+  }
+  if (a->grad_x) {
+    check_matrix(w, "weight", a->weight, a->n, a->k, a->weight_stride, e);
+    check_matrix(w, "grad_x", a->grad_x, a->m, a->k, a->grad_x_stride, e);
+  }
+  if (a->grad_weight) {
+    check_matrix(w, "x", a->x, a->m, a->k, a->x_stride, e);
+    check_matrix(w, "grad_weight", a->grad_weight, a->n, a->k, a->grad_weight_stride, e);
+  }
+  QVH_REQUIRE(reinterpret_cast<uintptr_t>(a->grad_bias) % e == 0, w + ": grad_bias is not aligned to its element type");
+}
+
+void check_workspace(const char* who, const void* ws, uint64_t have, size_t need) {
+  const std::string w(who);
+  QVH_REQUIRE(need == 0 || (ws != nullptr && have >= need), w + ": the workspace is too small");
+  QVH_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 16 == 0, w + ": the workspace must be 16-byte aligned");
+}
+
+}  // namespace
+}  // namespace qvh
+
+extern "C" {
+
+qvh_status qvh_linear_workspace(const qvh_linear_args* args, uint64_t* bytes) {
+  return qvh::guarded([&] {
+    QVH_REQUIRE(bytes != nullptr, "qvh_linear_workspace: null output");
+    qvh::check_linear("qvh_linear_workspace", args);
+    *bytes = qvh::plan_linear(*args, nullptr).bytes;
+  });
+}
+
+qvh_status qvh_linear_device(const qvh_linear_args* args, void* d_workspace, uint64_t workspace_bytes, void* stream) {
+  return qvh::guarded([&] {
+    using namespace qvh;
+    check_linear("qvh_linear_device", args);
+    const qvh_linear_args& a = *args;
+    if (a.m == 0 || a.n == 0) return;
+    const LinearRun r = plan_linear(a, d_workspace);
+    check_workspace("qvh_linear_device", d_workspace, workspace_bytes, r.bytes);
+    current_device();
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (r.few) {
+      with_dtype(a.dtype, [&](auto* t) { launch_few<std::remove_pointer_t<decltype(t)>>(a, s); });
+      return;
+    }
+    launch_prepare(a.dtype, r.x, r.w, s);
+    GemmArgs g;
+    g.a = r.x.op;
+    g.b = r.w.op;
+    g.m = static_cast<uint32_t>(a.m);
+    g.n = a.n;
+    g.k = a.k;
+    set_pairs(g, a.dtype);
+    run_product(Form::kRowsRows, a.dtype, g, a.bias, a.residual, a.residual_stride, a.out, a.out_stride, a.preactivation,
+                a.preactivation_stride, a.activation, r.plan, r.partial, s);
+  });
+}
+
+qvh_status qvh_linear_grad_workspace(const qvh_linear_grad_args* args, uint64_t* bytes) {
+  return qvh::guarded([&] {
+    QVH_REQUIRE(bytes != nullptr, "qvh_linear_grad_workspace: null output");
+    qvh::check_grad("qvh_linear_grad_workspace", args);
+    *bytes = qvh::plan_grad(*args, nullptr).bytes;
+  });
+}
+
+qvh_status qvh_linear_grad_device(const qvh_linear_grad_args* args, void* d_workspace, uint64_t workspace_bytes,
+                                  void* stream) {
+  return qvh::guarded([&] {
+    using namespace qvh;
+    check_grad("qvh_linear_grad_device", args);
+    const qvh_linear_grad_args& a = *args;
+    const GradRun r = plan_grad(a, d_workspace);
+    check_workspace("qvh_linear_grad_device", d_workspace, workspace_bytes, r.bytes);
+    current_device();
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (r.slope && r.sum_parts > 0) {
+      with_dtype(a.dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        hipLaunchKernelGGL((slope_kernel<T>), dim3(r.sum_parts, static_cast<unsigned>(ceil_div(a.n, 256))), dim3(256), 0, s,
+                           r.job);
+      });
+      QVH_HIP(hipGetLastError());
+    }
+    if (a.grad_bias && a.n > 0) {
+      with_dtype(a.dtype, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        hipLaunchKernelGGL((column_sum_kernel<T>), dim3(static_cast<unsigned>(ceil_div(a.n, 64))), dim3(256), 0, s,
+                           r.job.sums, r.sum_parts, a.n, static_cast<T*>(a.grad_bias));
+      });
+      QVH_HIP(hipGetLastError());
+    }
+    if (a.k == 0 || !(a.grad_x || a.grad_weight)) return;
+    launch_prepare(a.dtype, r.x, r.w, s);
+    GemmArgs g;
+    set_pairs(g, a.dtype);
+    g.a = r.dz;
+    if (a.grad_x && a.m > 0) {
+      g.b = r.w.op;
+      g.m = static_cast<uint32_t>(a.m);
+      g.n = a.k;
+      g.k = a.n;
+      run_product(Form::kRowsK, a.dtype, g, nullptr, nullptr, 0, a.grad_x, a.grad_x_stride, nullptr, 0, QVH_ACT_NONE,
+                  r.plan_x, r.partial_x, s);
+    }
+    if (a.grad_weight && a.n > 0) {
+      g.b = r.x.op;
+      g.m = a.n;
+      g.n = a.k;
+      g.k = static_cast<uint32_t>(a.m);
+      run_product(Form::kKK, a.dtype, g, nullptr, nullptr, 0, a.grad_weight, a.grad_weight_stride, nullptr, 0, QVH_ACT_NONE,
+                  r.plan_w, r.partial_w, s);
+    }
+  });
+}
+
+}  // extern "C"

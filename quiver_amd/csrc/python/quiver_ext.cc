@@ -167,6 +167,65 @@ PYBIND11_MODULE(_quiver, m) {
                               reinterpret_cast<void*>(stream)));
   });
 
+  // The encoder's operators (quiver_amd/encoder.py checks the tensors). They only enqueue, which is
+  // shorter than handing the GIL over and back.
+  const auto ptr = [](std::uintptr_t p) { return reinterpret_cast<void*>(p); };
+  m.def("_embed", [check, ptr](std::uintptr_t table, std::uint64_t rows, std::uint32_t dim, std::uint64_t stride, int dtype,
+                               std::uintptr_t tokens, int index_bytes, std::uint64_t count, float scale,
+                               std::uintptr_t out, std::uintptr_t stream) {
+    check(qvh_embed_device(ptr(table), rows, dim, stride, dtype, ptr(tokens), index_bytes, count, scale, ptr(out),
+                           ptr(stream)));
+  });
+  m.def("_embed_grad_workspace", [check](std::uint64_t rows, std::uint32_t dim, std::uint64_t count) {
+    std::uint64_t bytes = 0;
+    check(qvh_embed_grad_workspace(rows, dim, count, &bytes));
+    return bytes;
+  });
+  m.def("_embed_grad", [check, ptr](std::uintptr_t grad, std::uint64_t stride, std::uintptr_t tokens, int index_bytes,
+                                    std::uint64_t count, std::uint64_t rows, std::uint32_t dim, int dtype, float scale,
+                                    std::uintptr_t out, std::uintptr_t work, std::uint64_t work_bytes,
+                                    std::uintptr_t stream) {
+    check(qvh_embed_grad_device(ptr(grad), stride, ptr(tokens), index_bytes, count, rows, dim, dtype, scale, ptr(out),
+                                ptr(work), work_bytes, ptr(stream)));
+  });
+  // These two return the workspace they lack, in bytes, and enqueue nothing then.
+  m.def("_linear", [check, ptr](std::uint64_t m, std::uint32_t k, std::uint32_t n, int dtype, int act, std::uintptr_t x,
+                                std::uint64_t xs, std::uintptr_t w, std::uint64_t ws, std::uintptr_t bias,
+                                std::uintptr_t residual, std::uint64_t rs, std::uintptr_t out, std::uint64_t os,
+                                std::uintptr_t pre, std::uint64_t ps, std::uintptr_t work, std::uint64_t work_bytes,
+                                std::uintptr_t stream) -> std::uint64_t {
+    const qvh_linear_args a{m, k, n, dtype, act, ptr(x), xs, ptr(w), ws, ptr(bias), ptr(residual), rs, ptr(out), os, ptr(pre), ps};
+    std::uint64_t need = 0;
+    check(qvh_linear_workspace(&a, &need));
+    if (need > work_bytes) return need;
+    check(qvh_linear_device(&a, ptr(work), work_bytes, ptr(stream)));
+    return 0;
+  });
+  m.def("_linear_grad", [check, ptr](std::uint64_t m, std::uint32_t k, std::uint32_t n, int dtype, int act,
+                                     std::uintptr_t grad, std::uint64_t gs, std::uintptr_t pre, std::uint64_t ps,
+                                     std::uintptr_t x, std::uint64_t xs, std::uintptr_t w, std::uint64_t ws,
+                                     std::uintptr_t gx, std::uint64_t gxs, std::uintptr_t gw, std::uint64_t gws,
+                                     std::uintptr_t gb, std::uintptr_t work, std::uint64_t work_bytes,
+                                     std::uintptr_t stream) -> std::uint64_t {
+    const qvh_linear_grad_args a{m, k, n, dtype, act, ptr(grad), gs, ptr(pre), ps, ptr(x), xs, ptr(w), ws, ptr(gx), gxs, ptr(gw), gws, ptr(gb)};
+    std::uint64_t need = 0;
+    check(qvh_linear_grad_workspace(&a, &need));
+    if (need > work_bytes) return need;
+    check(qvh_linear_grad_device(&a, ptr(work), work_bytes, ptr(stream)));
+    return 0;
+  });
+  m.def("_orthogonalize_workspace", [check](std::uint64_t batch, std::uint32_t m, std::uint32_t n) {
+    std::uint64_t bytes = 0;
+    check(qvh_orthogonalize_workspace(batch, m, n, &bytes));
+    return bytes;
+  });
+  m.def("_orthogonalize", [check, ptr](std::uintptr_t update, std::uint64_t batch, std::uint32_t m, std::uint32_t n,
+                                       int dtype, std::uint32_t steps, float a, float b, float c, std::uintptr_t out,
+                                       std::uintptr_t work, std::uint64_t work_bytes, std::uintptr_t stream) {
+    check(qvh_orthogonalize_device(ptr(update), batch, m, n, dtype, steps, a, b, c, ptr(out), ptr(work), work_bytes,
+                                   ptr(stream)));
+  });
+
   m.def(
       "simd_isa",
       [] {
