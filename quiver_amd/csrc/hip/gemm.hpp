@@ -51,34 +51,57 @@ struct GemmOperand {
   uint64_t ld = 0, plane = 0, batch = 0;  // in elements
 };
 
-constexpr int kMaxPairs = 6;
-
 struct GemmArgs {
   GemmOperand a, b;
   uint32_t m = 0, n = 0, k = 0;
-  uint32_t pairs = 1;  // plane pairs
-  uint8_t pa[kMaxPairs] = {0}, pb[kMaxPairs] = {0};
+  uint32_t pairs = 1;        // pairs of planes, at most eight
+  uint32_t pa = 0, pb = 0;   // the planes of pair i: four bits each, from the lowest
   uint32_t tiles_m = 0, tiles_n = 0, splits = 1, batches = 1;
   float* partial = nullptr;  // [split][batch][m][n rounded up to 8] when splits > 1
 };
 
-enum class Activation : int { kNone = QVH_ACT_NONE, kRelu = QVH_ACT_RELU, kGelu = QVH_ACT_GELU, kSilu = QVH_ACT_SILU };
+/// The upper tail of the normal distribution at a >= 0 for 16-bit results, by the rational approximation
+/// 7.1.26 of Abramowitz and Stegun (error below 8e-8), and *e = exp(-z^2 / 2). About a fifth of erff's cost,
+/// which would take longer than a short product's matrix instructions.
+__device__ __forceinline__ float normal_tail(float a, float z, float* e) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.3275911f * 0.70710678f, 1.0f));
+  float p = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+  p = fmaf(t, p, 0.5f * 1.421413741f);
+  p = fmaf(t, p, 0.5f * -0.284496736f);
+  p = fmaf(t, p, 0.5f * 0.254829592f);
+  *e = __builtin_amdgcn_exp2f(z * z * -0.72134752f);
+  return p * t * *e;
+}
 
+/// FINE: for fp32 results.
+template <bool FINE>
 __device__ __forceinline__ float activate(float z, int act) {
   if (act == QVH_ACT_RELU) return z > 0.0f || z != z ? z : 0.0f;
-  if (act == QVH_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-  if (act == QVH_ACT_SILU) return z / (1.0f + __expf(-z));
+  if (act == QVH_ACT_GELU) {
+    if constexpr (FINE) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    // max(z, 0) - |z| tail(|z|), the product of +infinity and 0 kept out.
+    const float a = fmaxf(-z, fminf(z, 64.0f));
+    float e;
+    return fmaf(-a, normal_tail(a, z, &e), fmaxf(z, 0.0f));
+  }
+  if (act == QVH_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
   return z;
 }
 
 /// d activate / dz.
+template <bool FINE>
 __device__ __forceinline__ float activate_slope(float z, int act) {
   if (act == QVH_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
   if (act == QVH_ACT_GELU) {
-    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    if constexpr (FINE) {
+      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    }
+    float e;
+    const float tail = normal_tail(fabsf(z), z, &e);
+    return fmaf(z * 0.39894228f, e, z > 0.0f ? 1.0f - tail : tail);
   }
   if (act == QVH_ACT_SILU) {
-    const float s = 1.0f / (1.0f + __expf(-z));
+    const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-z));
     return s * (1.0f + z * (1.0f - s));
   }
   return 1.0f;
@@ -160,7 +183,7 @@ struct LinearEpilogue {
   __device__ __forceinline__ void one(uint32_t m, uint32_t n, float v) const {
     if (bias) v += static_cast<float>(bias[n]);
     if (keep) keep[m * ld_keep + n] = static_cast<T>(v);
-    v = activate(v, act);
+    v = activate<sizeof(T) == 4>(v, act);
     if (residual) v += static_cast<float>(residual[m * ld_residual + n]);
     out[m * ld_out + n] = static_cast<T>(v);
   }
@@ -181,13 +204,13 @@ struct LinearEpilogue {
     if (keep) store8(keep + m * ld_keep + n, v, left, vec_keep);
     if (act == QVH_ACT_RELU) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = activate(v[i], QVH_ACT_RELU);
+      for (int i = 0; i < 8; ++i) v[i] = activate<sizeof(T) == 4>(v[i], QVH_ACT_RELU);
     } else if (act == QVH_ACT_GELU) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = activate(v[i], QVH_ACT_GELU);
+      for (int i = 0; i < 8; ++i) v[i] = activate<sizeof(T) == 4>(v[i], QVH_ACT_GELU);
     } else if (act == QVH_ACT_SILU) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = activate(v[i], QVH_ACT_SILU);
+      for (int i = 0; i < 8; ++i) v[i] = activate<sizeof(T) == 4>(v[i], QVH_ACT_SILU);
     }
     if (residual) {
       float r[8];
@@ -211,41 +234,34 @@ struct PartialEpilogue {
 
 // ---- the kernel -------------------------------------------------------------------------------
 
-constexpr int kStep = 64;  // k per step
-
-/// The 16-byte pieces of one operand's R x 64 step: addresses for the loads into LDS, and fragments.
-template <class T, bool BY_K, int R, int WAVES>
+/// The 16-byte pieces of one operand's R x D step: addresses for the loads into LDS, and fragments.
+template <class T, bool BY_K, int R, int D, int WAVES>
 struct Stage {
-  static constexpr int kBytes = R * kStep * 2;
+  static constexpr int kBytes = R * D * 2;
   static constexpr int kLoads = kBytes / 1024 / WAVES;
-  static constexpr int kChunks = R / 8;              // 16-byte pieces per k, stored by k
-  static constexpr int kLines = 64 / kChunks;        // k per load, stored by k
+  static constexpr int kChunks = BY_K ? R / 8 : D / 8;  // 16-byte pieces per line (k, or row)
+  static constexpr int kLines = 64 / kChunks;           // lines per load
+  static_assert(D == 32 || D == 64, "a row is 64 or 128 bytes in LDS");
   static_assert(kLoads >= 1 && kBytes % (1024 * WAVES) == 0, "every wave loads whole kilobytes");
+
+  /// Piece c of a line lies at c ^ flip(line). LDS serves 256 bytes at a time, sixteen pieces: by rows, those of
+  /// sixteen neighbouring rows at one k fall on different banks (two rows, or four, share 256 bytes), by k
+  /// those of the four k that a transposing read takes at once.
+  static __device__ __forceinline__ uint32_t flip(uint32_t line) {
+    if constexpr (BY_K) return (line & (R / 32 - 1)) * 4;
+    return D == 64 ? line >> 1 & 7 : line >> 2 & 3;
+  }
 
   /// Byte offset (from the tile's first row and the step's first k) of what this lane loads in load i; the
   /// lanes fill LDS in order. `rows` and `depth`: how many of each there are from the tile's start on.
   static __device__ __forceinline__ uint32_t offset(int i, int wave, int lane, uint32_t ld, uint32_t rows, uint32_t depth) {
-    const int block = i * WAVES + wave;
-    if constexpr (BY_K) {
-      uint32_t k = static_cast<uint32_t>(block * kLines + lane / kChunks);
-      uint32_t c = static_cast<uint32_t>(lane % kChunks) ^ flip(k);
-      k = k < depth ? k : depth - 1;
-      const uint32_t last = (rows + 7) / 8 - 1;
-      c = c < last ? c : last;
-      return k * ld * 2 + c * 16;
-    } else {
-      uint32_t r = static_cast<uint32_t>(block * 8 + (lane >> 3));
-      uint32_t c = static_cast<uint32_t>((lane & 7) ^ (lane >> 3));
-      r = r < rows ? r : rows - 1;
-      const uint32_t last = (depth + 7) / 8 - 1;
-      c = c < last ? c : last;
-      return r * ld * 2 + c * 16;
-    }
+    uint32_t line = static_cast<uint32_t>((i * WAVES + wave) * kLines + lane / kChunks);
+    uint32_t c = static_cast<uint32_t>(lane % kChunks) ^ flip(line);
+    const uint32_t lines = BY_K ? depth : rows, last = ((BY_K ? rows : depth) + 7) / 8 - 1;
+    line = line < lines ? line : lines - 1;
+    c = c < last ? c : last;
+    return line * ld * 2 + c * 16;
   }
-
-  /// Stored by k, piece c of line k lies at c ^ flip(k): the four k that a transposing read takes at once
-  /// fall on different banks.
-  static __device__ __forceinline__ uint32_t flip(uint32_t k) { return (k & (R / 32 - 1)) * 4; }
 
   /// Fragment of rows row0 .. row0 + 31 (a multiple of 32) and k kk * 16 .. + 15.
   static __device__ __forceinline__ typename Frag<T>::x8 fragment(const char* lds, int row0, int kk, int lane) {
@@ -265,7 +281,8 @@ struct Stage {
       return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
       const int row = row0 + (lane & 31);
-      return *reinterpret_cast<const typename Frag<T>::x8*>(lds + row * 128 + (((kk * 2 + (lane >> 5)) ^ (lane & 7)) * 16));
+      return *reinterpret_cast<const typename Frag<T>::x8*>(
+          lds + row * (D * 2) + (((kk * 2 + (lane >> 5)) ^ flip(static_cast<uint32_t>(lane & 31))) * 16));
     }
   }
 };
@@ -300,17 +317,24 @@ __device__ __forceinline__ X8 clip(X8 f, int kk, int lane, uint32_t depth) {
   return f;
 }
 
-template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN, class Epi>
-__global__ void __launch_bounds__(WM* WN * 64, 2)
+/// Tile of a work-group, its waves, the depth of a step and the steps that LDS holds.
+template <int BM_, int BN_, int WM_, int WN_, int D_, int STAGES_>
+struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, D = D_, STAGES = STAGES_;
+};
+
+template <class T, bool AK, bool BK, class Shape, class Epi>
+__global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::BN / (Shape::WM * Shape::WN) > 128 * 64 ? 1 : 2)
     gemm_kernel(GemmArgs g, Epi epi) {
+  constexpr int BM = Shape::BM, BN = Shape::BN, WM = Shape::WM, WN = Shape::WN, kStep = Shape::D, kStages = Shape::STAGES;
   constexpr int kWaves = WM * WN;
-  using SA = Stage<T, AK, BM, kWaves>;
-  using SB = Stage<T, BK, BN, kWaves>;
+  using SA = Stage<T, AK, BM, kStep, kWaves>;
+  using SB = Stage<T, BK, BN, kStep, kWaves>;
   constexpr int kStageBytes = SA::kBytes + SB::kBytes;
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 blocks per wave
   constexpr int kSlabLd = BN / WN + 8;
   constexpr int kSlabBytes = 32 * kSlabLd * 4 * kWaves;
-  constexpr int kLds = 2 * kStageBytes > kSlabBytes ? 2 * kStageBytes : kSlabBytes;
+  constexpr int kLds = kStages * kStageBytes > kSlabBytes ? kStages * kStageBytes : kSlabBytes;
   __shared__ __attribute__((aligned(1024))) char s_mem[kLds];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -334,10 +358,12 @@ __global__ void __launch_bounds__(WM* WN * 64, 2)
 
   const uint32_t row0 = tm * BM, col0 = tn * BN;
   const uint32_t rows = g.m - row0, cols = g.n - col0;
-  const uint32_t ksteps = (g.k + kStep - 1) / kStep;
-  const uint32_t steps = ksteps * g.pairs;
+  // Steps that are 64 deep throughout, of all pairs, and a shorter last one per pair behind them.
+  const uint32_t ksteps = g.k / kStep, rest = g.k % kStep;
+  const uint32_t whole = ksteps * g.pairs, steps = whole + (rest ? g.pairs : 0);
   const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(steps) * split / g.splits);
   const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(steps) * (split + 1) / g.splits);
+  const uint32_t whole_end = end < whole ? end : whole;
 
   const T* const a0 = static_cast<const T*>(g.a.base) + z * g.a.batch + (AK ? uint64_t{row0} : row0 * g.a.ld);
   const T* const b0p = static_cast<const T*>(g.b.base) + z * g.b.batch + (BK ? uint64_t{col0} : col0 * g.b.ld);
@@ -350,30 +376,24 @@ __global__ void __launch_bounds__(WM* WN * 64, 2)
   const uint32_t lds0 = static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(s_mem)));
 
-  // Loads step `step` into half `buf`.
-  const auto load = [&](uint32_t step, int buf) {
-    const uint32_t pair = step / ksteps, ks = step - pair * ksteps;
-    const uint32_t k0 = ks * kStep;
-    const T* pa = a0 + g.pa[pair] * g.a.plane + (AK ? k0 * g.a.ld : uint64_t{k0});
-    const T* pb = b0p + g.pb[pair] * g.b.plane + (BK ? k0 * g.b.ld : uint64_t{k0});
+  // Where step ks of a pair begins, wave-uniform.
+  const auto begin_a = [&](uint32_t pair, uint32_t ks) {
+    const uint64_t k0 = static_cast<uint64_t>(ks) * kStep;
+    return a0 + (g.pa >> (4 * pair) & 15u) * g.a.plane + (AK ? k0 * g.a.ld : k0);
+  };
+  const auto begin_b = [&](uint32_t pair, uint32_t ks) {
+    const uint64_t k0 = static_cast<uint64_t>(ks) * kStep;
+    return b0p + (g.pb >> (4 * pair) & 15u) * g.b.plane + (BK ? k0 * g.b.ld : k0);
+  };
+  // Loads the step that begins at pa and pb into place `buf`, at the lanes' offsets.
+  const auto load = [&](const T* pa, const T* pb, int buf, const uint32_t(&at_a)[SA::kLoads],
+                        const uint32_t(&at_b)[SB::kLoads]) {
     const u32x4_t ra = buffer_resource(pa), rb = buffer_resource(pb);
-    const uint32_t la = lds0 + static_cast<uint32_t>(buf) * kStageBytes, lb = la + SA::kBytes;
-    const uint32_t depth = g.k - k0;
-    if (depth >= kStep) {
+    const uint32_t la = lds0 + static_cast<uint32_t>(buf) * kStageBytes + wave * 1024, lb = la + SA::kBytes;
 #pragma unroll
-      for (int i = 0; i < SA::kLoads; ++i) load_to_lds(la + (i * kWaves + wave) * 1024, oa[i], ra, 0);
+    for (int i = 0; i < SA::kLoads; ++i) load_to_lds(la + i * kWaves * 1024, at_a[i], ra, 0);
 #pragma unroll
-      for (int i = 0; i < SB::kLoads; ++i) load_to_lds(lb + (i * kWaves + wave) * 1024, ob[i], rb, 0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < SA::kLoads; ++i) {
-        load_to_lds(la + (i * kWaves + wave) * 1024, SA::offset(i, wave, lane, lda, rows, depth), ra, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < SB::kLoads; ++i) {
-        load_to_lds(lb + (i * kWaves + wave) * 1024, SB::offset(i, wave, lane, ldb, cols, depth), rb, 0);
-      }
-    }
+    for (int i = 0; i < SB::kLoads; ++i) load_to_lds(lb + i * kWaves * 1024, at_b[i], rb, 0);
   };
 
   f32x16_t acc[TM][TN];
@@ -384,43 +404,102 @@ __global__ void __launch_bounds__(WM* WN * 64, 2)
   }
 
   const int ra0 = wm * (BM / WM), rb0 = wn * (BN / WN);
-  const auto multiply = [&](int buf, uint32_t depth, auto whole) {
+  using X8 = typename Frag<T>::x8;
+  struct Fragments {
+    X8 a[TM], b[TN];
+  };
+  const auto fetch = [&](Fragments& f, int buf, int kk) {
     const char* la = s_mem + buf * kStageBytes;
-    const char* lb = la + SA::kBytes;
 #pragma unroll
-    for (int kk = 0; kk < kStep / 16; ++kk) {
-      if (!decltype(whole)::value && static_cast<uint32_t>(kk * 16) >= depth) break;
-      typename Frag<T>::x8 fa[TM], fb[TN];
+    for (int i = 0; i < TM; ++i) f.a[i] = SA::fragment(la, ra0 + 32 * i, kk, lane);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) fa[i] = SA::fragment(la, ra0 + 32 * i, kk, lane);
+    for (int j = 0; j < TN; ++j) f.b[j] = SB::fragment(la + SA::kBytes, rb0 + 32 * j, kk, lane);
+  };
+  const auto multiply = [&](const Fragments& f) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) fb[j] = SB::fragment(lb, rb0 + 32 * j, kk, lane);
-      if constexpr (!decltype(whole)::value) {
+    for (int i = 0; i < TM; ++i) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) fa[i] = clip(fa[i], kk, lane, depth);
-#pragma unroll
-        for (int j = 0; j < TN; ++j) fb[j] = clip(fb[j], kk, lane, depth);
-      }
-#pragma unroll
-      for (int i = 0; i < TM; ++i) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = Frag<T>::mfma(fa[i], fb[j], acc[i][j]);
-      }
+      for (int j = 0; j < TN; ++j) acc[i][j] = Frag<T>::mfma(f.a[i], f.b[j], acc[i][j]);
     }
   };
 
-  if (first < end) load(first, 0);
-  for (uint32_t s = first; s < end; ++s) {
-    const int buf = static_cast<int>((s - first) & 1);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of step s are in LDS
-    __syncthreads();                                  // everyone's are, and step s - 1 has been read
-    if (s + 1 < end) load(s + 1, buf ^ 1);
-    const uint32_t depth = g.k - s % ksteps * kStep;
-    if (depth >= kStep) {
-      multiply(buf, kStep, std::true_type{});
-    } else {
-      multiply(buf, depth, std::false_type{});
+  // Fragments are fetched one 16-deep slice ahead of their matrix instructions. The step's last slice is
+  // in registers before its instructions start: from then on the step's place in LDS is free for the step
+  // kStages on, and the next step's first slice is fetched while the last one is multiplied.
+  if (first < whole_end) {
+    constexpr int kLoads = SA::kLoads + SB::kLoads, kSlices = kStep / 16;
+    uint32_t pair = first / ksteps, ks = first % ksteps;  // of the next step to load
+    const T *pa = begin_a(pair, ks), *pb = begin_b(pair, ks);
+    const auto load_next = [&](int buf) {
+      load(pa, pb, buf, oa, ob);
+      pa += AK ? kStep * g.a.ld : kStep;
+      pb += BK ? kStep * g.b.ld : kStep;
+      if (++ks == ksteps) {
+        ks = 0;
+        ++pair;
+        pa = begin_a(pair, 0);
+        pb = begin_b(pair, 0);
+      }
+    };
+    Fragments f[2];
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+      if (first + i < whole_end) load_next(i);
     }
+    // All but the first step's loads may still be under way.
+    if (first + kStages <= whole_end) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");  // no fetch moves up across the barrier
+    fetch(f[0], 0, 0);
+    int buf = 0;
+    for (uint32_t s = first; s < whole_end; ++s) {
+#pragma unroll
+      for (int kk = 0; kk + 1 < kSlices; ++kk) {
+        fetch(f[(kk + 1) & 1], buf, kk + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(f[kk & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // This wave's fetches are done, and its loads of the next step have arrived.
+      if (s + kStages <= whole_end) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kLoads) : "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      }
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (s + kStages < whole_end) load_next(buf);
+      buf = buf + 1 == kStages ? 0 : buf + 1;
+      if (s + 1 < whole_end) fetch(f[0], buf, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(f[(kSlices - 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  for (uint32_t s = first < whole ? whole : first; s < end; ++s) {
+    uint32_t ta[SA::kLoads], tb[SB::kLoads];
+#pragma unroll
+    for (int i = 0; i < SA::kLoads; ++i) ta[i] = SA::offset(i, wave, lane, lda, rows, rest);
+#pragma unroll
+    for (int i = 0; i < SB::kLoads; ++i) tb[i] = SB::offset(i, wave, lane, ldb, cols, rest);
+    load(begin_a(s - whole, ksteps), begin_b(s - whole, ksteps), 0, ta, tb);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+#pragma unroll 1
+    for (int kk = 0; static_cast<uint32_t>(kk * 16) < rest; ++kk) {
+      Fragments f;
+      fetch(f, 0, kk);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) f.a[i] = clip(f.a[i], kk, lane, rest);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) f.b[j] = clip(f.b[j], kk, lane, rest);
+      multiply(f);
+    }
+    __syncthreads();
   }
   __syncthreads();
 
@@ -487,22 +566,22 @@ struct GemmPlan {
 
 GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t pairs, uint32_t batches);
 
-template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN, class Epi>
+template <class T, bool AK, bool BK, class Shape, class Epi>
 void launch_tile(GemmArgs g, const Epi& epi, hipStream_t s) {
-  g.tiles_m = static_cast<uint32_t>(ceil_div(g.m, BM));
-  g.tiles_n = static_cast<uint32_t>(ceil_div(g.n, BN));
+  g.tiles_m = static_cast<uint32_t>(ceil_div(g.m, Shape::BM));
+  g.tiles_n = static_cast<uint32_t>(ceil_div(g.n, Shape::BN));
   const uint64_t blocks = static_cast<uint64_t>(g.tiles_m) * g.tiles_n * g.splits;
   QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "the matrix product is too large");
   const dim3 grid(static_cast<unsigned>(blocks), g.batches);
   if (g.splits > 1) {
     const uint64_t ld = ceil_div(g.n, 8) * 8;
     const PartialEpilogue pe{g.partial, ld, ld * g.m};
-    hipLaunchKernelGGL((gemm_kernel<T, AK, BK, BM, BN, WM, WN, PartialEpilogue>), grid, dim3(WM * WN * 64), 0, s, g, pe);
+    hipLaunchKernelGGL((gemm_kernel<T, AK, BK, Shape, PartialEpilogue>), grid, dim3(Shape::WM * Shape::WN * 64), 0, s, g, pe);
     QVH_HIP(hipGetLastError());
     hipLaunchKernelGGL((gemm_join_kernel<Epi>), dim3(static_cast<unsigned>(ceil_div(ld / 8 * g.m, 256)), g.batches),
                        dim3(256), 0, s, g, epi);
   } else {
-    hipLaunchKernelGGL((gemm_kernel<T, AK, BK, BM, BN, WM, WN, Epi>), grid, dim3(WM * WN * 64), 0, s, g, epi);
+    hipLaunchKernelGGL((gemm_kernel<T, AK, BK, Shape, Epi>), grid, dim3(Shape::WM * Shape::WN * 64), 0, s, g, epi);
   }
   QVH_HIP(hipGetLastError());
 }
@@ -512,13 +591,17 @@ void launch_gemm(GemmArgs g, const Epi& epi, const GemmPlan& plan, void* partial
   if (g.m == 0 || g.n == 0 || g.batches == 0) return;
   g.splits = plan.splits;
   g.partial = static_cast<float*>(partial);
+#ifdef QVH_TRY
+  launch_tile<T, AK, BK, QVH_TRY>(g, epi, s);
+#else
   if (plan.tile == 2) {
-    launch_tile<T, AK, BK, 256, 256, 2, 4>(g, epi, s);
+    launch_tile<T, AK, BK, Tile<256, 256, 2, 4, 64, 2>>(g, epi, s);
   } else if (plan.tile == 1) {
-    launch_tile<T, AK, BK, 128, 128, 2, 2>(g, epi, s);
+    launch_tile<T, AK, BK, Tile<128, 128, 2, 2, 64, 2>>(g, epi, s);
   } else {
-    launch_tile<T, AK, BK, 64, 64, 2, 2>(g, epi, s);
+    launch_tile<T, AK, BK, Tile<64, 64, 2, 2, 64, 2>>(g, epi, s);
   }
+#endif
 }
 
 }  // namespace qvh

@@ -18,7 +18,7 @@ GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t pairs, uint32_t 
     p.tile = 1;
     p.bm = p.bn = 128;
   }
-  const uint64_t t = tiles(p.bm), steps = ceil_div(k, kStep) * pairs;
+  const uint64_t t = tiles(p.bm), steps = ceil_div(k, 64) * pairs;
   if (t > 0 && t < 192 && steps >= 16) {
     p.splits = static_cast<uint32_t>(std::min<uint64_t>({ceil_div(384, t), steps / 8, 64}));
   }
@@ -128,13 +128,13 @@ __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
         load8(static_cast<const T*>(a.pre) + r * a.ld_pre + c, z, left, a.vec_pre);
         if (a.act == QVH_ACT_RELU) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] *= activate_slope(z[i], QVH_ACT_RELU);
+          for (int i = 0; i < 8; ++i) g[i] *= activate_slope<sizeof(T) == 4>(z[i], QVH_ACT_RELU);
         } else if (a.act == QVH_ACT_GELU) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] *= activate_slope(z[i], QVH_ACT_GELU);
+          for (int i = 0; i < 8; ++i) g[i] *= activate_slope<sizeof(T) == 4>(z[i], QVH_ACT_GELU);
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] *= activate_slope(z[i], QVH_ACT_SILU);
+          for (int i = 0; i < 8; ++i) g[i] *= activate_slope<sizeof(T) == 4>(z[i], QVH_ACT_SILU);
         }
       }
       if (a.dz) store_prepared<T>(a.dz, r * a.ld + c, a.plane, g);
@@ -332,10 +332,9 @@ void launch_prepare(int dtype, const Prepared& a, const Prepared& b, hipStream_t
 void set_pairs(GemmArgs& g, int dtype) {
   g.pairs = 1;
   if (dtype != QVH_FP32) return;
-  const uint8_t pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
   g.pairs = 6;
-  std::copy(pa, pa + 6, g.pa);
-  std::copy(pb, pb + 6, g.pb);
+  g.pa = 0x001102;  // (2, 0), (0, 2), (1, 1), (1, 0), (0, 1), (0, 0)
+  g.pb = 0x010120;
 }
 
 void run_product(Form form, int dtype, GemmArgs g, const void* bias, const void* residual, uint64_t ld_residual,

@@ -203,8 +203,8 @@ GemmArgs product(const half_t* a, uint64_t lda, uint64_t plane_a, const half_t* 
   g.k = k;
   g.batches = static_cast<uint32_t>(batch);
   g.pairs = 3;
-  g.pa[1] = 1;  // (high, low), (low, high), (high, high)
-  g.pb[0] = 1;
+  g.pa = 0x010;  // (high, low), (low, high), (high, high)
+  g.pb = 0x001;
   return g;
 }
 
