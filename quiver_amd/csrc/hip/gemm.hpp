@@ -385,15 +385,18 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
     const uint64_t k0 = static_cast<uint64_t>(ks) * kStep;
     return b0p + (g.pb >> (4 * pair) & 15u) * g.b.plane + (BK ? k0 * g.b.ld : k0);
   };
-  // Loads the step that begins at pa and pb into place `buf`, at the lanes' offsets.
+  // Loads the step that begins at pa and pb into place `buf`, at the lanes' offsets: piece i of kPieces.
+  constexpr int kPieces = SA::kLoads + SB::kLoads;
+  const auto load_piece = [&](int i, u32x4_t ra, u32x4_t rb, int buf, const uint32_t(&at_a)[SA::kLoads],
+                              const uint32_t(&at_b)[SB::kLoads]) {
+    const uint32_t to = lds0 + static_cast<uint32_t>(buf) * kStageBytes + (i * kWaves + wave) * 1024;
+    load_to_lds(to, i < SA::kLoads ? at_a[i] : at_b[i - SA::kLoads], i < SA::kLoads ? ra : rb, 0);
+  };
   const auto load = [&](const T* pa, const T* pb, int buf, const uint32_t(&at_a)[SA::kLoads],
                         const uint32_t(&at_b)[SB::kLoads]) {
     const u32x4_t ra = buffer_resource(pa), rb = buffer_resource(pb);
-    const uint32_t la = lds0 + static_cast<uint32_t>(buf) * kStageBytes + wave * 1024, lb = la + SA::kBytes;
 #pragma unroll
-    for (int i = 0; i < SA::kLoads; ++i) load_to_lds(la + i * kWaves * 1024, at_a[i], ra, 0);
-#pragma unroll
-    for (int i = 0; i < SB::kLoads; ++i) load_to_lds(lb + i * kWaves * 1024, at_b[i], rb, 0);
+    for (int i = 0; i < kPieces; ++i) load_piece(i, ra, rb, buf, at_a, at_b);
   };
 
   f32x16_t acc[TM][TN];
@@ -427,11 +430,10 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
   // in registers before its instructions start: from then on the step's place in LDS is free for the step
   // kStages on, and the next step's first slice is fetched while the last one is multiplied.
   if (first < whole_end) {
-    constexpr int kLoads = SA::kLoads + SB::kLoads, kSlices = kStep / 16;
+    constexpr int kSlices = kStep / 16;
     uint32_t pair = first / ksteps, ks = first % ksteps;  // of the next step to load
     const T *pa = begin_a(pair, ks), *pb = begin_b(pair, ks);
-    const auto load_next = [&](int buf) {
-      load(pa, pb, buf, oa, ob);
+    const auto advance = [&] {
       pa += AK ? kStep * g.a.ld : kStep;
       pb += BK ? kStep * g.b.ld : kStep;
       if (++ks == ksteps) {
@@ -444,11 +446,14 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
     Fragments f[2];
 #pragma unroll
     for (int i = 0; i < kStages; ++i) {
-      if (first + i < whole_end) load_next(i);
+      if (first + i < whole_end) {
+        load(pa, pb, i, oa, ob);
+        advance();
+      }
     }
     // All but the first step's loads may still be under way.
     if (first + kStages <= whole_end) {
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kPieces) : "memory");
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
@@ -466,18 +471,31 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
       }
       // This wave's fetches are done, and its loads of the next step have arrived.
       if (s + kStages <= whole_end) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kLoads) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kPieces) : "memory");
       } else {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       }
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (s + kStages < whole_end) load_next(buf);
+      const bool more = s + kStages < whole_end;
+      const u32x4_t ra = buffer_resource(pa), rb = buffer_resource(pb);
+      const int free_buf = buf;
       buf = buf + 1 == kStages ? 0 : buf + 1;
       if (s + 1 < whole_end) fetch(f[0], buf, 0);
       __builtin_amdgcn_sched_barrier(0);
-      multiply(f[(kSlices - 1) & 1]);
-      __builtin_amdgcn_sched_barrier(0);
+      // The loads go out between the matrix instructions, which cover their issue.
+      constexpr int kLast = (kSlices - 1) & 1;
+#pragma unroll
+      for (int x = 0; x < TM * TN; ++x) {
+        acc[x / TN][x % TN] = Frag<T>::mfma(f[kLast].a[x / TN], f[kLast].b[x % TN], acc[x / TN][x % TN]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (more) {
+#pragma unroll
+          for (int i = x * kPieces / (TM * TN); i < (x + 1) * kPieces / (TM * TN); ++i) load_piece(i, ra, rb, free_buf, oa, ob);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (more) advance();
     }
   }
   for (uint32_t s = first < whole ? whole : first; s < end; ++s) {
