@@ -57,6 +57,8 @@ struct GemmArgs {
   uint32_t pairs = 1;        // pairs of planes, at most eight
   uint32_t pa = 0, pb = 0;   // the planes of pair i: four bits each, from the lowest
   uint32_t tiles_m = 0, tiles_n = 0, splits = 1, batches = 1;
+  uint32_t symmetric = 0;  // the product equals its transpose (m = n): tiles above the diagonal are mirrored
+  uint32_t side = 0;       // of a tile, where that is so
   float* partial = nullptr;  // [split][batch][m][n rounded up to 8] when splits > 1
 };
 
@@ -105,6 +107,21 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
     return s * (1.0f + z * (1.0f - s));
   }
   return 1.0f;
+}
+
+/// Row and eight-element piece of this thread where rows hold per_row pieces and work-groups of 256 threads take
+/// them in order. The 64-bit division only where the numbers need it.
+struct RowChunk {
+  uint64_t row;
+  uint32_t chunk;
+};
+__device__ __forceinline__ RowChunk row_and_chunk(uint32_t block, uint32_t per_row) {
+  if (block < (1u << 24)) {
+    const uint32_t i = block * 256 + threadIdx.x, r = i / per_row;
+    return {r, i - r * per_row};
+  }
+  const uint64_t i = static_cast<uint64_t>(block) * 256 + threadIdx.x, r = i / per_row;
+  return {r, static_cast<uint32_t>(i - r * per_row)};
 }
 
 /// Eight values as vector stores where the row is aligned and whole, else one by one.
@@ -342,7 +359,7 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
 
   // Work-groups go round the XCDs in order of their number; each XCD takes a contiguous run of tiles,
   // walked in bands of eight tile rows, so that its L2 serves the rows and columns they share.
-  const uint32_t per = g.tiles_m * g.tiles_n;
+  const uint32_t per = g.symmetric ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
   const uint32_t total = per * g.splits;
   uint32_t id = blockIdx.x;
   {
@@ -351,9 +368,18 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
   }
   const uint32_t split = id / per;
   const uint32_t tile = id % per;
-  const uint32_t band = 8 * g.tiles_n, b0 = tile / band * 8;
-  const uint32_t high = g.tiles_m - b0 < 8 ? g.tiles_m - b0 : 8;
-  const uint32_t tm = b0 + tile % band % high, tn = tile % band / high;
+  uint32_t tm, tn;
+  if (g.symmetric) {  // row by row of the lower triangle
+    tm = static_cast<uint32_t>((sqrtf(8.0f * static_cast<float>(tile) + 1.0f) - 1.0f) * 0.5f);
+    while (tm * (tm + 1) / 2 > tile) --tm;
+    while ((tm + 1) * (tm + 2) / 2 <= tile) ++tm;
+    tn = tile - tm * (tm + 1) / 2;
+  } else {
+    const uint32_t band = 8 * g.tiles_n, b0 = tile / band * 8;
+    const uint32_t high = g.tiles_m - b0 < 8 ? g.tiles_m - b0 : 8;
+    tm = b0 + tile % band % high;
+    tn = tile % band / high;
+  }
   const uint32_t z = blockIdx.y;
 
   const uint32_t row0 = tm * BM, col0 = tn * BN;
@@ -548,6 +574,18 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
       float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       if (m < g.m && n < g.n) epi(g.splits > 1 ? split * g.batches + z : z, m, n, g.n - n, v);
     }
+    if (g.symmetric && g.splits == 1 && tm != tn) {
+      // The same values at their mirrored places: a lane takes eight rows of one column.
+#pragma unroll
+      for (int q = 0; q < BN / WN / 16; ++q) {
+        const int c = q * 16 + lane / 4, r = lane % 4 * 8;
+        const uint32_t mm = col0 + static_cast<uint32_t>(rb0 + c), nn = row0 + static_cast<uint32_t>(ra0 + 32 * i + r);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = slab[(r + e) * kSlabLd + c];
+        if (mm < g.n && nn < g.m) epi(z, mm, nn, g.m - nn, v);
+      }
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
@@ -556,19 +594,37 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
 template <class Epi>
 __global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs g, Epi epi) {
   const uint32_t ld = (g.n + 7) / 8 * 8;
-  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const uint32_t per_row = ld / 8;
-  const uint64_t m = i / per_row;
+  const auto [m, chunk] = row_and_chunk(blockIdx.x, ld / 8);
   if (m >= g.m) return;
-  const uint32_t n = static_cast<uint32_t>(i % per_row) * 8;
-  const uint64_t batch = static_cast<uint64_t>(g.m) * ld;
+  const uint32_t n = chunk * 8;
+  const uint64_t batch = static_cast<uint64_t>(g.m) * ld, step = batch * g.batches;
+  const float* p = g.partial + blockIdx.y * batch;
   float v[8] = {};
-  for (uint32_t s = 0; s < g.splits; ++s) {
-    const float* p = g.partial + (static_cast<uint64_t>(s) * g.batches + blockIdx.y) * batch + m * ld + n;
-    float x[8];
-    load8(p, x, 8, true);
+  if (g.symmetric && n / g.side > m / g.side) {  // above the diagonal: from the mirrored place
+    p += n * static_cast<uint64_t>(ld) + m;
+    for (uint32_t s = 0; s < g.splits; ++s, p += step) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += x[e];
+      for (int e = 0; e < 8; ++e) v[e] += n + e < g.n ? p[e * static_cast<uint64_t>(ld)] : 0.0f;
+    }
+  } else {
+    p += m * ld + n;
+    uint32_t s = 0;
+    for (; s + 4 <= g.splits; s += 4, p += 4 * step) {  // four loads under way at a time
+      float x[4][8];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) load8(p + u * step, x[u], 8, true);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += x[u][e];
+      }
+    }
+    for (; s < g.splits; ++s, p += step) {
+      float x[8];
+      load8(p, x, 8, true);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += x[e];
+    }
   }
   epi(blockIdx.y, static_cast<uint32_t>(m), n, g.n - n, v);
 }
@@ -576,19 +632,22 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs g, Epi epi) {
 // ---- launching --------------------------------------------------------------------------------
 
 /// Tile shape and number of splits for a product; the same for the workspace's size and for the launch.
+/// `symmetric`: m = n and only the tiles on and below the diagonal are computed.
 struct GemmPlan {
-  int tile = 0;  // 0: 64 x 64, 1: 128 x 128, 2: 256 x 256
-  uint32_t bm = 64, bn = 64, splits = 1;
+  int tile = -1;  // 0: 64 x 64, 1: 128 x 128, 2: 256 x 256
+  uint32_t splits = 1;
   size_t partial_bytes = 0;
 };
 
-GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t pairs, uint32_t batches);
+GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t pairs, uint32_t batches, bool symmetric);
 
 template <class T, bool AK, bool BK, class Shape, class Epi>
 void launch_tile(GemmArgs g, const Epi& epi, hipStream_t s) {
   g.tiles_m = static_cast<uint32_t>(ceil_div(g.m, Shape::BM));
   g.tiles_n = static_cast<uint32_t>(ceil_div(g.n, Shape::BN));
-  const uint64_t blocks = static_cast<uint64_t>(g.tiles_m) * g.tiles_n * g.splits;
+  g.side = Shape::BM;
+  const uint64_t tiles = g.symmetric ? static_cast<uint64_t>(g.tiles_m) * (g.tiles_m + 1) / 2 : static_cast<uint64_t>(g.tiles_m) * g.tiles_n;
+  const uint64_t blocks = tiles * g.splits;
   QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "the matrix product is too large");
   const dim3 grid(static_cast<unsigned>(blocks), g.batches);
   if (g.splits > 1) {
@@ -609,9 +668,6 @@ void launch_gemm(GemmArgs g, const Epi& epi, const GemmPlan& plan, void* partial
   if (g.m == 0 || g.n == 0 || g.batches == 0) return;
   g.splits = plan.splits;
   g.partial = static_cast<float*>(partial);
-#ifdef QVH_TRY
-  launch_tile<T, AK, BK, QVH_TRY>(g, epi, s);
-#else
   if (plan.tile == 2) {
     launch_tile<T, AK, BK, Tile<256, 256, 2, 4, 64, 2>>(g, epi, s);
   } else if (plan.tile == 1) {
@@ -619,7 +675,6 @@ void launch_gemm(GemmArgs g, const Epi& epi, const GemmPlan& plan, void* partial
   } else {
     launch_tile<T, AK, BK, Tile<64, 64, 2, 2, 64, 2>>(g, epi, s);
   }
-#endif
 }
 
 }  // namespace qvh

@@ -1,6 +1,7 @@
 // The linear layer y = act(x w^T + b) + residual and its gradients: operand preparation, the few-row
 // kernel, and the choice between them and the tiled products (gemm.hpp).
 #include <algorithm>
+#include <cmath>
 
 #include "linear.hpp"
 
@@ -8,22 +9,45 @@ namespace qvh {
 
 // ---- plan -------------------------------------------------------------------------------------
 
-GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t pairs, uint32_t batches) {
-  GemmPlan p;
-  const auto tiles = [&](uint64_t t) { return ceil_div(m, t) * ceil_div(n, t) * batches; };
-  if (tiles(256) >= 192) {
-    p.tile = 2;
-    p.bm = p.bn = 256;
-  } else if (tiles(128) >= 128) {
-    p.tile = 1;
-    p.bm = p.bn = 128;
+// The estimate below is fitted to products from 128 x 128 x 64 to 10,000 x 768 x 4,608 with every tile and
+// split (bf16, both operands by rows): it picked the fastest or one within 15% of it. Both sides of
+// typical choices, in us: 1,024 x 1,024 x 4,096 as 64-tiles in one piece 37.2, in four 25.0, as 128-tiles in
+// one 47.1; 2,048^3 as 128-tiles 29.5, 256-tiles 51.0; 8,192 x 2,048 x 768 as 256-tiles 35.5, 128-tiles
+// 37.1, 64-tiles 51.2; 1,024 x 4,096 x 16,384 as 256-tiles in four pieces 131, 128-tiles in one 181.
+GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t pairs, uint32_t batches, bool symmetric) {
+  struct Cost {
+    uint64_t side, together;    // tile, and work-groups that a CU holds
+    double alone, shared, end;  // us per 64-deep step: one work-group on a CU, each of several; prologue and epilogue
+  };
+  constexpr Cost kCosts[3] = {{64, 4, 0.45, 0.22, 2.0}, {128, 2, 0.70, 0.53, 4.0}, {256, 1, 1.75, 1.75, 8.0}};
+  constexpr uint32_t kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+  constexpr double kCus = 256.0;
+  GemmPlan best;
+  double least = 0.0;
+  const uint64_t steps = ceil_div(k, 64) * pairs;
+  for (int t = 0; t < 3; ++t) {
+    const Cost& c = kCosts[t];
+    const uint64_t tm = ceil_div(m, c.side), tn = ceil_div(n, c.side);
+    const uint64_t tiles = (symmetric ? tm * (tm + 1) / 2 : tm * tn) * batches;
+    for (const uint32_t splits : kSplits) {
+      if (splits > 1 && steps < 2 * splits) break;
+      const double groups = static_cast<double>(tiles) * splits;
+      const double per_cu = std::ceil(groups / kCus);
+      const double rounds = std::ceil(per_cu / static_cast<double>(c.together));
+      const double at_once = std::ceil(per_cu / rounds);
+      const double step = std::max(c.alone, c.shared * at_once);
+      double us = rounds * (std::ceil(static_cast<double>(steps) / splits) * step + c.end + 0.5 * at_once);
+      // The partial sums go out and come back, through the last-level cache, in a launch of their own.
+      if (splits > 1) us += 4.0 + 0.1 * splits + static_cast<double>(splits) * batches * m * n * 8.0 / 7e6;
+      if (best.tile < 0 || us < least) {
+        least = us;
+        best.tile = t;
+        best.splits = splits;
+      }
+    }
   }
-  const uint64_t t = tiles(p.bm), steps = ceil_div(k, 64) * pairs;
-  if (t > 0 && t < 192 && steps >= 16) {
-    p.splits = static_cast<uint32_t>(std::min<uint64_t>({ceil_div(384, t), steps / 8, 64}));
-  }
-  if (p.splits > 1) p.partial_bytes = static_cast<size_t>(p.splits) * batches * m * (ceil_div(n, 8) * 8) * 4;
-  return p;
+  if (best.splits > 1) best.partial_bytes = static_cast<size_t>(best.splits) * batches * m * (ceil_div(n, 8) * 8) * 4;
+  return best;
 }
 
 namespace {
@@ -85,11 +109,10 @@ template <class T>
 __global__ void __launch_bounds__(256) prepare_kernel(PrepareArgs a, PrepareArgs b) {
   const bool second = blockIdx.x >= a.blocks;
   const PrepareArgs& p = second ? b : a;
-  const uint64_t i = static_cast<uint64_t>(second ? blockIdx.x - a.blocks : blockIdx.x) * 256 + threadIdx.x;
   const uint32_t per_row = static_cast<uint32_t>(p.ld / 8);
-  const uint64_t r = i / per_row;
+  const auto [r, chunk] = row_and_chunk(second ? blockIdx.x - a.blocks : blockIdx.x, per_row);
   if (r >= p.rows) return;
-  const uint32_t c = static_cast<uint32_t>(i - r * per_row) * 8;
+  const uint32_t c = chunk * 8;
   float v[8];
   load8(static_cast<const T*>(p.src) + r * p.stride + c, v, p.cols - c, p.vec);
   store_prepared<T>(p.dst, r * p.ld + c, p.plane, v);
@@ -399,7 +422,7 @@ LinearRun plan_linear(const qvh_linear_args& a, void* ws) {
   sp.base = static_cast<char*>(ws);
   r.x = prepare_operand(a.x, a.m, a.x_stride, a.k, a.dtype, sp);
   r.w = prepare_operand(a.weight, a.n, a.weight_stride, a.k, a.dtype, sp);
-  r.plan = gemm_plan(a.m, a.n, a.k, a.dtype == QVH_FP32 ? 6 : 1, 1);
+  r.plan = gemm_plan(a.m, a.n, a.k, a.dtype == QVH_FP32 ? 6 : 1, 1, false);
   r.partial = sp.take(r.plan.partial_bytes);
   r.bytes = sp.at;
   return r;
@@ -497,12 +520,12 @@ GradRun plan_grad(const qvh_linear_grad_args& a, void* ws) {
   if (products) {
     if (a.grad_x) {
       r.w = prepare_operand(a.weight, a.n, a.weight_stride, a.k, a.dtype, sp);
-      r.plan_x = gemm_plan(a.m, a.k, a.n, pairs, 1);
+      r.plan_x = gemm_plan(a.m, a.k, a.n, pairs, 1, false);
       r.partial_x = sp.take(r.plan_x.partial_bytes);
     }
     if (a.grad_weight) {
       r.x = prepare_operand(a.x, a.m, a.x_stride, a.k, a.dtype, sp);
-      r.plan_w = gemm_plan(a.n, a.k, a.m, pairs, 1);
+      r.plan_w = gemm_plan(a.n, a.k, a.m, pairs, 1, false);
       r.partial_w = sp.take(r.plan_w.partial_bytes);
     }
   }

@@ -19,22 +19,36 @@ namespace {
 
 constexpr uint32_t kMaxSide = 65536;
 constexpr float kScale = 4096.0f;
-constexpr uint32_t kNormParts = 64;
+constexpr uint32_t kNormParts = 256;
+
+/// Adds v over the work-group's four waves; the sum is in every thread.
+__device__ __forceinline__ double block_sum(double v, double* s_sum) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return ((s_sum[0] + s_sum[1]) + s_sum[2]) + s_sum[3];
+}
 
 template <class T>
-__global__ void __launch_bounds__(256) norm_kernel(const T* __restrict__ g, uint64_t count, double* __restrict__ parts) {
+__global__ void __launch_bounds__(256) norm_kernel(const T* __restrict__ g, uint64_t count, int vec,
+                                                   double* __restrict__ parts) {
   __shared__ double s_sum[4];
   const T* x = g + blockIdx.y * count;
   double sum = 0.0;
-  for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += kNormParts * 256) {
-    const double v = static_cast<double>(static_cast<float>(x[i]));
-    sum += v * v;
-  }
+  for (uint64_t i = (static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; i < count; i += kNormParts * 2048) {
+    float v[8];
+    load8(x + i, v, count - i < 8 ? static_cast<uint32_t>(count - i) : 8u, vec);
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-  if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) parts[blockIdx.y * kNormParts + blockIdx.x] = ((s_sum[0] + s_sum[1]) + s_sum[2]) + s_sum[3];
+    for (int e = 0; e < 8; ++e) sum += static_cast<double>(v[e]) * v[e];
+  }
+  sum = block_sum(sum, s_sum);
+  if (threadIdx.x == 0) parts[blockIdx.y * kNormParts + blockIdx.x] = sum;
+}
+
+/// 2^12 / norm from the sum of squares; nothing for a zero matrix, NaN where something is not finite.
+__device__ __forceinline__ double start_factor(double sum) {
+  return sum == 0.0 ? 0.0 : !(sum < __builtin_huge_val()) ? __builtin_nan("") : kScale / sqrt(sum);
 }
 
 /// high + low = v in fp16.
@@ -53,28 +67,18 @@ __device__ __forceinline__ void store_parts(half_t* p, uint64_t plane, const flo
 
 /// X = G / |G|_F in parts, rows padded with zeros to ld.
 template <class T>
-__global__ void __launch_bounds__(256) start_kernel(const T* __restrict__ g, uint32_t m, uint32_t n,
+__global__ void __launch_bounds__(256) start_kernel(const T* __restrict__ g, uint32_t m, uint32_t n, int vec,
                                                     const double* __restrict__ parts, half_t* __restrict__ x,
                                                     uint64_t ld, uint64_t plane) {
-  __shared__ double s_factor;
-  if (threadIdx.x < 64) {
-    double sum = parts[blockIdx.y * kNormParts + threadIdx.x];
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    // 2^12 / norm; nothing for a zero matrix, NaN where something is not finite.
-    if (threadIdx.x == 0) {
-      s_factor = sum == 0.0 ? 0.0f : !(sum < __builtin_huge_val()) ? __builtin_nan("") : kScale / sqrt(sum);
-    }
-  }
-  __syncthreads();
-  const double factor = s_factor;  // past fp32's range for an update near its smallest numbers
-  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const uint32_t per_row = static_cast<uint32_t>(ld / 8);
-  const uint64_t r = i / per_row;
+  __shared__ double s_sum[4];
+  static_assert(kNormParts == 256, "one part per thread");
+  // Past fp32's range for an update near its smallest numbers, so a double.
+  const double factor = start_factor(block_sum(parts[blockIdx.y * kNormParts + threadIdx.x], s_sum));
+  const auto [r, chunk] = row_and_chunk(blockIdx.x, static_cast<uint32_t>(ld / 8));
   if (r >= m) return;
-  const uint32_t c = static_cast<uint32_t>(i - r * per_row) * 8;
+  const uint32_t c = chunk * 8;
   float v[8];
-  load8(g + (static_cast<uint64_t>(blockIdx.y) * m + r) * n + c, v, n - c, false);
+  load8(g + (static_cast<uint64_t>(blockIdx.y) * m + r) * n + c, v, n - c, vec);
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = c + e < n ? static_cast<float>(v[e] * factor) : 0.0f;
   store_parts(x + blockIdx.y * 2 * plane + r * ld + c, plane, v);
@@ -130,6 +134,243 @@ __global__ void __launch_bounds__(256) parts_to_result_kernel(const half_t* __re
       static_cast<T>((static_cast<float>(p[0]) + static_cast<float>(p[plane])) / kScale);
 }
 
+// ---- small matrices: one work-group does all steps ---------------------------------------------
+//
+// Where X and S fit LDS (128 x 128, 64 x 512), the seventeen launches of a call would take several times
+// longer than their work. The waves each compute 32 x 32 blocks from LDS (sixteen waves with one block of X
+// each, or eight with up to five, which have the registers for it); P takes S's place, X the old
+// X's, between barriers. More rows than columns: the transpose is worked on. Rows are padded to an odd
+// number of 16-byte pieces, so that sixteen neighbouring rows at one k lie on different banks.
+
+constexpr uint32_t kSmallBlocks = 40;  // 32 x 32 blocks of X
+constexpr uint32_t kSmallLds = 160 * 1024;
+
+struct SmallShape {
+  uint32_t side, depth;     // rounded up to 32
+  uint32_t row_x, row_s;    // bytes
+  uint32_t bytes;
+};
+
+__host__ __device__ inline SmallShape small_shape(uint32_t m, uint32_t n) {
+  SmallShape s;
+  s.side = ((m < n ? m : n) + 31) / 32 * 32;
+  s.depth = ((m < n ? n : m) + 31) / 32 * 32;
+  s.row_x = s.depth * 2 + 16;
+  s.row_s = s.side * 2 + 16;
+  s.bytes = 2 * s.side * (s.row_x + s.row_s);
+  return s;
+}
+
+/// Whether a matrix is done by one work-group.
+inline bool is_small(uint32_t m, uint32_t n) {
+  if (std::max(m, n) > 2048) return false;
+  const SmallShape s = small_shape(m, n);
+  return s.bytes <= kSmallLds - 1024 && s.side / 32 * (s.depth / 32) <= kSmallBlocks;
+}
+
+/// BLOCKS: of X per wave.
+template <class T, int WAVES, int BLOCKS>
+__global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __restrict__ update, uint32_t m, uint32_t n,
+                                                                       uint32_t steps, float a, float b, float c,
+                                                                       T* __restrict__ out) {
+  using X8 = Frag<half_t>::x8;
+  using X4 = Frag<half_t>::x4;
+  extern __shared__ __attribute__((aligned(16))) char s_dyn[];
+  __shared__ double s_sum[WAVES];
+  const SmallShape sh = small_shape(m, n);
+  const bool tall = m > n;
+  const uint32_t lane = threadIdx.x & 63, j32 = lane & 31, h = lane >> 5;
+  const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)));
+  char* const x = s_dyn;                                // high part, low part
+  char* const s = s_dyn + 2 * sh.side * sh.row_x;
+  const uint32_t plane_x = sh.side * sh.row_x, plane_s = sh.side * sh.row_s;
+  const uint32_t count = m * n;
+  const T* g = update + static_cast<uint64_t>(blockIdx.x) * count;
+  T* o = out + static_cast<uint64_t>(blockIdx.x) * count;
+
+  double sum = 0.0;
+  for (uint32_t i = threadIdx.x; i < count; i += WAVES * 64) {
+    const double v = static_cast<double>(static_cast<float>(g[i]));
+    sum += v * v;
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if (lane == 0) s_sum[wave] = sum;
+  for (uint32_t i = threadIdx.x; i < sh.bytes / 16; i += WAVES * 64) {
+    *reinterpret_cast<f32x4_t*>(s_dyn + i * 16) = f32x4_t{};
+  }
+  __syncthreads();
+  sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) sum += s_sum[w];
+  const double factor = start_factor(sum);
+  for (uint32_t i = threadIdx.x; i < count; i += WAVES * 64) {
+    const uint32_t r = i / n, q = i - r * n;
+    half_t high, low;
+    split2(static_cast<float>(static_cast<float>(g[i]) * factor), high, low);
+    char* at = x + (tall ? q * sh.row_x + r * 2 : r * sh.row_x + q * 2);
+    *reinterpret_cast<half_t*>(at) = high;
+    *reinterpret_cast<half_t*>(at + plane_x) = low;
+  }
+  __syncthreads();
+
+  // 8 k of one row; rows by k.
+  const auto rows = [&](const char* base, uint32_t stride, uint32_t row0, uint32_t kk) {
+    return *reinterpret_cast<const X8*>(base + (row0 + j32) * stride + (kk * 16 + 8 * h) * 2);
+  };
+  const auto by_k = [&](const char* base, uint32_t stride, uint32_t col0, uint32_t kk) {
+    X4 part[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const uint32_t p = lane & 15, k = kk * 16 + 8 * h + 4 * q + (p >> 2);
+      const char* at = base + k * stride + (col0 + 16 * (lane >> 4 & 1) + 4 * (p & 3)) * 2;
+      part[q] = __builtin_bit_cast(X4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(at)));
+    }
+    return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  const auto three = [](X8 ah, X8 al, X8 bh, X8 bl, f32x16_t acc) {
+    acc = Frag<half_t>::mfma(al, bh, acc);
+    acc = Frag<half_t>::mfma(ah, bl, acc);
+    return Frag<half_t>::mfma(ah, bh, acc);
+  };
+  // Row of accumulator r of this lane within its block; the column is j32.
+  const auto row_of = [&](int r) { return static_cast<uint32_t>(8 * (r / 4) + r % 4) + 4 * h; };
+  const auto put = [&](char* base, uint32_t stride, uint32_t plane, uint32_t bi, uint32_t bj, const f32x16_t& v) {
+    char* at = base + (bi * 32 + 4 * h) * stride + (bj * 32 + j32) * 2;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      half_t high, low;
+      split2(v[r], high, low);
+      char* to = at + static_cast<uint32_t>(8 * (r / 4) + r % 4) * stride;
+      *reinterpret_cast<half_t*>(to) = high;
+      *reinterpret_cast<half_t*>(to + plane) = low;
+    }
+  };
+  // The block's mirror image: four neighbouring elements of a row at a time.
+  const auto put_mirrored = [&](char* base, uint32_t stride, uint32_t plane, uint32_t bi, uint32_t bj, const f32x16_t& v) {
+    char* at = base + (bj * 32 + j32) * stride + (bi * 32 + 4 * h) * 2;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      Pack<half_t, 4> high, low;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) split2(v[4 * q + e], high.v[e], low.v[e]);
+      *reinterpret_cast<Pack<half_t, 4>*>(at + q * 16) = high;
+      *reinterpret_cast<Pack<half_t, 4>*>(at + q * 16 + plane) = low;
+    }
+  };
+
+  const uint32_t sb = sh.side / 32, db = sh.depth / 32;
+  const uint32_t lower = sb * (sb + 1) / 2;  // at most 10 blocks of S up to 128 rows, 36 up to 256
+  const auto block_of = [](uint32_t t, uint32_t& bi, uint32_t& bj) {
+    bi = 0;
+    while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
+    bj = t - bi * (bi + 1) / 2;
+  };
+  // Addresses that follow from the wave's number are computed where they are used: kept over all steps, those
+  // of five blocks took 250 registers more than there are.
+  const auto fresh = [](uint32_t w) {
+    asm volatile("" : "+s"(w));
+    return w;
+  };
+  for (uint32_t step = 0; step < steps; ++step) {
+    // S = X X^T, the blocks on and below the diagonal and their mirror images.
+    for (uint32_t t = wave; t < lower; t += WAVES) {
+      uint32_t bi, bj;
+      block_of(t, bi, bj);
+      f32x16_t acc{};
+      for (uint32_t kk = 0; kk < sh.depth / 16; ++kk) {
+        acc = three(rows(x, sh.row_x, bi * 32, kk), rows(x + plane_x, sh.row_x, bi * 32, kk), rows(x, sh.row_x, bj * 32, kk),
+                    rows(x + plane_x, sh.row_x, bj * 32, kk), acc);
+      }
+      acc *= 1.0f / kScale;
+      put(s, sh.row_s, plane_s, bi, bj, acc);
+      if (bi != bj) put_mirrored(s, sh.row_s, plane_s, bi, bj, acc);
+    }
+    __syncthreads();
+    // P = a + b S + c S S in S's place.
+    f32x16_t kept[BLOCKS];
+#pragma unroll
+    for (int u = 0; u < BLOCKS; ++u) {
+      const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
+      if (t < lower) {
+        uint32_t bi, bj;
+        block_of(t, bi, bj);
+        f32x16_t acc{};
+        for (uint32_t kk = 0; kk < sh.side / 16; ++kk) {
+          acc = three(rows(s, sh.row_s, bi * 32, kk), rows(s + plane_s, sh.row_s, bi * 32, kk), rows(s, sh.row_s, bj * 32, kk),
+                      rows(s + plane_s, sh.row_s, bj * 32, kk), acc);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t row = bi * 32 + row_of(r), col = bj * 32 + j32;
+          const char* at = s + row * sh.row_s + col * 2;
+          const float sv = static_cast<float>(*reinterpret_cast<const half_t*>(at)) +
+                           static_cast<float>(*reinterpret_cast<const half_t*>(at + plane_s));
+          acc[r] = fmaf(b, sv, acc[r] * (c / kScale)) + (row == col ? a * kScale : 0.0f);
+        }
+        kept[u] = acc;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < BLOCKS; ++u) {
+      const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
+      if (t < lower) {
+        uint32_t bi, bj;
+        block_of(t, bi, bj);
+        put(s, sh.row_s, plane_s, bi, bj, kept[u]);
+        if (bi != bj) put_mirrored(s, sh.row_s, plane_s, bi, bj, kept[u]);
+      }
+    }
+    __syncthreads();
+    // P X in X's place; the last one is the result.
+#pragma unroll
+    for (int u = 0; u < BLOCKS; ++u) {
+      const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
+      if (t < sb * db) {
+        const uint32_t bi = t / db, bj = t % db;
+        f32x16_t acc{};
+        for (uint32_t kk = 0; kk < sh.side / 16; ++kk) {
+          acc = three(rows(s, sh.row_s, bi * 32, kk), rows(s + plane_s, sh.row_s, bi * 32, kk), by_k(x, sh.row_x, bj * 32, kk),
+                      by_k(x + plane_x, sh.row_x, bj * 32, kk), acc);
+        }
+        kept[u] = acc;
+      }
+    }
+    const bool last = step + 1 == steps;
+    if (!last) __syncthreads();
+#pragma unroll
+    for (int u = 0; u < BLOCKS; ++u) {
+      const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
+      if (t < sb * db) {
+        const uint32_t bi = t / db, bj = t % db;
+        if (!last) {
+          kept[u] *= 1.0f / kScale;
+          put(x, sh.row_x, plane_x, bi, bj, kept[u]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const uint32_t row = bi * 32 + row_of(r), col = bj * 32 + j32;
+            if (row < (tall ? n : m) && col < (tall ? m : n)) {
+              o[tall ? col * n + row : row * n + col] = static_cast<T>(kept[u][r] * (1.0f / (kScale * kScale)));
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (steps == 0) {
+    for (uint32_t i = threadIdx.x; i < count; i += WAVES * 64) {
+      const uint32_t r = i / n, q = i - r * n;
+      const char* at = x + (tall ? q * sh.row_x + r * 2 : r * sh.row_x + q * 2);
+      o[i] = static_cast<T>((static_cast<float>(*reinterpret_cast<const half_t*>(at)) +
+                             static_cast<float>(*reinterpret_cast<const half_t*>(at + plane_x))) /
+                            kScale);
+    }
+  }
+}
+
 struct OrthoLayout {
   uint32_t side;               // the smaller of m and n
   uint64_t ldx, lds;           // rounded up to 8
@@ -140,6 +381,7 @@ struct OrthoLayout {
 
 OrthoLayout ortho_layout(uint64_t batch, uint32_t m, uint32_t n) {
   OrthoLayout l{};
+  if (is_small(m, n)) return l;  // needs nothing
   const auto round = [](size_t b) { return (b + 255) / 256 * 256; };
   l.side = std::min(m, n);
   l.ldx = ceil_div(n, 8) * 8;
@@ -147,9 +389,9 @@ OrthoLayout ortho_layout(uint64_t batch, uint32_t m, uint32_t n) {
   l.plane_x = l.ldx * m;
   l.plane_s = l.lds * l.side;
   const uint32_t b = static_cast<uint32_t>(batch);
-  l.gram = gemm_plan(l.side, l.side, std::max(m, n), 3, b);
-  l.square = gemm_plan(l.side, l.side, l.side, 3, b);
-  l.update = gemm_plan(m, n, l.side, 3, b);
+  l.gram = gemm_plan(l.side, l.side, std::max(m, n), 3, b, true);
+  l.square = gemm_plan(l.side, l.side, l.side, 3, b, true);
+  l.update = gemm_plan(m, n, l.side, 3, b, false);
   size_t at = round(batch * kNormParts * 8);
   for (size_t& x : l.x) {
     x = at;
@@ -211,6 +453,25 @@ GemmArgs product(const half_t* a, uint64_t lda, uint64_t plane_a, const half_t* 
 template <class T>
 void orthogonalize(const T* update, uint64_t batch, uint32_t m, uint32_t n, uint32_t steps, float a, float b, float c,
                    T* out, char* ws, hipStream_t s) {
+  if (is_small(m, n)) {
+    const SmallShape sh = small_shape(m, n);
+    const auto go = [&](auto waves, auto blocks) {
+      constexpr int W = decltype(waves)::value;
+      const auto kernel = ortho_small_kernel<T, W, decltype(blocks)::value>;
+      static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                            hipFuncAttributeMaxDynamicSharedMemorySize, kSmallLds - 1024);
+      QVH_HIP(allowed);
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(batch)), dim3(W * 64), sh.bytes, s, update, m, n, steps,
+                         a, b, c, out);
+    };
+    if (sh.side / 32 * (sh.depth / 32) <= 16) {
+      go(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+    } else {
+      go(std::integral_constant<int, 8>{}, std::integral_constant<int, 5>{});
+    }
+    QVH_HIP(hipGetLastError());
+    return;
+  }
   const OrthoLayout l = ortho_layout(batch, m, n);
   double* norm = reinterpret_cast<double*>(ws + l.norm);
   half_t* x[2] = {reinterpret_cast<half_t*>(ws + l.x[0]), reinterpret_cast<half_t*>(ws + l.x[1])};
@@ -218,10 +479,14 @@ void orthogonalize(const T* update, uint64_t batch, uint32_t m, uint32_t n, uint
   half_t* poly = reinterpret_cast<half_t*>(ws + l.p);
   void* partial = ws + l.partial;
   const unsigned nb = static_cast<unsigned>(batch);
-  hipLaunchKernelGGL((norm_kernel<T>), dim3(kNormParts, nb), dim3(256), 0, s, update, static_cast<uint64_t>(m) * n, norm);
+  const bool aligned = reinterpret_cast<uintptr_t>(update) % 16 == 0;
+  const int vec_rows = aligned && n * sizeof(T) % 16 == 0;
+  const int vec_all = aligned && (batch == 1 || static_cast<uint64_t>(m) * n * sizeof(T) % 16 == 0);
+  hipLaunchKernelGGL((norm_kernel<T>), dim3(kNormParts, nb), dim3(256), 0, s, update, static_cast<uint64_t>(m) * n,
+                     vec_all, norm);
   QVH_HIP(hipGetLastError());
   hipLaunchKernelGGL((start_kernel<T>), dim3(static_cast<unsigned>(ceil_div(l.ldx / 8 * m, 256)), nb), dim3(256), 0, s,
-                     update, m, n, norm, x[0], l.ldx, l.plane_x);
+                     update, m, n, vec_rows, norm, x[0], l.ldx, l.plane_x);
   QVH_HIP(hipGetLastError());
   if (steps == 0) {
     hipLaunchKernelGGL((parts_to_result_kernel<T>), dim3(static_cast<unsigned>(ceil_div(static_cast<uint64_t>(m) * n, 256)), nb),
@@ -233,14 +498,16 @@ void orthogonalize(const T* update, uint64_t batch, uint32_t m, uint32_t n, uint
   for (uint32_t i = 0; i < steps; ++i) {
     const half_t* cur = x[i & 1];
     half_t* next = x[(i + 1) & 1];
-    const GemmArgs g1 = product(cur, l.ldx, l.plane_x, cur, l.ldx, l.plane_x, l.side, l.side, std::max(m, n), batch);
+    GemmArgs g1 = product(cur, l.ldx, l.plane_x, cur, l.ldx, l.plane_x, l.side, l.side, std::max(m, n), batch);
+    g1.symmetric = 1;
     const PartsEpilogue e1{gram, nullptr, l.lds, l.plane_s, 1.0f / kScale, 0.0f, 0.0f};
     if (tall) {
       launch_gemm<half_t, true, true>(g1, e1, l.gram, partial, s);
     } else {
       launch_gemm<half_t, false, false>(g1, e1, l.gram, partial, s);
     }
-    const GemmArgs g2 = product(gram, l.lds, l.plane_s, gram, l.lds, l.plane_s, l.side, l.side, l.side, batch);
+    GemmArgs g2 = product(gram, l.lds, l.plane_s, gram, l.lds, l.plane_s, l.side, l.side, l.side, batch);
+    g2.symmetric = 1;
     const PartsEpilogue e2{poly, gram, l.lds, l.plane_s, c / kScale, a * kScale, b};
     launch_gemm<half_t, false, false>(g2, e2, l.square, partial, s);
     // P is symmetric: it may be read by rows on either side.
@@ -290,7 +557,8 @@ qvh_status qvh_orthogonalize_device(const void* d_update, uint64_t batch, uint32
     QVH_REQUIRE(reinterpret_cast<uintptr_t>(d_update) % dtype_size(dtype) == 0 &&
                     reinterpret_cast<uintptr_t>(d_out) % dtype_size(dtype) == 0,
                 w + ": a buffer is not aligned to its element type");
-    QVH_REQUIRE(d_workspace != nullptr && workspace_bytes >= ortho_layout(batch, m, n).total, w + ": the workspace is too small");
+    const size_t need = ortho_layout(batch, m, n).total;
+    QVH_REQUIRE(need == 0 || (d_workspace != nullptr && workspace_bytes >= need), w + ": the workspace is too small");
     QVH_REQUIRE(reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, w + ": the workspace must be 16-byte aligned");
     current_device();
     with_dtype(dtype, [&](auto* t) {
