@@ -3,9 +3,9 @@
 //
 // Operands. Each is a 16-bit matrix, stored either by rows ([row][k], k contiguous) or by k ([k][row],
 // row contiguous): a layer's forward pass reads both by rows, its input gradient the weight by k, its
-// weight gradient both by k, so no pass ever transposes a matrix in memory. fp32 operands come as a
-// sum of 16-bit planes; the product then runs over the listed pairs of planes as if they followed each
-// other along k.
+// weight gradient both by k, so no pass ever transposes a matrix in memory. Operands of more than 16 bits
+// come as a sum of two or three 16-bit planes; a step then holds all of them, and every fragment that was
+// read from LDS enters two or three of the three or six products that count.
 //
 // A work-group takes a BM x BN tile in 64-deep steps. The steps go from memory straight into LDS
 // (16 bytes per lane, no registers), the next one while the present one is multiplied; LDS holds
@@ -54,11 +54,8 @@ struct GemmOperand {
 struct GemmArgs {
   GemmOperand a, b;
   uint32_t m = 0, n = 0, k = 0;
-  uint32_t pairs = 1;        // pairs of planes, at most eight
-  uint32_t pa = 0, pb = 0;   // the planes of pair i: four bits each, from the lowest
   uint32_t tiles_m = 0, tiles_n = 0, splits = 1, batches = 1;
   uint32_t symmetric = 0;  // the product equals its transpose (m = n): tiles above the diagonal are mirrored
-  uint32_t side = 0;       // of a tile, where that is so
   float* partial = nullptr;  // [split][batch][m][n rounded up to 8] when splits > 1
 };
 
@@ -334,20 +331,47 @@ __device__ __forceinline__ X8 clip(X8 f, int kk, int lane, uint32_t depth) {
   return f;
 }
 
-/// Tile of a work-group, its waves, the depth of a step and the steps that LDS holds.
-template <int BM_, int BN_, int WM_, int WN_, int D_, int STAGES_>
+/// Tile of a work-group, its waves, the depth of a step, the steps that LDS holds, and the operands' planes.
+template <int BM_, int BN_, int WM_, int WN_, int D_, int STAGES_, int PLANES_>
 struct Tile {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, D = D_, STAGES = STAGES_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, D = D_, STAGES = STAGES_, PLANES = PLANES_;
 };
+
+/// The pairs of planes whose products count, the smallest first. Two planes: all but low x low; three: those
+/// of at least 2^-16 of the product.
+template <int PLANES>
+struct Pairs;
+template <>
+struct Pairs<1> {
+  static constexpr int kCount = 1, kA[1] = {0}, kB[1] = {0};
+};
+template <>
+struct Pairs<2> {
+  static constexpr int kCount = 3, kA[3] = {1, 0, 0}, kB[3] = {0, 1, 0};
+};
+template <>
+struct Pairs<3> {
+  static constexpr int kCount = 6, kA[6] = {2, 0, 1, 1, 0, 0}, kB[6] = {0, 2, 1, 0, 1, 0};
+};
+
+/// Block t of the lower triangle, row by row.
+__device__ __forceinline__ void lower_block(uint32_t t, uint32_t& bi, uint32_t& bj) {
+  bi = static_cast<uint32_t>((sqrtf(8.0f * static_cast<float>(t) + 1.0f) - 1.0f) * 0.5f);
+  while (bi * (bi + 1) / 2 > t) --bi;
+  while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
+  bj = t - bi * (bi + 1) / 2;
+}
 
 template <class T, bool AK, bool BK, class Shape, class Epi>
 __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::BN / (Shape::WM * Shape::WN) > 128 * 64 ? 1 : 2)
     gemm_kernel(GemmArgs g, Epi epi) {
   constexpr int BM = Shape::BM, BN = Shape::BN, WM = Shape::WM, WN = Shape::WN, kStep = Shape::D, kStages = Shape::STAGES;
+  constexpr int kPlanes = Shape::PLANES;
+  using P = Pairs<kPlanes>;
   constexpr int kWaves = WM * WN;
   using SA = Stage<T, AK, BM, kStep, kWaves>;
   using SB = Stage<T, BK, BN, kStep, kWaves>;
-  constexpr int kStageBytes = SA::kBytes + SB::kBytes;
+  constexpr int kStageBytes = (SA::kBytes + SB::kBytes) * kPlanes;
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 blocks per wave
   constexpr int kSlabLd = BN / WN + 8;
   constexpr int kSlabBytes = 32 * kSlabLd * 4 * kWaves;
@@ -369,11 +393,8 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
   const uint32_t split = id / per;
   const uint32_t tile = id % per;
   uint32_t tm, tn;
-  if (g.symmetric) {  // row by row of the lower triangle
-    tm = static_cast<uint32_t>((sqrtf(8.0f * static_cast<float>(tile) + 1.0f) - 1.0f) * 0.5f);
-    while (tm * (tm + 1) / 2 > tile) --tm;
-    while ((tm + 1) * (tm + 2) / 2 <= tile) ++tm;
-    tn = tile - tm * (tm + 1) / 2;
+  if (g.symmetric) {
+    lower_block(tile, tm, tn);
   } else {
     const uint32_t band = 8 * g.tiles_n, b0 = tile / band * 8;
     const uint32_t high = g.tiles_m - b0 < 8 ? g.tiles_m - b0 : 8;
@@ -384,9 +405,8 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
 
   const uint32_t row0 = tm * BM, col0 = tn * BN;
   const uint32_t rows = g.m - row0, cols = g.n - col0;
-  // Steps that are 64 deep throughout, of all pairs, and a shorter last one per pair behind them.
-  const uint32_t ksteps = g.k / kStep, rest = g.k % kStep;
-  const uint32_t whole = ksteps * g.pairs, steps = whole + (rest ? g.pairs : 0);
+  const uint32_t whole = g.k / kStep, rest = g.k % kStep;  // the last step may be a shorter one
+  const uint32_t steps = whole + (rest ? 1 : 0);
   const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(steps) * split / g.splits);
   const uint32_t end = static_cast<uint32_t>(static_cast<uint64_t>(steps) * (split + 1) / g.splits);
   const uint32_t whole_end = end < whole ? end : whole;
@@ -402,27 +422,37 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
   const uint32_t lds0 = static_cast<uint32_t>(
       reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(s_mem)));
 
-  // Where step ks of a pair begins, wave-uniform.
-  const auto begin_a = [&](uint32_t pair, uint32_t ks) {
-    const uint64_t k0 = static_cast<uint64_t>(ks) * kStep;
-    return a0 + (g.pa >> (4 * pair) & 15u) * g.a.plane + (AK ? k0 * g.a.ld : k0);
+  // Loads the step that begins at pa and pb into place `buf`, at the lanes' offsets.
+  constexpr int kPieces = (SA::kLoads + SB::kLoads) * kPlanes;
+  struct Sources {
+    u32x4_t a[kPlanes], b[kPlanes];
   };
-  const auto begin_b = [&](uint32_t pair, uint32_t ks) {
-    const uint64_t k0 = static_cast<uint64_t>(ks) * kStep;
-    return b0p + (g.pb >> (4 * pair) & 15u) * g.b.plane + (BK ? k0 * g.b.ld : k0);
+  const auto sources = [&](uint32_t step) {
+    const uint64_t k0 = static_cast<uint64_t>(step) * kStep;
+    const T* pa = a0 + (AK ? k0 * g.a.ld : k0);
+    const T* pb = b0p + (BK ? k0 * g.b.ld : k0);
+    Sources s;
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) {
+      s.a[p] = buffer_resource(pa + p * g.a.plane);
+      s.b[p] = buffer_resource(pb + p * g.b.plane);
+    }
+    return s;
   };
-  // Loads the step that begins at pa and pb into place `buf`, at the lanes' offsets: piece i of kPieces.
-  constexpr int kPieces = SA::kLoads + SB::kLoads;
-  const auto load_piece = [&](int i, u32x4_t ra, u32x4_t rb, int buf, const uint32_t(&at_a)[SA::kLoads],
+  // In LDS: the planes of a, then those of b.
+  const auto load_piece = [&](int i, const Sources& s, int buf, const uint32_t(&at_a)[SA::kLoads],
                               const uint32_t(&at_b)[SB::kLoads]) {
     const uint32_t to = lds0 + static_cast<uint32_t>(buf) * kStageBytes + (i * kWaves + wave) * 1024;
-    load_to_lds(to, i < SA::kLoads ? at_a[i] : at_b[i - SA::kLoads], i < SA::kLoads ? ra : rb, 0);
+    constexpr int kOfA = SA::kLoads * kPlanes;
+    if (i < kOfA) {
+      load_to_lds(to, at_a[i % SA::kLoads], s.a[i / SA::kLoads], 0);
+    } else {
+      load_to_lds(to, at_b[(i - kOfA) % SB::kLoads], s.b[(i - kOfA) / SB::kLoads], 0);
+    }
   };
-  const auto load = [&](const T* pa, const T* pb, int buf, const uint32_t(&at_a)[SA::kLoads],
-                        const uint32_t(&at_b)[SB::kLoads]) {
-    const u32x4_t ra = buffer_resource(pa), rb = buffer_resource(pb);
+  const auto load = [&](const Sources& s, int buf, const uint32_t(&at_a)[SA::kLoads], const uint32_t(&at_b)[SB::kLoads]) {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) load_piece(i, ra, rb, buf, at_a, at_b);
+    for (int i = 0; i < kPieces; ++i) load_piece(i, s, buf, at_a, at_b);
   };
 
   f32x16_t acc[TM][TN];
@@ -435,21 +465,32 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
   const int ra0 = wm * (BM / WM), rb0 = wn * (BN / WN);
   using X8 = typename Frag<T>::x8;
   struct Fragments {
-    X8 a[TM], b[TN];
+    X8 a[kPlanes][TM], b[kPlanes][TN];
   };
   const auto fetch = [&](Fragments& f, int buf, int kk) {
     const char* la = s_mem + buf * kStageBytes;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) f.a[i] = SA::fragment(la, ra0 + 32 * i, kk, lane);
+    for (int p = 0; p < kPlanes; ++p) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) f.b[j] = SB::fragment(la + SA::kBytes, rb0 + 32 * j, kk, lane);
+      for (int i = 0; i < TM; ++i) f.a[p][i] = SA::fragment(la + p * SA::kBytes, ra0 + 32 * i, kk, lane);
+    }
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        f.b[p][j] = SB::fragment(la + kPlanes * SA::kBytes + p * SB::kBytes, rb0 + 32 * j, kk, lane);
+      }
+    }
+  };
+  // Matrix instruction x of a slice.
+  constexpr int kOps = TM * TN * P::kCount;
+  const auto step_of = [&](const Fragments& f, int x) {
+    const int i = x / TN % TM, j = x % TN, q = x / (TM * TN);
+    acc[i][j] = Frag<T>::mfma(f.a[P::kA[q]][i], f.b[P::kB[q]][j], acc[i][j]);
   };
   const auto multiply = [&](const Fragments& f) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-#pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = Frag<T>::mfma(f.a[i], f.b[j], acc[i][j]);
-    }
+    for (int x = 0; x < kOps; ++x) step_of(f, x);
   };
 
   // Fragments are fetched one 16-deep slice ahead of their matrix instructions. The step's last slice is
@@ -457,25 +498,10 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
   // kStages on, and the next step's first slice is fetched while the last one is multiplied.
   if (first < whole_end) {
     constexpr int kSlices = kStep / 16;
-    uint32_t pair = first / ksteps, ks = first % ksteps;  // of the next step to load
-    const T *pa = begin_a(pair, ks), *pb = begin_b(pair, ks);
-    const auto advance = [&] {
-      pa += AK ? kStep * g.a.ld : kStep;
-      pb += BK ? kStep * g.b.ld : kStep;
-      if (++ks == ksteps) {
-        ks = 0;
-        ++pair;
-        pa = begin_a(pair, 0);
-        pb = begin_b(pair, 0);
-      }
-    };
     Fragments f[2];
 #pragma unroll
     for (int i = 0; i < kStages; ++i) {
-      if (first + i < whole_end) {
-        load(pa, pb, i, oa, ob);
-        advance();
-      }
+      if (first + i < whole_end) load(sources(first + i), i, oa, ob);
     }
     // All but the first step's loads may still be under way.
     if (first + kStages <= whole_end) {
@@ -504,33 +530,31 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       const bool more = s + kStages < whole_end;
-      const u32x4_t ra = buffer_resource(pa), rb = buffer_resource(pb);
+      const Sources src = sources(s + kStages);
       const int free_buf = buf;
       buf = buf + 1 == kStages ? 0 : buf + 1;
       if (s + 1 < whole_end) fetch(f[0], buf, 0);
       __builtin_amdgcn_sched_barrier(0);
       // The loads go out between the matrix instructions, which cover their issue.
-      constexpr int kLast = (kSlices - 1) & 1;
 #pragma unroll
-      for (int x = 0; x < TM * TN; ++x) {
-        acc[x / TN][x % TN] = Frag<T>::mfma(f[kLast].a[x / TN], f[kLast].b[x % TN], acc[x / TN][x % TN]);
+      for (int x = 0; x < kOps; ++x) {
+        step_of(f[(kSlices - 1) & 1], x);
         __builtin_amdgcn_sched_barrier(0);
         if (more) {
 #pragma unroll
-          for (int i = x * kPieces / (TM * TN); i < (x + 1) * kPieces / (TM * TN); ++i) load_piece(i, ra, rb, free_buf, oa, ob);
+          for (int i = x * kPieces / kOps; i < (x + 1) * kPieces / kOps; ++i) load_piece(i, src, free_buf, oa, ob);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (more) advance();
     }
   }
-  for (uint32_t s = first < whole ? whole : first; s < end; ++s) {
+  if (rest && end == steps && first < end) {
     uint32_t ta[SA::kLoads], tb[SB::kLoads];
 #pragma unroll
     for (int i = 0; i < SA::kLoads; ++i) ta[i] = SA::offset(i, wave, lane, lda, rows, rest);
 #pragma unroll
     for (int i = 0; i < SB::kLoads; ++i) tb[i] = SB::offset(i, wave, lane, ldb, cols, rest);
-    load(begin_a(s - whole, ksteps), begin_b(s - whole, ksteps), 0, ta, tb);
+    load(sources(whole), 0, ta, tb);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 #pragma unroll 1
@@ -538,12 +562,14 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
       Fragments f;
       fetch(f, 0, kk);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) f.a[i] = clip(f.a[i], kk, lane, rest);
+      for (int p = 0; p < kPlanes; ++p) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) f.b[j] = clip(f.b[j], kk, lane, rest);
+        for (int i = 0; i < TM; ++i) f.a[p][i] = clip(f.a[p][i], kk, lane, rest);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) f.b[p][j] = clip(f.b[p][j], kk, lane, rest);
+      }
       multiply(f);
     }
-    __syncthreads();
   }
   __syncthreads();
 
@@ -590,63 +616,86 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
   }
 }
 
-/// Adds the splits' partial sums in order and runs the epilogue.
+/// Eight elements' partial sums, the splits in order.
+__device__ __forceinline__ void add_splits(const float* p, uint32_t splits, uint64_t step, float (&v)[8]) {
+  uint32_t s = 0;
+  for (; s + 4 <= splits; s += 4, p += 4 * step) {  // four loads under way at a time
+    float x[4][8];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) load8(p + u * step, x[u], 8, true);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += x[u][e];
+    }
+  }
+  for (; s < splits; ++s, p += step) {
+    float x[8];
+    load8(p, x, 8, true);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += x[e];
+  }
+}
+
+/// Adds the splits' partial sums and runs the epilogue.
 template <class Epi>
 __global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs g, Epi epi) {
   const uint32_t ld = (g.n + 7) / 8 * 8;
   const auto [m, chunk] = row_and_chunk(blockIdx.x, ld / 8);
   if (m >= g.m) return;
   const uint32_t n = chunk * 8;
-  const uint64_t batch = static_cast<uint64_t>(g.m) * ld, step = batch * g.batches;
-  const float* p = g.partial + blockIdx.y * batch;
+  const uint64_t batch = static_cast<uint64_t>(g.m) * ld;
   float v[8] = {};
-  if (g.symmetric && n / g.side > m / g.side) {  // above the diagonal: from the mirrored place
-    p += n * static_cast<uint64_t>(ld) + m;
-    for (uint32_t s = 0; s < g.splits; ++s, p += step) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += n + e < g.n ? p[e * static_cast<uint64_t>(ld)] : 0.0f;
-    }
-  } else {
-    p += m * ld + n;
-    uint32_t s = 0;
-    for (; s + 4 <= g.splits; s += 4, p += 4 * step) {  // four loads under way at a time
-      float x[4][8];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) load8(p + u * step, x[u], 8, true);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += x[u][e];
-      }
-    }
-    for (; s < g.splits; ++s, p += step) {
-      float x[8];
-      load8(p, x, 8, true);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += x[e];
-    }
-  }
+  add_splits(g.partial + blockIdx.y * batch + m * ld + n, g.splits, batch * g.batches, v);
   epi(blockIdx.y, static_cast<uint32_t>(m), n, g.n - n, v);
+}
+
+/// The same for a symmetric product, of which only the lower tiles have sums: work-groups of 128 threads per
+/// 32 x 32 block of the lower triangle, which go through LDS to their mirrored places.
+template <class Epi>
+__global__ void __launch_bounds__(128) gemm_join_symmetric_kernel(GemmArgs g, Epi epi) {
+  __shared__ float s_block[32][33];
+  uint32_t bi, bj;
+  lower_block(blockIdx.x, bi, bj);
+  const uint32_t ld = (g.n + 7) / 8 * 8;
+  const uint64_t batch = static_cast<uint64_t>(g.m) * ld;
+  const uint32_t r = threadIdx.x / 4, c = threadIdx.x % 4 * 8;
+  const uint32_t m = bi * 32 + r, n = bj * 32 + c;
+  float v[8] = {};
+  if (m < g.m && n < g.n) {
+    add_splits(g.partial + blockIdx.y * batch + m * static_cast<uint64_t>(ld) + n, g.splits, batch * g.batches, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s_block[r][c + e] = v[e];
+    epi(blockIdx.y, m, n, g.n - n, v);
+  }
+  if (bi == bj) return;
+  __syncthreads();
+  const uint32_t mm = bj * 32 + r, nn = bi * 32 + c;
+  if (mm < g.n && nn < g.m) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = s_block[c + e][r];
+    epi(blockIdx.y, mm, nn, g.m - nn, v);
+  }
 }
 
 // ---- launching --------------------------------------------------------------------------------
 
 /// Tile shape and number of splits for a product; the same for the workspace's size and for the launch.
-/// `symmetric`: m = n and only the tiles on and below the diagonal are computed.
 struct GemmPlan {
-  int tile = -1;  // 0: 64 x 64, 1: 128 x 128, 2: 256 x 256
+  int tile = 0;  // which of the three shapes
   uint32_t splits = 1;
   size_t partial_bytes = 0;
 };
 
-GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t pairs, uint32_t batches, bool symmetric);
+/// `symmetric`: m = n, and only the tiles on and below the diagonal are computed.
+GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, int planes, uint32_t batches, bool symmetric);
 
 template <class T, bool AK, bool BK, class Shape, class Epi>
 void launch_tile(GemmArgs g, const Epi& epi, hipStream_t s) {
   g.tiles_m = static_cast<uint32_t>(ceil_div(g.m, Shape::BM));
   g.tiles_n = static_cast<uint32_t>(ceil_div(g.n, Shape::BN));
-  g.side = Shape::BM;
-  const uint64_t tiles = g.symmetric ? static_cast<uint64_t>(g.tiles_m) * (g.tiles_m + 1) / 2 : static_cast<uint64_t>(g.tiles_m) * g.tiles_n;
+  const uint64_t tiles = g.symmetric ? static_cast<uint64_t>(g.tiles_m) * (g.tiles_m + 1) / 2
+                                     : static_cast<uint64_t>(g.tiles_m) * g.tiles_n;
   const uint64_t blocks = tiles * g.splits;
   QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "the matrix product is too large");
   const dim3 grid(static_cast<unsigned>(blocks), g.batches);
@@ -655,26 +704,56 @@ void launch_tile(GemmArgs g, const Epi& epi, hipStream_t s) {
     const PartialEpilogue pe{g.partial, ld, ld * g.m};
     hipLaunchKernelGGL((gemm_kernel<T, AK, BK, Shape, PartialEpilogue>), grid, dim3(Shape::WM * Shape::WN * 64), 0, s, g, pe);
     QVH_HIP(hipGetLastError());
-    hipLaunchKernelGGL((gemm_join_kernel<Epi>), dim3(static_cast<unsigned>(ceil_div(ld / 8 * g.m, 256)), g.batches),
-                       dim3(256), 0, s, g, epi);
+    if (g.symmetric) {
+      const uint32_t side = static_cast<uint32_t>(ceil_div(g.m, 32));
+      hipLaunchKernelGGL((gemm_join_symmetric_kernel<Epi>), dim3(side * (side + 1) / 2, g.batches), dim3(128), 0, s, g, epi);
+    } else {
+      hipLaunchKernelGGL((gemm_join_kernel<Epi>), dim3(static_cast<unsigned>(ceil_div(ld / 8 * g.m, 256)), g.batches),
+                         dim3(256), 0, s, g, epi);
+    }
   } else {
     hipLaunchKernelGGL((gemm_kernel<T, AK, BK, Shape, Epi>), grid, dim3(Shape::WM * Shape::WN * 64), 0, s, g, epi);
   }
   QVH_HIP(hipGetLastError());
 }
 
-template <class T, bool AK, bool BK, class Epi>
+/// The shapes by number of planes. With more than one a step is 32 deep, so that LDS holds two or three.
+template <int PLANES>
+struct Shapes;
+template <>
+struct Shapes<1> {
+  using S0 = Tile<64, 64, 2, 2, 64, 2, 1>;
+  using S1 = Tile<128, 128, 2, 2, 64, 2, 1>;
+  using S2 = Tile<256, 256, 2, 4, 64, 2, 1>;
+};
+template <>
+struct Shapes<2> {
+  using S0 = Tile<64, 64, 2, 2, 32, 3, 2>;
+  using S1 = Tile<128, 128, 2, 2, 32, 2, 2>;
+  using S2 = Tile<256, 128, 4, 2, 32, 3, 2>;
+};
+template <>
+struct Shapes<3> {
+  using S0 = Tile<64, 64, 2, 2, 32, 2, 3>;
+  using S1 = Tile<128, 128, 2, 4, 32, 3, 3>;
+  using S2 = Tile<256, 128, 4, 2, 32, 2, 3>;
+};
+
+template <class T, int PLANES, bool AK, bool BK, class Epi>
 void launch_gemm(GemmArgs g, const Epi& epi, const GemmPlan& plan, void* partial, hipStream_t s) {
   if (g.m == 0 || g.n == 0 || g.batches == 0) return;
   g.splits = plan.splits;
   g.partial = static_cast<float*>(partial);
   if (plan.tile == 2) {
-    launch_tile<T, AK, BK, Tile<256, 256, 2, 4, 64, 2>>(g, epi, s);
-  } else if (plan.tile == 1) {
-    launch_tile<T, AK, BK, Tile<128, 128, 2, 2, 64, 2>>(g, epi, s);
-  } else {
-    launch_tile<T, AK, BK, Tile<64, 64, 2, 2, 64, 2>>(g, epi, s);
+    // A symmetric product's tiles are square.
+    if constexpr (Shapes<PLANES>::S2::BM == Shapes<PLANES>::S2::BN) {
+      return launch_tile<T, AK, BK, typename Shapes<PLANES>::S2>(g, epi, s);
+    } else if (!g.symmetric) {
+      return launch_tile<T, AK, BK, typename Shapes<PLANES>::S2>(g, epi, s);
+    }
   }
+  if (plan.tile >= 1) return launch_tile<T, AK, BK, typename Shapes<PLANES>::S1>(g, epi, s);
+  launch_tile<T, AK, BK, typename Shapes<PLANES>::S0>(g, epi, s);
 }
 
 }  // namespace qvh

@@ -14,32 +14,36 @@ namespace qvh {
 // typical choices, in us: 1,024 x 1,024 x 4,096 as 64-tiles in one piece 37.2, in four 25.0, as 128-tiles in
 // one 47.1; 2,048^3 as 128-tiles 29.5, 256-tiles 51.0; 8,192 x 2,048 x 768 as 256-tiles 35.5, 128-tiles
 // 37.1, 64-tiles 51.2; 1,024 x 4,096 x 16,384 as 256-tiles in four pieces 131, 128-tiles in one 181.
-GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t pairs, uint32_t batches, bool symmetric) {
+GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, int planes, uint32_t batches, bool symmetric) {
   struct Cost {
-    uint64_t side, together;    // tile, and work-groups that a CU holds
-    double alone, shared, end;  // us per 64-deep step: one work-group on a CU, each of several; prologue and epilogue
+    uint64_t bm, bn, together;  // tile, and work-groups that a CU holds
+    double alone, shared, end;  // us per step: one work-group on a CU, each of several; prologue and epilogue
   };
-  constexpr Cost kCosts[3] = {{64, 4, 0.45, 0.22, 2.0}, {128, 2, 0.70, 0.53, 4.0}, {256, 1, 1.75, 1.75, 8.0}};
+  constexpr Cost kCosts[3][3] = {
+      {{64, 64, 4, 0.45, 0.22, 2.0}, {128, 128, 2, 0.70, 0.53, 4.0}, {256, 256, 1, 1.75, 1.75, 8.0}},
+      {{64, 64, 3, 0.40, 0.20, 2.0}, {128, 128, 2, 0.55, 0.45, 4.0}, {256, 128, 1, 0.95, 0.95, 6.0}},
+      {{64, 64, 3, 0.50, 0.35, 2.0}, {128, 128, 1, 0.95, 0.95, 4.0}, {256, 128, 1, 1.80, 1.80, 6.0}}};
   constexpr uint32_t kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
   constexpr double kCus = 256.0;
   GemmPlan best;
-  double least = 0.0;
-  const uint64_t steps = ceil_div(k, 64) * pairs;
+  double least = -1.0;
+  const uint64_t steps = ceil_div(k, planes == 1 ? 64 : 32);
   for (int t = 0; t < 3; ++t) {
-    const Cost& c = kCosts[t];
-    const uint64_t tm = ceil_div(m, c.side), tn = ceil_div(n, c.side);
+    const Cost& c = kCosts[planes - 1][t];
+    if (symmetric && c.bm != c.bn) continue;
+    const uint64_t tm = ceil_div(m, c.bm), tn = ceil_div(n, c.bn);
     const uint64_t tiles = (symmetric ? tm * (tm + 1) / 2 : tm * tn) * batches;
     for (const uint32_t splits : kSplits) {
       if (splits > 1 && steps < 2 * splits) break;
       const double groups = static_cast<double>(tiles) * splits;
       const double per_cu = std::ceil(groups / kCus);
       const double rounds = std::ceil(per_cu / static_cast<double>(c.together));
-      const double at_once = std::ceil(per_cu / rounds);
+      const double at_once = std::ceil(per_cu / std::max(rounds, 1.0));
       const double step = std::max(c.alone, c.shared * at_once);
       double us = rounds * (std::ceil(static_cast<double>(steps) / splits) * step + c.end + 0.5 * at_once);
       // The partial sums go out and come back, through the last-level cache, in a launch of their own.
       if (splits > 1) us += 4.0 + 0.1 * splits + static_cast<double>(splits) * batches * m * n * 8.0 / 7e6;
-      if (best.tile < 0 || us < least) {
+      if (least < 0.0 || us < least) {
         least = us;
         best.tile = t;
         best.splits = splits;
@@ -55,7 +59,7 @@ namespace {
 constexpr uint64_t kMaxRows = uint64_t{1} << 31, kMaxStride = uint64_t{1} << 22;
 constexpr uint32_t kMaxWidth = 1u << 20;
 constexpr uint64_t kFewRows = 64;  // x rows that the few-row kernel takes
-constexpr uint32_t kPlanes = 3;    // bf16 parts of an fp32 value
+constexpr int kPlanes = 3;         // bf16 parts of an fp32 value
 
 // ---- operand preparation ----------------------------------------------------------------------
 
@@ -351,15 +355,6 @@ void launch_prepare(int dtype, const Prepared& a, const Prepared& b, hipStream_t
   QVH_HIP(hipGetLastError());
 }
 
-/// The pairs of parts whose products make up fp32's, the smallest first.
-void set_pairs(GemmArgs& g, int dtype) {
-  g.pairs = 1;
-  if (dtype != QVH_FP32) return;
-  g.pairs = 6;
-  g.pa = 0x001102;  // (2, 0), (0, 2), (1, 1), (1, 0), (0, 1), (0, 0)
-  g.pb = 0x010120;
-}
-
 void run_product(Form form, int dtype, GemmArgs g, const void* bias, const void* residual, uint64_t ld_residual,
                  void* out, uint64_t ld_out, void* keep, uint64_t ld_keep, int act, const GemmPlan& plan, void* partial,
                  hipStream_t s) {
@@ -422,7 +417,7 @@ LinearRun plan_linear(const qvh_linear_args& a, void* ws) {
   sp.base = static_cast<char*>(ws);
   r.x = prepare_operand(a.x, a.m, a.x_stride, a.k, a.dtype, sp);
   r.w = prepare_operand(a.weight, a.n, a.weight_stride, a.k, a.dtype, sp);
-  r.plan = gemm_plan(a.m, a.n, a.k, a.dtype == QVH_FP32 ? 6 : 1, 1, false);
+  r.plan = gemm_plan(a.m, a.n, a.k, a.dtype == QVH_FP32 ? kPlanes : 1, 1, false);
   r.partial = sp.take(r.plan.partial_bytes);
   r.bytes = sp.at;
   return r;
@@ -483,7 +478,7 @@ GradRun plan_grad(const qvh_linear_grad_args& a, void* ws) {
   GradRun r;
   if (a.n == 0 || (a.m == 0 && a.k == 0)) return r;
   const size_t e = dtype_size(a.dtype);
-  const uint32_t pairs = a.dtype == QVH_FP32 ? 6 : 1;
+  const int planes = a.dtype == QVH_FP32 ? kPlanes : 1;
   Space sp;
   sp.base = static_cast<char*>(ws);
   const bool products = (a.grad_x || a.grad_weight) && a.k > 0;
@@ -520,12 +515,12 @@ GradRun plan_grad(const qvh_linear_grad_args& a, void* ws) {
   if (products) {
     if (a.grad_x) {
       r.w = prepare_operand(a.weight, a.n, a.weight_stride, a.k, a.dtype, sp);
-      r.plan_x = gemm_plan(a.m, a.k, a.n, pairs, 1, false);
+      r.plan_x = gemm_plan(a.m, a.k, a.n, planes, 1, false);
       r.partial_x = sp.take(r.plan_x.partial_bytes);
     }
     if (a.grad_weight) {
       r.x = prepare_operand(a.x, a.m, a.x_stride, a.k, a.dtype, sp);
-      r.plan_w = gemm_plan(a.n, a.k, a.m, pairs, 1, false);
+      r.plan_w = gemm_plan(a.n, a.k, a.m, planes, 1, false);
       r.partial_w = sp.take(r.plan_w.partial_bytes);
     }
   }
@@ -594,7 +589,6 @@ qvh_status qvh_linear_device(const qvh_linear_args* args, void* d_workspace, uin
     g.m = static_cast<uint32_t>(a.m);
     g.n = a.n;
     g.k = a.k;
-    set_pairs(g, a.dtype);
     run_product(Form::kRowsRows, a.dtype, g, a.bias, a.residual, a.residual_stride, a.out, a.out_stride, a.preactivation,
                 a.preactivation_stride, a.activation, r.plan, r.partial, s);
   });
@@ -637,7 +631,6 @@ qvh_status qvh_linear_grad_device(const qvh_linear_grad_args* args, void* d_work
     if (a.k == 0 || !(a.grad_x || a.grad_weight)) return;
     launch_prepare(a.dtype, r.x, r.w, s);
     GemmArgs g;
-    set_pairs(g, a.dtype);
     g.a = r.dz;
     if (a.grad_x && a.m > 0) {
       g.b = r.w.op;

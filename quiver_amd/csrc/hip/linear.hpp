@@ -14,11 +14,11 @@ void gemm_bf16(Form form, const GemmArgs& g, const LinearEpilogue<bhalf_t>& e, c
 /// bf16 planes of fp32 operands, fp32 results.
 void gemm_fp32(Form form, const GemmArgs& g, const LinearEpilogue<float>& e, const GemmPlan& p, void* partial, hipStream_t s);
 
-template <class T, class Epi>
+template <class T, int PLANES, class Epi>
 void gemm_forms(Form form, const GemmArgs& g, const Epi& e, const GemmPlan& p, void* partial, hipStream_t s) {
-  if (form == Form::kRowsRows) return launch_gemm<T, false, false>(g, e, p, partial, s);
-  if (form == Form::kRowsK) return launch_gemm<T, false, true>(g, e, p, partial, s);
-  launch_gemm<T, true, true>(g, e, p, partial, s);
+  if (form == Form::kRowsRows) return launch_gemm<T, PLANES, false, false>(g, e, p, partial, s);
+  if (form == Form::kRowsK) return launch_gemm<T, PLANES, false, true>(g, e, p, partial, s);
+  launch_gemm<T, PLANES, true, true>(g, e, p, partial, s);
 }
 
 }  // namespace qvh
