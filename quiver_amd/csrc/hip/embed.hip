@@ -92,80 +92,91 @@ void launch_embed(const void* table, uint64_t rows, uint32_t dim, uint64_t strid
 
 constexpr uint32_t kOwnTokens = 2048;
 
-/// Adds N gradient rows, in order: the loads first, so that they are in flight together.
-template <class T, int V, int N>
-__device__ __forceinline__ void add_rows(const T* __restrict__ grad, uint64_t stride, uint32_t col, bool in,
-                                         uint32_t entries, uint64_t& mask, float (&acc)[V]) {
-  float g[N][V];
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const int bit = __builtin_ctzll(mask);
-    mask &= mask - 1;
-    const uint32_t pos = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(entries), bit)) & 0xFFFFu;
-    if (in) {
-      load_floats<T, V>(grad + static_cast<uint64_t>(pos) * stride + col, g[j]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k) g[j][k] = 0.0f;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) acc[k] += g[j][k];
-  }
-}
-
 /// One wave per `own` rows (at most 64): lists the batch's tokens that fall into its rows, then per row
-/// adds their gradient rows in order of position.
-template <class T, int V, class I>
+/// the positions of its tokens, whose gradient rows are added: 64 / G at a time, each by G lanes that take
+/// V columns, every such share in order of position and the shares in order.
+template <class T, int V, int G, class I>
 __global__ void __launch_bounds__(256) embed_grad_own_kernel(const T* __restrict__ grad, uint64_t stride,
                                                              const I* __restrict__ tokens, uint32_t count, uint32_t rows,
                                                              uint32_t dim, uint32_t own, float scale,
                                                              T* __restrict__ out) {
+  constexpr uint32_t kShares = 64 / G, kAhead = V >= 8 ? 8 : 16;
   __shared__ uint32_t s_list[4][kOwnTokens];  // (row - first) << 16 | position
+  __shared__ uint16_t s_match[4][kOwnTokens];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint64_t first = (static_cast<uint64_t>(blockIdx.x) * 4 + wave) * own;
   const uint32_t held = first < rows ? (rows - first < own ? static_cast<uint32_t>(rows - first) : own) : 0u;
   uint32_t* list = s_list[wave];
+  uint16_t* match = s_match[wave];
   uint32_t found = 0;
   const uint64_t below = (uint64_t{1} << lane) - 1;
-#pragma unroll 4
-  for (uint32_t b = 0; b < count; b += 64) {
-    const uint32_t t = b + lane;
-    const int64_t tok = t < count ? static_cast<int64_t>(tokens[t]) : -1;
-    const uint64_t r = static_cast<uint64_t>(tok) - first;  // wraps to a large value below the first row
-    const bool mine = tok >= 0 && r < held;
-    const uint64_t mask = __builtin_amdgcn_ballot_w64(mine);
-    if (mine) list[found + __popcll(mask & below)] = static_cast<uint32_t>(r) << 16 | t;
-    found += static_cast<uint32_t>(__popcll(mask));
+  for (uint32_t b0 = 0; b0 < count; b0 += 512) {
+    int64_t tok[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t t = b0 + u * 64 + lane;
+      tok[u] = t < count ? static_cast<int64_t>(tokens[t]) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint64_t r = static_cast<uint64_t>(tok[u]) - first;  // wraps to a large value below the first row
+      const bool mine = tok[u] >= 0 && r < held;
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(mine);
+      if (mine) list[found + __popcll(mask & below)] = static_cast<uint32_t>(r) << 16 | (b0 + u * 64 + lane);
+      found += static_cast<uint32_t>(__popcll(mask));
+    }
   }
-  __syncthreads();
+  const uint32_t share = lane / G;
   for (uint32_t r = 0; r < held; ++r) {
-    for (uint32_t c0 = 0; c0 < dim; c0 += 64 * V) {
-      const uint32_t c = c0 + lane * V;
+    uint32_t n = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's own LDS accesses stay in order
+    for (uint32_t b = 0; b < found; b += 64) {
+      const uint32_t e = b + lane < found ? list[b + lane] : 0xFFFFFFFFu;
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(e >> 16 == r);
+      if (e >> 16 == r) match[n + __popcll(mask & below)] = static_cast<uint16_t>(e);
+      n += static_cast<uint32_t>(__popcll(mask));
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (uint32_t c0 = 0; c0 < dim; c0 += G * V) {
+      const uint32_t c = c0 + lane % G * V;
       const bool in = c < dim;
       float acc[V] = {};
-      for (uint32_t b = 0; b < found; b += 64) {
-        const uint32_t e = b + lane < found ? list[b + lane] : 0xFFFFFFFFu;
-        uint64_t mask = __builtin_amdgcn_ballot_w64(e >> 16 == r);
-        while (__popcll(mask) >= 8) add_rows<T, V, 8>(grad, stride, c, in, e, mask, acc);
-        if (__popcll(mask) >= 4) add_rows<T, V, 4>(grad, stride, c, in, e, mask, acc);
-        while (mask) add_rows<T, V, 1>(grad, stride, c, in, e, mask, acc);
+      for (uint32_t j0 = 0; j0 < n; j0 += kShares * kAhead) {
+        float x[kAhead][V];
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u) {
+          const uint32_t j = j0 + u * kShares + share;
+          if (in && j < n) {
+            load_floats<T, V>(grad + static_cast<uint64_t>(match[j]) * stride + c, x[u]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k) x[u][k] = 0.0f;
+          }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u) {
+#pragma unroll
+          for (int k = 0; k < V; ++k) acc[k] += x[u][k];
+        }
+      }
+#pragma unroll
+      for (int off = G; off < 64; off <<= 1) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] += __shfl_xor(acc[k], off, 64);
       }
 #pragma unroll
       for (int k = 0; k < V; ++k) acc[k] *= scale;
-      if (in) store_floats<T, V>(out + (first + r) * dim + c, acc);
+      if (in && share == 0) store_floats<T, V>(out + (first + r) * dim + c, acc);
     }
   }
 }
 
 // ---- sorting (key, position) pairs ------------------------------------------------------------
 //
-// Stable counting passes of at most 8 bits. Each of `parts` work-groups has a contiguous part of the
-// list; count[part][digit] gives every part its place per digit. The first pass's counts are taken by a
-// launch of their own, a later pass's by the scatter of the pass before it, which knows where its
-// pairs land (integer additions: their order changes nothing).
+// Stable counting passes of at most 8 bits, each a count and a scatter. Each of `parts` work-groups has a
+// contiguous part of the list; count[part][digit] gives every part its place per digit. (A scatter that
+// also counts the next pass's digits by atomics, knowing where its pairs land, took 33 us of 262,144
+// tokens instead of 5 + 6: frequent words all count in one place.)
 
 constexpr uint32_t kParts = 128, kBins = 256;
 constexpr uint32_t kSortWaves = 8;
@@ -177,23 +188,22 @@ __device__ __forceinline__ uint32_t token_key(const I* tokens, uint64_t t, uint3
   return tok >= 0 && static_cast<uint64_t>(tok) < rows ? static_cast<uint32_t>(tok) : rows;
 }
 
-template <class I>
-__global__ void __launch_bounds__(256) count_kernel(const I* __restrict__ tokens, uint32_t count, uint32_t part,
-                                                    uint32_t rows, uint32_t digit_mask, uint32_t* __restrict__ counts,
-                                                    uint32_t* __restrict__ next_counts) {
+template <class I, bool FIRST>
+__global__ void __launch_bounds__(512) count_kernel(const I* __restrict__ tokens, const uint32_t* __restrict__ keys,
+                                                    uint32_t count, uint32_t part, uint32_t rows, uint32_t shift,
+                                                    uint32_t digit_mask, uint32_t* __restrict__ counts) {
   __shared__ uint32_t s_bins[kBins];
-  s_bins[threadIdx.x] = 0;
-  next_counts[blockIdx.x * kBins + threadIdx.x] = 0;  // a second and a third pass's
-  next_counts[(gridDim.x + blockIdx.x) * kBins + threadIdx.x] = 0;
-  next_counts[(2 * gridDim.x + blockIdx.x) * kBins + threadIdx.x] = 0;
+  if (threadIdx.x < kBins) s_bins[threadIdx.x] = 0;
   __syncthreads();
   const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * part;
   const uint64_t end = begin + part < count ? begin + part : count;
-  for (uint64_t t = begin + threadIdx.x; t < end; t += 256) {
-    atomicAdd(&s_bins[token_key(tokens, t, rows) & digit_mask], 1u);
+#pragma unroll 4
+  for (uint64_t t = begin + threadIdx.x; t < end; t += 512) {
+    const uint32_t key = FIRST ? token_key(tokens, t, rows) : keys[t];
+    atomicAdd(&s_bins[key >> shift & digit_mask], 1u);
   }
   __syncthreads();
-  counts[blockIdx.x * kBins + threadIdx.x] = s_bins[threadIdx.x];
+  if (threadIdx.x < kBins) counts[blockIdx.x * kBins + threadIdx.x] = s_bins[threadIdx.x];
 }
 
 /// One pass. FIRST reads the tokens themselves (positions are the list's order).
@@ -201,10 +211,10 @@ template <class I, bool FIRST>
 __global__ void __launch_bounds__(kSortWaves * 64) scatter_kernel(
     const I* __restrict__ tokens, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ positions,
     uint32_t count, uint32_t part, uint32_t rows, uint32_t shift, uint32_t bits, const uint32_t* __restrict__ counts,
-    uint32_t* __restrict__ next_counts, uint32_t next_shift, uint32_t next_mask, uint32_t* __restrict__ out_keys,
-    uint32_t* __restrict__ out_positions) {
+    uint32_t* __restrict__ out_keys, uint32_t* __restrict__ out_positions) {
   __shared__ uint32_t s_at[kSortWaves][kBins];
   __shared__ uint32_t s_scan[kBins];
+  __shared__ uint32_t s_half[2][kBins];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t digit_mask = (1u << bits) - 1;
   for (uint32_t i = tid; i < kSortWaves * kBins; i += kSortWaves * 64) (&s_at[0][0])[i] = 0;
@@ -220,23 +230,39 @@ __global__ void __launch_bounds__(kSortWaves * 64) scatter_kernel(
     const uint32_t key = FIRST ? token_key(tokens, i, rows) : keys[i];
     atomicAdd(&s_at[wave][key >> shift & digit_mask], 1u);
   }
-  // This part's place per digit: all pairs of smaller digits, and this digit's in earlier parts.
+  // This part's place per digit: all pairs of smaller digits, and this digit's in earlier parts. Two threads
+  // per digit, each over half of the parts.
+  const uint32_t digit_of = tid % kBins, half = tid / kBins;
   uint32_t before = 0, all = 0;
-  if (tid < kBins) {
-#pragma unroll 8
-    for (uint32_t p = 0; p < gridDim.x; ++p) {
-      const uint32_t n = counts[p * kBins + tid];
+  {
+    const uint32_t p0 = half ? (gridDim.x + 1) / 2 : 0u, p1 = half ? gridDim.x : (gridDim.x + 1) / 2;
+#pragma unroll 16
+    for (uint32_t p = p0; p < p1; ++p) {
+      const uint32_t n = counts[p * kBins + digit_of];
       before += p < blockIdx.x ? n : 0u;
       all += n;
     }
-    s_scan[tid] = all;
+  }
+  if (half) {
+    s_half[0][digit_of] = before;
+    s_half[1][digit_of] = all;
   }
   __syncthreads();
-  for (uint32_t d = 1; d < kBins; d <<= 1) {
-    const uint32_t add = tid < kBins && tid >= d ? s_scan[tid - d] : 0u;
-    __syncthreads();
-    if (tid < kBins) s_scan[tid] += add;
-    __syncthreads();
+  if (!half) {
+    before += s_half[0][tid];
+    all += s_half[1][tid];
+    // Inclusive sums over the 256 digits: within the waves, then across the four.
+    uint32_t run = all;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t up = static_cast<uint32_t>(__shfl_up(static_cast<int>(run), d, 64));
+      run += lane >= static_cast<uint32_t>(d) ? up : 0u;
+    }
+    s_scan[tid] = run;
+  }
+  __syncthreads();
+  if (tid < kBins) {
+    for (uint32_t w = 0; w < wave; ++w) before += s_scan[w * 64 + 63];
   }
   if (tid < kBins) {
     uint32_t at = s_scan[tid] - all + before;
@@ -269,14 +295,13 @@ __global__ void __launch_bounds__(kSortWaves * 64) scatter_kernel(
       const uint32_t to = base + rank;
       out_keys[to] = key;
       out_positions[to] = pos;
-      if (next_counts) atomicAdd(&next_counts[to / part * kBins + (key >> next_shift & next_mask)], 1u);
     }
   }
 }
 
 // ---- sums over the sorted list ----------------------------------------------------------------
 
-constexpr uint32_t kPiece = 64;     // sorted entries that one group of lanes adds
+constexpr uint32_t kMostEntries = 2048;  // sorted entries of a work-group's pieces
 constexpr uint32_t kZeroRows = 64;  // table rows that one work-group checks for having no token
 
 struct SumArgs {
@@ -288,6 +313,7 @@ struct SumArgs {
   float scale;
   void* out;
   float* partial;  // [piece][2][dim]: the run that came from the piece before, the one that goes on
+  uint32_t piece;  // sorted entries that one group of lanes adds
   uint32_t pieces, sum_blocks, slabs;
   uint32_t cpr;
 };
@@ -331,14 +357,15 @@ template <class T, int V, int G>
 __global__ void __launch_bounds__(256) embed_grad_sum_kernel(SumArgs a) {
   constexpr uint32_t kGroups = 256 / G;
   constexpr int kAhead = 8;
-  __shared__ uint32_t s_key[kGroups * kPiece];
-  __shared__ uint32_t s_pos[kGroups * kPiece];
+  __shared__ uint32_t s_key[kMostEntries];
+  __shared__ uint32_t s_pos[kMostEntries];
+  const uint32_t length = a.piece;
   if (blockIdx.x >= a.sum_blocks) {
     if (blockIdx.y == 0) zero_rows<T, V>(a, blockIdx.x - a.sum_blocks, s_key);
     return;
   }
-  const uint64_t block0 = static_cast<uint64_t>(blockIdx.x) * (kGroups * kPiece);
-  for (uint32_t i = threadIdx.x; i < kGroups * kPiece; i += 256) {
+  const uint64_t block0 = static_cast<uint64_t>(blockIdx.x) * (kGroups * length);
+  for (uint32_t i = threadIdx.x; i < kGroups * length; i += 256) {
     const uint64_t e = block0 + i;
     s_key[i] = e < a.count ? a.keys[e] : a.rows;
     s_pos[i] = e < a.count ? a.positions[e] : 0u;
@@ -346,12 +373,12 @@ __global__ void __launch_bounds__(256) embed_grad_sum_kernel(SumArgs a) {
   __syncthreads();
   const uint32_t group = threadIdx.x / G;
   const uint64_t piece = static_cast<uint64_t>(blockIdx.x) * kGroups + group;
-  const uint64_t e0 = piece * kPiece;
+  const uint64_t e0 = piece * length;
   const uint32_t col = (blockIdx.y * G + threadIdx.x % G) * V;
   if (e0 >= a.count || col >= a.dim) return;
-  const uint32_t n = a.count - e0 < kPiece ? static_cast<uint32_t>(a.count - e0) : kPiece;
-  const uint32_t* key = s_key + group * kPiece;
-  const uint32_t* pos = s_pos + group * kPiece;
+  const uint32_t n = a.count - e0 < length ? static_cast<uint32_t>(a.count - e0) : length;
+  const uint32_t* key = s_key + group * length;
+  const uint32_t* pos = s_pos + group * length;
   const uint32_t from = e0 > 0 ? a.keys[e0 - 1] : a.rows;                // the run that came in, if any
   const uint32_t onto = e0 + n < a.count ? a.keys[e0 + n] : a.rows;      // the run that goes on, if any
   const T* grad = static_cast<const T*>(a.grad) + col;
@@ -365,8 +392,14 @@ __global__ void __launch_bounds__(256) embed_grad_sum_kernel(SumArgs a) {
     const bool came = began == 0 && from == cur, goes = end == n && onto == cur;
     if (came || goes) {
       float* p = partial + (came ? 0u : a.dim);
+      constexpr int kWide = V < 4 ? V : 4;
 #pragma unroll
-      for (int k = 0; k < V; ++k) p[k] = acc[k];
+      for (int k = 0; k < V; k += kWide) {
+        float part[kWide];
+#pragma unroll
+        for (int e = 0; e < kWide; ++e) part[e] = acc[k + e];
+        store_floats<float, kWide>(p + k, part);
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < V; ++k) acc[k] *= a.scale;
@@ -402,45 +435,52 @@ __global__ void __launch_bounds__(256) embed_grad_sum_kernel(SumArgs a) {
   flush(n);
 }
 
-/// Work-group per piece: where a run begins in this piece and goes on, its partial sums are added in
-/// order (four waves take contiguous shares of them) and the row is written.
-template <class T>
+/// Work-group per piece and 64 W columns: where a run begins in this piece and goes on, its partial sums
+/// are added in order (four waves take contiguous shares of them) and the row is written.
+template <class T, int W>
 __global__ void __launch_bounds__(256) embed_grad_join_kernel(SumArgs a) {
-  __shared__ float s_sum[4][64];
-  const uint64_t e0 = static_cast<uint64_t>(blockIdx.x) * kPiece, e1 = e0 + kPiece;
+  __shared__ float s_sum[4][64 * W];
+  const uint64_t e0 = static_cast<uint64_t>(blockIdx.x) * a.piece, e1 = e0 + a.piece;
   if (e1 >= a.count) return;  // nothing goes on from the last piece
-  const uint32_t cur = a.keys[e1 - 1];
-  if (cur == a.rows || a.keys[e1] != cur) return;
-  if (e0 > 0 && a.keys[e0] == cur && a.keys[e0 - 1] == cur) return;  // began earlier
+  const uint32_t cur = a.keys[e1 - 1], next = a.keys[e1], lead = a.keys[e0], from = e0 > 0 ? a.keys[e0 - 1] : a.rows;
+  if (cur == a.rows || next != cur) return;
+  if (lead == cur && from == cur) return;  // began earlier
   const uint32_t end = static_cast<uint32_t>(e1) +
                        lower_bound(a.keys + e1, a.count - static_cast<uint32_t>(e1), cur + 1);
-  const uint32_t last = (end - 1) / kPiece;             // pieces blockIdx.x .. last hold the run
+  const uint32_t last = (end - 1) / a.piece;  // pieces blockIdx.x .. last hold the run
   const uint32_t n = last - blockIdx.x + 1;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t share = (n + 3) / 4;
   const uint32_t p0 = wave * share < n ? wave * share : n, p1 = p0 + share < n ? p0 + share : n;
-  for (uint32_t c0 = blockIdx.y * 64; c0 < a.dim; c0 += gridDim.y * 64) {
-    const uint32_t c = c0 + lane;
-    float acc = 0.0f;
-    if (c < a.dim) {
+  const uint32_t c = (blockIdx.y * 64 + lane) * W;
+  float acc[W] = {};
+  if (c < a.dim) {
 #pragma unroll 8
-      for (uint32_t p = p0; p < p1; ++p) {
-        acc += a.partial[((static_cast<uint64_t>(blockIdx.x) + p) * 2 + (p == 0 ? 1 : 0)) * a.dim + c];
-      }
+    for (uint32_t p = p0; p < p1; ++p) {
+      float x[W];
+      load_floats<float, W>(a.partial + ((static_cast<uint64_t>(blockIdx.x) + p) * 2 + (p == 0 ? 1 : 0)) * a.dim + c, x);
+#pragma unroll
+      for (int k = 0; k < W; ++k) acc[k] += x[k];
     }
-    __syncthreads();
-    s_sum[wave][lane] = acc;
-    __syncthreads();
-    if (wave == 0 && c < a.dim) {
-      const float sum = ((s_sum[0][lane] + s_sum[1][lane]) + s_sum[2][lane]) + s_sum[3][lane];
-      static_cast<T*>(a.out)[static_cast<uint64_t>(cur) * a.dim + c] = static_cast<T>(sum * a.scale);
+  }
+#pragma unroll
+  for (int k = 0; k < W; ++k) s_sum[wave][lane * W + k] = acc[k];
+  __syncthreads();
+  if (wave == 0 && c < a.dim) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const uint32_t i = lane * W + k;
+      acc[k] = (((s_sum[0][i] + s_sum[1][i]) + s_sum[2][i]) + s_sum[3][i]) * a.scale;
     }
+    T* to = static_cast<T*>(a.out) + static_cast<uint64_t>(cur) * a.dim + c;
+#pragma unroll
+    for (int k = 0; k < W; ++k) to[k] = static_cast<T>(acc[k]);
   }
 }
 
 /// Where the parts of the workspace lie, in bytes.
 struct GradLayout {
-  uint32_t parts, part, passes;
+  uint32_t parts, part, passes, piece;
   size_t counts, keys[2], positions[2], partial, total;
 };
 
@@ -453,7 +493,13 @@ GradLayout grad_layout(uint64_t rows, uint32_t dim, uint64_t count) {
   uint32_t bits = 0;
   while (bits < 32 && (rows >> bits) != 0) ++bits;
   l.passes = std::max(1u, (bits + 7) / 8);
-  size_t at = round(4 * static_cast<size_t>(l.parts) * kBins * 4);
+  // About 2,048 waves of pieces, where there are so many tokens: long pieces have fewer runs to join. Rows of
+  // dim / 8 to dim pieces of 16 bytes: counted as dim / 8 here, for every type.
+  const uint64_t lanes = std::min<uint64_t>(std::max<uint64_t>(ceil_div(dim, 8), 8), 64);
+  const uint64_t slabs = ceil_div(dim, 512);
+  l.piece = 16;
+  while (l.piece < 256 && l.piece < 8 * lanes && ceil_div(count, 2 * l.piece) * slabs * lanes >= 2048 * 64) l.piece *= 2;
+  size_t at = round(static_cast<size_t>(l.parts) * kBins * 4);
   for (int i = 0; i < 2; ++i) {
     l.keys[i] = at;
     at += round(count * 4);
@@ -461,7 +507,7 @@ GradLayout grad_layout(uint64_t rows, uint32_t dim, uint64_t count) {
     at += round(count * 4);
   }
   l.partial = at;
-  l.total = at + round(ceil_div(count, kPiece) * 2 * dim * 4);
+  l.total = at + round(ceil_div(count, l.piece) * 2 * dim * 4);
   return l;
 }
 
@@ -474,10 +520,20 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
     const uint32_t own = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(rows / 8192, 4), 64));
     with_width<T>(width, [&](auto v) {
       constexpr int V = decltype(v)::value;
-      hipLaunchKernelGGL((embed_grad_own_kernel<T, V, I>), dim3(static_cast<unsigned>(ceil_div(rows, 4 * own))),
-                         dim3(256), 0, s, static_cast<const T*>(grad), stride, static_cast<const I*>(tokens),
-                         static_cast<uint32_t>(count), static_cast<uint32_t>(rows), dim, own, scale,
-                         static_cast<T*>(out));
+      const auto go = [&](auto group) {
+        hipLaunchKernelGGL((embed_grad_own_kernel<T, V, decltype(group)::value, I>),
+                           dim3(static_cast<unsigned>(ceil_div(rows, 4 * own))), dim3(256), 0, s,
+                           static_cast<const T*>(grad), stride, static_cast<const I*>(tokens),
+                           static_cast<uint32_t>(count), static_cast<uint32_t>(rows), dim, own, scale,
+                           static_cast<T*>(out));
+      };
+      if (dim / V <= 16) {
+        go(std::integral_constant<int, 16>{});
+      } else if (dim / V <= 32) {
+        go(std::integral_constant<int, 32>{});
+      } else {
+        go(std::integral_constant<int, 64>{});
+      }
     });
     QVH_HIP(hipGetLastError());
     return;
@@ -488,22 +544,17 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
   while (bits < 32 && (rows >> bits) != 0) ++bits;
   const uint32_t digit = (bits + l.passes - 1) / l.passes;
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + l.counts);
-  const size_t counts_step = static_cast<size_t>(l.parts) * kBins;
   uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(ws + l.keys[0]), reinterpret_cast<uint32_t*>(ws + l.keys[1])};
   uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + l.positions[0]), reinterpret_cast<uint32_t*>(ws + l.positions[1])};
-  hipLaunchKernelGGL((count_kernel<I>), dim3(l.parts), dim3(256), 0, s, static_cast<const I*>(tokens), n, l.part, r,
-                     (1u << digit) - 1, counts, counts + counts_step);
-  QVH_HIP(hipGetLastError());
   for (uint32_t p = 0; p < l.passes; ++p) {
-    uint32_t* next = p + 1 < l.passes ? counts + (p + 1) * counts_step : nullptr;
-    const uint32_t next_mask = (1u << digit) - 1;
-    uint32_t* ok = keys[p & 1];
-    uint32_t* op = pos[p & 1];
+    const uint32_t *ik = keys[(p & 1) ^ 1], *ip = pos[(p & 1) ^ 1];
     const auto pass = [&](auto first) {
       constexpr bool F = decltype(first)::value;
+      hipLaunchKernelGGL((count_kernel<I, F>), dim3(l.parts), dim3(512), 0, s, static_cast<const I*>(tokens), ik, n, l.part, r,
+                         p * digit, (1u << digit) - 1, counts);
+      QVH_HIP(hipGetLastError());
       hipLaunchKernelGGL((scatter_kernel<I, F>), dim3(l.parts), dim3(kSortWaves * 64), 0, s,
-                         static_cast<const I*>(tokens), keys[(p & 1) ^ 1], pos[(p & 1) ^ 1], n, l.part, r, p * digit,
-                         digit, counts + p * counts_step, next, (p + 1) * digit, next_mask, ok, op);
+                         static_cast<const I*>(tokens), ik, ip, n, l.part, r, p * digit, digit, counts, keys[p & 1], pos[p & 1]);
     };
     if (p == 0) {
       pass(std::true_type{});
@@ -525,11 +576,13 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
     a.scale = scale;
     a.out = out;
     a.partial = reinterpret_cast<float*>(ws + l.partial);
-    a.pieces = static_cast<uint32_t>(ceil_div(count, kPiece));
+    a.piece = l.piece;
+    a.pieces = static_cast<uint32_t>(ceil_div(count, l.piece));
     a.cpr = dim / V;
     const uint32_t zero_blocks = static_cast<uint32_t>(ceil_div(rows, kZeroRows));
     const auto sum = [&](auto group) {
       constexpr int G = decltype(group)::value;
+      QVH_REQUIRE(256 / G * a.piece <= kMostEntries, "qvh_embed_grad_device: pieces past the work-group's memory");
       a.sum_blocks = static_cast<uint32_t>(ceil_div(a.pieces, 256 / G));
       a.slabs = static_cast<uint32_t>(ceil_div(a.cpr, G));
       hipLaunchKernelGGL((embed_grad_sum_kernel<T, V, G>), dim3(a.sum_blocks + zero_blocks, a.slabs), dim3(256), 0, s, a);
@@ -545,8 +598,11 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
     }
     QVH_HIP(hipGetLastError());
     if (a.pieces > 1) {
-      hipLaunchKernelGGL((embed_grad_join_kernel<T>), dim3(a.pieces, std::min<uint32_t>(ceil_div(dim, 64), 16)), dim3(256),
-                         0, s, a);
+      if (dim % 4 == 0) {
+        hipLaunchKernelGGL((embed_grad_join_kernel<T, 4>), dim3(a.pieces, ceil_div(dim, 256)), dim3(256), 0, s, a);
+      } else {
+        hipLaunchKernelGGL((embed_grad_join_kernel<T, 1>), dim3(a.pieces, ceil_div(dim, 64)), dim3(256), 0, s, a);
+      }
       QVH_HIP(hipGetLastError());
     }
   });

@@ -42,7 +42,7 @@ GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, int planes, uint32_t batc
       const double step = std::max(c.alone, c.shared * at_once);
       double us = rounds * (std::ceil(static_cast<double>(steps) / splits) * step + c.end + 0.5 * at_once);
       // The partial sums go out and come back, through the last-level cache, in a launch of their own.
-      if (splits > 1) us += 4.0 + 0.1 * splits + static_cast<double>(splits) * batches * m * n * 8.0 / 7e6;
+      if (splits > 1) us += 5.5 + 0.1 * splits + static_cast<double>(splits) * batches * m * n * 8.0 / 7e6;
       if (least < 0.0 || us < least) {
         least = us;
         best.tile = t;

@@ -232,21 +232,9 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
     acc = Frag<half_t>::mfma(ah, bl, acc);
     return Frag<half_t>::mfma(ah, bh, acc);
   };
-  // Row of accumulator r of this lane within its block; the column is j32.
-  const auto row_of = [&](int r) { return static_cast<uint32_t>(8 * (r / 4) + r % 4) + 4 * h; };
+  // Block v of a product, transposed: lane j32 holds a row of what is stored, four neighbouring columns at a
+  // time, so that the stores are of 8 bytes (as rows of the block itself they would be of two).
   const auto put = [&](char* base, uint32_t stride, uint32_t plane, uint32_t bi, uint32_t bj, const f32x16_t& v) {
-    char* at = base + (bi * 32 + 4 * h) * stride + (bj * 32 + j32) * 2;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      half_t high, low;
-      split2(v[r], high, low);
-      char* to = at + static_cast<uint32_t>(8 * (r / 4) + r % 4) * stride;
-      *reinterpret_cast<half_t*>(to) = high;
-      *reinterpret_cast<half_t*>(to + plane) = low;
-    }
-  };
-  // The block's mirror image: four neighbouring elements of a row at a time.
-  const auto put_mirrored = [&](char* base, uint32_t stride, uint32_t plane, uint32_t bi, uint32_t bj, const f32x16_t& v) {
     char* at = base + (bj * 32 + j32) * stride + (bi * 32 + 4 * h) * 2;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -259,12 +247,6 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
   };
 
   const uint32_t sb = sh.side / 32, db = sh.depth / 32;
-  const uint32_t lower = sb * (sb + 1) / 2;  // at most 10 blocks of S up to 128 rows, 36 up to 256
-  const auto block_of = [](uint32_t t, uint32_t& bi, uint32_t& bj) {
-    bi = 0;
-    while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
-    bj = t - bi * (bi + 1) / 2;
-  };
   // Addresses that follow from the wave's number are computed where they are used: kept over all steps, those
   // of five blocks took 250 registers more than there are.
   const auto fresh = [](uint32_t w) {
@@ -272,18 +254,20 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
     return w;
   };
   for (uint32_t step = 0; step < steps; ++step) {
-    // S = X X^T, the blocks on and below the diagonal and their mirror images.
-    for (uint32_t t = wave; t < lower; t += WAVES) {
-      uint32_t bi, bj;
-      block_of(t, bi, bj);
-      f32x16_t acc{};
-      for (uint32_t kk = 0; kk < sh.depth / 16; ++kk) {
-        acc = three(rows(x, sh.row_x, bi * 32, kk), rows(x + plane_x, sh.row_x, bi * 32, kk), rows(x, sh.row_x, bj * 32, kk),
-                    rows(x + plane_x, sh.row_x, bj * 32, kk), acc);
+    // S = X X^T. All blocks: the waves that its symmetry would save have nothing else to do.
+#pragma unroll
+    for (int u = 0; u < BLOCKS; ++u) {
+      const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
+      if (t < sb * sb) {
+        const uint32_t bi = t / sb, bj = t % sb;
+        f32x16_t acc{};
+        for (uint32_t kk = 0; kk < sh.depth / 16; ++kk) {
+          acc = three(rows(x, sh.row_x, bi * 32, kk), rows(x + plane_x, sh.row_x, bi * 32, kk), rows(x, sh.row_x, bj * 32, kk),
+                      rows(x + plane_x, sh.row_x, bj * 32, kk), acc);
+        }
+        acc *= 1.0f / kScale;
+        put(s, sh.row_s, plane_s, bi, bj, acc);
       }
-      acc *= 1.0f / kScale;
-      put(s, sh.row_s, plane_s, bi, bj, acc);
-      if (bi != bj) put_mirrored(s, sh.row_s, plane_s, bi, bj, acc);
     }
     __syncthreads();
     // P = a + b S + c S S in S's place.
@@ -291,21 +275,24 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
 #pragma unroll
     for (int u = 0; u < BLOCKS; ++u) {
       const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
-      if (t < lower) {
-        uint32_t bi, bj;
-        block_of(t, bi, bj);
+      if (t < sb * sb) {
+        const uint32_t bi = t / sb, bj = t % sb;
         f32x16_t acc{};
         for (uint32_t kk = 0; kk < sh.side / 16; ++kk) {
           acc = three(rows(s, sh.row_s, bi * 32, kk), rows(s + plane_s, sh.row_s, bi * 32, kk), rows(s, sh.row_s, bj * 32, kk),
                       rows(s + plane_s, sh.row_s, bj * 32, kk), acc);
         }
+        const char* at = s + (bj * 32 + j32) * sh.row_s + (bi * 32 + 4 * h) * 2;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const uint32_t row = bi * 32 + row_of(r), col = bj * 32 + j32;
-          const char* at = s + row * sh.row_s + col * 2;
-          const float sv = static_cast<float>(*reinterpret_cast<const half_t*>(at)) +
-                           static_cast<float>(*reinterpret_cast<const half_t*>(at + plane_s));
-          acc[r] = fmaf(b, sv, acc[r] * (c / kScale)) + (row == col ? a * kScale : 0.0f);
+        for (int q = 0; q < 4; ++q) {
+          const Pack<half_t, 4> high = *reinterpret_cast<const Pack<half_t, 4>*>(at + q * 16);
+          const Pack<half_t, 4> low = *reinterpret_cast<const Pack<half_t, 4>*>(at + q * 16 + plane_s);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float sv = static_cast<float>(high.v[e]) + static_cast<float>(low.v[e]);
+            const bool diagonal = bi == bj && static_cast<uint32_t>(8 * q + e) + 4 * h == j32;
+            acc[4 * q + e] = fmaf(b, sv, acc[4 * q + e] * (c / kScale)) + (diagonal ? a * kScale : 0.0f);
+          }
         }
         kept[u] = acc;
       }
@@ -314,24 +301,19 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
 #pragma unroll
     for (int u = 0; u < BLOCKS; ++u) {
       const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
-      if (t < lower) {
-        uint32_t bi, bj;
-        block_of(t, bi, bj);
-        put(s, sh.row_s, plane_s, bi, bj, kept[u]);
-        if (bi != bj) put_mirrored(s, sh.row_s, plane_s, bi, bj, kept[u]);
-      }
+      if (t < sb * sb) put(s, sh.row_s, plane_s, t / sb, t % sb, kept[u]);
     }
     __syncthreads();
-    // P X in X's place; the last one is the result.
+    // P X in X's place, computed as its transpose (P is symmetric); the last one is the result.
 #pragma unroll
     for (int u = 0; u < BLOCKS; ++u) {
       const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
       if (t < sb * db) {
-        const uint32_t bi = t / db, bj = t % db;
+        const uint32_t bi = t / sb, bj = t % sb;  // columns of X, rows of P
         f32x16_t acc{};
         for (uint32_t kk = 0; kk < sh.side / 16; ++kk) {
-          acc = three(rows(s, sh.row_s, bi * 32, kk), rows(s + plane_s, sh.row_s, bi * 32, kk), by_k(x, sh.row_x, bj * 32, kk),
-                      by_k(x + plane_x, sh.row_x, bj * 32, kk), acc);
+          acc = three(by_k(x, sh.row_x, bi * 32, kk), by_k(x + plane_x, sh.row_x, bi * 32, kk), rows(s, sh.row_s, bj * 32, kk),
+                      rows(s + plane_s, sh.row_s, bj * 32, kk), acc);
         }
         kept[u] = acc;
       }
@@ -342,14 +324,15 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
     for (int u = 0; u < BLOCKS; ++u) {
       const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
       if (t < sb * db) {
-        const uint32_t bi = t / db, bj = t % db;
+        const uint32_t bi = t / sb, bj = t % sb;
         if (!last) {
           kept[u] *= 1.0f / kScale;
           put(x, sh.row_x, plane_x, bi, bj, kept[u]);
         } else {
+          const uint32_t row = bj * 32 + j32;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const uint32_t row = bi * 32 + row_of(r), col = bj * 32 + j32;
+            const uint32_t col = bi * 32 + static_cast<uint32_t>(8 * (r / 4) + r % 4) + 4 * h;
             if (row < (tall ? n : m) && col < (tall ? m : n)) {
               o[tall ? col * n + row : row * n + col] = static_cast<T>(kept[u][r] * (1.0f / (kScale * kScale)));
             }
@@ -460,7 +443,7 @@ void orthogonalize(const T* update, uint64_t batch, uint32_t m, uint32_t n, uint
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(batch)), dim3(W * 64), sh.bytes, s, update, m, n, steps,
                          a, b, c, out);
     };
-    if (sh.side / 32 * (sh.depth / 32) <= 16) {
+    if (sh.side / 32 * (sh.depth / 32) <= 16) {  // side <= depth, so S has no more blocks than X
       go(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
     } else {
       go(std::integral_constant<int, 8>{}, std::integral_constant<int, 5>{});
