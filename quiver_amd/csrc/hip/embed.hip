@@ -493,12 +493,13 @@ GradLayout grad_layout(uint64_t rows, uint32_t dim, uint64_t count) {
   uint32_t bits = 0;
   while (bits < 32 && (rows >> bits) != 0) ++bits;
   l.passes = std::max(1u, (bits + 7) / 8);
-  // About 2,048 waves of pieces, where there are so many tokens: long pieces have fewer runs to join. Rows of
+  // About 8,192 waves of pieces, where there are so many tokens: long pieces have fewer runs to join, short
+  // ones more loads under way (262,144 x 1,024 bf16: 256 entries 263 us a call, 128 208, 64 193). Rows of
   // dim / 8 to dim pieces of 16 bytes: counted as dim / 8 here, for every type.
   const uint64_t lanes = std::min<uint64_t>(std::max<uint64_t>(ceil_div(dim, 8), 8), 64);
   const uint64_t slabs = ceil_div(dim, 512);
   l.piece = 16;
-  while (l.piece < 256 && l.piece < 8 * lanes && ceil_div(count, 2 * l.piece) * slabs * lanes >= 2048 * 64) l.piece *= 2;
+  while (l.piece < 256 && l.piece < 8 * lanes && ceil_div(count, 2 * l.piece) * slabs * lanes >= 8192 * 64) l.piece *= 2;
   size_t at = round(static_cast<size_t>(l.parts) * kBins * 4);
   for (int i = 0; i < 2; ++i) {
     l.keys[i] = at;

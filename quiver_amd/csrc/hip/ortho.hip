@@ -187,11 +187,22 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
   const T* g = update + static_cast<uint64_t>(blockIdx.x) * count;
   T* o = out + static_cast<uint64_t>(blockIdx.x) * count;
 
+  // Rows over the waves, columns over the lanes: f(row, column) for every element, loads of four rows at once.
+  const auto each = [&](auto&& f) {
+    for (uint32_t q = lane; q < n; q += 64) {
+      for (uint32_t r0 = wave; r0 < m; r0 += 4 * WAVES) {
+        float v[4];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) v[u] = r0 + u * WAVES < m ? static_cast<float>(g[(r0 + u * WAVES) * n + q]) : 0.0f;
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+          if (r0 + u * WAVES < m) f(r0 + u * WAVES, q, v[u]);
+        }
+      }
+    }
+  };
   double sum = 0.0;
-  for (uint32_t i = threadIdx.x; i < count; i += WAVES * 64) {
-    const double v = static_cast<double>(static_cast<float>(g[i]));
-    sum += v * v;
-  }
+  each([&](uint32_t, uint32_t, float v) { sum = fma(static_cast<double>(v), static_cast<double>(v), sum); });
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
   if (lane == 0) s_sum[wave] = sum;
@@ -203,14 +214,13 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) sum += s_sum[w];
   const double factor = start_factor(sum);
-  for (uint32_t i = threadIdx.x; i < count; i += WAVES * 64) {
-    const uint32_t r = i / n, q = i - r * n;
+  each([&](uint32_t r, uint32_t q, float v) {
     half_t high, low;
-    split2(static_cast<float>(static_cast<float>(g[i]) * factor), high, low);
+    split2(static_cast<float>(v * factor), high, low);
     char* at = x + (tall ? q * sh.row_x + r * 2 : r * sh.row_x + q * 2);
     *reinterpret_cast<half_t*>(at) = high;
     *reinterpret_cast<half_t*>(at + plane_x) = low;
-  }
+  });
   __syncthreads();
 
   // 8 k of one row; rows by k.
@@ -227,11 +237,29 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
     }
     return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  const auto three = [](X8 ah, X8 al, X8 bh, X8 bl, f32x16_t acc) {
-    acc = Frag<half_t>::mfma(al, bh, acc);
-    acc = Frag<half_t>::mfma(ah, bl, acc);
-    return Frag<half_t>::mfma(ah, bh, acc);
+  // A block of a product over `slices` (an even number of) 16-deep slices: the small terms by themselves, so
+  // that the matrix instructions wait less for one another, and two slices' fragments fetched at a time.
+  const auto product_of = [](uint32_t slices, auto&& a_at, auto&& b_at) {
+    f32x16_t small{}, large{};
+    for (uint32_t kk = 0; kk < slices; kk += 2) {
+      X8 ah[2], al[2], bh[2], bl[2];
+#pragma unroll
+      for (uint32_t u = 0; u < 2; ++u) {
+        ah[u] = a_at(0, kk + u);
+        bl[u] = b_at(1, kk + u);
+        al[u] = a_at(1, kk + u);
+        bh[u] = b_at(0, kk + u);
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < 2; ++u) {
+        small = Frag<half_t>::mfma(ah[u], bl[u], small);
+        large = Frag<half_t>::mfma(ah[u], bh[u], large);
+        small = Frag<half_t>::mfma(al[u], bh[u], small);
+      }
+    }
+    return large + small;
   };
+
   // Block v of a product, transposed: lane j32 holds a row of what is stored, four neighbouring columns at a
   // time, so that the stores are of 8 bytes (as rows of the block itself they would be of two).
   const auto put = [&](char* base, uint32_t stride, uint32_t plane, uint32_t bi, uint32_t bj, const f32x16_t& v) {
@@ -260,13 +288,10 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
       const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
       if (t < sb * sb) {
         const uint32_t bi = t / sb, bj = t % sb;
-        f32x16_t acc{};
-        for (uint32_t kk = 0; kk < sh.depth / 16; ++kk) {
-          acc = three(rows(x, sh.row_x, bi * 32, kk), rows(x + plane_x, sh.row_x, bi * 32, kk), rows(x, sh.row_x, bj * 32, kk),
-                      rows(x + plane_x, sh.row_x, bj * 32, kk), acc);
-        }
-        acc *= 1.0f / kScale;
-        put(s, sh.row_s, plane_s, bi, bj, acc);
+        const f32x16_t acc = product_of(
+            sh.depth / 16, [&](uint32_t p, uint32_t kk) { return rows(x + p * plane_x, sh.row_x, bi * 32, kk); },
+            [&](uint32_t p, uint32_t kk) { return rows(x + p * plane_x, sh.row_x, bj * 32, kk); });
+        put(s, sh.row_s, plane_s, bi, bj, acc * (1.0f / kScale));
       }
     }
     __syncthreads();
@@ -277,11 +302,9 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
       const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
       if (t < sb * sb) {
         const uint32_t bi = t / sb, bj = t % sb;
-        f32x16_t acc{};
-        for (uint32_t kk = 0; kk < sh.side / 16; ++kk) {
-          acc = three(rows(s, sh.row_s, bi * 32, kk), rows(s + plane_s, sh.row_s, bi * 32, kk), rows(s, sh.row_s, bj * 32, kk),
-                      rows(s + plane_s, sh.row_s, bj * 32, kk), acc);
-        }
+        f32x16_t acc = product_of(
+            sh.side / 16, [&](uint32_t p, uint32_t kk) { return rows(s + p * plane_s, sh.row_s, bi * 32, kk); },
+            [&](uint32_t p, uint32_t kk) { return rows(s + p * plane_s, sh.row_s, bj * 32, kk); });
         const char* at = s + (bj * 32 + j32) * sh.row_s + (bi * 32 + 4 * h) * 2;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -310,12 +333,9 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
       const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
       if (t < sb * db) {
         const uint32_t bi = t / sb, bj = t % sb;  // columns of X, rows of P
-        f32x16_t acc{};
-        for (uint32_t kk = 0; kk < sh.side / 16; ++kk) {
-          acc = three(by_k(x, sh.row_x, bi * 32, kk), by_k(x + plane_x, sh.row_x, bi * 32, kk), rows(s, sh.row_s, bj * 32, kk),
-                      rows(s + plane_s, sh.row_s, bj * 32, kk), acc);
-        }
-        kept[u] = acc;
+        kept[u] = product_of(
+            sh.side / 16, [&](uint32_t p, uint32_t kk) { return by_k(x + p * plane_x, sh.row_x, bi * 32, kk); },
+            [&](uint32_t p, uint32_t kk) { return rows(s + p * plane_s, sh.row_s, bj * 32, kk); });
       }
     }
     const bool last = step + 1 == steps;
@@ -388,18 +408,33 @@ OrthoLayout ortho_layout(uint64_t batch, uint32_t m, uint32_t n) {
   return l;
 }
 
-/// Whether no step can push a singular value of [0, 1] past 3.5 or the polynomial past 15.
+/// Whether no step can push a singular value of [0, 1] past 3.5 or the polynomial past 15. On [0, top] both
+/// are largest at an end or where their derivative is zero, which for q = s^2 is a quadratic's or a
+/// line's zero.
 bool bounded(uint32_t steps, double a, double b, double c) {
   double top = 1.0;
   for (uint32_t i = 0; i < steps; ++i) {
     double next = 0.0;
-    for (int j = 0; j <= 4096; ++j) {
-      const double s = top * j / 4096, p = a + b * s * s + c * s * s * s * s;
-      if (!(std::fabs(p) <= 15.0) || !(std::fabs(b) * s * s <= 200.0)) return false;
-      next = std::max(next, std::fabs(s * p));
+    bool small = true;
+    const auto at = [&](double q) {
+      if (!(q > 0.0)) q = 0.0;
+      if (q > top * top) return;
+      const double p = a + b * q + c * q * q;
+      small = small && std::fabs(p) <= 15.0;
+      next = std::max(next, std::fabs(std::sqrt(q) * p));
+    };
+    at(0.0);
+    at(top * top);
+    if (c != 0.0) at(-b / (2.0 * c));
+    const double root = 9.0 * b * b - 20.0 * a * c;  // of a + 3 b q + 5 c q^2
+    if (c != 0.0 && root >= 0.0) {
+      at((-3.0 * b + std::sqrt(root)) / (10.0 * c));
+      at((-3.0 * b - std::sqrt(root)) / (10.0 * c));
+    } else if (c == 0.0 && b != 0.0) {
+      at(-a / (3.0 * b));
     }
-    if (!(next <= 3.5)) return false;
-    if (next <= top) return true;  // never leaves [0, top] from here on
+    if (!small || !(next <= 3.5)) return false;  // NaN coefficients among them
+    if (next <= top) return true;                // stays in [0, top] from here on
     top = next;
   }
   return true;
