@@ -25,12 +25,15 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
+/// What a lane holds of one row of a 32 x 32 block: `kEach` neighbouring k, lanes 32 .. 63 the next ones.
 template <class T>
 struct Frag;
 template <>
 struct Frag<half_t> {
   typedef half_t x8 __attribute__((ext_vector_type(8)));
   typedef half_t x4 __attribute__((ext_vector_type(4)));
+  typedef x8 type;
+  static constexpr int kEach = 8;
   static __device__ __forceinline__ f32x16_t mfma(x8 a, x8 b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
@@ -39,13 +42,28 @@ template <>
 struct Frag<bhalf_t> {
   typedef bhalf_t x8 __attribute__((ext_vector_type(8)));
   typedef bhalf_t x4 __attribute__((ext_vector_type(4)));
+  typedef x8 type;
+  static constexpr int kEach = 8;
   static __device__ __forceinline__ f32x16_t mfma(x8 a, x8 b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
 };
 
+template <>
+struct Frag<float> {
+  typedef f32x4_t type;
+  static constexpr int kEach = 4;
+  // The instruction takes one k per lane and half: four of them, each with the halves' k of one index.
+  static __device__ __forceinline__ f32x16_t mfma(f32x4_t a, f32x4_t b, f32x16_t c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
 /// One operand: element (row, k) of plane p at base[p * plane + row * ld + k], or [.. k * ld + row] where
-/// it is stored by k. 16-byte aligned, ld % 8 == 0, and the contiguous extent rounded up to 8 is readable.
+/// it is stored by k. Loaded 16 bytes at a time: base and rows 16-byte aligned, the contiguous extent rounded
+/// up to 16 bytes readable. Four bytes at a time: base, rows and the extent in whole dwords.
 struct GemmOperand {
   const void* base = nullptr;
   uint64_t ld = 0, plane = 0, batch = 0;  // in elements
@@ -190,8 +208,8 @@ struct LinearEpilogue {
   uint64_t ld_residual = 0, ld_out = 0, ld_keep = 0;
   int act = QVH_ACT_NONE;
   int vec_bias = 0, vec_residual = 0, vec_out = 0, vec_keep = 0;
-  GemmArgs direct;  // fp32: the product itself, for elements that come out as NaN
-  int a_by_k = 0, b_by_k = 0;
+  GemmArgs direct;  // fp32 by planes: the product itself, for elements that come out as NaN
+  int a_by_k = 0, b_by_k = 0, planes = 0;
 
   /// The same for one element.
   __device__ __forceinline__ void one(uint32_t m, uint32_t n, float v) const {
@@ -206,7 +224,9 @@ struct LinearEpilogue {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll 1
       for (int i = 0; i < 8; ++i) {
-        if (v[i] != v[i] && static_cast<uint32_t>(i) < left) v[i] = direct_element(direct, a_by_k, b_by_k, 3, m, n + i);
+        if (planes > 0 && v[i] != v[i] && static_cast<uint32_t>(i) < left) {
+          v[i] = direct_element(direct, a_by_k, b_by_k, planes, m, n + i);
+        }
       }
     }
     if (bias) {
@@ -248,38 +268,49 @@ struct PartialEpilogue {
 
 // ---- the kernel -------------------------------------------------------------------------------
 
-/// The 16-byte pieces of one operand's R x D step: addresses for the loads into LDS, and fragments.
-template <class T, bool BY_K, int R, int D, int WAVES>
+/// The 16-byte pieces of one operand's R x D step: addresses for the loads into LDS (WIDE bytes per lane), and
+/// fragments.
+template <class T, bool BY_K, int R, int D, int WAVES, int WIDE>
 struct Stage {
-  static constexpr int kBytes = R * D * 2;
-  static constexpr int kLoads = kBytes / 1024 / WAVES;
-  static constexpr int kChunks = BY_K ? R / 8 : D / 8;  // 16-byte pieces per line (k, or row)
-  static constexpr int kLines = 64 / kChunks;           // lines per load
-  static_assert(D == 32 || D == 64, "a row is 64 or 128 bytes in LDS");
-  static_assert(kLoads >= 1 && kBytes % (1024 * WAVES) == 0, "every wave loads whole kilobytes");
+  static constexpr int kEach = Frag<T>::kEach, kElem = sizeof(T);
+  static constexpr int kBytes = R * D * kElem;
+  static constexpr int kLoads = kBytes / (64 * WIDE) / WAVES;
+  static constexpr int kLine = (BY_K ? R : D) * kElem;  // bytes per line: a k, or a row
+  static_assert(BY_K || kLine == 64 || kLine == 128, "a row is 64 or 128 bytes in LDS");
+  static_assert(WIDE == 16 || WIDE == 4, "bytes that a lane loads");
+  static_assert(kLoads >= 1 && kBytes % (64 * WIDE * WAVES) == 0, "every wave makes whole loads");
 
   /// Piece c of a line lies at c ^ flip(line). LDS serves 256 bytes at a time, sixteen pieces: by rows, those of
   /// sixteen neighbouring rows at one k fall on different banks (two rows, or four, share 256 bytes), by k
-  /// those of the four k that a transposing read takes at once.
+  /// those of the k that one read takes.
   static __device__ __forceinline__ uint32_t flip(uint32_t line) {
-    if constexpr (BY_K) return (line & (R / 32 - 1)) * 4;
-    return D == 64 ? line >> 1 & 7 : line >> 2 & 3;
+    if constexpr (BY_K) return kElem == 4 ? (line >> 2 & 1) * 8 : (line & (R / 32 - 1)) * 4;
+    return kLine == 128 ? line >> 1 & 7 : line >> 2 & 3;
   }
 
   /// Byte offset (from the tile's first row and the step's first k) of what this lane loads in load i; the
   /// lanes fill LDS in order. `rows` and `depth`: how many of each there are from the tile's start on.
   static __device__ __forceinline__ uint32_t offset(int i, int wave, int lane, uint32_t ld, uint32_t rows, uint32_t depth) {
-    uint32_t line = static_cast<uint32_t>((i * WAVES + wave) * kLines + lane / kChunks);
-    uint32_t c = static_cast<uint32_t>(lane % kChunks) ^ flip(line);
-    const uint32_t lines = BY_K ? depth : rows, last = ((BY_K ? rows : depth) + 7) / 8 - 1;
+    const uint32_t at = static_cast<uint32_t>(((i * WAVES + wave) * 64 + lane) * WIDE);
+    uint32_t line = at / kLine;
+    const uint32_t lines = BY_K ? depth : rows, extent = (BY_K ? rows : depth) * kElem;
+    uint32_t byte = ((at % kLine / 16) ^ flip(line)) * 16 + at % 16;
     line = line < lines ? line : lines - 1;
-    c = c < last ? c : last;
-    return line * ld * 2 + c * 16;
+    const uint32_t last = WIDE == 16 ? (extent + 15) / 16 * 16 - 16 : extent - 4;
+    byte = byte < last ? byte : last;
+    return line * ld * kElem + byte;
   }
 
-  /// Fragment of rows row0 .. row0 + 31 (a multiple of 32) and k kk * 16 .. + 15.
-  static __device__ __forceinline__ typename Frag<T>::x8 fragment(const char* lds, int row0, int kk, int lane) {
-    if constexpr (BY_K) {
+  /// Fragment of rows row0 .. row0 + 31 (a multiple of 32) and slice kk of 2 kEach k.
+  static __device__ __forceinline__ typename Frag<T>::type fragment(const char* lds, int row0, int kk, int lane) {
+    if constexpr (BY_K && kElem == 4) {
+      const int k = kk * 8 + 4 * (lane >> 5), row = row0 + (lane & 31);
+      const char* at = lds + k * kLine + ((static_cast<uint32_t>(row / 4) ^ flip(static_cast<uint32_t>(k))) * 16 + row % 4 * 4);
+      f32x4_t f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = *reinterpret_cast<const float*>(at + e * kLine);
+      return f;
+    } else if constexpr (BY_K) {
       typedef typename Frag<T>::x4 x4;
       x4 part[2];
 #pragma unroll
@@ -287,7 +318,7 @@ struct Stage {
         const int p = lane & 15, j = p >> 2;
         const int k = kk * 16 + 8 * (lane >> 5) + 4 * q + j;
         const uint32_t chunk = static_cast<uint32_t>(row0 / 8 + 2 * (lane >> 4 & 1) + (p >> 1 & 1));
-        const char* at = lds + k * (R * 2) + ((chunk ^ flip(static_cast<uint32_t>(4 * q + j))) * 16 + (p & 1) * 8);
+        const char* at = lds + k * kLine + ((chunk ^ flip(static_cast<uint32_t>(4 * q + j))) * 16 + (p & 1) * 8);
         const s16x4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (__attribute__((address_space(3))) s16x4_t*)(at));
         part[q] = __builtin_bit_cast(x4, v);
@@ -295,19 +326,28 @@ struct Stage {
       return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
     } else {
       const int row = row0 + (lane & 31);
-      return *reinterpret_cast<const typename Frag<T>::x8*>(
-          lds + row * (D * 2) + (((kk * 2 + (lane >> 5)) ^ flip(static_cast<uint32_t>(lane & 31))) * 16));
+      return *reinterpret_cast<const typename Frag<T>::type*>(
+          lds + row * kLine + (((kk * 2 + (lane >> 5)) ^ flip(static_cast<uint32_t>(lane & 31))) * 16));
     }
   }
 };
 
-/// 64 lanes x 16 bytes from rsrc + offset + scalar into LDS at lds (wave-uniform), in lane order. Nothing
-/// waits for it but s_waitcnt vmcnt.
-__device__ __forceinline__ void load_to_lds(uint32_t lds, uint32_t offset, u32x4_t rsrc, uint32_t scalar) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-               :
-               : "s"(lds), "v"(offset), "s"(rsrc), "s"(scalar)
-               : "memory");
+/// 64 lanes x WIDE bytes from rsrc + offset into LDS at lds (wave-uniform), in lane order. Nothing waits for it
+/// but s_waitcnt vmcnt. The instructions in front keep the distances that the hardware asks for between a
+/// lane read or m0 and the load (the compiler does not look into the block).
+template <int WIDE>
+__device__ __forceinline__ void load_to_lds(uint32_t lds, uint32_t offset, u32x4_t rsrc) {
+  if constexpr (WIDE == 16) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds), "v"(offset), "s"(rsrc)
+                 : "memory");
+  } else {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds), "v"(offset), "s"(rsrc)
+                 : "memory");
+  }
 }
 
 __device__ __forceinline__ u32x4_t buffer_resource(const void* base) {
@@ -321,20 +361,21 @@ __device__ __forceinline__ u32x4_t buffer_resource(const void* base) {
 }
 
 /// Elements of a fragment at or past `depth` (k counted from the fragment's step) become zero.
-template <class X8>
-__device__ __forceinline__ X8 clip(X8 f, int kk, int lane, uint32_t depth) {
-  const int first = kk * 16 + 8 * (lane >> 5);
+template <int EACH, class F>
+__device__ __forceinline__ F clip(F f, int kk, int lane, uint32_t depth) {
+  const int first = (kk * 2 + (lane >> 5)) * EACH;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < EACH; ++e) {
     if (static_cast<uint32_t>(first + e) >= depth) f[e] = 0;
   }
   return f;
 }
 
-/// Tile of a work-group, its waves, the depth of a step, the steps that LDS holds, and the operands' planes.
-template <int BM_, int BN_, int WM_, int WN_, int D_, int STAGES_, int PLANES_>
+/// Tile of a work-group, its waves, the depth of a step, the steps that LDS holds, the operands' planes, and the
+/// bytes that a lane loads at a time.
+template <int BM_, int BN_, int WM_, int WN_, int D_, int STAGES_, int PLANES_, int WIDE_ = 16>
 struct Tile {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, D = D_, STAGES = STAGES_, PLANES = PLANES_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, D = D_, STAGES = STAGES_, PLANES = PLANES_, WIDE = WIDE_;
 };
 
 /// The pairs of planes whose products count, the smallest first. Two planes: all but low x low; three: those
@@ -369,8 +410,8 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
   constexpr int kPlanes = Shape::PLANES;
   using P = Pairs<kPlanes>;
   constexpr int kWaves = WM * WN;
-  using SA = Stage<T, AK, BM, kStep, kWaves>;
-  using SB = Stage<T, BK, BN, kStep, kWaves>;
+  using SA = Stage<T, AK, BM, kStep, kWaves, Shape::WIDE>;
+  using SB = Stage<T, BK, BN, kStep, kWaves, Shape::WIDE>;
   constexpr int kStageBytes = (SA::kBytes + SB::kBytes) * kPlanes;
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 blocks per wave
   constexpr int kSlabLd = BN / WN + 8;
@@ -442,12 +483,12 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
   // In LDS: the planes of a, then those of b.
   const auto load_piece = [&](int i, const Sources& s, int buf, const uint32_t(&at_a)[SA::kLoads],
                               const uint32_t(&at_b)[SB::kLoads]) {
-    const uint32_t to = lds0 + static_cast<uint32_t>(buf) * kStageBytes + (i * kWaves + wave) * 1024;
+    const uint32_t to = lds0 + static_cast<uint32_t>(buf) * kStageBytes + (i * kWaves + wave) * (64 * Shape::WIDE);
     constexpr int kOfA = SA::kLoads * kPlanes;
     if (i < kOfA) {
-      load_to_lds(to, at_a[i % SA::kLoads], s.a[i / SA::kLoads], 0);
+      load_to_lds<Shape::WIDE>(to, at_a[i % SA::kLoads], s.a[i / SA::kLoads]);
     } else {
-      load_to_lds(to, at_b[(i - kOfA) % SB::kLoads], s.b[(i - kOfA) / SB::kLoads], 0);
+      load_to_lds<Shape::WIDE>(to, at_b[(i - kOfA) % SB::kLoads], s.b[(i - kOfA) / SB::kLoads]);
     }
   };
   const auto load = [&](const Sources& s, int buf, const uint32_t(&at_a)[SA::kLoads], const uint32_t(&at_b)[SB::kLoads]) {
@@ -463,9 +504,9 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
   }
 
   const int ra0 = wm * (BM / WM), rb0 = wn * (BN / WN);
-  using X8 = typename Frag<T>::x8;
+  constexpr int kDepth = 2 * Frag<T>::kEach;  // k of a slice
   struct Fragments {
-    X8 a[kPlanes][TM], b[kPlanes][TN];
+    typename Frag<T>::type a[kPlanes][TM], b[kPlanes][TN];
   };
   const auto fetch = [&](Fragments& f, int buf, int kk) {
     const char* la = s_mem + buf * kStageBytes;
@@ -493,11 +534,11 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
     for (int x = 0; x < kOps; ++x) step_of(f, x);
   };
 
-  // Fragments are fetched one 16-deep slice ahead of their matrix instructions. The step's last slice is
+  // Fragments are fetched one slice ahead of their matrix instructions. The step's last slice is
   // in registers before its instructions start: from then on the step's place in LDS is free for the step
   // kStages on, and the next step's first slice is fetched while the last one is multiplied.
   if (first < whole_end) {
-    constexpr int kSlices = kStep / 16;
+    constexpr int kSlices = kStep / kDepth;
     Fragments f[2];
 #pragma unroll
     for (int i = 0; i < kStages; ++i) {
@@ -558,15 +599,15 @@ __global__ void __launch_bounds__(Shape::WM* Shape::WN * 64, Shape::BM* Shape::B
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 #pragma unroll 1
-    for (int kk = 0; static_cast<uint32_t>(kk * 16) < rest; ++kk) {
+    for (int kk = 0; static_cast<uint32_t>(kk * kDepth) < rest; ++kk) {
       Fragments f;
       fetch(f, 0, kk);
 #pragma unroll
       for (int p = 0; p < kPlanes; ++p) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) f.a[p][i] = clip(f.a[p][i], kk, lane, rest);
+        for (int i = 0; i < TM; ++i) f.a[p][i] = clip<Frag<T>::kEach>(f.a[p][i], kk, lane, rest);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) f.b[p][j] = clip(f.b[p][j], kk, lane, rest);
+        for (int j = 0; j < TN; ++j) f.b[p][j] = clip<Frag<T>::kEach>(f.b[p][j], kk, lane, rest);
       }
       multiply(f);
     }
@@ -682,13 +723,16 @@ __global__ void __launch_bounds__(128) gemm_join_symmetric_kernel(GemmArgs g, Ep
 
 /// Tile shape and number of splits for a product; the same for the workspace's size and for the launch.
 struct GemmPlan {
-  int tile = 0;  // which of the three shapes
+  int tile = 0;  // which of the kind's shapes
   uint32_t splits = 1;
   size_t partial_bytes = 0;
+  double us = 0.0;  // the estimate that chose them
 };
 
+enum class Kind : int;
+
 /// `symmetric`: m = n, and only the tiles on and below the diagonal are computed.
-GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, int planes, uint32_t batches, bool symmetric);
+GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, Kind kind, uint32_t batches, bool symmetric);
 
 template <class T, bool AK, bool BK, class Shape, class Epi>
 void launch_tile(GemmArgs g, const Epi& epi, hipStream_t s) {
@@ -717,43 +761,67 @@ void launch_tile(GemmArgs g, const Epi& epi, hipStream_t s) {
   QVH_HIP(hipGetLastError());
 }
 
-/// The shapes by number of planes. With more than one a step is 32 deep, so that LDS holds two or three.
-template <int PLANES>
+/// How a product reads its operands, and the shapes it may take. With more than one plane a step is 32 deep, so
+/// that LDS holds two or three.
+enum class Kind : int {
+  kPlane1 = 0,  // 16-bit operands
+  kPlane2 = 1,  // two 16-bit planes
+  kPlane3 = 2,  // three 16-bit planes
+  kFloat = 3,   // fp32 operands on fp32 matrix instructions
+  kNarrow = 4,  // 16-bit operands, loaded four bytes at a time
+  kFloatNarrow = 5
+};
+template <Kind K>
 struct Shapes;
 template <>
-struct Shapes<1> {
+struct Shapes<Kind::kPlane1> {
   using S0 = Tile<64, 64, 2, 2, 64, 2, 1>;
   using S1 = Tile<128, 128, 2, 2, 64, 2, 1>;
   using S2 = Tile<256, 256, 2, 4, 64, 2, 1>;
 };
 template <>
-struct Shapes<2> {
+struct Shapes<Kind::kPlane2> {
   using S0 = Tile<64, 64, 2, 2, 32, 3, 2>;
   using S1 = Tile<128, 128, 2, 2, 32, 2, 2>;
   using S2 = Tile<256, 128, 4, 2, 32, 3, 2>;
 };
 template <>
-struct Shapes<3> {
+struct Shapes<Kind::kPlane3> {
   using S0 = Tile<64, 64, 2, 2, 32, 2, 3>;
   using S1 = Tile<128, 128, 2, 4, 32, 3, 3>;
   using S2 = Tile<256, 128, 4, 2, 32, 2, 3>;
 };
+template <>
+struct Shapes<Kind::kFloat> {
+  using S0 = Tile<64, 64, 2, 2, 32, 3, 1>;
+  using S1 = Tile<128, 128, 2, 2, 32, 2, 1>;
+  using S2 = void;
+};
+template <>
+struct Shapes<Kind::kNarrow> {
+  using S0 = Tile<64, 64, 2, 2, 64, 2, 1, 4>;
+  using S1 = Tile<128, 128, 2, 2, 64, 2, 1, 4>;
+  using S2 = void;
+};
+template <>
+struct Shapes<Kind::kFloatNarrow> {
+  using S0 = Tile<64, 64, 2, 2, 32, 3, 1, 4>;
+  using S1 = Tile<128, 128, 2, 2, 32, 2, 1, 4>;
+  using S2 = void;
+};
 
-template <class T, int PLANES, bool AK, bool BK, class Epi>
+template <class T, Kind K, bool AK, bool BK, class Epi>
 void launch_gemm(GemmArgs g, const Epi& epi, const GemmPlan& plan, void* partial, hipStream_t s) {
   if (g.m == 0 || g.n == 0 || g.batches == 0) return;
   g.splits = plan.splits;
   g.partial = static_cast<float*>(partial);
-  if (plan.tile == 2) {
+  using S = Shapes<K>;
+  if constexpr (!std::is_void_v<typename S::S2>) {
     // A symmetric product's tiles are square.
-    if constexpr (Shapes<PLANES>::S2::BM == Shapes<PLANES>::S2::BN) {
-      return launch_tile<T, AK, BK, typename Shapes<PLANES>::S2>(g, epi, s);
-    } else if (!g.symmetric) {
-      return launch_tile<T, AK, BK, typename Shapes<PLANES>::S2>(g, epi, s);
-    }
+    if (plan.tile == 2 && (S::S2::BM == S::S2::BN || !g.symmetric)) return launch_tile<T, AK, BK, typename S::S2>(g, epi, s);
   }
-  if (plan.tile >= 1) return launch_tile<T, AK, BK, typename Shapes<PLANES>::S1>(g, epi, s);
-  launch_tile<T, AK, BK, typename Shapes<PLANES>::S0>(g, epi, s);
+  if (plan.tile >= 1) return launch_tile<T, AK, BK, typename S::S1>(g, epi, s);
+  launch_tile<T, AK, BK, typename S::S0>(g, epi, s);
 }
 
 }  // namespace qvh

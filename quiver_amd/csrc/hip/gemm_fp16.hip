@@ -3,9 +3,10 @@
 
 namespace qvh {
 
-void gemm_fp16(Form form, const GemmArgs& g, const LinearEpilogue<half_t>& e, const GemmPlan& p, void* partial,
+void gemm_fp16(Form form, Kind kind, const GemmArgs& g, const LinearEpilogue<half_t>& e, const GemmPlan& p, void* partial,
                hipStream_t s) {
-  gemm_forms<half_t, 1>(form, g, e, p, partial, s);
+  if (kind == Kind::kNarrow) return gemm_forms<half_t, Kind::kNarrow>(form, g, e, p, partial, s);
+  gemm_forms<half_t, Kind::kPlane1>(form, g, e, p, partial, s);
 }
 
 }  // namespace qvh

@@ -14,23 +14,26 @@ namespace qvh {
 // typical choices, in us: 1,024 x 1,024 x 4,096 as 64-tiles in one piece 37.2, in four 25.0, as 128-tiles in
 // one 47.1; 2,048^3 as 128-tiles 29.5, 256-tiles 51.0; 8,192 x 2,048 x 768 as 256-tiles 35.5, 128-tiles
 // 37.1, 64-tiles 51.2; 1,024 x 4,096 x 16,384 as 256-tiles in four pieces 131, 128-tiles in one 181.
-GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, int planes, uint32_t batches, bool symmetric) {
+GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, Kind kind, uint32_t batches, bool symmetric) {
   struct Cost {
     uint64_t bm, bn, together;  // tile, and work-groups that a CU holds
     double alone, shared, end;  // us per step: one work-group on a CU, each of several; prologue and epilogue
   };
-  constexpr Cost kCosts[3][3] = {
+  constexpr Cost kCosts[6][3] = {
       {{64, 64, 4, 0.45, 0.22, 2.0}, {128, 128, 2, 0.70, 0.53, 4.0}, {256, 256, 1, 1.75, 1.75, 8.0}},
       {{64, 64, 3, 0.40, 0.20, 2.0}, {128, 128, 2, 0.55, 0.45, 4.0}, {256, 128, 1, 0.95, 0.95, 6.0}},
-      {{64, 64, 3, 0.50, 0.35, 2.0}, {128, 128, 1, 0.95, 0.95, 4.0}, {256, 128, 1, 1.80, 1.80, 6.0}}};
+      {{64, 64, 3, 0.50, 0.35, 2.0}, {128, 128, 1, 0.95, 0.95, 4.0}, {256, 128, 1, 1.80, 1.80, 6.0}},
+      {{64, 64, 3, 0.55, 0.52, 2.0}, {128, 128, 2, 2.10, 2.00, 4.0}, {}},
+      {{64, 64, 4, 0.70, 0.50, 2.0}, {128, 128, 2, 1.20, 1.00, 4.0}, {}},
+      {{64, 64, 3, 0.70, 0.60, 2.0}, {128, 128, 2, 2.30, 2.10, 4.0}, {}}};
   constexpr uint32_t kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
   constexpr double kCus = 256.0;
   GemmPlan best;
   double least = -1.0;
-  const uint64_t steps = ceil_div(k, planes == 1 ? 64 : 32);
+  const uint64_t steps = ceil_div(k, kind == Kind::kPlane1 || kind == Kind::kNarrow ? 64 : 32);
   for (int t = 0; t < 3; ++t) {
-    const Cost& c = kCosts[planes - 1][t];
-    if (symmetric && c.bm != c.bn) continue;
+    const Cost& c = kCosts[static_cast<int>(kind)][t];
+    if (c.bm == 0 || (symmetric && c.bm != c.bn)) continue;
     const uint64_t tm = ceil_div(m, c.bm), tn = ceil_div(n, c.bn);
     const uint64_t tiles = (symmetric ? tm * (tm + 1) / 2 : tm * tn) * batches;
     for (const uint32_t splits : kSplits) {
@@ -50,6 +53,7 @@ GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, int planes, uint32_t batc
       }
     }
   }
+  best.us = least;
   if (best.splits > 1) best.partial_bytes = static_cast<size_t>(best.splits) * batches * m * (ceil_div(n, 8) * 8) * 4;
   return best;
 }
@@ -131,6 +135,7 @@ struct SlopeArgs {
   uint32_t cols;
   int act, vec_grad, vec_pre;
   void* dz;  // as PrepareArgs::dst, or null
+  int plain;  // dz in its own type, also where that is fp32
   uint64_t ld, plane;
   float* sums;  // [work-group][cols rounded up to 8], or null
   uint32_t rows_each;
@@ -164,7 +169,13 @@ __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
           for (int i = 0; i < 8; ++i) g[i] *= activate_slope<sizeof(T) == 4>(z[i], QVH_ACT_SILU);
         }
       }
-      if (a.dz) store_prepared<T>(a.dz, r * a.ld + c, a.plane, g);
+      if (a.dz) {
+        if (sizeof(T) == 4 && a.plain) {
+          store8(static_cast<T*>(a.dz) + r * a.ld + c, g, 8, true);  // zeros behind the last column
+        } else {
+          store_prepared<T>(a.dz, r * a.ld + c, a.plane, g);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[i] += g[i];
     }
@@ -292,8 +303,14 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_rows_kernel(const T* __res
 
 // ---- host side --------------------------------------------------------------------------------
 
-bool aligned_rows(const void* p, uint64_t stride, uint64_t cols, size_t elem) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * elem % 16 == 0 && cols * elem % 16 == 0;
+/// How the tiled products can read a matrix: 16 bytes at a time, four, or only a copy of it.
+enum class Fit { kWide, kDwords, kNot };
+
+Fit fit_of(const void* p, uint64_t stride, uint64_t cols, size_t elem) {
+  const auto whole = [&](uint64_t bytes) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * elem % bytes == 0 && cols * elem % bytes == 0;
+  };
+  return whole(16) ? Fit::kWide : whole(4) ? Fit::kDwords : Fit::kNot;
 }
 
 /// 8 elements at a time: base and stride allow 16-byte accesses.
@@ -311,35 +328,58 @@ struct Space {
   }
 };
 
-/// A matrix as an operand of the tiled product: itself where it can be read as it is, else a copy to be made.
+/// A matrix as an operand of a tiled product: itself, or a copy to be made.
 struct Prepared {
   GemmOperand op;
   PrepareArgs job;
   bool copy = false;
 };
 
-Prepared prepare_operand(const void* src, uint64_t rows, uint64_t stride, uint32_t cols, int dtype, Space& ws) {
+struct Matrix {
+  const void* p;
+  uint64_t rows, stride;
+  uint32_t cols;
+};
+
+Prepared as_it_is(const Matrix& x) {
   Prepared p;
-  if (dtype != QVH_FP32 && aligned_rows(src, stride, cols, 2)) {
-    p.op.base = src;
-    p.op.ld = stride;
-    return p;
-  }
+  p.op.base = x.p;
+  p.op.ld = x.stride;
+  return p;
+}
+
+/// Aligned rows, zeros behind the last column; fp32 in its three parts.
+Prepared copy_of(const Matrix& x, int dtype, Space& ws) {
+  Prepared p;
   p.copy = true;
-  p.job.src = src;
-  p.job.rows = rows;
-  p.job.stride = stride;
-  p.job.cols = cols;
-  p.job.ld = ceil_div(cols, 8) * 8;
-  p.job.plane = p.job.ld * rows;
+  p.job.src = x.p;
+  p.job.rows = x.rows;
+  p.job.stride = x.stride;
+  p.job.cols = x.cols;
+  p.job.ld = ceil_div(x.cols, 8) * 8;
+  p.job.plane = p.job.ld * x.rows;
   p.job.dst = ws.take(p.job.plane * (dtype == QVH_FP32 ? kPlanes : 1) * 2);
-  p.job.vec = vec8(src, stride, dtype_size(dtype));
-  p.job.blocks = static_cast<uint32_t>(ceil_div(p.job.ld / 8 * rows, 256));
+  p.job.vec = vec8(x.p, x.stride, dtype_size(dtype));
+  const uint64_t blocks = ceil_div(p.job.ld / 8 * x.rows, 256);
+  QVH_REQUIRE(blocks <= 0x3FFFFFFFu, "the matrix product is too large");
+  p.job.blocks = static_cast<uint32_t>(blocks);
   p.op.base = p.job.dst;
   p.op.ld = p.job.ld;
   p.op.plane = p.job.plane;
   return p;
 }
+
+/// us of a launch that copies `elements`.
+double copy_us(int dtype, double elements) { return 6.0 + elements * (dtype == QVH_FP32 ? 10.0 : 4.0) / 3.5e6; }
+
+/// The kind that reads both operands as they are; for 16-bit types only where both fit.
+Kind direct_kind(int dtype, Fit a, Fit b) {
+  const bool wide = a == Fit::kWide && b == Fit::kWide;
+  if (dtype == QVH_FP32) return wide ? Kind::kFloat : Kind::kFloatNarrow;
+  return wide ? Kind::kPlane1 : Kind::kNarrow;
+}
+
+Kind copied_kind(int dtype) { return dtype == QVH_FP32 ? Kind::kPlane3 : Kind::kPlane1; }
 
 void launch_prepare(int dtype, const Prepared& a, const Prepared& b, hipStream_t s) {
   const PrepareArgs none;
@@ -355,7 +395,7 @@ void launch_prepare(int dtype, const Prepared& a, const Prepared& b, hipStream_t
   QVH_HIP(hipGetLastError());
 }
 
-void run_product(Form form, int dtype, GemmArgs g, const void* bias, const void* residual, uint64_t ld_residual,
+void run_product(Form form, Kind kind, int dtype, GemmArgs g, const void* bias, const void* residual, uint64_t ld_residual,
                  void* out, uint64_t ld_out, void* keep, uint64_t ld_keep, int act, const GemmPlan& plan, void* partial,
                  hipStream_t s) {
   with_dtype(dtype, [&](auto* t) {
@@ -376,12 +416,13 @@ void run_product(Form form, int dtype, GemmArgs g, const void* bias, const void*
     e.direct = g;
     e.a_by_k = form == Form::kKK;
     e.b_by_k = form != Form::kRowsRows;
+    e.planes = kind == Kind::kPlane3 ? kPlanes : 0;
     if constexpr (std::is_same_v<T, float>) {
-      gemm_fp32(form, g, e, plan, partial, s);
+      gemm_fp32(form, kind, g, e, plan, partial, s);
     } else if constexpr (std::is_same_v<T, half_t>) {
-      gemm_fp16(form, g, e, plan, partial, s);
+      gemm_fp16(form, kind, g, e, plan, partial, s);
     } else {
-      gemm_bf16(form, g, e, plan, partial, s);
+      gemm_bf16(form, kind, g, e, plan, partial, s);
     }
   });
 }
@@ -402,12 +443,15 @@ void check_matrix(const std::string& w, const char* name, const void* p, uint64_
 
 struct LinearRun {
   bool few = false;
+  Kind kind = Kind::kPlane1;
   Prepared x, w;
   GemmPlan plan;
   void* partial = nullptr;
   size_t bytes = 0;
 };
 
+// fp32: the fp32 matrix instructions read the operands as they are; the bf16 ones, sixteen times as fast, need
+// copies in three parts and then six products.
 LinearRun plan_linear(const qvh_linear_args& a, void* ws) {
   LinearRun r;
   if (a.m == 0 || a.n == 0) return r;
@@ -415,9 +459,26 @@ LinearRun plan_linear(const qvh_linear_args& a, void* ws) {
   if (r.few) return r;
   Space sp;
   sp.base = static_cast<char*>(ws);
-  r.x = prepare_operand(a.x, a.m, a.x_stride, a.k, a.dtype, sp);
-  r.w = prepare_operand(a.weight, a.n, a.weight_stride, a.k, a.dtype, sp);
-  r.plan = gemm_plan(a.m, a.n, a.k, a.dtype == QVH_FP32 ? kPlanes : 1, 1, false);
+  const size_t e = dtype_size(a.dtype);
+  const Matrix x{a.x, a.m, a.x_stride, a.k}, w{a.weight, a.n, a.weight_stride, a.k};
+  const Fit fx = fit_of(a.x, a.x_stride, a.k, e), fw = fit_of(a.weight, a.weight_stride, a.k, e);
+  const bool all = a.dtype == QVH_FP32;  // copies are made of everything, in parts
+  const bool copy_x = all || fx != Fit::kWide, copy_w = all || fw != Fit::kWide;
+  r.kind = copied_kind(a.dtype);
+  r.plan = gemm_plan(a.m, a.n, a.k, r.kind, 1, false);
+  bool copies = copy_x || copy_w;
+  if (copies && (all || (fx != Fit::kNot && fw != Fit::kNot))) {
+    const double elements = (copy_x ? static_cast<double>(a.m) * a.k : 0.0) + (copy_w ? static_cast<double>(a.n) * a.k : 0.0);
+    const Kind direct = direct_kind(a.dtype, fx, fw);
+    const GemmPlan p = gemm_plan(a.m, a.n, a.k, direct, 1, false);
+    if (p.us < r.plan.us + copy_us(a.dtype, elements)) {
+      copies = false;
+      r.kind = direct;
+      r.plan = p;
+    }
+  }
+  r.x = copies && copy_x ? copy_of(x, a.dtype, sp) : as_it_is(x);
+  r.w = copies && copy_w ? copy_of(w, a.dtype, sp) : as_it_is(w);
   r.partial = sp.take(r.plan.partial_bytes);
   r.bytes = sp.at;
   return r;
@@ -469,6 +530,7 @@ struct GradRun {
   uint32_t sum_parts = 0;
   GemmOperand dz;
   Prepared x, w;
+  Kind kind_x = Kind::kPlane1, kind_w = Kind::kPlane1;
   GemmPlan plan_x, plan_w;
   void *partial_x = nullptr, *partial_w = nullptr;
   size_t bytes = 0;
@@ -478,12 +540,32 @@ GradRun plan_grad(const qvh_linear_grad_args& a, void* ws) {
   GradRun r;
   if (a.n == 0 || (a.m == 0 && a.k == 0)) return r;
   const size_t e = dtype_size(a.dtype);
-  const int planes = a.dtype == QVH_FP32 ? kPlanes : 1;
   Space sp;
   sp.base = static_cast<char*>(ws);
-  const bool products = (a.grad_x || a.grad_weight) && a.k > 0;
-  const bool as_is = a.activation == QVH_ACT_NONE && a.dtype != QVH_FP32 && aligned_rows(a.grad, a.grad_stride, a.n, 2);
-  r.slope = (products && !as_is) || a.grad_bias;
+  const bool of_x = a.grad_x && a.k > 0, of_w = a.grad_weight && a.k > 0;
+  const bool fp32 = a.dtype == QVH_FP32;
+  const Matrix x{a.x, a.m, a.x_stride, a.k}, w{a.weight, a.n, a.weight_stride, a.k};
+  const Fit fx = fit_of(a.x, a.x_stride, a.k, e), fw = fit_of(a.weight, a.weight_stride, a.k, e);
+
+  // fp32: both products on fp32 instructions, or both on parts. dz is grad itself where there is no
+  // activation and the products can read it.
+  bool parts = false;
+  if (fp32 && (of_x || of_w)) {
+    double direct = 0.0, split = copy_us(a.dtype, static_cast<double>(a.m) * a.n);
+    if (of_x) {
+      direct += gemm_plan(a.m, a.k, a.n, direct_kind(a.dtype, Fit::kWide, fw), 1, false).us;
+      split += gemm_plan(a.m, a.k, a.n, Kind::kPlane3, 1, false).us + static_cast<double>(a.n) * a.k * 10.0 / 3.5e6;
+    }
+    if (of_w) {
+      direct += gemm_plan(a.n, a.k, a.m, direct_kind(a.dtype, Fit::kWide, fx), 1, false).us;
+      split += gemm_plan(a.n, a.k, a.m, Kind::kPlane3, 1, false).us + static_cast<double>(a.m) * a.k * 10.0 / 3.5e6;
+    }
+    parts = split < direct;
+  }
+  Fit fz = fit_of(a.grad, a.grad_stride, a.n, e);
+  const bool as_is = a.activation == QVH_ACT_NONE && !parts && (fz == Fit::kWide || (fp32 && fz == Fit::kDwords));
+  const bool writes = (of_x || of_w) && !as_is;
+  r.slope = writes || a.grad_bias;
   if (r.slope) {
     SlopeArgs& j = r.job;
     j.grad = a.grad;
@@ -497,33 +579,49 @@ GradRun plan_grad(const qvh_linear_grad_args& a, void* ws) {
     j.vec_pre = vec8(a.preactivation, a.preactivation_stride, e);
     j.ld = ceil_div(a.n, 8) * 8;
     j.plane = j.ld * a.m;
-    if (products && !as_is) j.dz = sp.take(j.plane * (a.dtype == QVH_FP32 ? kPlanes : 1) * 2);
+    j.plain = !parts;
+    if (writes) j.dz = sp.take(j.plane * (parts ? kPlanes * 2 : e));
     // Work-groups of 256 columns; rows spread over about a thousand of them, at least 16 rows each.
     const uint64_t across = ceil_div(a.n, 256);
     j.rows_each = static_cast<uint32_t>(std::max<uint64_t>(16, ceil_div(ceil_div(a.m, 8), ceil_div(1024, across)) * 8));
     r.sum_parts = static_cast<uint32_t>(ceil_div(a.m, j.rows_each));
     if (a.grad_bias) j.sums = static_cast<float*>(sp.take(static_cast<size_t>(r.sum_parts) * j.ld * 4));
-    r.dz.base = j.dz;
-    r.dz.ld = j.ld;
-    r.dz.plane = j.plane;
   }
-  if (as_is) {
+  if (writes) {
+    r.dz.base = r.job.dz;
+    r.dz.ld = r.job.ld;
+    r.dz.plane = r.job.plane;
+    fz = Fit::kWide;
+  } else {
     r.dz.base = a.grad;
     r.dz.ld = a.grad_stride;
-    r.dz.plane = 0;
   }
-  if (products) {
-    if (a.grad_x) {
-      r.w = prepare_operand(a.weight, a.n, a.weight_stride, a.k, a.dtype, sp);
-      r.plan_x = gemm_plan(a.m, a.k, a.n, planes, 1, false);
-      r.partial_x = sp.take(r.plan_x.partial_bytes);
+  const auto product = [&](const Matrix& other, Fit fit, uint64_t m, uint64_t depth, Prepared& prepared, Kind& kind,
+                           GemmPlan& plan, void*& partial) {
+    if (parts) {
+      kind = Kind::kPlane3;
+      plan = gemm_plan(m, a.k, depth, kind, 1, false);
+      prepared = copy_of(other, a.dtype, sp);
+    } else if (fp32 || (fit == Fit::kWide && fz == Fit::kWide)) {
+      kind = direct_kind(a.dtype, fz, fit);
+      plan = gemm_plan(m, a.k, depth, kind, 1, false);
+      prepared = as_it_is(other);
+    } else {  // 16-bit: dz is wide by now
+      kind = Kind::kPlane1;
+      plan = gemm_plan(m, a.k, depth, kind, 1, false);
+      prepared = as_it_is(other);
+      const GemmPlan narrow = gemm_plan(m, a.k, depth, Kind::kNarrow, 1, false);
+      if (fit == Fit::kDwords && narrow.us < plan.us + copy_us(a.dtype, static_cast<double>(other.rows) * other.cols)) {
+        kind = Kind::kNarrow;
+        plan = narrow;
+      } else {
+        prepared = copy_of(other, a.dtype, sp);
+      }
     }
-    if (a.grad_weight) {
-      r.x = prepare_operand(a.x, a.m, a.x_stride, a.k, a.dtype, sp);
-      r.plan_w = gemm_plan(a.n, a.k, a.m, planes, 1, false);
-      r.partial_w = sp.take(r.plan_w.partial_bytes);
-    }
-  }
+    partial = sp.take(plan.partial_bytes);
+  };
+  if (of_x) product(w, fw, a.m, a.n, r.w, r.kind_x, r.plan_x, r.partial_x);
+  if (of_w) product(x, fx, a.n, a.m, r.x, r.kind_w, r.plan_w, r.partial_w);
   r.bytes = sp.at;
   return r;
 }
@@ -589,7 +687,7 @@ qvh_status qvh_linear_device(const qvh_linear_args* args, void* d_workspace, uin
     g.m = static_cast<uint32_t>(a.m);
     g.n = a.n;
     g.k = a.k;
-    run_product(Form::kRowsRows, a.dtype, g, a.bias, a.residual, a.residual_stride, a.out, a.out_stride, a.preactivation,
+    run_product(Form::kRowsRows, r.kind, a.dtype, g, a.bias, a.residual, a.residual_stride, a.out, a.out_stride, a.preactivation,
                 a.preactivation_stride, a.activation, r.plan, r.partial, s);
   });
 }
@@ -637,7 +735,7 @@ qvh_status qvh_linear_grad_device(const qvh_linear_grad_args* args, void* d_work
       g.m = static_cast<uint32_t>(a.m);
       g.n = a.k;
       g.k = a.n;
-      run_product(Form::kRowsK, a.dtype, g, nullptr, nullptr, 0, a.grad_x, a.grad_x_stride, nullptr, 0, QVH_ACT_NONE,
+      run_product(Form::kRowsK, r.kind_x, a.dtype, g, nullptr, nullptr, 0, a.grad_x, a.grad_x_stride, nullptr, 0, QVH_ACT_NONE,
                   r.plan_x, r.partial_x, s);
     }
     if (a.grad_weight && a.n > 0) {
@@ -645,7 +743,7 @@ qvh_status qvh_linear_grad_device(const qvh_linear_grad_args* args, void* d_work
       g.m = a.n;
       g.n = a.k;
       g.k = static_cast<uint32_t>(a.m);
-      run_product(Form::kKK, a.dtype, g, nullptr, nullptr, 0, a.grad_weight, a.grad_weight_stride, nullptr, 0, QVH_ACT_NONE,
+      run_product(Form::kKK, r.kind_w, a.dtype, g, nullptr, nullptr, 0, a.grad_weight, a.grad_weight_stride, nullptr, 0, QVH_ACT_NONE,
                   r.plan_w, r.partial_w, s);
     }
   });

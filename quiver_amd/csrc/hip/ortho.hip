@@ -391,9 +391,9 @@ OrthoLayout ortho_layout(uint64_t batch, uint32_t m, uint32_t n) {
   l.plane_x = l.ldx * m;
   l.plane_s = l.lds * l.side;
   const uint32_t b = static_cast<uint32_t>(batch);
-  l.gram = gemm_plan(l.side, l.side, std::max(m, n), 2, b, true);
-  l.square = gemm_plan(l.side, l.side, l.side, 2, b, true);
-  l.update = gemm_plan(m, n, l.side, 2, b, false);
+  l.gram = gemm_plan(l.side, l.side, std::max(m, n), Kind::kPlane2, b, true);
+  l.square = gemm_plan(l.side, l.side, l.side, Kind::kPlane2, b, true);
+  l.update = gemm_plan(m, n, l.side, Kind::kPlane2, b, false);
   size_t at = round(batch * kNormParts * 8);
   for (size_t& x : l.x) {
     x = at;
@@ -516,22 +516,22 @@ void orthogonalize(const T* update, uint64_t batch, uint32_t m, uint32_t n, uint
     g1.symmetric = 1;
     const PartsEpilogue e1{gram, nullptr, l.lds, l.plane_s, 1.0f / kScale, 0.0f, 0.0f};
     if (tall) {
-      launch_gemm<half_t, 2, true, true>(g1, e1, l.gram, partial, s);
+      launch_gemm<half_t, Kind::kPlane2, true, true>(g1, e1, l.gram, partial, s);
     } else {
-      launch_gemm<half_t, 2, false, false>(g1, e1, l.gram, partial, s);
+      launch_gemm<half_t, Kind::kPlane2, false, false>(g1, e1, l.gram, partial, s);
     }
     GemmArgs g2 = product(gram, l.lds, l.plane_s, gram, l.lds, l.plane_s, l.side, l.side, l.side, batch);
     g2.symmetric = 1;
     const PartsEpilogue e2{poly, gram, l.lds, l.plane_s, c / kScale, a * kScale, b};
-    launch_gemm<half_t, 2, false, false>(g2, e2, l.square, partial, s);
+    launch_gemm<half_t, Kind::kPlane2, false, false>(g2, e2, l.square, partial, s);
     // P is symmetric: it may be read by rows on either side.
     const GemmArgs g3 = tall ? product(cur, l.ldx, l.plane_x, poly, l.lds, l.plane_s, m, n, l.side, batch)
                              : product(poly, l.lds, l.plane_s, cur, l.ldx, l.plane_x, m, n, l.side, batch);
     const auto third = [&](const auto& e) {
       if (tall) {
-        launch_gemm<half_t, 2, false, false>(g3, e, l.update, partial, s);
+        launch_gemm<half_t, Kind::kPlane2, false, false>(g3, e, l.update, partial, s);
       } else {
-        launch_gemm<half_t, 2, false, true>(g3, e, l.update, partial, s);
+        launch_gemm<half_t, Kind::kPlane2, false, true>(g3, e, l.update, partial, s);
       }
     };
     if (i + 1 < steps) {

@@ -27,11 +27,12 @@ _MAX_STRIDE = 1 << 22
 
 _torch = None
 _dtypes = {}
+_raw_stream = None
 
 
 def _load_torch():
     """torch, once it is known to share this library's HIP runtime."""
-    global _torch
+    global _torch, _raw_stream
     if _torch is None:
         import torch
 
@@ -41,6 +42,8 @@ def _load_torch():
                              f"({', '.join(sorted(runtimes))}), so device tensors cannot be shared: "
                              "import torch before quiver_amd")
         _dtypes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        # The current stream's handle alone; torch.cuda.current_stream makes an object of it, at 2 us a call.
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         _torch = torch
     return _torch
 
@@ -98,6 +101,8 @@ def _activation(name) -> int:
 
 
 def _stream(device) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(device.index)
     return _torch.cuda.current_stream(device).cuda_stream
 
 
