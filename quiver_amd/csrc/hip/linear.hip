@@ -23,9 +23,9 @@ GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, Kind kind, uint32_t batch
       {{64, 64, 4, 0.45, 0.22, 2.0}, {128, 128, 2, 0.70, 0.53, 4.0}, {256, 256, 1, 1.75, 1.75, 8.0}},
       {{64, 64, 3, 0.40, 0.20, 2.0}, {128, 128, 2, 0.55, 0.45, 4.0}, {256, 128, 1, 0.95, 0.95, 6.0}},
       {{64, 64, 3, 0.50, 0.35, 2.0}, {128, 128, 1, 0.95, 0.95, 4.0}, {256, 128, 1, 1.80, 1.80, 6.0}},
-      {{64, 64, 3, 0.55, 0.52, 2.0}, {128, 128, 2, 2.10, 2.00, 4.0}, {}},
-      {{64, 64, 4, 0.70, 0.50, 2.0}, {128, 128, 2, 1.20, 1.00, 4.0}, {}},
-      {{64, 64, 3, 0.70, 0.60, 2.0}, {128, 128, 2, 2.30, 2.10, 4.0}, {}}};
+      {{64, 64, 3, 0.70, 0.52, 2.0}, {128, 128, 2, 2.10, 2.00, 4.0}, {}},
+      {{64, 64, 4, 0.56, 0.35, 2.0}, {128, 128, 2, 1.05, 0.75, 4.0}, {}},
+      {{64, 64, 3, 0.90, 0.62, 2.0}, {128, 128, 2, 2.40, 2.10, 4.0}, {}}};
   constexpr uint32_t kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
   constexpr double kCus = 256.0;
   GemmPlan best;
@@ -451,7 +451,9 @@ struct LinearRun {
 };
 
 // fp32: the fp32 matrix instructions read the operands as they are; the bf16 ones, sixteen times as fast, need
-// copies in three parts and then six products.
+// copies in three parts and then six products. Both sides, copies included, in us: 512^3 12 and 22, 1,024^3 28
+// and 41, 2,048^3 140 and 112, 10,000 x 768 x 768 114 and 92. 16-bit rows that are whole dwords but not whole
+// 16-byte pieces, read as they are and copied: 1,003 x 98 x 384 5.2 and 8.1, 2,048^2 x 2,046 39 and 45.
 LinearRun plan_linear(const qvh_linear_args& a, void* ws) {
   LinearRun r;
   if (a.m == 0 || a.n == 0) return r;
