@@ -23,17 +23,17 @@ constexpr uint32_t kMaxDim = 32768;
 
 // ---- lookup -----------------------------------------------------------------------------------
 
-/// Chunk c of the output is V elements; U chunks per thread, 256 apart, so that each thread has U
-/// independent row reads in flight.
+/// Piece c of a row is V elements (vector_width), cpr pieces a row; U pieces per thread, 256 apart, so that each
+/// thread has U independent row reads in flight.
 template <class T, int V, class I, int U>
 __global__ void __launch_bounds__(256) embed_kernel(const T* __restrict__ table, uint64_t rows, uint64_t stride,
-                                                    const I* __restrict__ tokens, uint64_t count, uint32_t cpr,
-                                                    uint32_t magic, float scale, T* __restrict__ out) {
+                                                    const I* __restrict__ tokens, uint64_t count, uint32_t dim,
+                                                    uint32_t cpr, uint32_t magic, float scale, T* __restrict__ out) {
   const uint64_t first = static_cast<uint64_t>(blockIdx.x) * (256 * U);
   const uint64_t t0 = first / cpr;
   const uint32_t lead = static_cast<uint32_t>(first - t0 * cpr);
   const uint64_t total = count * cpr;
-  uint64_t at[U];
+  uint64_t at[U], row[U];
   uint32_t col[U];
   int64_t tok[U];
 #pragma unroll
@@ -42,7 +42,9 @@ __global__ void __launch_bounds__(256) embed_kernel(const T* __restrict__ table,
     const uint32_t i = lead + u * 256 + threadIdx.x;
     const uint32_t q = cpr == 1 ? i : __umulhi(i, magic);
     at[u] = first + u * 256 + threadIdx.x;
+    row[u] = t0 + q;
     col[u] = (i - q * cpr) * V;
+    col[u] = col[u] < dim - V ? col[u] : dim - V;
     tok[u] = at[u] < total ? static_cast<int64_t>(tokens[t0 + q]) : -1;
   }
   float x[U][V];
@@ -59,16 +61,16 @@ __global__ void __launch_bounds__(256) embed_kernel(const T* __restrict__ table,
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (at[u] < total) store_floats<T, V>(out + at[u] * V, x[u]);
+    if (at[u] < total) store_floats<T, V>(out + row[u] * dim + col[u], x[u]);
   }
 }
 
 template <class T, class I>
 void launch_embed(const void* table, uint64_t rows, uint32_t dim, uint64_t stride, const void* tokens, uint64_t count,
                   float scale, void* out, hipStream_t s) {
-  with_width<T>(vector_width(sizeof(T), {dim, stride}, {table, out}), [&](auto width) {
+  with_width<T>(vector_width(sizeof(T), dim), [&](auto width) {
     constexpr int V = decltype(width)::value;
-    const uint32_t cpr = dim / V;
+    const uint32_t cpr = static_cast<uint32_t>(ceil_div(dim, V));
     const uint32_t magic = cpr == 1 ? 0u : static_cast<uint32_t>((uint64_t{1} << 32) / cpr + 1);
     const uint64_t total = count * cpr;
     const auto go = [&](auto unroll) {
@@ -76,7 +78,7 @@ void launch_embed(const void* table, uint64_t rows, uint32_t dim, uint64_t strid
       const uint64_t blocks = ceil_div(total, 256 * U);
       QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "qvh_embed_device: too many tokens");
       hipLaunchKernelGGL((embed_kernel<T, V, I, U>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s,
-                         static_cast<const T*>(table), rows, stride, static_cast<const I*>(tokens), count, cpr, magic,
+                         static_cast<const T*>(table), rows, stride, static_cast<const I*>(tokens), count, dim, cpr, magic,
                          scale, static_cast<T*>(out));
     };
     if (total < 256 * 1024) {
@@ -138,8 +140,9 @@ __global__ void __launch_bounds__(256) embed_grad_own_kernel(const T* __restrict
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     for (uint32_t c0 = 0; c0 < dim; c0 += G * V) {
-      const uint32_t c = c0 + lane % G * V;
+      uint32_t c = c0 + lane % G * V;
       const bool in = c < dim;
+      c = c < dim - V ? c : dim - V;
       float acc[V] = {};
       for (uint32_t j0 = 0; j0 < n; j0 += kShares * kAhead) {
         float x[kAhead][V];
@@ -347,8 +350,8 @@ __device__ __forceinline__ void zero_rows(const SumArgs& a, uint32_t block, uint
   const float zero[V] = {};
   T* out = static_cast<T*>(a.out) + r0 * a.dim;
   for (uint32_t i = threadIdx.x; i < kZeroRows * a.cpr; i += 256) {
-    const uint32_t row = i / a.cpr;
-    if (!s_flag[row]) store_floats<T, V>(out + static_cast<uint64_t>(i) * V, zero);
+    const uint32_t row = i / a.cpr, c = (i - row * a.cpr) * V;
+    if (!s_flag[row]) store_floats<T, V>(out + static_cast<uint64_t>(row) * a.dim + (c < a.dim - V ? c : a.dim - V), zero);
   }
 }
 
@@ -374,8 +377,9 @@ __global__ void __launch_bounds__(256) embed_grad_sum_kernel(SumArgs a) {
   const uint32_t group = threadIdx.x / G;
   const uint64_t piece = static_cast<uint64_t>(blockIdx.x) * kGroups + group;
   const uint64_t e0 = piece * length;
-  const uint32_t col = (blockIdx.y * G + threadIdx.x % G) * V;
+  uint32_t col = (blockIdx.y * G + threadIdx.x % G) * V;
   if (e0 >= a.count || col >= a.dim) return;
+  col = col < a.dim - V ? col : a.dim - V;
   const uint32_t n = a.count - e0 < length ? static_cast<uint32_t>(a.count - e0) : length;
   const uint32_t* key = s_key + group * length;
   const uint32_t* pos = s_pos + group * length;
@@ -452,9 +456,11 @@ __global__ void __launch_bounds__(256) embed_grad_join_kernel(SumArgs a) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t share = (n + 3) / 4;
   const uint32_t p0 = wave * share < n ? wave * share : n, p1 = p0 + share < n ? p0 + share : n;
-  const uint32_t c = (blockIdx.y * 64 + lane) * W;
+  uint32_t c = (blockIdx.y * 64 + lane) * W;
+  const bool in = c < a.dim;
+  c = c < a.dim - W ? c : a.dim - W;
   float acc[W] = {};
-  if (c < a.dim) {
+  if (in) {
 #pragma unroll 8
     for (uint32_t p = p0; p < p1; ++p) {
       float x[W];
@@ -466,15 +472,13 @@ __global__ void __launch_bounds__(256) embed_grad_join_kernel(SumArgs a) {
 #pragma unroll
   for (int k = 0; k < W; ++k) s_sum[wave][lane * W + k] = acc[k];
   __syncthreads();
-  if (wave == 0 && c < a.dim) {
+  if (wave == 0 && in) {
 #pragma unroll
     for (int k = 0; k < W; ++k) {
       const uint32_t i = lane * W + k;
       acc[k] = (((s_sum[0][i] + s_sum[1][i]) + s_sum[2][i]) + s_sum[3][i]) * a.scale;
     }
-    T* to = static_cast<T*>(a.out) + static_cast<uint64_t>(cur) * a.dim + c;
-#pragma unroll
-    for (int k = 0; k < W; ++k) to[k] = static_cast<T>(acc[k]);
+    store_floats<T, W>(static_cast<T*>(a.out) + static_cast<uint64_t>(cur) * a.dim + c, acc);
   }
 }
 
@@ -515,7 +519,7 @@ GradLayout grad_layout(uint64_t rows, uint32_t dim, uint64_t count) {
 template <class T, class I>
 void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, uint64_t count, uint64_t rows,
                        uint32_t dim, float scale, void* out, char* ws, hipStream_t s) {
-  const int width = vector_width(sizeof(T), {dim, stride}, {grad, out});
+  const int width = vector_width(sizeof(T), dim);
   if (count <= kOwnTokens) {
     // As few rows per wave as the device holds waves for at once: a wave's rows follow one another, each
     // waiting for its gradient rows (10,000 rows, 1,000 tokens of 128 fp32: four rows 13 us, two 11).
@@ -531,9 +535,9 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
                            static_cast<uint32_t>(count), static_cast<uint32_t>(rows), dim, own, scale,
                            static_cast<T*>(out));
       };
-      if (dim / V <= 16) {
+      if (ceil_div(dim, V) <= 16) {
         go(std::integral_constant<int, 16>{});
-      } else if (dim / V <= 32) {
+      } else if (ceil_div(dim, V) <= 32) {
         go(std::integral_constant<int, 32>{});
       } else {
         go(std::integral_constant<int, 64>{});
@@ -582,7 +586,7 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
     a.partial = reinterpret_cast<float*>(ws + l.partial);
     a.piece = l.piece;
     a.pieces = static_cast<uint32_t>(ceil_div(count, l.piece));
-    a.cpr = dim / V;
+    a.cpr = static_cast<uint32_t>(ceil_div(dim, V));
     const uint32_t zero_blocks = static_cast<uint32_t>(ceil_div(rows, kZeroRows));
     const auto sum = [&](auto group) {
       constexpr int G = decltype(group)::value;
@@ -602,7 +606,7 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
     }
     QVH_HIP(hipGetLastError());
     if (a.pieces > 1) {
-      if (dim % 4 == 0) {
+      if (dim >= 4) {
         hipLaunchKernelGGL((embed_grad_join_kernel<T, 4>), dim3(a.pieces, ceil_div(dim, 256)), dim3(256), 0, s, a);
       } else {
         hipLaunchKernelGGL((embed_grad_join_kernel<T, 1>), dim3(a.pieces, ceil_div(dim, 64)), dim3(256), 0, s, a);
@@ -632,6 +636,9 @@ qvh_status qvh_embed_device(const void* d_table, uint64_t rows, uint32_t dim, ui
   return qvh::guarded([&] {
     using namespace qvh;
     check_embed("qvh_embed_device", rows, dim, dtype, index_bytes, count);
+    QVH_REQUIRE(reinterpret_cast<uintptr_t>(d_table) % dtype_size(dtype) == 0 && reinterpret_cast<uintptr_t>(d_out) % dtype_size(dtype) == 0 &&
+                    reinterpret_cast<uintptr_t>(d_tokens) % index_bytes == 0,
+                "qvh_embed_device: a buffer is not aligned to its element type");
     QVH_REQUIRE(row_stride >= dim || rows <= 1, "qvh_embed_device: the row stride must be at least dim");
     if (count == 0) return;
     QVH_REQUIRE((d_table || rows == 0) && d_tokens && d_out, "qvh_embed_device: null buffer");
@@ -663,6 +670,9 @@ qvh_status qvh_embed_grad_device(const void* d_grad, uint64_t row_stride, const 
   return qvh::guarded([&] {
     using namespace qvh;
     check_embed("qvh_embed_grad_device", rows, dim, dtype, index_bytes, count);
+    QVH_REQUIRE(reinterpret_cast<uintptr_t>(d_grad) % dtype_size(dtype) == 0 && reinterpret_cast<uintptr_t>(d_out) % dtype_size(dtype) == 0 &&
+                    reinterpret_cast<uintptr_t>(d_tokens) % index_bytes == 0,
+                "qvh_embed_grad_device: a buffer is not aligned to its element type");
     QVH_REQUIRE(row_stride >= dim || count <= 1, "qvh_embed_grad_device: the row stride must be at least dim");
     if (rows == 0) return;
     QVH_REQUIRE(((d_grad && d_tokens) || count == 0) && d_out, "qvh_embed_grad_device: null buffer");

@@ -139,10 +139,10 @@ __device__ __forceinline__ RowChunk row_and_chunk(uint32_t block, uint32_t per_r
   return {r, static_cast<uint32_t>(i - r * per_row)};
 }
 
-/// Eight values as vector stores where the row is aligned and whole, else one by one.
+/// Eight values as vector accesses, or those of them that the row still has one by one.
 template <class T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8], uint32_t left, bool vec) {
-  if (vec && left >= 8) {
+__device__ __forceinline__ void store8(T* p, const float (&v)[8], uint32_t left) {
+  if (left >= 8) {
     if constexpr (sizeof(T) == 2) {
       store_floats<T, 8>(p, v);
     } else {
@@ -159,8 +159,8 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], uint32_t left,
 }
 
 template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8], uint32_t left, bool vec) {
-  if (vec && left >= 8) {
+__device__ __forceinline__ void load8(const T* p, float (&v)[8], uint32_t left) {
+  if (left >= 8) {
     if constexpr (sizeof(T) == 2) {
       load_floats<T, 8>(p, v);
     } else {
@@ -207,7 +207,6 @@ struct LinearEpilogue {
   T* keep = nullptr;
   uint64_t ld_residual = 0, ld_out = 0, ld_keep = 0;
   int act = QVH_ACT_NONE;
-  int vec_bias = 0, vec_residual = 0, vec_out = 0, vec_keep = 0;
   GemmArgs direct;  // fp32 by planes: the product itself, for elements that come out as NaN
   int a_by_k = 0, b_by_k = 0, planes = 0;
 
@@ -231,11 +230,11 @@ struct LinearEpilogue {
     }
     if (bias) {
       float b[8];
-      load8(bias + n, b, left, vec_bias);
+      load8(bias + n, b, left);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += b[i];
     }
-    if (keep) store8(keep + m * ld_keep + n, v, left, vec_keep);
+    if (keep) store8(keep + m * ld_keep + n, v, left);
     if (act == QVH_ACT_RELU) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = activate<sizeof(T) == 4>(v[i], QVH_ACT_RELU);
@@ -248,11 +247,11 @@ struct LinearEpilogue {
     }
     if (residual) {
       float r[8];
-      load8(residual + m * ld_residual + n, r, left, vec_residual);
+      load8(residual + m * ld_residual + n, r, left);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += r[i];
     }
-    store8(out + m * ld_out + n, v, left, vec_out);
+    store8(out + m * ld_out + n, v, left);
   }
 };
 
@@ -261,8 +260,7 @@ struct PartialEpilogue {
   float* out;
   uint64_t ld, batch;
   __device__ __forceinline__ void operator()(uint32_t z, uint32_t m, uint32_t n, uint32_t, float (&v)[8]) const {
-    const uint32_t whole = 8;
-    store8(out + z * batch + m * ld + n, v, whole, true);
+    store8(out + z * batch + m * ld + n, v, 8);
   }
 };
 
@@ -663,7 +661,7 @@ __device__ __forceinline__ void add_splits(const float* p, uint32_t splits, uint
   for (; s + 4 <= splits; s += 4, p += 4 * step) {  // four loads under way at a time
     float x[4][8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load8(p + u * step, x[u], 8, true);
+    for (int u = 0; u < 4; ++u) load8(p + u * step, x[u], 8);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
 #pragma unroll
@@ -672,7 +670,7 @@ __device__ __forceinline__ void add_splits(const float* p, uint32_t splits, uint
   }
   for (; s < splits; ++s, p += step) {
     float x[8];
-    load8(p, x, 8, true);
+    load8(p, x, 8);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += x[e];
   }
@@ -775,7 +773,7 @@ template <Kind K>
 struct Shapes;
 template <>
 struct Shapes<Kind::kPlane1> {
-  using S0 = Tile<64, 64, 2, 2, 64, 2, 1>;
+  using S0 = Tile<64, 64, 2, 2, 64, 3, 1>;
   using S1 = Tile<128, 128, 2, 2, 64, 2, 1>;
   using S2 = Tile<256, 256, 2, 4, 64, 2, 1>;
 };

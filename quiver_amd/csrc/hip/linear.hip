@@ -74,7 +74,6 @@ struct PrepareArgs {
   void* dst = nullptr;  // [planes][rows][ld], ld = cols rounded up to 8, zeros behind the columns
   uint64_t ld = 0, plane = 0;
   uint32_t blocks = 0;
-  int vec = 0;
 };
 
 /// The three bf16 parts of an fp32 value, each the rounding of what the ones before it leave: their sum is
@@ -122,7 +121,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(PrepareArgs a, PrepareArgs
   if (r >= p.rows) return;
   const uint32_t c = chunk * 8;
   float v[8];
-  load8(static_cast<const T*>(p.src) + r * p.stride + c, v, p.cols - c, p.vec);
+  load8(static_cast<const T*>(p.src) + r * p.stride + c, v, p.cols - c);
   store_prepared<T>(p.dst, r * p.ld + c, p.plane, v);
 }
 
@@ -133,7 +132,7 @@ struct SlopeArgs {
   const void* pre;
   uint64_t rows, ld_grad, ld_pre;
   uint32_t cols;
-  int act, vec_grad, vec_pre;
+  int act;
   void* dz;  // as PrepareArgs::dst, or null
   int plain;  // dz in its own type, also where that is fp32
   uint64_t ld, plane;
@@ -154,10 +153,10 @@ __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
 #pragma unroll 2
     for (uint64_t r = r0 + part; r < r1; r += 8) {
       float g[8];
-      load8(static_cast<const T*>(a.grad) + r * a.ld_grad + c, g, left, a.vec_grad);
+      load8(static_cast<const T*>(a.grad) + r * a.ld_grad + c, g, left);
       if (a.act != QVH_ACT_NONE) {
         float z[8];
-        load8(static_cast<const T*>(a.pre) + r * a.ld_pre + c, z, left, a.vec_pre);
+        load8(static_cast<const T*>(a.pre) + r * a.ld_pre + c, z, left);
         if (a.act == QVH_ACT_RELU) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) g[i] *= activate_slope<sizeof(T) == 4>(z[i], QVH_ACT_RELU);
@@ -171,7 +170,7 @@ __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
       }
       if (a.dz) {
         if (sizeof(T) == 4 && a.plain) {
-          store8(static_cast<T*>(a.dz) + r * a.ld + c, g, 8, true);  // zeros behind the last column
+          store8(static_cast<T*>(a.dz) + r * a.ld + c, g, 8);  // zeros behind the last column
         } else {
           store_prepared<T>(a.dz, r * a.ld + c, a.plane, g);
         }
@@ -221,21 +220,13 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict
 constexpr int kFewWaves = 8;
 
 template <class T>
-__device__ __forceinline__ void load_k(const T* row, uint32_t k, uint32_t depth, bool vec, typename Frag<T>::x8& f) {
-  if (vec && k + 8 <= depth) {
-    f = *reinterpret_cast<const typename Frag<T>::x8*>(row + k);
+__device__ __forceinline__ void load_k(const T* row, uint32_t k, uint32_t depth, typename Frag<T>::type& f) {
+  constexpr int kEach = Frag<T>::kEach;
+  if (k + kEach <= depth) {
+    f = reinterpret_cast<const Loose<T, kEach>*>(row + k)->v;
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = k + e < depth ? row[k + e] : static_cast<T>(0.0f);
-  }
-}
-
-__device__ __forceinline__ void load_k(const float* row, uint32_t k, uint32_t depth, bool vec, f32x4_t& f) {
-  if (vec && k + 4 <= depth) {
-    f = *reinterpret_cast<const f32x4_t*>(row + k);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = k + e < depth ? row[k + e] : 0.0f;
+    for (int e = 0; e < kEach; ++e) f[e] = k + e < depth ? row[k + e] : static_cast<T>(0.0f);
   }
 }
 
@@ -251,22 +242,13 @@ __device__ __forceinline__ f32x4_t mfma16(f32x4_t a, f32x4_t b, f32x4_t c) {
   return c;
 }
 
-template <class T>
-struct FewFrag {
-  using type = typename Frag<T>::x8;
-};
-template <>
-struct FewFrag<float> {
-  using type = f32x4_t;
-};
-
 template <class T, int MT>
 __global__ void __launch_bounds__(kFewWaves * 64) few_rows_kernel(const T* __restrict__ x, uint64_t ldx,
                                                                   const T* __restrict__ w, uint64_t ldw, uint32_t m,
-                                                                  uint32_t n, uint32_t k, int vec_x, int vec_w,
+                                                                  uint32_t n, uint32_t k,
                                                                   LinearEpilogue<T> epi) {
-  using F = typename FewFrag<T>::type;
-  constexpr uint32_t kEach = sizeof(F) / sizeof(T);  // k per lane and step
+  using F = typename Frag<T>::type;
+  constexpr uint32_t kEach = Frag<T>::kEach;  // k per lane and step
   constexpr uint32_t kDepth = kEach * 4;
   __shared__ float s_sum[kFewWaves][16 * MT][17];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, h = lane >> 4;
@@ -279,9 +261,9 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_rows_kernel(const T* __res
 #pragma unroll 4
   for (uint32_t k0 = wave * kDepth; k0 < k; k0 += kFewWaves * kDepth) {
     F fw, fx[MT];
-    load_k(wr, k0 + h * kEach, k, vec_w, fw);
+    load_k<T>(wr, k0 + h * kEach, k, fw);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) load_k(xr[t], k0 + h * kEach, k, vec_x, fx[t]);
+    for (int t = 0; t < MT; ++t) load_k<T>(xr[t], k0 + h * kEach, k, fx[t]);
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = mfma16(fw, fx[t], acc[t]);
   }
@@ -311,11 +293,6 @@ Fit fit_of(const void* p, uint64_t stride, uint64_t cols, size_t elem) {
     return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * elem % bytes == 0 && cols * elem % bytes == 0;
   };
   return whole(16) ? Fit::kWide : whole(4) ? Fit::kDwords : Fit::kNot;
-}
-
-/// 8 elements at a time: base and stride allow 16-byte accesses.
-int vec8(const void* p, uint64_t stride, size_t elem) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * elem % 16 == 0;
 }
 
 struct Space {
@@ -359,7 +336,6 @@ Prepared copy_of(const Matrix& x, int dtype, Space& ws) {
   p.job.ld = ceil_div(x.cols, 8) * 8;
   p.job.plane = p.job.ld * x.rows;
   p.job.dst = ws.take(p.job.plane * (dtype == QVH_FP32 ? kPlanes : 1) * 2);
-  p.job.vec = vec8(x.p, x.stride, dtype_size(dtype));
   const uint64_t blocks = ceil_div(p.job.ld / 8 * x.rows, 256);
   QVH_REQUIRE(blocks <= 0x3FFFFFFFu, "the matrix product is too large");
   p.job.blocks = static_cast<uint32_t>(blocks);
@@ -409,10 +385,6 @@ void run_product(Form form, Kind kind, int dtype, GemmArgs g, const void* bias, 
     e.ld_out = ld_out;
     e.ld_keep = ld_keep;
     e.act = act;
-    e.vec_bias = vec8(bias, 8, sizeof(T));
-    e.vec_residual = vec8(residual, ld_residual, sizeof(T));
-    e.vec_out = vec8(out, ld_out, sizeof(T));
-    e.vec_keep = vec8(keep, ld_keep, sizeof(T));
     e.direct = g;
     e.a_by_k = form == Form::kKK;
     e.b_by_k = form != Form::kRowsRows;
@@ -513,8 +485,7 @@ void launch_few(const qvh_linear_args& a, hipStream_t s) {
   const auto go = [&](auto tiles) {
     hipLaunchKernelGGL((few_rows_kernel<T, decltype(tiles)::value>), dim3(static_cast<unsigned>(ceil_div(a.n, 16))),
                        dim3(kFewWaves * 64), 0, s, static_cast<const T*>(a.x), a.x_stride,
-                       static_cast<const T*>(a.weight), a.weight_stride, static_cast<uint32_t>(a.m), a.n, a.k,
-                       vec8(a.x, a.x_stride, sizeof(T)), vec8(a.weight, a.weight_stride, sizeof(T)), e);
+                       static_cast<const T*>(a.weight), a.weight_stride, static_cast<uint32_t>(a.m), a.n, a.k, e);
   };
   if (a.m <= 16) {
     go(std::integral_constant<int, 1>{});
@@ -577,8 +548,6 @@ GradRun plan_grad(const qvh_linear_grad_args& a, void* ws) {
     j.ld_pre = a.preactivation_stride;
     j.cols = a.n;
     j.act = a.activation;
-    j.vec_grad = vec8(a.grad, a.grad_stride, e);
-    j.vec_pre = vec8(a.preactivation, a.preactivation_stride, e);
     j.ld = ceil_div(a.n, 8) * 8;
     j.plane = j.ld * a.m;
     j.plain = !parts;

@@ -30,14 +30,14 @@ __device__ __forceinline__ double block_sum(double v, double* s_sum) {
 }
 
 template <class T>
-__global__ void __launch_bounds__(256) norm_kernel(const T* __restrict__ g, uint64_t count, int vec,
+__global__ void __launch_bounds__(256) norm_kernel(const T* __restrict__ g, uint64_t count,
                                                    double* __restrict__ parts) {
   __shared__ double s_sum[4];
   const T* x = g + blockIdx.y * count;
   double sum = 0.0;
   for (uint64_t i = (static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; i < count; i += kNormParts * 2048) {
     float v[8];
-    load8(x + i, v, count - i < 8 ? static_cast<uint32_t>(count - i) : 8u, vec);
+    load8(x + i, v, count - i < 8 ? static_cast<uint32_t>(count - i) : 8u);
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum += static_cast<double>(v[e]) * v[e];
   }
@@ -66,7 +66,7 @@ __device__ __forceinline__ void store_parts(half_t* p, uint64_t plane, const flo
 
 /// X = G / |G|_F in parts, rows padded with zeros to ld.
 template <class T>
-__global__ void __launch_bounds__(256) start_kernel(const T* __restrict__ g, uint32_t m, uint32_t n, int vec,
+__global__ void __launch_bounds__(256) start_kernel(const T* __restrict__ g, uint32_t m, uint32_t n,
                                                     const double* __restrict__ parts, half_t* __restrict__ x,
                                                     uint64_t ld, uint64_t plane) {
   __shared__ double s_sum[4];
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(256) start_kernel(const T* __restrict__ g, uin
   if (r >= m) return;
   const uint32_t c = chunk * 8;
   float v[8];
-  load8(g + (static_cast<uint64_t>(blockIdx.y) * m + r) * n + c, v, n - c, vec);
+  load8(g + (static_cast<uint64_t>(blockIdx.y) * m + r) * n + c, v, n - c);
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = c + e < n ? static_cast<float>(v[e] * factor) : 0.0f;
   store_parts(x + blockIdx.y * 2 * plane + r * ld + c, plane, v);
@@ -114,11 +114,10 @@ struct ResultEpilogue {
   T* out;
   uint64_t ld, batch;
   float scale;
-  int vec;
   __device__ __forceinline__ void operator()(uint32_t z, uint32_t m, uint32_t n, uint32_t left, float (&v)[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= scale;
-    store8(out + z * batch + m * ld + n, v, left, vec);
+    store8(out + z * batch + m * ld + n, v, left);
   }
 };
 
@@ -493,14 +492,10 @@ void orthogonalize(const T* update, uint64_t batch, uint32_t m, uint32_t n, uint
   half_t* poly = reinterpret_cast<half_t*>(ws + l.p);
   void* partial = ws + l.partial;
   const unsigned nb = static_cast<unsigned>(batch);
-  const bool aligned = reinterpret_cast<uintptr_t>(update) % 16 == 0;
-  const int vec_rows = aligned && n * sizeof(T) % 16 == 0;
-  const int vec_all = aligned && (batch == 1 || static_cast<uint64_t>(m) * n * sizeof(T) % 16 == 0);
-  hipLaunchKernelGGL((norm_kernel<T>), dim3(kNormParts, nb), dim3(256), 0, s, update, static_cast<uint64_t>(m) * n,
-                     vec_all, norm);
+  hipLaunchKernelGGL((norm_kernel<T>), dim3(kNormParts, nb), dim3(256), 0, s, update, static_cast<uint64_t>(m) * n, norm);
   QVH_HIP(hipGetLastError());
   hipLaunchKernelGGL((start_kernel<T>), dim3(static_cast<unsigned>(ceil_div(l.ldx / 8 * m, 256)), nb), dim3(256), 0, s,
-                     update, m, n, vec_rows, norm, x[0], l.ldx, l.plane_x);
+                     update, m, n, norm, x[0], l.ldx, l.plane_x);
   QVH_HIP(hipGetLastError());
   if (steps == 0) {
     hipLaunchKernelGGL((parts_to_result_kernel<T>), dim3(static_cast<unsigned>(ceil_div(static_cast<uint64_t>(m) * n, 256)), nb),
@@ -537,8 +532,7 @@ void orthogonalize(const T* update, uint64_t batch, uint32_t m, uint32_t n, uint
     if (i + 1 < steps) {
       third(PartsEpilogue{next, nullptr, l.ldx, l.plane_x, 1.0f / kScale, 0.0f, 0.0f});
     } else {
-      const int vec = reinterpret_cast<uintptr_t>(out) % 16 == 0 && n * sizeof(T) % 16 == 0;
-      third(ResultEpilogue<T>{out, n, static_cast<uint64_t>(m) * n, 1.0f / (kScale * kScale), vec});
+      third(ResultEpilogue<T>{out, n, static_cast<uint64_t>(m) * n, 1.0f / (kScale * kScale)});
     }
   }
 }

@@ -1,7 +1,6 @@
 // Element types of the encoder operators (fp32, fp16, bf16) and their loads and stores by whole vectors.
 #pragma once
 
-#include <initializer_list>
 #include <type_traits>
 
 #include "common.hpp"
@@ -32,32 +31,40 @@ struct alignas(sizeof(T) * V) Pack {
   T v[V];
 };
 
+/// The same in global memory, aligned to T alone: the hardware takes vector accesses at any address.
+template <class T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+  typedef T vec __attribute__((ext_vector_type(V)));
+  vec v;
+};
+template <class T>
+struct Loose<T, 1> {
+  T v[1];
+};
+
 template <class T, int V>
 __device__ __forceinline__ void load_floats(const T* p, float (&out)[V]) {
-  const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
+  const auto k = reinterpret_cast<const Loose<T, V>*>(p)->v;
 #pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = static_cast<float>(k.v[i]);
+  for (int i = 0; i < V; ++i) out[i] = static_cast<float>(k[i]);
 }
 
 /// Rounds to nearest even, once.
 template <class T, int V>
 __device__ __forceinline__ void store_floats(T* p, const float (&in)[V]) {
-  Pack<T, V> k;
+  Loose<T, V> k;
 #pragma unroll
   for (int i = 0; i < V; ++i) k.v[i] = static_cast<T>(in[i]);
-  *reinterpret_cast<Pack<T, V>*>(p) = k;
+  *reinterpret_cast<Loose<T, V>*>(p) = k;
 }
 
-/// The largest power of two of elements, at most 16 bytes, that divides the row length, the row
-/// strides and the base addresses.
-inline int vector_width(size_t elem, std::initializer_list<uint64_t> lengths, std::initializer_list<const void*> bases) {
-  uint64_t bits = 16 / elem;
-  for (uint64_t n : lengths) bits |= n;
-  for (const void* p : bases) {
-    QVH_REQUIRE(reinterpret_cast<uintptr_t>(p) % elem == 0, "a buffer is not aligned to its element type");
-    bits |= reinterpret_cast<uintptr_t>(p) / elem;
-  }
-  return static_cast<int>(bits & (~bits + 1));
+/// The widest access that a row of `n` elements has room for. A row is taken in ceil(n / V) pieces, the last
+/// one moved back so that it ends with the row: the elements it shares with the piece before are read twice
+/// and written twice with the same values, which costs less than narrow accesses of odd rows.
+inline int vector_width(size_t elem, uint64_t n) {
+  int v = static_cast<int>(16 / elem);
+  while (static_cast<uint64_t>(v) > n) v /= 2;
+  return v;
 }
 
 /// Calls f with std::integral_constant<int, v> for the v in {1, 2, 4, 8} that is given (8 only for 16-bit types).
