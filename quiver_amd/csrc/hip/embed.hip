@@ -179,7 +179,8 @@ __global__ void __launch_bounds__(256) embed_grad_own_kernel(const T* __restrict
 // Stable counting passes of at most 8 bits, each a count and a scatter. Each of `parts` work-groups has a
 // contiguous part of the list; count[part][digit] gives every part its place per digit. (A scatter that
 // also counts the next pass's digits by atomics, knowing where its pairs land, took 33 us of 262,144
-// tokens instead of 5 + 6: frequent words all count in one place.)
+// tokens instead of 5 + 7: frequent words all count in one place.) Nor does one work-group that
+// makes all passes in its LDS gain: 16 us at 5,651 tokens, the four launches 19 with their gaps.
 
 constexpr uint32_t kParts = 128, kBins = 256;
 constexpr uint32_t kSortWaves = 8;
@@ -209,19 +210,56 @@ __global__ void __launch_bounds__(512) count_kernel(const I* __restrict__ tokens
   if (threadIdx.x < kBins) counts[blockIdx.x * kBins + threadIdx.x] = s_bins[threadIdx.x];
 }
 
-/// One pass. FIRST reads the tokens themselves (positions are the list's order).
-template <class I, bool FIRST>
+/// Lanes that hold the same digit as this one (those of `in` only).
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, uint32_t bits, bool in) {
+  uint64_t same = __builtin_amdgcn_ballot_w64(in);
+  for (uint32_t k = 0; k < bits; ++k) {
+    const uint64_t ones = __builtin_amdgcn_ballot_w64((digit >> k & 1u) != 0);
+    same &= (digit >> k & 1u) ? ones : ~ones;
+  }
+  return same;
+}
+
+/// The place of this lane's pair: *next (the wave's next place for the digit, in LDS) plus its rank among the
+/// lanes with the same digit.
+__device__ __forceinline__ uint32_t take_place(uint32_t* next, uint64_t same, bool in) {
+  const uint32_t rank = static_cast<uint32_t>(__popcll(same & ((uint64_t{1} << (threadIdx.x & 63)) - 1)));
+  uint32_t base = 0;
+  if (in && rank == 0) base = atomicAdd(next, static_cast<uint32_t>(__popcll(same)));
+  base = static_cast<uint32_t>(__shfl(static_cast<int>(base), in ? __builtin_ctzll(same) : 0, 64));
+  return base + rank;
+}
+
+/// Sum of `v` over the threads below, of the first 256; s_waves has four entries. All threads call it.
+__device__ __forceinline__ uint32_t scan_256(uint32_t v, uint32_t* s_waves) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t run = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t up = static_cast<uint32_t>(__shfl_up(static_cast<int>(run), d, 64));
+    run += lane >= static_cast<uint32_t>(d) ? up : 0u;
+  }
+  if (wave < 4 && lane == 63) s_waves[wave] = run;
+  __syncthreads();
+  if (wave < 4) {
+    for (uint32_t w = 0; w < wave; ++w) run += s_waves[w];
+  }
+  return run - v;
+}
+
+/// One pass. FIRST reads the tokens themselves (positions are the list's order); HELD: a wave's share is at most
+/// kHeld rounds, which are loaded once, at the start.
+constexpr uint32_t kHeld = 4;
+template <class I, bool FIRST, bool HELD>
 __global__ void __launch_bounds__(kSortWaves * 64) scatter_kernel(
     const I* __restrict__ tokens, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ positions,
     uint32_t count, uint32_t part, uint32_t rows, uint32_t shift, uint32_t bits, const uint32_t* __restrict__ counts,
     uint32_t* __restrict__ out_keys, uint32_t* __restrict__ out_positions) {
   __shared__ uint32_t s_at[kSortWaves][kBins];
-  __shared__ uint32_t s_scan[kBins];
   __shared__ uint32_t s_half[2][kBins];
+  __shared__ uint32_t s_waves[4];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t digit_mask = (1u << bits) - 1;
-  for (uint32_t i = tid; i < kSortWaves * kBins; i += kSortWaves * 64) (&s_at[0][0])[i] = 0;
-  __syncthreads();
 
   // A wave's share of the part is contiguous: the pairs' order is the waves' order.
   const uint64_t begin = static_cast<uint64_t>(blockIdx.x) * part;
@@ -229,9 +267,15 @@ __global__ void __launch_bounds__(kSortWaves * 64) scatter_kernel(
   const uint32_t share = static_cast<uint32_t>(ceil_div(part, kSortWaves * 64)) * 64;
   const uint64_t w0 = begin + static_cast<uint64_t>(wave) * share;
   const uint64_t w1 = w0 + share < end ? w0 + share : end;
-  for (uint64_t i = w0 + lane; i < w1; i += 64) {
-    const uint32_t key = FIRST ? token_key(tokens, i, rows) : keys[i];
-    atomicAdd(&s_at[wave][key >> shift & digit_mask], 1u);
+  const auto key_at = [&](uint64_t i) { return i < w1 ? (FIRST ? token_key(tokens, i, rows) : keys[i]) : 0u; };
+  const auto position_at = [&](uint64_t i) { return FIRST ? static_cast<uint32_t>(i) : i < w1 ? positions[i] : 0u; };
+  uint32_t key[kHeld], pos[kHeld];
+  if constexpr (HELD) {
+#pragma unroll
+    for (uint32_t u = 0; u < kHeld; ++u) {
+      key[u] = key_at(w0 + u * 64 + lane);
+      pos[u] = position_at(w0 + u * 64 + lane);
+    }
   }
   // This part's place per digit: all pairs of smaller digits, and this digit's in earlier parts. Two threads
   // per digit, each over half of the parts.
@@ -239,36 +283,37 @@ __global__ void __launch_bounds__(kSortWaves * 64) scatter_kernel(
   uint32_t before = 0, all = 0;
   {
     const uint32_t p0 = half ? (gridDim.x + 1) / 2 : 0u, p1 = half ? gridDim.x : (gridDim.x + 1) / 2;
-#pragma unroll 16
-    for (uint32_t p = p0; p < p1; ++p) {
-      const uint32_t n = counts[p * kBins + digit_of];
-      before += p < blockIdx.x ? n : 0u;
-      all += n;
+    for (uint32_t p = p0; p < p1; p += 16) {
+      uint32_t n[16];  // loads in flight together; past the half's end its last one again, for nothing
+#pragma unroll
+      for (uint32_t u = 0; u < 16; ++u) n[u] = counts[(p + u < p1 ? p + u : p1 - 1) * kBins + digit_of];
+#pragma unroll
+      for (uint32_t u = 0; u < 16; ++u) {
+        before += p + u < p1 && p + u < blockIdx.x ? n[u] : 0u;
+        all += p + u < p1 ? n[u] : 0u;
+      }
     }
   }
+  for (uint32_t i = tid; i < kSortWaves * kBins; i += kSortWaves * 64) (&s_at[0][0])[i] = 0;
   if (half) {
     s_half[0][digit_of] = before;
     s_half[1][digit_of] = all;
   }
   __syncthreads();
+  if constexpr (HELD) {
+#pragma unroll
+    for (uint32_t u = 0; u < kHeld; ++u) {
+      if (w0 + u * 64 + lane < w1) atomicAdd(&s_at[wave][key[u] >> shift & digit_mask], 1u);
+    }
+  } else {
+    for (uint64_t i = w0 + lane; i < w1; i += 64) atomicAdd(&s_at[wave][key_at(i) >> shift & digit_mask], 1u);
+  }
   if (!half) {
     before += s_half[0][tid];
     all += s_half[1][tid];
-    // Inclusive sums over the 256 digits: within the waves, then across the four.
-    uint32_t run = all;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t up = static_cast<uint32_t>(__shfl_up(static_cast<int>(run), d, 64));
-      run += lane >= static_cast<uint32_t>(d) ? up : 0u;
-    }
-    s_scan[tid] = run;
   }
-  __syncthreads();
-  if (tid < kBins) {
-    for (uint32_t w = 0; w < wave; ++w) before += s_scan[w * 64 + 63];
-  }
-  if (tid < kBins) {
-    uint32_t at = s_scan[tid] - all + before;
+  uint32_t at = scan_256(half ? 0u : all, s_waves) + before;  // its barrier is behind the waves' counts
+  if (!half) {
 #pragma unroll
     for (uint32_t w = 0; w < kSortWaves; ++w) {
       const uint32_t n = s_at[w][tid];
@@ -277,28 +322,20 @@ __global__ void __launch_bounds__(kSortWaves * 64) scatter_kernel(
     }
   }
   __syncthreads();
-  const uint64_t below = (uint64_t{1} << lane) - 1;
-  for (uint64_t b = w0; b < w1; b += 64) {
-    const uint64_t i = b + lane;
+  const auto place = [&](uint64_t i, uint32_t k, uint32_t p) {
     const bool in = i < w1;
-    const uint32_t key = in ? (FIRST ? token_key(tokens, i, rows) : keys[i]) : 0u;
-    const uint32_t pos = in ? (FIRST ? static_cast<uint32_t>(i) : positions[i]) : 0u;
-    const uint32_t digit = key >> shift & digit_mask;
-    // Lanes with this lane's digit.
-    uint64_t same = __builtin_amdgcn_ballot_w64(in);
-    for (uint32_t k = 0; k < bits; ++k) {
-      const uint64_t ones = __builtin_amdgcn_ballot_w64((digit >> k & 1u) != 0);
-      same &= (digit >> k & 1u) ? ones : ~ones;
-    }
-    const uint32_t rank = static_cast<uint32_t>(__popcll(same & below));
-    uint32_t base = 0;
-    if (in && rank == 0) base = atomicAdd(&s_at[wave][digit], static_cast<uint32_t>(__popcll(same)));
-    base = static_cast<uint32_t>(__shfl(static_cast<int>(base), in ? __builtin_ctzll(same) : 0, 64));
+    const uint32_t digit = k >> shift & digit_mask;
+    const uint32_t to = take_place(&s_at[wave][digit], same_digit(digit, bits, in), in);
     if (in) {
-      const uint32_t to = base + rank;
-      out_keys[to] = key;
-      out_positions[to] = pos;
+      out_keys[to] = k;
+      out_positions[to] = p;
     }
+  };
+  if constexpr (HELD) {
+#pragma unroll
+    for (uint32_t u = 0; u < kHeld; ++u) place(w0 + u * 64 + lane, key[u], pos[u]);
+  } else {
+    for (uint64_t b = w0; b < w1; b += 64) place(b + lane, key_at(b + lane), position_at(b + lane));
   }
 }
 
@@ -329,6 +366,20 @@ __device__ __forceinline__ uint32_t lower_bound(const uint32_t* keys, uint32_t n
     const bool right = keys[lo + half] < key;
     lo = right ? lo + half + 1 : lo;
     n = right ? n - half - 1 : half;
+  }
+  return lo;
+}
+
+/// The same for a whole wave that looks for one key: 64 probes at a time (a run's end among 262,144 entries
+/// in three steps for eighteen: 262,144 x 1,024 joined in 16 us for 19).
+__device__ __forceinline__ uint32_t wave_lower_bound(const uint32_t* keys, uint32_t n, uint32_t key) {
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t lo = 0;
+  while (n > 0) {
+    const uint32_t step = (n + 63) / 64, i = (lane + 1) * step - 1;
+    const uint32_t c = static_cast<uint32_t>(__popcll(__builtin_amdgcn_ballot_w64(i < n && keys[lo + i] < key)));
+    lo += c * step;  // the probe behind it, if there is one, is not below the key
+    n = n - c * step < step - 1 ? n - c * step : step - 1;
   }
   return lo;
 }
@@ -439,46 +490,78 @@ __global__ void __launch_bounds__(256) embed_grad_sum_kernel(SumArgs a) {
   flush(n);
 }
 
-/// Work-group per piece and 64 W columns: where a run begins in this piece and goes on, its partial sums
-/// are added in order (four waves take contiguous shares of them) and the row is written.
+/// Work-group per sixteen pieces and 64 W columns: where a run begins in a piece and goes on, its partial
+/// sums are added in order and the row is written. A run of few pieces is its wave's own; a long one is
+/// shared by the sixteen waves in contiguous parts, since the longest run decides the time: of 262,144
+/// tokens the most frequent has 1,600 pieces of 16, which four waves read in 32 us (a work-group per piece
+/// or per four pieces, no matter) and sixteen in 18.
+constexpr uint32_t kJoinWaves = 16, kJoinAlone = 16;
 template <class T, int W>
-__global__ void __launch_bounds__(256) embed_grad_join_kernel(SumArgs a) {
-  __shared__ float s_sum[4][64 * W];
-  const uint64_t e0 = static_cast<uint64_t>(blockIdx.x) * a.piece, e1 = e0 + a.piece;
-  if (e1 >= a.count) return;  // nothing goes on from the last piece
-  const uint32_t cur = a.keys[e1 - 1], next = a.keys[e1], lead = a.keys[e0], from = e0 > 0 ? a.keys[e0 - 1] : a.rows;
-  if (cur == a.rows || next != cur) return;
-  if (lead == cur && from == cur) return;  // began earlier
-  const uint32_t end = static_cast<uint32_t>(e1) +
-                       lower_bound(a.keys + e1, a.count - static_cast<uint32_t>(e1), cur + 1);
-  const uint32_t last = (end - 1) / a.piece;  // pieces blockIdx.x .. last hold the run
-  const uint32_t n = last - blockIdx.x + 1;
+__global__ void __launch_bounds__(kJoinWaves * 64) embed_grad_join_kernel(SumArgs a) {
+  __shared__ float s_sum[kJoinWaves][64 * W];
+  __shared__ uint32_t s_end[kJoinWaves];  // one past a long run's last entry
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t share = (n + 3) / 4;
-  const uint32_t p0 = wave * share < n ? wave * share : n, p1 = p0 + share < n ? p0 + share : n;
+  const uint32_t first = blockIdx.x * kJoinWaves;
   uint32_t c = (blockIdx.y * 64 + lane) * W;
   const bool in = c < a.dim;
   c = c < a.dim - W ? c : a.dim - W;
-  float acc[W] = {};
-  if (in) {
+  // Pieces p0 .. p1 of the run that begins in `begin`, where it is the part that goes on.
+  const auto add = [&](uint32_t begin, uint32_t p0, uint32_t p1, float (&acc)[W]) {
 #pragma unroll 8
     for (uint32_t p = p0; p < p1; ++p) {
       float x[W];
-      load_floats<float, W>(a.partial + ((static_cast<uint64_t>(blockIdx.x) + p) * 2 + (p == 0 ? 1 : 0)) * a.dim + c, x);
+      load_floats<float, W>(a.partial + (static_cast<uint64_t>(p) * 2 + (p == begin ? 1 : 0)) * a.dim + c, x);
 #pragma unroll
       for (int k = 0; k < W; ++k) acc[k] += x[k];
     }
-  }
+  };
+  const auto write = [&](uint32_t row, float (&acc)[W]) {
 #pragma unroll
-  for (int k = 0; k < W; ++k) s_sum[wave][lane * W + k] = acc[k];
-  __syncthreads();
-  if (wave == 0 && in) {
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-      const uint32_t i = lane * W + k;
-      acc[k] = (((s_sum[0][i] + s_sum[1][i]) + s_sum[2][i]) + s_sum[3][i]) * a.scale;
+    for (int k = 0; k < W; ++k) acc[k] *= a.scale;
+    store_floats<T, W>(static_cast<T*>(a.out) + static_cast<uint64_t>(row) * a.dim + c, acc);
+  };
+
+  const uint64_t e0 = static_cast<uint64_t>(first + wave) * a.piece, e1 = e0 + a.piece;
+  uint32_t shared_end = 0;
+  if (e1 < a.count) {  // nothing goes on from the last piece
+    const uint32_t cur = a.keys[e1 - 1], next = a.keys[e1], lead = a.keys[e0], from = e0 > 0 ? a.keys[e0 - 1] : a.rows;
+    const bool earlier = lead == cur && from == cur;
+    if (cur != a.rows && next == cur && !earlier) {
+      const uint32_t end = static_cast<uint32_t>(e1) +
+                           wave_lower_bound(a.keys + e1, a.count - static_cast<uint32_t>(e1), cur + 1);
+      const uint32_t last = (end - 1) / a.piece;
+      if (last - (first + wave) < kJoinAlone) {
+        float acc[W] = {};
+        if (in) {
+          add(first + wave, first + wave, last + 1, acc);
+          write(cur, acc);
+        }
+      } else {
+        shared_end = end;
+      }
     }
-    store_floats<T, W>(static_cast<T*>(a.out) + static_cast<uint64_t>(cur) * a.dim + c, acc);
+  }
+  if (lane == 0) s_end[wave] = shared_end;
+  __syncthreads();
+  for (uint32_t b = 0; b < kJoinWaves; ++b) {
+    if (s_end[b] == 0) continue;
+    const uint32_t begin = first + b, end = (s_end[b] - 1) / a.piece + 1;  // pieces begin .. end - 1 hold the run
+    const uint32_t share = (end - begin + kJoinWaves - 1) / kJoinWaves;
+    const uint32_t p0 = begin + wave * share < end ? begin + wave * share : end, p1 = p0 + share < end ? p0 + share : end;
+    float acc[W] = {};
+    if (in) add(begin, p0, p1, acc);
+#pragma unroll
+    for (int k = 0; k < W; ++k) s_sum[wave][lane * W + k] = acc[k];
+    __syncthreads();
+    if (wave == 0 && in) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        acc[k] = 0.0f;
+        for (uint32_t w = 0; w < kJoinWaves; ++w) acc[k] += s_sum[w][lane * W + k];
+      }
+      write(a.keys[s_end[b] - 1], acc);
+    }
+    __syncthreads();
   }
 }
 
@@ -554,30 +637,30 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
   uint32_t* counts = reinterpret_cast<uint32_t*>(ws + l.counts);
   uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(ws + l.keys[0]), reinterpret_cast<uint32_t*>(ws + l.keys[1])};
   uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + l.positions[0]), reinterpret_cast<uint32_t*>(ws + l.positions[1])};
+  const uint32_t sorted = (l.passes - 1) & 1;  // which of the two halves of keys and pos
+  const bool held = l.part <= kSortWaves * 64 * kHeld;
   for (uint32_t p = 0; p < l.passes; ++p) {
     const uint32_t *ik = keys[(p & 1) ^ 1], *ip = pos[(p & 1) ^ 1];
-    const auto pass = [&](auto first) {
+    const auto pass = [&](auto first, auto hold) {
       constexpr bool F = decltype(first)::value;
-      hipLaunchKernelGGL((count_kernel<I, F>), dim3(l.parts), dim3(512), 0, s, static_cast<const I*>(tokens), ik, n, l.part, r,
-                         p * digit, (1u << digit) - 1, counts);
+      hipLaunchKernelGGL((count_kernel<I, F>), dim3(l.parts), dim3(512), 0, s, static_cast<const I*>(tokens), ik, n, l.part,
+                         r, p * digit, (1u << digit) - 1, counts);
       QVH_HIP(hipGetLastError());
-      hipLaunchKernelGGL((scatter_kernel<I, F>), dim3(l.parts), dim3(kSortWaves * 64), 0, s,
-                         static_cast<const I*>(tokens), ik, ip, n, l.part, r, p * digit, digit, counts, keys[p & 1], pos[p & 1]);
+      hipLaunchKernelGGL((scatter_kernel<I, F, decltype(hold)::value>), dim3(l.parts), dim3(kSortWaves * 64), 0, s,
+                         static_cast<const I*>(tokens), ik, ip, n, l.part, r, p * digit, digit, counts, keys[p & 1],
+                         pos[p & 1]);
+      QVH_HIP(hipGetLastError());
     };
-    if (p == 0) {
-      pass(std::true_type{});
-    } else {
-      pass(std::false_type{});
-    }
-    QVH_HIP(hipGetLastError());
+    const auto either = [&](auto first) { held ? pass(first, std::true_type{}) : pass(first, std::false_type{}); };
+    p == 0 ? either(std::true_type{}) : either(std::false_type{});
   }
   with_width<T>(width, [&](auto v) {
     constexpr int V = decltype(v)::value;
     SumArgs a{};
     a.grad = grad;
     a.stride = stride;
-    a.keys = keys[(l.passes - 1) & 1];
-    a.positions = pos[(l.passes - 1) & 1];
+    a.keys = keys[sorted];
+    a.positions = pos[sorted];
     a.count = n;
     a.rows = r;
     a.dim = dim;
@@ -606,10 +689,11 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
     }
     QVH_HIP(hipGetLastError());
     if (a.pieces > 1) {
+      const unsigned blocks = static_cast<unsigned>(ceil_div(a.pieces, kJoinWaves));
       if (dim >= 4) {
-        hipLaunchKernelGGL((embed_grad_join_kernel<T, 4>), dim3(a.pieces, ceil_div(dim, 256)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((embed_grad_join_kernel<T, 4>), dim3(blocks, ceil_div(dim, 256)), dim3(kJoinWaves * 64), 0, s, a);
       } else {
-        hipLaunchKernelGGL((embed_grad_join_kernel<T, 1>), dim3(a.pieces, ceil_div(dim, 64)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((embed_grad_join_kernel<T, 1>), dim3(blocks, ceil_div(dim, 64)), dim3(kJoinWaves * 64), 0, s, a);
       }
       QVH_HIP(hipGetLastError());
     }
