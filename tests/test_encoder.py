@@ -95,12 +95,16 @@ def _linear(**change):
     return a
 
 
+# A float32 product large enough to be made of 16-bit parts, which lie in a workspace.
+SPLIT = dict(m=4096, k=1024, n=1024, x_stride=1024, weight_stride=1024, out_stride=1024)
+
+
 @pytest.mark.parametrize("change,word", [
     (dict(dtype=4), "dtype"), (dict(activation=7), "activation"), (dict(m=2**31), "m must"), (dict(k=2**20 + 1), "k and n"),
     (dict(n=2**21), "k and n"), (dict(x=None), "x is null"), (dict(weight=None), "weight is null"),
     (dict(out=None), "out is null"), (dict(x_stride=31), "stride"), (dict(x_stride=2**22 + 1), "stride"),
     (dict(out_stride=15), "stride"), (dict(residual=1 << 20, residual_stride=3), "stride"),
-    (dict(x=(1 << 20) + 1), "aligned"), (dict(bias=(1 << 20) + 1), "aligned"), (dict(dtype=0, x_stride=32), "workspace")])
+    (dict(x=(1 << 20) + 1), "aligned"), (dict(bias=(1 << 20) + 1), "aligned"), (dict(dtype=0, **SPLIT), "workspace")])
 def test_linear_refuses(lib, change, word):
     _refused(lib, lib.qvh_linear_device(C.byref(_linear(**change)), None, C.c_uint64(0), None), word)
 
@@ -108,7 +112,9 @@ def test_linear_refuses(lib, change, word):
 def test_linear_workspace(lib):
     size = C.c_uint64(1)
     assert lib.qvh_linear_workspace(C.byref(_linear(m=4)), C.byref(size)) == 0 and size.value == 0
-    assert lib.qvh_linear_workspace(C.byref(_linear(dtype=0)), C.byref(size)) == 0 and size.value >= 6 * 100 * 32
+    assert lib.qvh_linear_workspace(C.byref(_linear(dtype=0)), C.byref(size)) == 0 and size.value == 0  # read as it is
+    assert lib.qvh_linear_workspace(C.byref(_linear(dtype=0, **SPLIT)), C.byref(size)) == 0
+    assert size.value >= 6 * (4096 + 1024) * 1024  # three 16-bit parts of both operands
     _refused(lib, lib.qvh_linear_workspace(None, C.byref(size)), "null")
     _refused(lib, lib.qvh_linear_workspace(C.byref(_linear()), None), "null")
 
