@@ -294,7 +294,7 @@ struct Stage {
     const uint32_t lines = BY_K ? depth : rows, extent = (BY_K ? rows : depth) * kElem;
     uint32_t byte = ((at % kLine / 16) ^ flip(line)) * 16 + at % 16;
     line = line < lines ? line : lines - 1;
-    const uint32_t last = WIDE == 16 ? (extent + 15) / 16 * 16 - 16 : extent - 4;
+    const uint32_t last = (extent + WIDE - 1) / WIDE * WIDE - WIDE;  // rows that end inside it are padded to whole ones
     byte = byte < last ? byte : last;
     return line * ld * kElem + byte;
   }

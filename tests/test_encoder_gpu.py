@@ -369,6 +369,22 @@ def test_linear_grad(dtype, m, k, n):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m,k,n", [(24, 938, 117), (90, 30, 1), (2, 2, 3), (70, 338, 65), (513, 6, 129), (5001, 66, 63), (130, 1644, 515)])
+def test_linear_grad_of_even_rows_and_odd_ones(dtype, m, k, n):
+    """Rows of x and w that are whole dwords but not whole 16-byte pieces, next to odd rows of the gradient."""
+    test_linear_grad(dtype, m, k, n)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m,k,n", [(65, 2, 1), (100, 1030, 77), (1000, 4094, 66), (3000, 18, 515), (2049, 514, 1027)])
+def test_linear_of_even_rows(dtype, m, k, n):
+    g = torch.Generator().manual_seed(m + k)
+    _say("linear", dtype, m, k, n)
+    x, w, b = _randn(g, m, k, dtype=dtype), _randn(g, n, k, dtype=dtype, std=1 / math.sqrt(k)), _randn(g, n, dtype=dtype)
+    _check_linear(dtype, x, w, b, "silu", _randn(g, m, n, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_linear_grad_views_and_parts(dtype):
     g = torch.Generator().manual_seed(4)
     _say("linear_grad views", dtype)
