@@ -62,7 +62,7 @@ namespace {
 
 constexpr uint64_t kMaxRows = uint64_t{1} << 31, kMaxStride = uint64_t{1} << 22;
 constexpr uint32_t kMaxWidth = 1u << 20;
-constexpr uint64_t kFewRows = 64;  // x rows that the few-row kernel takes
+constexpr uint64_t kSumRows = 128;  // rows whose column sums one work-group makes
 constexpr int kPlanes = 3;         // bf16 parts of an fp32 value
 
 // ---- operand preparation ----------------------------------------------------------------------
@@ -113,11 +113,11 @@ __device__ __forceinline__ void store_prepared(void* dst, uint64_t at, uint64_t 
 /// Copies up to two matrices into rows that the tiled product can read: aligned, padded with zeros, fp32 in
 /// its three parts.
 template <class T>
-__global__ void __launch_bounds__(256) prepare_kernel(PrepareArgs a, PrepareArgs b) {
-  const bool second = blockIdx.x >= a.blocks;
+__device__ __forceinline__ void prepare_rows(uint32_t block, const PrepareArgs& a, const PrepareArgs& b) {
+  const bool second = block >= a.blocks;
   const PrepareArgs& p = second ? b : a;
   const uint32_t per_row = static_cast<uint32_t>(p.ld / 8);
-  const auto [r, chunk] = row_and_chunk(second ? blockIdx.x - a.blocks : blockIdx.x, per_row);
+  const auto [r, chunk] = row_and_chunk(second ? block - a.blocks : block, per_row);
   if (r >= p.rows) return;
   const uint32_t c = chunk * 8;
   float v[8];
@@ -125,8 +125,13 @@ __global__ void __launch_bounds__(256) prepare_kernel(PrepareArgs a, PrepareArgs
   store_prepared<T>(p.dst, r * p.ld + c, p.plane, v);
 }
 
+template <class T>
+__global__ void __launch_bounds__(256) prepare_kernel(PrepareArgs a, PrepareArgs b) {
+  prepare_rows<T>(blockIdx.x, a, b);
+}
+
 /// dz = grad * act'(z) (stored if asked for) and its column sums over this work-group's rows. A thread
-/// has eight columns; eight threads share them, each taking every eighth row.
+/// has eight columns; 256 / LX threads share them, each taking every 256 / LX-th row.
 struct SlopeArgs {
   const void* grad;
   const void* pre;
@@ -137,21 +142,29 @@ struct SlopeArgs {
   int plain;  // dz in its own type, also where that is fp32
   uint64_t ld, plane;
   float* sums;  // [work-group][cols rounded up to 8], or null
-  uint32_t rows_each;
+  void* total;  // the sums themselves, where one work-group has all rows, or null
+  uint32_t rows_each, across, blocks;
 };
 
-template <class T>
-__global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
-  __shared__ float s_sum[8][32 * 8 + 4];
-  const uint32_t lane = threadIdx.x % 32, part = threadIdx.x / 32;
-  const uint32_t c = (blockIdx.y * 32 + lane) * 8;
-  const uint64_t r0 = static_cast<uint64_t>(blockIdx.x) * a.rows_each;
+/// Work-groups past the slope's make the copies of x and w.
+template <class T, int LX>
+__global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a, PrepareArgs copy_a, PrepareArgs copy_b) {
+  constexpr uint32_t kRows = 256 / LX, kCols = LX * 8;
+  __shared__ float s_sum[kRows][kCols + 4];
+  if (blockIdx.x >= a.blocks) {
+    prepare_rows<T>(blockIdx.x - a.blocks, copy_a, copy_b);
+    return;
+  }
+  const uint32_t group = blockIdx.x / a.across, across = blockIdx.x - group * a.across;
+  const uint32_t lane = threadIdx.x % LX, part = threadIdx.x / LX;
+  const uint32_t c = across * kCols + lane * 8;
+  const uint64_t r0 = static_cast<uint64_t>(group) * a.rows_each;
   const uint64_t r1 = r0 + a.rows_each < a.rows ? r0 + a.rows_each : a.rows;
   float sum[8] = {};
   if (c < a.cols) {
     const uint32_t left = a.cols - c;
 #pragma unroll 2
-    for (uint64_t r = r0 + part; r < r1; r += 8) {
+    for (uint64_t r = r0 + part; r < r1; r += kRows) {
       float g[8];
       load8(static_cast<const T*>(a.grad) + r * a.ld_grad + c, g, left);
       if (a.act != QVH_ACT_NONE) {
@@ -179,17 +192,21 @@ __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a) {
       for (int i = 0; i < 8; ++i) sum[i] += g[i];
     }
   }
-  if (!a.sums) return;
+  if (!a.sums && !a.total) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) s_sum[part][lane * 8 + i] = sum[i];
   __syncthreads();
   const uint32_t ld = (a.cols + 7) / 8 * 8;
-  const uint32_t col = blockIdx.y * 256 + threadIdx.x;
-  if (col < ld) {
+  const uint32_t col = across * kCols + threadIdx.x;
+  if (threadIdx.x < kCols && col < ld) {
     float t = 0.0f;
-#pragma unroll
-    for (int p = 0; p < 8; ++p) t += s_sum[p][threadIdx.x];
-    a.sums[static_cast<uint64_t>(blockIdx.x) * ld + col] = t;
+#pragma unroll 8
+    for (uint32_t p = 0; p < kRows; ++p) t += s_sum[p][threadIdx.x];
+    if (a.sums) {
+      a.sums[static_cast<uint64_t>(group) * ld + col] = t;
+    } else if (col < a.cols) {
+      static_cast<T*>(a.total)[col] = static_cast<T>(t);
+    }
   }
 }
 
@@ -213,9 +230,11 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict
 
 // ---- few rows ---------------------------------------------------------------------------------
 //
-// For a handful of rows of x the weight is the traffic: every work-group reads 16 of its rows once,
-// straight into the fragments of the matrix unit, its eight waves taking every eighth step of k, and
-// adds the waves' sums in LDS.
+// Small products in one launch, whatever their rows' alignment: every work-group reads 16 rows of the weight
+// and up to 64 of x straight into the fragments of the matrix unit, its eight waves taking every eighth step
+// of k, and adds the waves' sums in LDS. One row of x: the weight is the traffic. Many: the loads, of 64
+// bytes from each of 16 rows, are what takes the time, 0.4 us a step for 16 rows of x and 1.1 for 64
+// (loading four steps ahead changes nothing), so that long k is better split and joined.
 
 constexpr int kFewWaves = 8;
 
@@ -252,11 +271,11 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_rows_kernel(const T* __res
   constexpr uint32_t kDepth = kEach * 4;
   __shared__ float s_sum[kFewWaves][16 * MT][17];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, h = lane >> 4;
-  const uint32_t n0 = blockIdx.x * 16;
+  const uint32_t n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
   const T* wr = w + static_cast<uint64_t>(n0 + i < n ? n0 + i : n - 1) * ldw;
   const T* xr[MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) xr[t] = x + static_cast<uint64_t>(16 * t + i < m ? 16 * t + i : m - 1) * ldx;
+  for (int t = 0; t < MT; ++t) xr[t] = x + static_cast<uint64_t>(m0 + 16 * t + i < m ? m0 + 16 * t + i : m - 1) * ldx;
   f32x4_t acc[MT] = {};
 #pragma unroll 4
   for (uint32_t k0 = wave * kDepth; k0 < k; k0 += kFewWaves * kDepth) {
@@ -279,7 +298,7 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_rows_kernel(const T* __res
     float sum = 0.0f;
 #pragma unroll
     for (int v = 0; v < kFewWaves; ++v) sum += s_sum[v][row][col];
-    if (row < m && n0 + col < n) epi.one(row, n0 + col, sum);
+    if (m0 + row < m && n0 + col < n) epi.one(m0 + row, n0 + col, sum);
   }
 }
 
@@ -413,6 +432,17 @@ void check_matrix(const std::string& w, const char* name, const void* p, uint64_
   QVH_REQUIRE((stride >= cols || rows <= 1) && stride <= kMaxStride, w + ": " + name + "'s stride must be in [row length, 2^22]");
 }
 
+/// us of the few-row kernel, fitted to 204 products from 1 x 64 x 64 to 3,721 x 2,019 x 65, bf16 and fp32. Taken
+/// where it promises to beat the tiled products, it was the slower by more than 12% in 12 of them (by rows of x
+/// alone, up to 64, in far more: 13% slower than the better one on average, against 2%). Both sides, few rows
+/// first: 64 x 512 x 1,024 4.5 and 4.9, 64 x 4,096 x 1,024 19.8 and 9.0, 614 x 96 x 74 2.7 and 3.9.
+double few_us(uint64_t m, uint32_t k, uint32_t n, int dtype) {
+  const uint64_t groups = ceil_div(m, 64) * ceil_div(n, 16);
+  double step = m <= 16 ? 0.42 : m <= 32 ? 0.64 : 1.07;
+  if (dtype != QVH_FP32 && k % 2 != 0) step *= 2.7;  // rows that begin inside a dword
+  return 2.0 + static_cast<double>(ceil_div(groups, 256)) * (0.3 + static_cast<double>(ceil_div(k, dtype == QVH_FP32 ? 128 : 256)) * step);
+}
+
 struct LinearRun {
   bool few = false;
   Kind kind = Kind::kPlane1;
@@ -429,8 +459,6 @@ struct LinearRun {
 LinearRun plan_linear(const qvh_linear_args& a, void* ws) {
   LinearRun r;
   if (a.m == 0 || a.n == 0) return r;
-  r.few = a.m <= kFewRows;
-  if (r.few) return r;
   Space sp;
   sp.base = static_cast<char*>(ws);
   const size_t e = dtype_size(a.dtype);
@@ -438,11 +466,11 @@ LinearRun plan_linear(const qvh_linear_args& a, void* ws) {
   const Fit fx = fit_of(a.x, a.x_stride, a.k, e), fw = fit_of(a.weight, a.weight_stride, a.k, e);
   const bool all = a.dtype == QVH_FP32;  // copies are made of everything, in parts
   const bool copy_x = all || fx != Fit::kWide, copy_w = all || fw != Fit::kWide;
+  const double elements = (copy_x ? static_cast<double>(a.m) * a.k : 0.0) + (copy_w ? static_cast<double>(a.n) * a.k : 0.0);
   r.kind = copied_kind(a.dtype);
   r.plan = gemm_plan(a.m, a.n, a.k, r.kind, 1, false);
   bool copies = copy_x || copy_w;
   if (copies && (all || (fx != Fit::kNot && fw != Fit::kNot))) {
-    const double elements = (copy_x ? static_cast<double>(a.m) * a.k : 0.0) + (copy_w ? static_cast<double>(a.n) * a.k : 0.0);
     const Kind direct = direct_kind(a.dtype, fx, fw);
     const GemmPlan p = gemm_plan(a.m, a.n, a.k, direct, 1, false);
     if (p.us < r.plan.us + copy_us(a.dtype, elements)) {
@@ -451,6 +479,8 @@ LinearRun plan_linear(const qvh_linear_args& a, void* ws) {
       r.plan = p;
     }
   }
+  r.few = ceil_div(a.m, 64) <= 65535 && few_us(a.m, a.k, a.n, a.dtype) < r.plan.us + (copies ? copy_us(a.dtype, elements) : 0.0);
+  if (r.few) return r;
   r.x = copies && copy_x ? copy_of(x, a.dtype, sp) : as_it_is(x);
   r.w = copies && copy_w ? copy_of(w, a.dtype, sp) : as_it_is(w);
   r.partial = sp.take(r.plan.partial_bytes);
@@ -483,7 +513,7 @@ void launch_few(const qvh_linear_args& a, hipStream_t s) {
   e.ld_keep = a.preactivation_stride;
   e.act = a.activation;
   const auto go = [&](auto tiles) {
-    hipLaunchKernelGGL((few_rows_kernel<T, decltype(tiles)::value>), dim3(static_cast<unsigned>(ceil_div(a.n, 16))),
+    hipLaunchKernelGGL((few_rows_kernel<T, decltype(tiles)::value>), dim3(static_cast<unsigned>(ceil_div(a.n, 16)), static_cast<unsigned>(ceil_div(a.m, 64))),
                        dim3(kFewWaves * 64), 0, s, static_cast<const T*>(a.x), a.x_stride,
                        static_cast<const T*>(a.weight), a.weight_stride, static_cast<uint32_t>(a.m), a.n, a.k, e);
   };
@@ -499,6 +529,7 @@ void launch_few(const qvh_linear_args& a, hipStream_t s) {
 
 struct GradRun {
   bool slope = false;  // dz is written or summed
+  bool one = false;    // by work-groups that have all rows
   SlopeArgs job{};
   uint32_t sum_parts = 0;
   GemmOperand dz;
@@ -552,11 +583,21 @@ GradRun plan_grad(const qvh_linear_grad_args& a, void* ws) {
     j.plane = j.ld * a.m;
     j.plain = !parts;
     if (writes) j.dz = sp.take(j.plane * (parts ? kPlanes * 2 : e));
-    // Work-groups of 256 columns; rows spread over about a thousand of them, at least 16 rows each.
-    const uint64_t across = ceil_div(a.n, 256);
-    j.rows_each = static_cast<uint32_t>(std::max<uint64_t>(16, ceil_div(ceil_div(a.m, 8), ceil_div(1024, across)) * 8));
-    r.sum_parts = static_cast<uint32_t>(ceil_div(a.m, j.rows_each));
-    if (a.grad_bias) j.sums = static_cast<float*>(sp.take(static_cast<size_t>(r.sum_parts) * j.ld * 4));
+    // A work-group with all rows of 64 columns saves the launch that adds up the parts; its threads then walk
+    // down up to four rows each. Otherwise 256 columns, rows spread over about a thousand work-groups, at
+    // least 16 rows each. (All of linear_grad, bf16: 90 x 1,024 x 80 16.7 us against 21.2; with up to 256
+    // rows allowed 255 x 511 x 4,095 took 38.2 against 28.8.)
+    r.one = a.grad_bias && a.m <= kSumRows;
+    j.across = static_cast<uint32_t>(ceil_div(a.n, r.one ? 64 : 256));
+    j.rows_each = r.one ? static_cast<uint32_t>(std::max<uint64_t>(a.m, 1))
+                        : static_cast<uint32_t>(std::max<uint64_t>(16, ceil_div(ceil_div(a.m, 8), ceil_div(1024, j.across)) * 8));
+    r.sum_parts = r.one ? 1 : static_cast<uint32_t>(ceil_div(a.m, j.rows_each));
+    j.blocks = r.sum_parts * j.across;
+    if (r.one) {
+      j.total = a.grad_bias;
+    } else if (a.grad_bias) {
+      j.sums = static_cast<float*>(sp.take(static_cast<size_t>(r.sum_parts) * j.ld * 4));
+    }
   }
   if (writes) {
     r.dz.base = r.job.dz;
@@ -681,15 +722,23 @@ qvh_status qvh_linear_grad_device(const qvh_linear_grad_args* args, void* d_work
     check_workspace("qvh_linear_grad_device", d_workspace, workspace_bytes, r.bytes);
     current_device();
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (r.slope && r.sum_parts > 0) {
+    const bool products = a.k > 0 && (a.grad_x || a.grad_weight);
+    if (r.slope && r.job.blocks > 0) {
+      const PrepareArgs none;
+      const PrepareArgs& first = r.x.copy ? r.x.job : r.w.copy ? r.w.job : none;
+      const PrepareArgs& second = r.x.copy && r.w.copy ? r.w.job : none;
+      const uint64_t blocks = static_cast<uint64_t>(r.job.blocks) + first.blocks + second.blocks;
+      QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "the matrix product is too large");
       with_dtype(a.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        hipLaunchKernelGGL((slope_kernel<T>), dim3(r.sum_parts, static_cast<unsigned>(ceil_div(a.n, 256))), dim3(256), 0, s,
-                           r.job);
+        const auto kernel = r.one ? slope_kernel<T, 8> : slope_kernel<T, 32>;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, r.job, first, second);
       });
       QVH_HIP(hipGetLastError());
+    } else if (products) {
+      launch_prepare(a.dtype, r.x, r.w, s);
     }
-    if (a.grad_bias && a.n > 0) {
+    if (a.grad_bias && a.n > 0 && !r.one) {
       with_dtype(a.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         hipLaunchKernelGGL((column_sum_kernel<T>), dim3(static_cast<unsigned>(ceil_div(a.n, 64))), dim3(256), 0, s,
@@ -697,8 +746,7 @@ qvh_status qvh_linear_grad_device(const qvh_linear_grad_args* args, void* d_work
       });
       QVH_HIP(hipGetLastError());
     }
-    if (a.k == 0 || !(a.grad_x || a.grad_weight)) return;
-    launch_prepare(a.dtype, r.x, r.w, s);
+    if (!products) return;
     GemmArgs g;
     g.a = r.dz;
     if (a.grad_x && a.m > 0) {
