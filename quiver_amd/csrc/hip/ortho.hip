@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(256) parts_to_result_kernel(const half_t* __re
 // number of 16-byte pieces, so that sixteen neighbouring rows at one k lie on different banks.
 
 constexpr uint32_t kSmallBlocks = 40;  // 32 x 32 blocks of X
-constexpr uint32_t kSmallLds = 160 * 1024;
+constexpr uint32_t kSmallLds = 160 * 1024;  // what a work-group may have
 
 struct SmallShape {
   uint32_t side, depth;     // rounded up to 32
@@ -158,6 +158,9 @@ __host__ __device__ inline SmallShape small_shape(uint32_t m, uint32_t n) {
   s.bytes = 2 * s.side * (s.row_x + s.row_s);
   return s;
 }
+
+/// Waves for it: their registers hold its blocks.
+inline uint32_t small_waves(const SmallShape& s) { return s.side / 32 * (s.depth / 32) <= 16 ? 16 : 8; }
 
 /// Whether a matrix is done by one work-group.
 inline bool is_small(uint32_t m, uint32_t n) {
@@ -186,22 +189,35 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
   const T* g = update + static_cast<uint64_t>(blockIdx.x) * count;
   T* o = out + static_cast<uint64_t>(blockIdx.x) * count;
 
-  // Rows over the waves, columns over the lanes: f(row, column) for every element, loads of four rows at once.
+  // f(index, value) for this thread's elements of the update, in the order they lie, four vectors loaded at once.
+  constexpr uint32_t kVec = 16 / sizeof(T), kThreads = WAVES * 64;
   const auto each = [&](auto&& f) {
-    for (uint32_t q = lane; q < n; q += 64) {
-      for (uint32_t r0 = wave; r0 < m; r0 += 4 * WAVES) {
-        float v[4];
+    const uint32_t vectors = count / kVec;
+    for (uint32_t i0 = threadIdx.x; i0 < vectors; i0 += 4 * kThreads) {
+      float v[4][kVec];
 #pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) v[u] = r0 + u * WAVES < m ? static_cast<float>(g[(r0 + u * WAVES) * n + q]) : 0.0f;
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) {
-          if (r0 + u * WAVES < m) f(r0 + u * WAVES, q, v[u]);
-        }
+      for (uint32_t u = 0; u < 4; ++u) {
+        if (i0 + u * kThreads < vectors) load_floats<T, kVec>(g + (i0 + u * kThreads) * kVec, v[u]);
       }
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        if (i0 + u * kThreads < vectors) f((i0 + u * kThreads) * kVec, v[u], kVec);
+      }
+    }
+    const uint32_t left = count % kVec;
+    if (threadIdx.x < left) {
+      float v[kVec];
+      v[0] = static_cast<float>(g[count - left + threadIdx.x]);
+      f(count - left + threadIdx.x, v, 1u);
     }
   };
   double sum = 0.0;
-  each([&](uint32_t, uint32_t, float v) { sum = fma(static_cast<double>(v), static_cast<double>(v), sum); });
+  each([&](uint32_t, const float (&v)[kVec], uint32_t valid) {
+#pragma unroll
+    for (uint32_t e = 0; e < kVec; ++e) {
+      if (e < valid) sum = fma(static_cast<double>(v[e]), static_cast<double>(v[e]), sum);
+    }
+  });
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
   if (lane == 0) s_sum[wave] = sum;
@@ -213,12 +229,22 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) sum += s_sum[w];
   const double factor = start_factor(sum);
-  each([&](uint32_t r, uint32_t q, float v) {
-    half_t high, low;
-    split2(static_cast<float>(v * factor), high, low);
-    char* at = x + (tall ? q * sh.row_x + r * 2 : r * sh.row_x + q * 2);
-    *reinterpret_cast<half_t*>(at) = high;
-    *reinterpret_cast<half_t*>(at + plane_x) = low;
+  each([&](uint32_t i, const float (&v)[kVec], uint32_t valid) {
+    uint32_t r = i / n, q = i - r * n;
+#pragma unroll
+    for (uint32_t e = 0; e < kVec; ++e) {
+      if (e < valid) {
+        half_t high, low;
+        split2(static_cast<float>(v[e] * factor), high, low);
+        char* at = x + (tall ? q * sh.row_x + r * 2 : r * sh.row_x + q * 2);
+        *reinterpret_cast<half_t*>(at) = high;
+        *reinterpret_cast<half_t*>(at + plane_x) = low;
+      }
+      if (++q == n) {
+        q = 0;
+        ++r;
+      }
+    }
   });
   __syncthreads();
 
@@ -236,11 +262,12 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
     }
     return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  // A block of a product over `slices` (an even number of) 16-deep slices: the small terms by themselves, so
-  // that the matrix instructions wait less for one another, and two slices' fragments fetched at a time.
-  const auto product_of = [](uint32_t slices, auto&& a_at, auto&& b_at) {
+  // A block of a product over 16-deep slices `from` .. `to` - 1, an even number of them: the small terms by
+  // themselves, so that the matrix instructions wait less for one another, and two slices' fragments
+  // fetched at a time.
+  const auto product_of = [](uint32_t from, uint32_t to, auto&& a_at, auto&& b_at) {
     f32x16_t small{}, large{};
-    for (uint32_t kk = 0; kk < slices; kk += 2) {
+    for (uint32_t kk = from; kk < to; kk += 2) {
       X8 ah[2], al[2], bh[2], bl[2];
 #pragma unroll
       for (uint32_t u = 0; u < 2; ++u) {
@@ -274,6 +301,11 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
   };
 
   const uint32_t sb = sh.side / 32, db = sh.depth / 32;
+  // Waves to a block of S: a KB of its place each. Adding up their parts takes 1.5 us a step, 32 k less for a wave
+  // save 0.15 (32 x 1,100 bf16: 78 us a call with one wave, 58 with five; 64 x 256: 37 with one, 43 with four).
+  f32x4_t* const s_part = reinterpret_cast<f32x4_t*>(s);
+  const uint32_t most = sb == 1 ? 5 : WAVES / (sb * sb) < 4 ? WAVES / (sb * sb) : 4;
+  const uint32_t ways = db - db / (most > 0 ? most : 1) >= 12 ? most : 1;
   // Addresses that follow from the wave's number are computed where they are used: kept over all steps, those
   // of five blocks took 250 registers more than there are.
   const auto fresh = [](uint32_t w) {
@@ -281,16 +313,43 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
     return w;
   };
   for (uint32_t step = 0; step < steps; ++step) {
-    // S = X X^T. All blocks: the waves that its symmetry would save have nothing else to do.
-#pragma unroll
-    for (int u = 0; u < BLOCKS; ++u) {
-      const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
+    // S = X X^T. All blocks: the waves that its symmetry would save have nothing else to do. Where there are
+    // several waves to a block and k is long, each takes a part of it; the first adds the parts up, four rows
+    // at a time, which lie in S's place until then.
+    const auto x_rows = [&](uint32_t row0) {
+      return [&, row0](uint32_t p, uint32_t kk) { return rows(x + p * plane_x, sh.row_x, row0, kk); };
+    };
+    if (ways > 1) {
+      const uint32_t t = fresh(wave) / ways, way = fresh(wave) % ways;
+      const uint32_t bi = t / sb, bj = t % sb, pairs = sh.depth / 32;
+      f32x16_t acc{};
       if (t < sb * sb) {
-        const uint32_t bi = t / sb, bj = t % sb;
-        const f32x16_t acc = product_of(
-            sh.depth / 16, [&](uint32_t p, uint32_t kk) { return rows(x + p * plane_x, sh.row_x, bi * 32, kk); },
-            [&](uint32_t p, uint32_t kk) { return rows(x + p * plane_x, sh.row_x, bj * 32, kk); });
-        put(s, sh.row_s, plane_s, bi, bj, acc * (1.0f / kScale));
+        acc = product_of(pairs * way / ways * 2, pairs * (way + 1) / ways * 2, x_rows(bi * 32), x_rows(bj * 32));
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f32x4_t part;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[e] = acc[4 * q + e];
+        if (t < sb * sb) s_part[wave * 64 + lane] = part;
+        __syncthreads();
+        if (t < sb * sb && way == 0) {
+          for (uint32_t v = 1; v < ways; ++v) part += s_part[(wave + v) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[4 * q + e] = part[e];
+        }
+        __syncthreads();
+      }
+      if (t < sb * sb && way == 0) put(s, sh.row_s, plane_s, bi, bj, acc * (1.0f / kScale));
+    } else {
+#pragma unroll
+      for (int u = 0; u < BLOCKS; ++u) {
+        const uint32_t t = fresh(wave) + static_cast<uint32_t>(u) * WAVES;
+        if (t < sb * sb) {
+          const uint32_t bi = t / sb, bj = t % sb;
+          const f32x16_t acc = product_of(0, sh.depth / 16, x_rows(bi * 32), x_rows(bj * 32));
+          put(s, sh.row_s, plane_s, bi, bj, acc * (1.0f / kScale));
+        }
       }
     }
     __syncthreads();
@@ -302,7 +361,7 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
       if (t < sb * sb) {
         const uint32_t bi = t / sb, bj = t % sb;
         f32x16_t acc = product_of(
-            sh.side / 16, [&](uint32_t p, uint32_t kk) { return rows(s + p * plane_s, sh.row_s, bi * 32, kk); },
+            0, sh.side / 16, [&](uint32_t p, uint32_t kk) { return rows(s + p * plane_s, sh.row_s, bi * 32, kk); },
             [&](uint32_t p, uint32_t kk) { return rows(s + p * plane_s, sh.row_s, bj * 32, kk); });
         const char* at = s + (bj * 32 + j32) * sh.row_s + (bi * 32 + 4 * h) * 2;
 #pragma unroll
@@ -333,7 +392,7 @@ __global__ void __launch_bounds__(WAVES * 64) ortho_small_kernel(const T* __rest
       if (t < sb * db) {
         const uint32_t bi = t / sb, bj = t % sb;  // columns of X, rows of P
         kept[u] = product_of(
-            sh.side / 16, [&](uint32_t p, uint32_t kk) { return by_k(x + p * plane_x, sh.row_x, bi * 32, kk); },
+            0, sh.side / 16, [&](uint32_t p, uint32_t kk) { return by_k(x + p * plane_x, sh.row_x, bi * 32, kk); },
             [&](uint32_t p, uint32_t kk) { return rows(s + p * plane_s, sh.row_s, bj * 32, kk); });
       }
     }
@@ -477,7 +536,7 @@ void orthogonalize(const T* update, uint64_t batch, uint32_t m, uint32_t n, uint
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(batch)), dim3(W * 64), sh.bytes, s, update, m, n, steps,
                          a, b, c, out);
     };
-    if (sh.side / 32 * (sh.depth / 32) <= 16) {  // side <= depth, so S has no more blocks than X
+    if (small_waves(sh) == 16) {  // side <= depth, so S has no more blocks than X
       go(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
     } else {
       go(std::integral_constant<int, 8>{}, std::integral_constant<int, 5>{});
