@@ -759,8 +759,9 @@ void launch_tile(GemmArgs g, const Epi& epi, hipStream_t s) {
   QVH_HIP(hipGetLastError());
 }
 
-/// How a product reads its operands, and the shapes it may take. With more than one plane a step is 32 deep, so
-/// that LDS holds two or three.
+/// How a product reads its operands, and the shapes it may take. A row of a 64-deep step is a whole 128-byte line
+/// of the L2, of a 32-deep one half of it; with more than one plane only the small tiles, or one work-group on
+/// a CU, have the LDS for two such steps.
 enum class Kind : int {
   kPlane1 = 0,  // 16-bit operands
   kPlane2 = 1,  // two 16-bit planes
@@ -779,9 +780,10 @@ struct Shapes<Kind::kPlane1> {
 };
 template <>
 struct Shapes<Kind::kPlane2> {
-  using S0 = Tile<64, 64, 2, 2, 32, 3, 2>;
+  using S0 = Tile<64, 64, 2, 2, 64, 2, 2>;
   using S1 = Tile<128, 128, 2, 2, 32, 2, 2>;
   using S2 = Tile<256, 128, 4, 2, 32, 3, 2>;
+  using Alone = Tile<128, 128, 2, 4, 64, 2, 2>;
 };
 template <>
 struct Shapes<Kind::kPlane3> {
@@ -817,6 +819,12 @@ void launch_gemm(GemmArgs g, const Epi& epi, const GemmPlan& plan, void* partial
   if constexpr (!std::is_void_v<typename S::S2>) {
     // A symmetric product's tiles are square.
     if (plan.tile == 2 && (S::S2::BM == S::S2::BN || !g.symmetric)) return launch_tile<T, AK, BK, typename S::S2>(g, epi, s);
+  }
+  if constexpr (K == Kind::kPlane2) {
+    // The deep tile where every work-group has a CU to itself; past that two shallow ones on a CU hide each
+    // other's waits (orthogonalisation of 1,024 x 4,096 393 us, 364 with it; six of 678 x 1,096 451, 482).
+    const uint64_t groups = ceil_div(g.m, 128) * ceil_div(g.n, 128) * g.splits * g.batches;
+    if (plan.tile == 1 && groups <= 256) return launch_tile<T, AK, BK, typename S::Alone>(g, epi, s);
   }
   if (plan.tile >= 1) return launch_tile<T, AK, BK, typename S::S1>(g, epi, s);
   launch_tile<T, AK, BK, typename S::S0>(g, epi, s);

@@ -277,7 +277,6 @@ __global__ void __launch_bounds__(kFewWaves * 64) few_rows_kernel(const T* __res
 #pragma unroll
   for (int t = 0; t < MT; ++t) xr[t] = x + static_cast<uint64_t>(m0 + 16 * t + i < m ? m0 + 16 * t + i : m - 1) * ldx;
   f32x4_t acc[MT] = {};
-#pragma unroll 4
   for (uint32_t k0 = wave * kDepth; k0 < k; k0 += kFewWaves * kDepth) {
     F fw, fx[MT];
     load_k<T>(wr, k0 + h * kEach, k, fw);
