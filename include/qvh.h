@@ -358,8 +358,9 @@ qvh_status qvh_embed_device(const void* d_table, uint64_t rows, uint32_t dim, ui
                             const void* d_tokens, int index_bytes, uint64_t count, float scale, void* d_out,
                             void* stream);
 
-/* The table's gradient out[rows][dim]: scale * the sum of grad[t] over the tokens t that name the row, in
- * order of t; zero for rows that no token names. Tokens outside the table add nothing. */
+/* The table's gradient out[rows][dim]: scale * the fp32 sum of grad[t] over the tokens t that name the row, in
+ * an order that depends on the tokens alone; zero for rows that no token names. Tokens outside the table
+ * add nothing. */
 qvh_status qvh_embed_grad_workspace(uint64_t rows, uint32_t dim, uint64_t count, uint64_t* bytes);
 qvh_status qvh_embed_grad_device(const void* d_grad, uint64_t row_stride, const void* d_tokens, int index_bytes,
                                  uint64_t count, uint64_t rows, uint32_t dim, int dtype, float scale, void* d_out,
@@ -368,8 +369,9 @@ qvh_status qvh_embed_grad_device(const void* d_grad, uint64_t row_stride, const 
 /* A linear layer: z = x w^T + bias, out = act(z) + residual, with x [m][k], w [n][k], bias [n] (nullable),
  * residual [m][n] (nullable), out [m][n]; z is also stored to `preactivation` (nullable), which the
  * backward pass of an activation takes. out may be the residual's own buffer, and no other overlap is
- * allowed. m is below 2^31, k and n at most 2^20, strides at most 2^22. fp32 products run as sums of
- * three bf16 parts of each operand (24 bits; what is dropped is below fp32's own rounding). */
+ * allowed. m is below 2^31, k and n at most 2^20, strides at most 2^22. fp32 products run on fp32 matrix
+ * instructions, large ones as sums of three bf16 parts of each operand (24 bits; what is dropped is below
+ * fp32's own rounding). */
 typedef struct qvh_linear_args {
   uint64_t m;
   uint32_t k, n;

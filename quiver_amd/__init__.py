@@ -16,6 +16,10 @@ distances (float32) come back as tensors on the same device, without a round tri
 memory. torch must be imported before quiver_amd for this: torch ships its own HIP runtime, and
 memory of one runtime copy cannot be used by another (a ValueError says so). The scans run as hand-written HIP kernels on the GPU (``quiver_amd/lib/libqvh.so``);
 there is no CPU fallback: without a gfx950 device, adding or searching raises ``ValueError``.
+
+In front of an index, ``embed``, ``linear`` and their gradients ``embed_grad``, ``linear_grad``, and
+``orthogonalize`` make and train the vectors on torch tensors (quiver_amd/encoder.py;
+examples/encoder_search.py trains a small text encoder, indexes its vectors and searches them).
 """
 
 from __future__ import annotations

@@ -3,7 +3,7 @@
 // Lookup: y[t] = scale * table[token[t]], a row of zeros where the token is outside the table. One
 // pass that reads each named row and writes each output row; memory traffic is the whole cost.
 //
-// Gradient: dE[v] = scale * sum of dy[t] over the t with token[t] = v, in order of t, in fp32. The
+// Gradient: dE[v] = scale * sum of dy[t] over the t with token[t] = v, in fp32. The
 // tokens are sorted (stable, least significant digit first), so equal tokens are neighbours; waves
 // then sum fixed pieces of the sorted list, and runs that cross a piece are joined in order by a
 // second launch. Which partial sums are formed depends on the tokens alone, never on timing, so a
@@ -23,46 +23,29 @@ constexpr uint32_t kMaxDim = 32768;
 
 // ---- lookup -----------------------------------------------------------------------------------
 
-/// Piece c of a row is V elements (vector_width), cpr pieces a row; U pieces per thread, 256 apart, so that each
-/// thread has U independent row reads in flight.
-template <class T, int V, class I, int U>
+/// Piece c of a row is V elements (vector_width), cpr pieces a row, a piece per thread. Bound by memory: 250,007
+/// tokens of 100 fp32 (a fifth of them padding) in a table of 1.18 million rows 23.6 us, 182 MB at 7.7 TB/s with the
+/// frequent rows from the caches; 24 tokens of 768 bf16 2.4 us, the launch. Four pieces per thread, 256 apart, are
+/// no faster at any size (2,048 x 1,024 bf16 3.4 us, one piece 2.8; 250,007 x 100 26.8, 26.2).
+template <class T, int V, class I>
 __global__ void __launch_bounds__(256) embed_kernel(const T* __restrict__ table, uint64_t rows, uint64_t stride,
                                                     const I* __restrict__ tokens, uint64_t count, uint32_t dim,
                                                     uint32_t cpr, uint32_t magic, float scale, T* __restrict__ out) {
-  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * (256 * U);
-  const uint64_t t0 = first / cpr;
-  const uint32_t lead = static_cast<uint32_t>(first - t0 * cpr);
-  const uint64_t total = count * cpr;
-  uint64_t at[U], row[U];
-  uint32_t col[U];
-  int64_t tok[U];
+  // The work-group's first piece by a division; (lead + index) / cpr by a multiplication: exact below 2^32 / cpr.
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * 256, t0 = first / cpr;
+  const uint32_t i = static_cast<uint32_t>(first - t0 * cpr) + threadIdx.x;
+  const uint32_t q = cpr == 1 ? i : __umulhi(i, magic);
+  uint32_t col = (i - q * cpr) * V;
+  col = col < dim - V ? col : dim - V;
+  if (t0 + q >= count) return;
+  const int64_t tok = static_cast<int64_t>(tokens[t0 + q]);
+  float x[V] = {};
+  if (tok >= 0 && static_cast<uint64_t>(tok) < rows) {
+    load_floats<T, V>(table + static_cast<uint64_t>(tok) * stride + col, x);
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    // (lead + index) / cpr by a multiplication: exact below 2^32 / cpr.
-    const uint32_t i = lead + u * 256 + threadIdx.x;
-    const uint32_t q = cpr == 1 ? i : __umulhi(i, magic);
-    at[u] = first + u * 256 + threadIdx.x;
-    row[u] = t0 + q;
-    col[u] = (i - q * cpr) * V;
-    col[u] = col[u] < dim - V ? col[u] : dim - V;
-    tok[u] = at[u] < total ? static_cast<int64_t>(tokens[t0 + q]) : -1;
+    for (int e = 0; e < V; ++e) x[e] *= scale;
   }
-  float x[U][V];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (tok[u] >= 0 && static_cast<uint64_t>(tok[u]) < rows) {
-      load_floats<T, V>(table + static_cast<uint64_t>(tok[u]) * stride + col[u], x[u]);
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[u][i] *= scale;
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[u][i] = 0.0f;
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (at[u] < total) store_floats<T, V>(out + row[u] * dim + col[u], x[u]);
-  }
+  store_floats<T, V>(out + (t0 + q) * dim + col, x);
 }
 
 template <class T, class I>
@@ -72,28 +55,47 @@ void launch_embed(const void* table, uint64_t rows, uint32_t dim, uint64_t strid
     constexpr int V = decltype(width)::value;
     const uint32_t cpr = static_cast<uint32_t>(ceil_div(dim, V));
     const uint32_t magic = cpr == 1 ? 0u : static_cast<uint32_t>((uint64_t{1} << 32) / cpr + 1);
-    const uint64_t total = count * cpr;
-    const auto go = [&](auto unroll) {
-      constexpr int U = decltype(unroll)::value;
-      const uint64_t blocks = ceil_div(total, 256 * U);
-      QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "qvh_embed_device: too many tokens");
-      hipLaunchKernelGGL((embed_kernel<T, V, I, U>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s,
-                         static_cast<const T*>(table), rows, stride, static_cast<const I*>(tokens), count, dim, cpr, magic,
-                         scale, static_cast<T*>(out));
-    };
-    if (total < 256 * 1024) {
-      go(std::integral_constant<int, 1>{});
-    } else {
-      go(std::integral_constant<int, 4>{});
-    }
+    const uint64_t blocks = ceil_div(count * cpr, 256);
+    QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "qvh_embed_device: too many tokens");
+    hipLaunchKernelGGL((embed_kernel<T, V, I>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s,
+                       static_cast<const T*>(table), rows, stride, static_cast<const I*>(tokens), count, dim, cpr, magic, scale,
+                       static_cast<T*>(out));
   });
   QVH_HIP(hipGetLastError());
 }
 
 // ---- gradient of a small batch: rows look for their tokens ------------------------------------
 
-constexpr uint32_t kOwnTokens = 2048;
+constexpr uint32_t kOwnTokens = 2048;  // what LDS has room for
 
+/// Rows per wave: as few as there are waves at once, since a wave's rows follow one another, each waiting for its
+/// gradient rows (10,000 rows, 1,000 tokens of 128 fp32: four rows 13 us, two 11).
+uint32_t own_rows(uint64_t rows, uint64_t count) {
+  const uint64_t lds = std::max<uint64_t>(count, 1) * 24;  // per work-group of four waves
+  const uint64_t at_once = 256 * 4 * std::min<uint64_t>(8, 160 * 1024 / lds);
+  return static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(ceil_div(rows, at_once), 1), 64));
+}
+
+/// Whether a batch is small enough for rows to look for their tokens: by estimates of both ways, in us. The own way
+/// is slow where one wave has many tokens to add, one round of loads after another, or many rows to write; the
+/// sorted one is six launches or more. (No dtype: rows of 16-bit and 32-bit elements take as many rounds.) Both
+/// sides, own way first: 10,000 rows of 128, fp16, 512 tokens 8.2 and 24.4, 2,048 tokens 29.5 and 26.6; 32,000
+/// rows of 1,024, 512 tokens 63 and 35; a million rows of 100, 512 tokens 189 and 58; 1,000 of 64, 2,048 tokens
+/// 15.6 and 27.1.
+bool rows_look(uint64_t rows, uint32_t dim, uint64_t count) {
+  if (count > kOwnTokens) return false;
+  const uint64_t pieces = ceil_div(dim, 8), lanes = pieces <= 16 ? 16 : pieces <= 32 ? 32 : 64;
+  const uint64_t rounds = ceil_div(count, 64 / lanes * 8) * ceil_div(pieces, lanes);
+  const uint64_t waves = ceil_div(rows, own_rows(rows, count));
+  const uint64_t turns = ceil_div(waves, 256 * 4 * std::min<uint64_t>(8, 160 * 1024 / (std::max<uint64_t>(count, 1) * 24)));
+  const double own = 3.0 + 0.25 * static_cast<double>(rounds) + 1.3 * static_cast<double>(turns * own_rows(rows, count));
+  const int passes = rows < 256 ? 1 : rows < 65536 ? 2 : rows < (1u << 24) ? 3 : 4;
+  const double sorted = 9.0 + 7.5 * passes + static_cast<double>(rows) * dim / 3e6;
+  return own < sorted;
+}
+
+/// 1,000 tokens in 10,000 rows of 128 fp32: 9.8 us, where the 5 MB of the table and 0.5 MB of gradients would
+/// take 1.1; bound by the chain token, match, gradient row of the wave with the most frequent tokens.
 /// One wave per `own` rows (at most 64): lists the batch's tokens that fall into its rows, then per row
 /// the positions of its tokens, whose gradient rows are added: 64 / G at a time, each by G lanes that take
 /// V columns, every such share in order of position and the shares in order.
@@ -406,7 +408,9 @@ __device__ __forceinline__ void zero_rows(const SumArgs& a, uint32_t block, uint
   }
 }
 
-/// Groups of G lanes, each adding one piece of the list over G * V columns (slab blockIdx.y).
+/// Groups of G lanes, each adding one piece of the list over G * V columns (slab blockIdx.y). Bound by memory: of
+/// 262,144 tokens of 1,024 bf16 in 32,000 rows (537 MB read, 66 MB written) 143 us, 4.2 TB/s, where a copy
+/// reaches 4.98; it reads rows in an order of its own, 1 KB of each.
 template <class T, int V, int G>
 __global__ void __launch_bounds__(256) embed_grad_sum_kernel(SumArgs a) {
   constexpr uint32_t kGroups = 256 / G;
@@ -573,7 +577,7 @@ struct GradLayout {
 
 GradLayout grad_layout(uint64_t rows, uint32_t dim, uint64_t count) {
   GradLayout l{};
-  if (count <= kOwnTokens) return l;
+  if (rows_look(rows, dim, count)) return l;
   const auto round = [](size_t b) { return (b + 255) / 256 * 256; };
   l.part = static_cast<uint32_t>(std::max<uint64_t>(ceil_div(count, kParts), 1024));
   l.parts = static_cast<uint32_t>(ceil_div(count, l.part));
@@ -603,12 +607,8 @@ template <class T, class I>
 void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, uint64_t count, uint64_t rows,
                        uint32_t dim, float scale, void* out, char* ws, hipStream_t s) {
   const int width = vector_width(sizeof(T), dim);
-  if (count <= kOwnTokens) {
-    // As few rows per wave as the device holds waves for at once: a wave's rows follow one another, each
-    // waiting for its gradient rows (10,000 rows, 1,000 tokens of 128 fp32: four rows 13 us, two 11).
-    const uint32_t lds = static_cast<uint32_t>(std::max<uint64_t>(count, 1)) * 24;
-    const uint64_t at_once = 256 * 4 * std::min<uint64_t>(8, 160 * 1024 / lds);
-    const uint32_t own = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(ceil_div(rows, at_once), 1), 64));
+  if (rows_look(rows, dim, count)) {
+    const uint32_t lds = static_cast<uint32_t>(std::max<uint64_t>(count, 1)) * 24, own = own_rows(rows, count);
     with_width<T>(width, [&](auto v) {
       constexpr int V = decltype(v)::value;
       const auto go = [&](auto group) {

@@ -1,19 +1,30 @@
-// Matrix product of the encoder operators on the 16-bit matrix unit: C[m][n] = sum_k A(m, k) B(n, k),
-// accumulated in fp32, with an epilogue.
+// Matrix product of the encoder operators on the matrix unit: C[m][n] = sum_k A(m, k) B(n, k), accumulated in
+// fp32, with an epilogue.
 //
-// Operands. Each is a 16-bit matrix, stored either by rows ([row][k], k contiguous) or by k ([k][row],
-// row contiguous): a layer's forward pass reads both by rows, its input gradient the weight by k, its
-// weight gradient both by k, so no pass ever transposes a matrix in memory. Operands of more than 16 bits
-// come as a sum of two or three 16-bit planes; a step then holds all of them, and every fragment that was
-// read from LDS enters two or three of the three or six products that count.
+// Operands. Each is stored either by rows ([row][k], k contiguous) or by k ([k][row], row contiguous): a
+// layer's forward pass reads both by rows, its input gradient the weight by k, its weight gradient both by
+// k, so no pass ever transposes a matrix in memory. Elements are of 16 bits, or fp32 for the fp32
+// instructions. Operands of more than 16 bits may also come as a sum of two or three 16-bit planes; a step then
+// holds all of them, and every fragment that was read from LDS enters two or three of the three or six
+// products that count.
 //
-// A work-group takes a BM x BN tile in 64-deep steps. The steps go from memory straight into LDS
-// (16 bytes per lane, no registers), the next one while the present one is multiplied; LDS holds
-// each row's (or each k's) 16-byte pieces permuted so that the fragments of the matrix unit are read
-// without bank conflicts, and because such loads fill LDS in lane order the permutation is in the
-// addresses that the lanes load from. Nothing is read outside the operands: rows and k past the end
-// are clamped to the last one, the results of clamped rows are not stored, and elements past the last
-// k are replaced by zeros in registers, in the last step only.
+// A work-group takes a BM x BN tile in steps of 64 or 32 k. The steps go from memory straight into LDS
+// (16 bytes per lane where the rows are aligned so, 4 otherwise; no registers), the next one or two while the
+// present one is multiplied; LDS holds each row's (or each k's) 16-byte pieces permuted so that the
+// fragments of the matrix unit are read without bank conflicts, and because such loads fill LDS in lane order
+// the permutation is in the addresses that the lanes load from. Nothing is read outside the operands: rows
+// and k past the end are clamped to the last one, the results of clamped rows are not stored, and elements past
+// the last k are replaced by zeros in registers, in the last step only.
+//
+// Work-groups go to the XCDs in runs of neighbouring tiles, so that an L2 reads an operand about once: 16,384 x
+// 1,024 x 4,096 bf16 fetches 203 MB, of operands of 42 of which every XCD needs the weight's 8.
+//
+// What bounds it. Large products, by the matrix unit and the clock under load: 8,192^3 bf16 about 1,200 TFLOP/s, its
+// instructions busy 63% of the time at 1.7 GHz (the installed library: 1,500). A layer of 16,384 x 1,024 x 4,096 with GELU and the
+// kept pre-activation, by its 16 steps' start and the 268 MB that its epilogue writes at the end of every tile:
+// 187 us, 735 TFLOP/s, the main loop alone 115. Small products, by the latency of a step (0.4 to 0.7 us) and a
+// launch. Tried without gain: five or more steps ahead, loads spread over several slices, prefetches into the L2,
+// wave priorities, tiles of 256 x 256 with four waves.
 #pragma once
 
 #include "types16.hpp"
@@ -676,7 +687,8 @@ __device__ __forceinline__ void add_splits(const float* p, uint32_t splits, uint
   }
 }
 
-/// Adds the splits' partial sums and runs the epilogue.
+/// Adds the splits' partial sums and runs the epilogue. Four splits of 4,096 x 1,024: 67 MB from the last-level
+/// cache and 8 out in 13 us.
 template <class Epi>
 __global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs g, Epi epi) {
   const uint32_t ld = (g.n + 7) / 8 * 8;
@@ -689,8 +701,9 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs g, Epi epi) {
   epi(blockIdx.y, static_cast<uint32_t>(m), n, g.n - n, v);
 }
 
-/// The same for a symmetric product, of which only the lower tiles have sums: work-groups of 128 threads per
-/// 32 x 32 block of the lower triangle, which go through LDS to their mirrored places.
+/// The same for a symmetric product (1,024 x 1,024 in three splits 5 us), of which only the lower tiles have
+/// sums: work-groups of 128 threads per 32 x 32 block of the lower triangle, which go through LDS to their
+/// mirrored places.
 template <class Epi>
 __global__ void __launch_bounds__(128) gemm_join_symmetric_kernel(GemmArgs g, Epi epi) {
   __shared__ float s_block[32][33];

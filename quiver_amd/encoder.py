@@ -132,8 +132,8 @@ def embed(table, tokens, scale: float = 1.0):
 def embed_grad(grad, tokens, rows: int, scale: float = 1.0):
     """The table's gradient [rows, dim] from the gradient of ``embed``'s result.
 
-    Each row is ``scale`` times the sum of the gradients of the tokens that name it, in their order, in
-    fp32; zero where no token does. Tokens outside the table add nothing.
+    Each row is ``scale`` times the sum of the gradients of the tokens that name it, in fp32 and in an order
+    that depends on the tokens alone; zero where no token does. Tokens outside the table add nothing.
     """
     _check("grad", grad)
     device = grad.device

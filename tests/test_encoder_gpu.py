@@ -138,6 +138,30 @@ def test_embed_grad(dtype, rows, dim, count):
     _check_embed_grad(grad, tok.int(), rows, dtype)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,dim,count", [
+    (1000, 64, 2048), (3000, 768, 300), (3000, 768, 1000), (32_000, 1024, 512), (300_000, 100, 100), (200, 512, 2047),
+    (65_536, 3, 40), (1, 1, 2048), (255, 9, 1900)])
+def test_embed_grad_of_small_batches(dtype, rows, dim, count):
+    """Either side of the choice between rows that look for their tokens and sorted tokens, frequent tokens first."""
+    g = torch.Generator().manual_seed(rows + dim + count)
+    _say("embed_grad small", dtype, rows, dim, count)
+    grad = _randn(g, count, dim, dtype=dtype)
+    tok = (torch.exp(torch.rand(count, generator=g, dtype=torch.float64) * math.log(rows + 1.0)) - 1).long().clamp(0, rows - 1)
+    _check_embed_grad(grad, tok.to(_gpu()), rows, dtype)
+
+
+@pytest.mark.parametrize("dim", [1, 30, 300])
+def test_embed_grad_joins_short_and_long_runs(dim):
+    """Runs of 1 to 4,000 tokens, so that some end in their piece, some in the next ones and some far behind."""
+    _say("embed_grad joins", dim)
+    g = torch.Generator().manual_seed(dim)
+    lengths = [1, 4000, 15, 16, 17, 1, 250, 256, 260, 272, 3, 31, 32, 33, 2000, 700, 8, 8, 8]
+    tok = torch.repeat_interleave(torch.arange(len(lengths)) * 3, torch.tensor(lengths))
+    tok = tok[torch.randperm(len(tok), generator=g)].to(_gpu())
+    _check_embed_grad(_randn(g, len(tok), dim, dtype="fp32"), tok, 60, "fp32")
+
+
 @pytest.mark.parametrize("count", [700, 2048, 6400, 6401, 50_000])
 @pytest.mark.parametrize("kind", ["one token", "two tokens", "blocks", "padding", "falling", "last row"])
 def test_embed_grad_runs(kind, count):
@@ -476,6 +500,13 @@ def test_orthogonalize(dtype, shape):
         size = want.flatten(-2).norm(dim=-1)
         assert bool((err <= bound + ROUND[dtype] * size).all()), (steps, err.max().item(), bound)
         assert torch.equal(got, quiver.orthogonalize(u, steps=steps, coefficients=co))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(128, 128), (64, 512), (512, 64), (32, 1100), (1100, 26), (2, 5, 1100), (64, 200), (79, 1220), (1024, 96),
+                                   (128, 1300), (1, 2048), (2049, 2), (640, 640), (3, 384, 300)])
+def test_orthogonalize_long_and_large(dtype, shape):
+    test_orthogonalize(dtype, shape)
 
 
 def test_orthogonalize_makes_singular_values_alike():
