@@ -23,29 +23,48 @@ constexpr uint32_t kMaxDim = 32768;
 
 // ---- lookup -----------------------------------------------------------------------------------
 
-/// Piece c of a row is V elements (vector_width), cpr pieces a row, a piece per thread. Bound by memory: 250,007
-/// tokens of 100 fp32 (a fifth of them padding) in a table of 1.18 million rows 23.6 us, 182 MB at 7.7 TB/s with the
-/// frequent rows from the caches; 24 tokens of 768 bf16 2.4 us, the launch. Four pieces per thread, 256 apart, are
-/// no faster at any size (2,048 x 1,024 bf16 3.4 us, one piece 2.8; 250,007 x 100 26.8, 26.2).
-template <class T, int V, class I>
+/// Piece c of a row is V elements (vector_width), cpr pieces a row; U pieces per thread, 256 apart, so that each
+/// thread has U independent row reads in flight. Bound by memory: 250,007 tokens of 100 fp32 (a fifth of them
+/// padding) in a table of 1.18 million rows 31.6 us a call with the table in HBM, 182 MB at 5.8 TB/s; 24 tokens
+/// of 768 bf16 2.4 us, the launch.
+template <class T, int V, class I, int U>
 __global__ void __launch_bounds__(256) embed_kernel(const T* __restrict__ table, uint64_t rows, uint64_t stride,
                                                     const I* __restrict__ tokens, uint64_t count, uint32_t dim,
                                                     uint32_t cpr, uint32_t magic, float scale, T* __restrict__ out) {
-  // The work-group's first piece by a division; (lead + index) / cpr by a multiplication: exact below 2^32 / cpr.
-  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * 256, t0 = first / cpr;
-  const uint32_t i = static_cast<uint32_t>(first - t0 * cpr) + threadIdx.x;
-  const uint32_t q = cpr == 1 ? i : __umulhi(i, magic);
-  uint32_t col = (i - q * cpr) * V;
-  col = col < dim - V ? col : dim - V;
-  if (t0 + q >= count) return;
-  const int64_t tok = static_cast<int64_t>(tokens[t0 + q]);
-  float x[V] = {};
-  if (tok >= 0 && static_cast<uint64_t>(tok) < rows) {
-    load_floats<T, V>(table + static_cast<uint64_t>(tok) * stride + col, x);
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * (256 * U);
+  const uint64_t t0 = first / cpr;
+  const uint32_t lead = static_cast<uint32_t>(first - t0 * cpr);
+  const uint64_t total = count * cpr;
+  uint64_t at[U], row[U];
+  uint32_t col[U];
+  int64_t tok[U];
 #pragma unroll
-    for (int e = 0; e < V; ++e) x[e] *= scale;
+  for (int u = 0; u < U; ++u) {
+    // (lead + index) / cpr by a multiplication: exact below 2^32 / cpr.
+    const uint32_t i = lead + u * 256 + threadIdx.x;
+    const uint32_t q = cpr == 1 ? i : __umulhi(i, magic);
+    at[u] = first + u * 256 + threadIdx.x;
+    row[u] = t0 + q;
+    col[u] = (i - q * cpr) * V;
+    col[u] = col[u] < dim - V ? col[u] : dim - V;
+    tok[u] = at[u] < total ? static_cast<int64_t>(tokens[t0 + q]) : -1;
   }
-  store_floats<T, V>(out + (t0 + q) * dim + col, x);
+  float x[U][V];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (tok[u] >= 0 && static_cast<uint64_t>(tok[u]) < rows) {
+      load_floats<T, V>(table + static_cast<uint64_t>(tok[u]) * stride + col[u], x[u]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[u][i] *= scale;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[u][i] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (at[u] < total) store_floats<T, V>(out + row[u] * dim + col[u], x[u]);
+  }
 }
 
 template <class T, class I>
@@ -55,11 +74,23 @@ void launch_embed(const void* table, uint64_t rows, uint32_t dim, uint64_t strid
     constexpr int V = decltype(width)::value;
     const uint32_t cpr = static_cast<uint32_t>(ceil_div(dim, V));
     const uint32_t magic = cpr == 1 ? 0u : static_cast<uint32_t>((uint64_t{1} << 32) / cpr + 1);
-    const uint64_t blocks = ceil_div(count * cpr, 256);
-    QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "qvh_embed_device: too many tokens");
-    hipLaunchKernelGGL((embed_kernel<T, V, I>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s,
-                       static_cast<const T*>(table), rows, stride, static_cast<const I*>(tokens), count, dim, cpr, magic, scale,
-                       static_cast<T*>(out));
+    const uint64_t total = count * cpr;
+    const auto go = [&](auto unroll) {
+      constexpr int U = decltype(unroll)::value;
+      const uint64_t blocks = ceil_div(total, 256 * U);
+      QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "qvh_embed_device: too many tokens");
+      hipLaunchKernelGGL((embed_kernel<T, V, I, U>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s,
+                         static_cast<const T*>(table), rows, stride, static_cast<const I*>(tokens), count, dim, cpr, magic,
+                         scale, static_cast<T*>(out));
+    };
+    // Two pieces per thread where the device is full several times over; below, one. Both sides, one and two, with
+    // the tables in HBM: 250,007 x 100 fp32 35.1 and 32.0 us, 60,000 x 1,024 bf16 40.3 and 36.0; 16,000 x 100
+    // fp32 3.8 and 4.2. (Four: 33.1, 36.4, 4.8.)
+    if (total < (1u << 21)) {
+      go(std::integral_constant<int, 1>{});
+    } else {
+      go(std::integral_constant<int, 2>{});
+    }
   });
   QVH_HIP(hipGetLastError());
 }
