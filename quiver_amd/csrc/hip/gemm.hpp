@@ -141,12 +141,12 @@ struct RowChunk {
   uint64_t row;
   uint32_t chunk;
 };
-__device__ __forceinline__ RowChunk row_and_chunk(uint32_t block, uint32_t per_row) {
+__device__ __forceinline__ RowChunk row_and_chunk(uint32_t block, uint32_t per_row, uint32_t thread) {
   if (block < (1u << 24)) {
-    const uint32_t i = block * 256 + threadIdx.x, r = i / per_row;
+    const uint32_t i = block * 256 + thread, r = i / per_row;
     return {r, i - r * per_row};
   }
-  const uint64_t i = static_cast<uint64_t>(block) * 256 + threadIdx.x, r = i / per_row;
+  const uint64_t i = static_cast<uint64_t>(block) * 256 + thread, r = i / per_row;
   return {r, static_cast<uint32_t>(i - r * per_row)};
 }
 
@@ -209,6 +209,31 @@ __device__ __forceinline__ float direct_element(const GemmArgs& g, bool a_by_k, 
   return sum;
 }
 
+/// Column sums of work-groups that share the rows, [part][cols rounded up to 8], to be added up.
+struct ColumnSums {
+  const float* parts = nullptr;
+  uint32_t count = 0, cols = 0;
+};
+
+/// 64 columns' parts, in order: four waves take contiguous shares of them.
+template <class T>
+__device__ __forceinline__ void add_columns(const ColumnSums& a, uint32_t block, T* __restrict__ out) {
+  __shared__ float s_sum[4][64];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ld = (a.cols + 7) / 8 * 8;
+  const uint32_t c = block * 64 + lane, share = (a.count + 3) / 4;
+  const uint32_t p0 = wave * share < a.count ? wave * share : a.count, p1 = p0 + share < a.count ? p0 + share : a.count;
+  float t = 0.0f;
+  if (c < a.cols) {
+#pragma unroll 8
+    for (uint32_t p = p0; p < p1; ++p) t += a.parts[static_cast<uint64_t>(p) * ld + c];
+  }
+  s_sum[wave][lane] = t;
+  __syncthreads();
+  if (wave == 0 && c < a.cols) {
+    out[c] = static_cast<T>(((s_sum[0][lane] + s_sum[1][lane]) + s_sum[2][lane]) + s_sum[3][lane]);
+  }
+}
+
 /// y = act(acc + bias) + residual, the sum in front of the activation kept where it is asked for.
 template <class T>
 struct LinearEpilogue {
@@ -220,6 +245,9 @@ struct LinearEpilogue {
   int act = QVH_ACT_NONE;
   GemmArgs direct;  // fp32 by planes: the product itself, for elements that come out as NaN
   int a_by_k = 0, b_by_k = 0, planes = 0;
+  // Column sums that the launch which joins a product's splits adds up besides, and where they go.
+  ColumnSums columns;
+  T* column_out = nullptr;
 
   /// The same for one element.
   __device__ __forceinline__ void one(uint32_t m, uint32_t n, float v) const {
@@ -687,12 +715,24 @@ __device__ __forceinline__ void add_splits(const float* p, uint32_t splits, uint
   }
 }
 
-/// Adds the splits' partial sums and runs the epilogue. Four splits of 4,096 x 1,024: 67 MB from the last-level
-/// cache and 8 out in 13 us.
 template <class Epi>
-__global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs g, Epi epi) {
+struct HasColumns {
+  static constexpr bool value = false;
+};
+template <class T>
+struct HasColumns<LinearEpilogue<T>> {
+  static constexpr bool value = true;
+};
+
+/// Adds the splits' partial sums and runs the epilogue. Four splits of 4,096 x 1,024: 67 MB from the last-level
+/// cache and 8 out in 13 us. Work-groups from `blocks` on add column sums.
+template <class Epi>
+__global__ void __launch_bounds__(256) gemm_join_kernel(GemmArgs g, Epi epi, uint32_t blocks) {
+  if constexpr (HasColumns<Epi>::value) {
+    if (blockIdx.x >= blocks) return add_columns(epi.columns, blockIdx.x - blocks, epi.column_out);
+  }
   const uint32_t ld = (g.n + 7) / 8 * 8;
-  const auto [m, chunk] = row_and_chunk(blockIdx.x, ld / 8);
+  const auto [m, chunk] = row_and_chunk(blockIdx.x, ld / 8, threadIdx.x);
   if (m >= g.m) return;
   const uint32_t n = chunk * 8;
   const uint64_t batch = static_cast<uint64_t>(g.m) * ld;
@@ -763,8 +803,10 @@ void launch_tile(GemmArgs g, const Epi& epi, hipStream_t s) {
       const uint32_t side = static_cast<uint32_t>(ceil_div(g.m, 32));
       hipLaunchKernelGGL((gemm_join_symmetric_kernel<Epi>), dim3(side * (side + 1) / 2, g.batches), dim3(128), 0, s, g, epi);
     } else {
-      hipLaunchKernelGGL((gemm_join_kernel<Epi>), dim3(static_cast<unsigned>(ceil_div(ld / 8 * g.m, 256)), g.batches),
-                         dim3(256), 0, s, g, epi);
+      const uint32_t join = static_cast<uint32_t>(ceil_div(ld / 8 * g.m, 256));
+      uint32_t more = 0;
+      if constexpr (HasColumns<Epi>::value) more = static_cast<uint32_t>(ceil_div(epi.columns.cols, 64));
+      hipLaunchKernelGGL((gemm_join_kernel<Epi>), dim3(join + more, g.batches), dim3(256), 0, s, g, epi, join);
     }
   } else {
     hipLaunchKernelGGL((gemm_kernel<T, AK, BK, Shape, Epi>), grid, dim3(Shape::WM * Shape::WN * 64), 0, s, g, epi);

@@ -62,7 +62,7 @@ namespace {
 
 constexpr uint64_t kMaxRows = uint64_t{1} << 31, kMaxStride = uint64_t{1} << 22;
 constexpr uint32_t kMaxWidth = 1u << 20;
-constexpr uint64_t kSumRows = 128;  // rows whose column sums one work-group makes
+constexpr uint64_t kSumRows = 512;  // rows whose column sums one work-group makes
 constexpr int kPlanes = 3;         // bf16 parts of an fp32 value
 
 // ---- operand preparation ----------------------------------------------------------------------
@@ -113,11 +113,11 @@ __device__ __forceinline__ void store_prepared(void* dst, uint64_t at, uint64_t 
 /// Copies up to two matrices into rows that the tiled product can read: aligned, padded with zeros, fp32 in
 /// its three parts. Bound by memory: 10,000 x 768 and 768 x 768 fp32 83 MB in 14 us.
 template <class T>
-__device__ __forceinline__ void prepare_rows(uint32_t block, const PrepareArgs& a, const PrepareArgs& b) {
+__device__ __forceinline__ void prepare_rows(uint32_t block, uint32_t thread, const PrepareArgs& a, const PrepareArgs& b) {
   const bool second = block >= a.blocks;
   const PrepareArgs& p = second ? b : a;
   const uint32_t per_row = static_cast<uint32_t>(p.ld / 8);
-  const auto [r, chunk] = row_and_chunk(second ? block - a.blocks : block, per_row);
+  const auto [r, chunk] = row_and_chunk(second ? block - a.blocks : block, per_row, thread);
   if (r >= p.rows) return;
   const uint32_t c = chunk * 8;
   float v[8];
@@ -127,11 +127,11 @@ __device__ __forceinline__ void prepare_rows(uint32_t block, const PrepareArgs& 
 
 template <class T>
 __global__ void __launch_bounds__(256) prepare_kernel(PrepareArgs a, PrepareArgs b) {
-  prepare_rows<T>(blockIdx.x, a, b);
+  prepare_rows<T>(blockIdx.x, threadIdx.x, a, b);
 }
 
 /// dz = grad * act'(z) (stored if asked for) and its column sums over this work-group's rows. A thread
-/// has eight columns; 256 / LX threads share them, each taking every 256 / LX-th row. Bound by memory: 16,384 x
+/// has eight columns; LY threads share them, each taking every LY-th row. Bound by memory: 16,384 x
 /// 4,096 bf16 with GELU 403 MB in 87 us, 4.6 TB/s. dz is written for 16-bit results in their type: it feeds
 /// the matrix unit, which takes no wider ones (an error of 2^-9 of each term, as the gradient itself has).
 struct SlopeArgs {
@@ -149,12 +149,13 @@ struct SlopeArgs {
 };
 
 /// Work-groups past the slope's make the copies of x and w.
-template <class T, int LX>
-__global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a, PrepareArgs copy_a, PrepareArgs copy_b) {
-  constexpr uint32_t kRows = 256 / LX, kCols = LX * 8;
+template <class T, int LX, int LY>
+__global__ void __launch_bounds__(LX* LY) slope_kernel(SlopeArgs a, PrepareArgs copy_a, PrepareArgs copy_b) {
+  constexpr uint32_t kRows = LY, kCols = LX * 8, kParts = LX * LY / 256;
   __shared__ float s_sum[kRows][kCols + 4];
   if (blockIdx.x >= a.blocks) {
-    prepare_rows<T>(blockIdx.x - a.blocks, copy_a, copy_b);
+    const uint32_t block = (blockIdx.x - a.blocks) * kParts + threadIdx.x / 256;
+    if (block < copy_a.blocks + copy_b.blocks) prepare_rows<T>(block, threadIdx.x % 256, copy_a, copy_b);
     return;
   }
   const uint32_t group = blockIdx.x / a.across, across = blockIdx.x - group * a.across;
@@ -212,22 +213,10 @@ __global__ void __launch_bounds__(256) slope_kernel(SlopeArgs a, PrepareArgs cop
   }
 }
 
-/// Adds the work-groups' column sums in order: four waves take contiguous shares of them.
+/// Adds the work-groups' column sums, where no launch of a product does.
 template <class T>
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ sums, uint32_t parts, uint32_t cols,
-                                                         T* __restrict__ out) {
-  __shared__ float s_sum[4][64];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ld = (cols + 7) / 8 * 8;
-  const uint32_t c = blockIdx.x * 64 + lane, share = (parts + 3) / 4;
-  const uint32_t p0 = wave * share < parts ? wave * share : parts, p1 = p0 + share < parts ? p0 + share : parts;
-  float t = 0.0f;
-  if (c < cols) {
-#pragma unroll 8
-    for (uint32_t p = p0; p < p1; ++p) t += sums[static_cast<uint64_t>(p) * ld + c];
-  }
-  s_sum[wave][lane] = t;
-  __syncthreads();
-  if (wave == 0 && c < cols) out[c] = static_cast<T>(((s_sum[0][lane] + s_sum[1][lane]) + s_sum[2][lane]) + s_sum[3][lane]);
+__global__ void __launch_bounds__(256) column_sum_kernel(ColumnSums a, T* __restrict__ out) {
+  add_columns(a, blockIdx.x, out);
 }
 
 // ---- few rows ---------------------------------------------------------------------------------
@@ -393,10 +382,12 @@ void launch_prepare(int dtype, const Prepared& a, const Prepared& b, hipStream_t
 
 void run_product(Form form, Kind kind, int dtype, GemmArgs g, const void* bias, const void* residual, uint64_t ld_residual,
                  void* out, uint64_t ld_out, void* keep, uint64_t ld_keep, int act, const GemmPlan& plan, void* partial,
-                 hipStream_t s) {
+                 hipStream_t s, const ColumnSums& columns = {}, void* column_out = nullptr) {
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     LinearEpilogue<T> e;
+    e.columns = columns;
+    e.column_out = static_cast<T*>(column_out);
     e.bias = static_cast<const T*>(bias);
     e.residual = static_cast<const T*>(residual);
     e.out = static_cast<T*>(out);
@@ -584,10 +575,9 @@ GradRun plan_grad(const qvh_linear_grad_args& a, void* ws) {
     j.plane = j.ld * a.m;
     j.plain = !parts;
     if (writes) j.dz = sp.take(j.plane * (parts ? kPlanes * 2 : e));
-    // A work-group with all rows of 64 columns saves the launch that adds up the parts; its threads then walk
-    // down up to four rows each. Otherwise 256 columns, rows spread over about a thousand work-groups, at
-    // least 16 rows each. (All of linear_grad, bf16: 90 x 1,024 x 80 16.7 us against 21.2; with up to 256
-    // rows allowed 255 x 511 x 4,095 took 38.2 against 28.8.)
+    // A work-group with all rows of 64 columns saves the launch that adds up the parts; its threads (256, or 1,024)
+    // then walk down up to four rows each. Otherwise 256 columns, rows spread over about a thousand
+    // work-groups, at least 16 rows each. (All of linear_grad, bf16: 90 x 1,024 x 80 16.7 us against 21.2.)
     r.one = a.grad_bias && a.m <= kSumRows;
     j.across = static_cast<uint32_t>(ceil_div(a.n, r.one ? 64 : 256));
     j.rows_each = r.one ? static_cast<uint32_t>(std::max<uint64_t>(a.m, 1))
@@ -728,24 +718,35 @@ qvh_status qvh_linear_grad_device(const qvh_linear_grad_args* args, void* d_work
       const PrepareArgs none;
       const PrepareArgs& first = r.x.copy ? r.x.job : r.w.copy ? r.w.job : none;
       const PrepareArgs& second = r.x.copy && r.w.copy ? r.w.job : none;
-      const uint64_t blocks = static_cast<uint64_t>(r.job.blocks) + first.blocks + second.blocks;
-      QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "the matrix product is too large");
+      const uint64_t copies = static_cast<uint64_t>(first.blocks) + second.blocks;
+      QVH_REQUIRE(r.job.blocks + copies <= 0x7FFFFFFFu, "the matrix product is too large");
       with_dtype(a.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        const auto kernel = r.one ? slope_kernel<T, 8> : slope_kernel<T, 32>;
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, r.job, first, second);
+        const bool tall = r.one && a.m > 128;
+        const auto kernel = tall ? slope_kernel<T, 8, 128> : r.one ? slope_kernel<T, 8, 32> : slope_kernel<T, 32, 8>;
+        const uint64_t groups = r.job.blocks + ceil_div(copies, tall ? 4 : 1);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(tall ? 1024 : 256), 0, s, r.job, first, second);
       });
       QVH_HIP(hipGetLastError());
     } else if (products) {
       launch_prepare(a.dtype, r.x, r.w, s);
     }
+    // The parts are added by the launch that joins the weight gradient's splits, or by one of their own.
+    ColumnSums columns;
     if (a.grad_bias && a.n > 0 && !r.one) {
+      columns.parts = r.job.sums;
+      columns.count = r.sum_parts;
+      columns.cols = a.n;
+    }
+    const bool joined = products && a.grad_weight && r.plan_w.splits > 1;
+    if (columns.cols > 0 && !joined) {
       with_dtype(a.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        hipLaunchKernelGGL((column_sum_kernel<T>), dim3(static_cast<unsigned>(ceil_div(a.n, 64))), dim3(256), 0, s,
-                           r.job.sums, r.sum_parts, a.n, static_cast<T*>(a.grad_bias));
+        hipLaunchKernelGGL((column_sum_kernel<T>), dim3(static_cast<unsigned>(ceil_div(a.n, 64))), dim3(256), 0, s, columns,
+                           static_cast<T*>(a.grad_bias));
       });
       QVH_HIP(hipGetLastError());
+      columns = ColumnSums{};
     }
     if (!products) return;
     GemmArgs g;
@@ -764,7 +765,7 @@ qvh_status qvh_linear_grad_device(const qvh_linear_grad_args* args, void* d_work
       g.n = a.k;
       g.k = static_cast<uint32_t>(a.m);
       run_product(Form::kKK, r.kind_w, a.dtype, g, nullptr, nullptr, 0, a.grad_weight, a.grad_weight_stride, nullptr, 0, QVH_ACT_NONE,
-                  r.plan_w, r.partial_w, s);
+                  r.plan_w, r.partial_w, s, columns, a.grad_bias);
     }
   });
 }

@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(256) start_kernel(const T* __restrict__ g, uin
   static_assert(kNormParts == 256, "one part per thread");
   // Past fp32's range for an update near its smallest numbers, so a double.
   const double factor = start_factor(block_sum(parts[blockIdx.y * kNormParts + threadIdx.x], s_sum));
-  const auto [r, chunk] = row_and_chunk(blockIdx.x, static_cast<uint32_t>(ld / 8));
+  const auto [r, chunk] = row_and_chunk(blockIdx.x, static_cast<uint32_t>(ld / 8), threadIdx.x);
   if (r >= m) return;
   const uint32_t c = chunk * 8;
   float v[8];

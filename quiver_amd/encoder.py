@@ -26,13 +26,14 @@ _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
 _MAX_STRIDE = 1 << 22
 
 _torch = None
+_tensor = None
 _dtypes = {}
 _raw_stream = None
 
 
 def _load_torch():
     """torch, once it is known to share this library's HIP runtime."""
-    global _torch, _raw_stream
+    global _torch, _tensor, _raw_stream
     if _torch is None:
         import torch
 
@@ -44,12 +45,15 @@ def _load_torch():
         _dtypes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
         # The current stream's handle alone; torch.cuda.current_stream makes an object of it, at 2 us a call.
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _tensor = torch.Tensor
         _torch = torch
     return _torch
 
 
 def _check(name: str, x, device=None, dtype=None):
     """A floating device tensor, on `device` and of `dtype` where those are given."""
+    if dtype is not None and x.__class__ is _tensor and x.dtype is dtype and x.device == device:
+        return  # what nearly every call finds, in a third of the time
     torch = _load_torch()
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor in GPU memory")
@@ -68,11 +72,13 @@ def _check(name: str, x, device=None, dtype=None):
 
 def _rows(x, cols: int):
     """x as rows of `cols` contiguous elements, and the elements between rows."""
-    if x.dim() != 2:
-        x = x.reshape(x.numel() // cols if cols else 0, cols)
-    stride = x.stride(0)
     if x.is_contiguous():
         return x, cols
+    if x.dim() != 2:
+        x = x.reshape(x.numel() // cols if cols else 0, cols)
+        if x.is_contiguous():
+            return x, cols
+    stride = x.stride(0)
     if x.stride(1) != 1 or stride < cols or stride > _MAX_STRIDE:
         return x.contiguous(), cols
     return x, stride
@@ -84,13 +90,13 @@ def _tokens(tokens, device):
         raise TypeError("tokens must be a torch tensor in GPU memory")
     if tokens.device != device:
         raise ValueError(f"tokens are on {tokens.device}, the other tensors on {device}")
-    if tokens.dtype == torch.int64:
+    if tokens.dtype is torch.int64:
         size = 8
-    elif tokens.dtype == torch.int32:
+    elif tokens.dtype is torch.int32:
         size = 4
     else:
         raise ValueError(f"tokens must be int32 or int64, got {tokens.dtype}")
-    return tokens.contiguous(), size
+    return tokens if tokens.is_contiguous() else tokens.contiguous(), size
 
 
 def _activation(name) -> int:
@@ -177,7 +183,7 @@ def linear(x, weight, bias=None, activation: Optional[str] = None, residual=None
         _check("bias", bias, device, dtype)
         if bias.shape != (n,):
             raise ValueError(f"bias must have shape ({n},), got {tuple(bias.shape)}")
-        br = bias.contiguous()
+        br = bias if bias.is_contiguous() else bias.contiguous()
     if residual is not None:
         _check("residual", residual, device, dtype)
         if residual.shape != shape:
@@ -224,7 +230,7 @@ def linear_grad(grad, x, weight, preactivation=None, activation: Optional[str] =
     gr, gs = _rows(grad, n)
     xr, xs = _rows(x, k)
     wr, ws = _rows(weight, k)
-    m = gr.shape[0] if n else x.numel() // k if k else 0
+    m = grad.numel() // n if n else x.numel() // k if k else 0
     gx = x.new_empty(x.shape) if inputs else None
     gw = weight.new_empty((n, k))
     gb = weight.new_empty((n,)) if bias else None
