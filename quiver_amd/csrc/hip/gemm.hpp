@@ -215,19 +215,25 @@ struct ColumnSums {
   uint32_t count = 0, cols = 0;
 };
 
-/// 64 columns' parts, in order: four waves take contiguous shares of them.
+__device__ __forceinline__ float sum8(const float (&t)[8]) {
+  return ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
+}
+
+/// 64 columns' parts: four waves take contiguous shares of them.
 template <class T>
 __device__ __forceinline__ void add_columns(const ColumnSums& a, uint32_t block, T* __restrict__ out) {
   __shared__ float s_sum[4][64];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ld = (a.cols + 7) / 8 * 8;
   const uint32_t c = block * 64 + lane, share = (a.count + 3) / 4;
   const uint32_t p0 = wave * share < a.count ? wave * share : a.count, p1 = p0 + share < a.count ? p0 + share : a.count;
-  float t = 0.0f;
+  float t[8] = {};  // every eighth part each: eight loads under way, and short sums
   if (c < a.cols) {
-#pragma unroll 8
-    for (uint32_t p = p0; p < p1; ++p) t += a.parts[static_cast<uint64_t>(p) * ld + c];
+    for (uint32_t p = p0; p < p1; p += 8) {
+#pragma unroll
+      for (uint32_t u = 0; u < 8; ++u) t[u] += p + u < p1 ? a.parts[static_cast<uint64_t>(p + u) * ld + c] : 0.0f;
+    }
   }
-  s_sum[wave][lane] = t;
+  s_sum[wave][lane] = sum8(t);
   __syncthreads();
   if (wave == 0 && c < a.cols) {
     out[c] = static_cast<T>(((s_sum[0][lane] + s_sum[1][lane]) + s_sum[2][lane]) + s_sum[3][lane]);

@@ -202,9 +202,12 @@ __global__ void __launch_bounds__(LX* LY) slope_kernel(SlopeArgs a, PrepareArgs 
   const uint32_t ld = (a.cols + 7) / 8 * 8;
   const uint32_t col = across * kCols + threadIdx.x;
   if (threadIdx.x < kCols && col < ld) {
-    float t = 0.0f;
-#pragma unroll 8
-    for (uint32_t p = 0; p < kRows; ++p) t += s_sum[p][threadIdx.x];
+    float eight[8] = {};
+    for (uint32_t p = 0; p < kRows; p += 8) {
+#pragma unroll
+      for (uint32_t u = 0; u < 8; ++u) eight[u] += s_sum[p + u][threadIdx.x];
+    }
+    const float t = sum8(eight);
     if (a.sums) {
       a.sums[static_cast<uint64_t>(group) * ld + col] = t;
     } else if (col < a.cols) {
@@ -431,7 +434,7 @@ void check_matrix(const std::string& w, const char* name, const void* p, uint64_
 double few_us(uint64_t m, uint32_t k, uint32_t n, int dtype) {
   const uint64_t groups = ceil_div(m, 64) * ceil_div(n, 16);
   double step = m <= 16 ? 0.42 : m <= 32 ? 0.64 : 1.07;
-  if (dtype != QVH_FP32 && k % 2 != 0) step *= 2.7;  // rows that begin inside a dword
+  if (dtype != QVH_FP32 && k % 2 != 0) step *= 3.2;  // rows that begin inside a dword
   return 2.0 + static_cast<double>(ceil_div(groups, 256)) * (0.3 + static_cast<double>(ceil_div(k, dtype == QVH_FP32 ? 128 : 256)) * step);
 }
 

@@ -188,16 +188,18 @@ PYBIND11_MODULE(_quiver, m) {
     check(qvh_embed_grad_device(ptr(grad), stride, ptr(tokens), index_bytes, count, rows, dim, dtype, scale, ptr(out),
                                 ptr(work), work_bytes, ptr(stream)));
   });
-  // These two return the workspace they lack, in bytes, and enqueue nothing then.
+  // Without a workspace these two return the size of the one they need and enqueue nothing, or enqueue and return 0.
   m.def("_linear", [check, ptr](std::uint64_t m, std::uint32_t k, std::uint32_t n, int dtype, int act, std::uintptr_t x,
                                 std::uint64_t xs, std::uintptr_t w, std::uint64_t ws, std::uintptr_t bias,
                                 std::uintptr_t residual, std::uint64_t rs, std::uintptr_t out, std::uint64_t os,
                                 std::uintptr_t pre, std::uint64_t ps, std::uintptr_t work, std::uint64_t work_bytes,
                                 std::uintptr_t stream) -> std::uint64_t {
     const qvh_linear_args a{m, k, n, dtype, act, ptr(x), xs, ptr(w), ws, ptr(bias), ptr(residual), rs, ptr(out), os, ptr(pre), ps};
-    std::uint64_t need = 0;
-    check(qvh_linear_workspace(&a, &need));
-    if (need > work_bytes) return need;
+    if (work_bytes == 0) {
+      std::uint64_t need = 0;
+      check(qvh_linear_workspace(&a, &need));
+      if (need > 0) return need;
+    }
     check(qvh_linear_device(&a, ptr(work), work_bytes, ptr(stream)));
     return 0;
   });
@@ -208,9 +210,11 @@ PYBIND11_MODULE(_quiver, m) {
                                      std::uintptr_t gb, std::uintptr_t work, std::uint64_t work_bytes,
                                      std::uintptr_t stream) -> std::uint64_t {
     const qvh_linear_grad_args a{m, k, n, dtype, act, ptr(grad), gs, ptr(pre), ps, ptr(x), xs, ptr(w), ws, ptr(gx), gxs, ptr(gw), gws, ptr(gb)};
-    std::uint64_t need = 0;
-    check(qvh_linear_grad_workspace(&a, &need));
-    if (need > work_bytes) return need;
+    if (work_bytes == 0) {
+      std::uint64_t need = 0;
+      check(qvh_linear_grad_workspace(&a, &need));
+      if (need > 0) return need;
+    }
     check(qvh_linear_grad_device(&a, ptr(work), work_bytes, ptr(stream)));
     return 0;
   });
