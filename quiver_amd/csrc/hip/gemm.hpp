@@ -150,16 +150,25 @@ __device__ __forceinline__ RowChunk row_and_chunk(uint32_t block, uint32_t per_r
   return {r, static_cast<uint32_t>(i - r * per_row)};
 }
 
-/// Eight values as vector accesses, or those of them that the row still has one by one.
-template <class T>
+/// Eight values as vector accesses, or those of them that the row still has one by one. STREAM: past the caches.
+template <bool STREAM = false, class T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8], uint32_t left) {
   if (left >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      store_floats<T, 8>(p, v);
-    } else {
-      const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
-      store_floats<T, 4>(p, lo);
-      store_floats<T, 4>(p + 4, hi);
+    constexpr int kEach = 16 / sizeof(T);
+    typedef T elements __attribute__((ext_vector_type(kEach)));
+    typedef uint32_t dwords __attribute__((ext_vector_type(4), aligned(2)));  // elements would be streamed one by one
+#pragma unroll
+    for (int i = 0; i < 8; i += kEach) {
+      elements x;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) x[e] = static_cast<T>(v[i + e]);
+      dwords* to = reinterpret_cast<dwords*>(p + i);
+      const u32x4_t bits = __builtin_bit_cast(u32x4_t, x);
+      if constexpr (STREAM) {
+        __builtin_nontemporal_store(bits, to);
+      } else {
+        *to = bits;
+      }
     }
   } else {
 #pragma unroll
@@ -265,6 +274,11 @@ struct LinearEpilogue {
   }
 
   __device__ __forceinline__ void operator()(uint32_t, uint32_t m, uint32_t n, uint32_t left, float (&v)[8]) const {
+    apply<false>(m, n, left, v);
+  }
+
+  template <bool STREAM>
+  __device__ __forceinline__ void apply(uint32_t m, uint32_t n, uint32_t left, float (&v)[8]) const {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll 1
       for (int i = 0; i < 8; ++i) {
@@ -279,7 +293,7 @@ struct LinearEpilogue {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += b[i];
     }
-    if (keep) store8(keep + m * ld_keep + n, v, left);
+    if (keep) store8<STREAM>(keep + m * ld_keep + n, v, left);
     if (act == QVH_ACT_RELU) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = activate<sizeof(T) == 4>(v[i], QVH_ACT_RELU);
@@ -296,7 +310,16 @@ struct LinearEpilogue {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] += r[i];
     }
-    store8(out + m * ld_out + n, v, left);
+    store8<STREAM>(out + m * ld_out + n, v, left);
+  }
+};
+
+/// The same for results too large for the L2s.
+template <class T>
+struct StreamedEpilogue {
+  LinearEpilogue<T> of;
+  __device__ __forceinline__ void operator()(uint32_t, uint32_t m, uint32_t n, uint32_t left, float (&v)[8]) const {
+    of.template apply<true>(m, n, left, v);
   }
 };
 

@@ -428,7 +428,7 @@ void check_matrix(const std::string& w, const char* name, const void* p, uint64_
 }
 
 /// us of the few-row kernel, fitted to 204 products from 1 x 64 x 64 to 3,721 x 2,019 x 65, bf16 and fp32. Taken
-/// where it promises to beat the tiled products, it was the slower by more than 12% in 12 of them (by rows of x
+/// where it promises to beat the tiled products, it was the slower by more than 12% in 10 of them (by rows of x
 /// alone, up to 64, in far more: 13% slower than the better one on average, against 2%). Both sides, few rows
 /// first: 64 x 512 x 1,024 4.5 and 4.9, 64 x 4,096 x 1,024 19.8 and 9.0, 614 x 96 x 74 2.7 and 3.9.
 double few_us(uint64_t m, uint32_t k, uint32_t n, int dtype) {

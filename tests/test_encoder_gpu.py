@@ -280,6 +280,13 @@ def test_linear(dtype, m, k, n):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m,k,n", [(4111, 72, 4501), (8200, 64, 2056)])
+def test_linear_of_large_results(dtype, m, k, n):
+    """Results of more than 32 MB, with rows that begin anywhere and a last tile that ends anywhere."""
+    test_linear(dtype, m, k, n)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("m", [5, 200])
 def test_linear_views(dtype, m):
     """Rows with a stride, columns that start off alignment, leading dimensions, transposes."""
