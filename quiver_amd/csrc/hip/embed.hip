@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(256) embed_kernel(const T* __restrict__ table,
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (at[u] < total) store_floats<T, V>(out + row[u] * dim + col[u], x[u]);
+    if (at[u] < total) store_floats<T, V, (U > 1)>(out + row[u] * dim + col[u], x[u]);
   }
 }
 
@@ -85,7 +85,8 @@ void launch_embed(const void* table, uint64_t rows, uint32_t dim, uint64_t strid
     };
     // Two pieces per thread where the device is full several times over; below, one. Both sides, one and two, with
     // the tables in HBM: 250,007 x 100 fp32 35.1 and 32.0 us, 60,000 x 1,024 bf16 40.3 and 36.0; 16,000 x 100
-    // fp32 3.8 and 4.2. (Four: 33.1, 36.4, 4.8.)
+    // fp32 3.8 and 4.2. (Four: 33.1, 36.4, 4.8.) The result, of 32 MB or more then, is stored past the L2s: 250,007 x
+    // 1,024 bf16 162 us through them, 143 past; 250,007 x 100 fp32 31.9 and 32.7.
     if (total < (1u << 21)) {
       go(std::integral_constant<int, 1>{});
     } else {
@@ -442,7 +443,7 @@ __device__ __forceinline__ void zero_rows(const SumArgs& a, uint32_t block, uint
 /// Groups of G lanes, each adding one piece of the list over G * V columns (slab blockIdx.y). Bound by memory: of
 /// 262,144 tokens of 1,024 bf16 in 32,000 rows (537 MB read, 66 MB written) 143 us, 4.2 TB/s, where a copy
 /// reaches 4.98; it reads rows in an order of its own, 1 KB of each.
-template <class T, int V, int G>
+template <class T, int V, int G, bool STREAM>
 __global__ void __launch_bounds__(256) embed_grad_sum_kernel(SumArgs a) {
   constexpr uint32_t kGroups = 256 / G;
   constexpr int kAhead = 8;
@@ -503,7 +504,7 @@ __global__ void __launch_bounds__(256) embed_grad_sum_kernel(SumArgs a) {
     for (int u = 0; u < kAhead; ++u) {
       kk[u] = j + u < n ? key[j + u] : a.rows;
       if (kk[u] != a.rows) {
-        load_floats<T, V>(grad + static_cast<uint64_t>(pos[j + u]) * a.stride, x[u]);
+        load_floats<T, V, STREAM>(grad + static_cast<uint64_t>(pos[j + u]) * a.stride, x[u]);
       } else {
 #pragma unroll
         for (int k = 0; k < V; ++k) x[u][k] = 0.0f;
@@ -707,7 +708,12 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
       QVH_REQUIRE(256 / G * a.piece <= kMostEntries, "qvh_embed_grad_device: pieces past the work-group's memory");
       a.sum_blocks = static_cast<uint32_t>(ceil_div(a.pieces, 256 / G));
       a.slabs = static_cast<uint32_t>(ceil_div(a.cpr, G));
-      hipLaunchKernelGGL((embed_grad_sum_kernel<T, V, G>), dim3(a.sum_blocks + zero_blocks, a.slabs), dim3(256), 0, s, a);
+      // Gradients that the L2s cannot hold are read past them, so that the partial sums stay for the join. Both sides,
+      // through and past: 250,007 x 100 bf16 146 and 131 us a call, 262,144 x 1,024 193 and 184; 100,000 x 128
+      // (26 MB) 44 and 47.
+      const bool stream = count * dim * sizeof(T) >= kStreamed;
+      const auto kernel = stream ? embed_grad_sum_kernel<T, V, G, true> : embed_grad_sum_kernel<T, V, G, false>;
+      hipLaunchKernelGGL(kernel, dim3(a.sum_blocks + zero_blocks, a.slabs), dim3(256), 0, s, a);
     };
     if (a.cpr <= 8) {
       sum(std::integral_constant<int, 8>{});

@@ -154,21 +154,12 @@ __device__ __forceinline__ RowChunk row_and_chunk(uint32_t block, uint32_t per_r
 template <bool STREAM = false, class T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8], uint32_t left) {
   if (left >= 8) {
-    constexpr int kEach = 16 / sizeof(T);
-    typedef T elements __attribute__((ext_vector_type(kEach)));
-    typedef uint32_t dwords __attribute__((ext_vector_type(4), aligned(2)));  // elements would be streamed one by one
-#pragma unroll
-    for (int i = 0; i < 8; i += kEach) {
-      elements x;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) x[e] = static_cast<T>(v[i + e]);
-      dwords* to = reinterpret_cast<dwords*>(p + i);
-      const u32x4_t bits = __builtin_bit_cast(u32x4_t, x);
-      if constexpr (STREAM) {
-        __builtin_nontemporal_store(bits, to);
-      } else {
-        *to = bits;
-      }
+    if constexpr (sizeof(T) == 2) {
+      store_floats<T, 8, STREAM>(p, v);
+    } else {
+      const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+      store_floats<T, 4, STREAM>(p, lo);
+      store_floats<T, 4, STREAM>(p + 4, hi);
     }
   } else {
 #pragma unroll
@@ -178,15 +169,15 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], uint32_t left)
   }
 }
 
-template <class T>
+template <bool STREAM = false, class T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8], uint32_t left) {
   if (left >= 8) {
     if constexpr (sizeof(T) == 2) {
-      load_floats<T, 8>(p, v);
+      load_floats<T, 8, STREAM>(p, v);
     } else {
       float lo[4], hi[4];
-      load_floats<T, 4>(p, lo);
-      load_floats<T, 4>(p + 4, hi);
+      load_floats<T, 4, STREAM>(p, lo);
+      load_floats<T, 4, STREAM>(p + 4, hi);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         v[i] = lo[i];

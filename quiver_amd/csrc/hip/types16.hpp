@@ -42,20 +42,44 @@ struct Loose<T, 1> {
   T v[1];
 };
 
-template <class T, int V>
+/// From so many bytes on, as much as the L2s hold together, what is read or written once goes past them.
+constexpr uint64_t kStreamed = uint64_t{32} << 20;
+
+/// Sixteen bytes aligned to two: a vector of smaller elements would be streamed one by one.
+typedef uint32_t dwords_t __attribute__((ext_vector_type(4)));
+typedef uint32_t loose_dwords_t __attribute__((ext_vector_type(4), aligned(2)));
+
+/// STREAM: past the caches, where V elements are 16 bytes.
+template <class T, int V, bool STREAM = false>
 __device__ __forceinline__ void load_floats(const T* p, float (&out)[V]) {
-  const auto k = reinterpret_cast<const Loose<T, V>*>(p)->v;
+  if constexpr (STREAM && V * sizeof(T) == 16) {
+    typedef T elements __attribute__((ext_vector_type(V)));
+    const dwords_t bits = __builtin_nontemporal_load(reinterpret_cast<const loose_dwords_t*>(p));
+    const elements k = __builtin_bit_cast(elements, bits);
 #pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = static_cast<float>(k[i]);
+    for (int i = 0; i < V; ++i) out[i] = static_cast<float>(k[i]);
+  } else {
+    const auto k = reinterpret_cast<const Loose<T, V>*>(p)->v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = static_cast<float>(k[i]);
+  }
 }
 
 /// Rounds to nearest even, once.
-template <class T, int V>
+template <class T, int V, bool STREAM = false>
 __device__ __forceinline__ void store_floats(T* p, const float (&in)[V]) {
-  Loose<T, V> k;
+  if constexpr (STREAM && V * sizeof(T) == 16) {
+    typedef T elements __attribute__((ext_vector_type(V)));
+    elements k;
 #pragma unroll
-  for (int i = 0; i < V; ++i) k.v[i] = static_cast<T>(in[i]);
-  *reinterpret_cast<Loose<T, V>*>(p) = k;
+    for (int i = 0; i < V; ++i) k[i] = static_cast<T>(in[i]);
+    __builtin_nontemporal_store(__builtin_bit_cast(dwords_t, k), reinterpret_cast<loose_dwords_t*>(p));
+  } else {
+    Loose<T, V> k;
+#pragma unroll
+    for (int i = 0; i < V; ++i) k.v[i] = static_cast<T>(in[i]);
+    *reinterpret_cast<Loose<T, V>*>(p) = k;
+  }
 }
 
 /// The widest access that a row of `n` elements has room for. A row is taken in ceil(n / V) pieces, the last

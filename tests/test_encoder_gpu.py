@@ -151,6 +151,18 @@ def test_embed_grad_of_small_batches(dtype, rows, dim, count):
     _check_embed_grad(grad, tok.to(_gpu()), rows, dtype)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,dim,count", [(5000, 201, 90_000), (300, 64, 300_001)])
+def test_embedding_of_large_batches(dtype, rows, dim, count):
+    """More than 32 MB of gradients and of looked-up rows, odd rows among them."""
+    test_embed_grad(dtype, rows, dim, count)
+    g = torch.Generator().manual_seed(rows)
+    table = _randn(g, rows, dim, dtype=dtype)
+    tok = torch.randint(-1, rows, (count,), generator=g).to(_gpu())
+    want = torch.where(tok[:, None] >= 0, table[tok.clamp(min=0)], torch.zeros((), dtype=TYPES[dtype], device=_gpu()))
+    assert torch.equal(quiver.embed(table, tok), want)
+
+
 @pytest.mark.parametrize("dim", [1, 30, 300])
 def test_embed_grad_joins_short_and_long_runs(dim):
     """Runs of 1 to 4,000 tokens, so that some end in their piece, some in the next ones and some far behind."""
@@ -413,6 +425,12 @@ def test_linear_of_even_rows(dtype, m, k, n):
     _say("linear", dtype, m, k, n)
     x, w, b = _randn(g, m, k, dtype=dtype), _randn(g, n, k, dtype=dtype, std=1 / math.sqrt(k)), _randn(g, n, dtype=dtype)
     _check_linear(dtype, x, w, b, "silu", _randn(g, m, n, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m,k,n", [(4201, 40, 4101), (20_000, 24, 1000)])
+def test_linear_grad_of_large_gradients(dtype, m, k, n):
+    test_linear_grad(dtype, m, k, n)
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
