@@ -25,8 +25,8 @@ constexpr uint32_t kMaxDim = 32768;
 
 /// Piece c of a row is V elements (vector_width), cpr pieces a row; U pieces per thread, 256 apart, so that each
 /// thread has U independent row reads in flight. Bound by memory: 250,007 tokens of 100 fp32 (a fifth of them
-/// padding) in a table of 1.18 million rows 31.6 us a call with the table in HBM, 182 MB at 5.8 TB/s; 24 tokens
-/// of 768 bf16 2.4 us, the launch.
+/// padding) in a table of 1.18 million rows 22 us, the 182 MB it moves at 8 TB/s, some of the rows from the
+/// caches; 24 tokens of 768 bf16 2.4 us, the launch.
 template <class T, int V, class I, int U>
 __global__ void __launch_bounds__(256) embed_kernel(const T* __restrict__ table, uint64_t rows, uint64_t stride,
                                                     const I* __restrict__ tokens, uint64_t count, uint32_t dim,
@@ -441,7 +441,7 @@ __device__ __forceinline__ void zero_rows(const SumArgs& a, uint32_t block, uint
 }
 
 /// Groups of G lanes, each adding one piece of the list over G * V columns (slab blockIdx.y). Bound by memory: of
-/// 262,144 tokens of 1,024 bf16 in 32,000 rows (537 MB read, 66 MB written) 143 us, 4.2 TB/s, where a copy
+/// 262,144 tokens of 1,024 bf16 in 32,000 rows (537 MB read, 66 MB written) 140 us, 4.3 TB/s, where a copy
 /// reaches 4.98; it reads rows in an order of its own, 1 KB of each.
 template <class T, int V, int G, bool STREAM>
 __global__ void __launch_bounds__(256) embed_grad_sum_kernel(SumArgs a) {

@@ -22,7 +22,7 @@
 // What bounds it. Large products, by the matrix unit and the clock under load: 8,192^3 bf16 about 1,200 TFLOP/s, its
 // instructions busy 63% of the time at 1.7 GHz (the installed library: 1,500). A layer of 16,384 x 1,024 x 4,096 with GELU and the
 // kept pre-activation, by its 16 steps' start and the 268 MB that its epilogue writes at the end of every tile:
-// 175 us, 785 TFLOP/s, the main loop alone 115. Small products, by the latency of a step (0.4 to 0.7 us) and a
+// 171 us, 800 TFLOP/s, the main loop alone 115. Small products, by the latency of a step (0.4 to 0.7 us) and a
 // launch. Tried without gain: five or more steps ahead, loads spread over several slices, prefetches into the L2,
 // wave priorities, tiles of 256 x 256 with four waves.
 #pragma once
