@@ -671,7 +671,7 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
   uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + l.positions[0]), reinterpret_cast<uint32_t*>(ws + l.positions[1])};
   const uint32_t sorted = (l.passes - 1) & 1;  // which of the two halves of keys and pos
   const bool held = l.part <= kSortWaves * 64 * kHeld;
-  for (uint32_t p = 0; p < l.passes; ++p) {
+  for (uint32_t p = 0; p < l.passes && n > 0; ++p) {  // without tokens there is nothing to sort, and rows to clear all the same
     const uint32_t *ik = keys[(p & 1) ^ 1], *ip = pos[(p & 1) ^ 1];
     const auto pass = [&](auto first, auto hold) {
       constexpr bool F = decltype(first)::value;
