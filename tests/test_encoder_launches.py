@@ -1,11 +1,15 @@
 """The encoder's launches, recorded on the CPU by a stand-in for the HIP runtime (tests/launches.py)."""
 
 import json
+import math
 import os
+import random
 import subprocess
 import sys
 
 import pytest
+
+from encoder_paths import GRAD, LINEAR, ORTHO
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -40,3 +44,59 @@ def test_embed_grad_without_tokens_clears_the_rows(launches, rows, dim, dtype):
     kernel, = _kernels(answer)
     grid = answer["launches"][0][1]
     assert kernel == "embed_grad_own_kernel" or (kernel == "embed_grad_sum_kernel" and grid * 64 >= rows)
+
+
+# ---- the kernels that the shapes of test_encoder_paths_gpu.py take ------------------------------
+
+
+def _products(answers):
+    return {kernel for a in answers for kernel in _kernels(a) if kernel.startswith("gemm_kernel")}
+
+
+def _calls(dtype):
+    for act in ("gelu", "none"):
+        for name, shapes in (("linear", LINEAR[dtype]), ("linear_grad", GRAD[dtype])):
+            for m, k, n in shapes:
+                yield [name, dict(m=m, k=k, n=n, dtype=dtype, act=act)]
+
+
+def _any_calls(rng, count, dtype):
+    """Layers and gradients over all sizes, half of the rows in whole 16-byte pieces, some not aligned to them."""
+    size = lambda lo, hi: int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))  # noqa: E731
+    for _ in range(count):
+        whole = rng.choice([1, 8])
+        m, k, n = size(1, 200_000), size(1, 20_000), size(1, 20_000)
+        args = dict(m=m, k=max(whole, k // whole * whole), n=max(whole, n // whole * whole), dtype=dtype,
+                    act=rng.choice(["none", "gelu"]))
+        if args["m"] * max(args["n"], args["k"]) < 1 << 32:
+            yield ["linear", dict(args, offset=rng.choice([0, 0, 1]))]
+            yield ["linear_grad", dict(args, inputs=rng.random() < 0.8, weight=rng.random() < 0.8)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_tested_shapes_take_every_product_kernel(launches, dtype):
+    tested = _products(launches(*_calls(dtype)))
+    taken = _products(launches(*_any_calls(random.Random(3), 6000, dtype)))
+    assert taken <= tested, sorted(taken - tested)
+
+
+def test_tested_orthogonalisations_take_every_product_kernel(launches):
+    tested = _products(launches(*(["orthogonalize", dict(m=m, n=n, batch=b, steps=2)] for m, n, b in ORTHO)))
+    rng = random.Random(4)
+    size = lambda hi: int(round(math.exp(rng.uniform(0, math.log(hi)))))  # noqa: E731
+    taken = _products(launches(*(["orthogonalize", dict(m=size(16384), n=size(16384), steps=2, batch=rng.choice([1, 1, 2, 6, 12, size(200)]))]
+                                 for _ in range(6000))))
+    assert taken <= tested, sorted(taken - tested)
+
+
+def test_fp16_goes_as_bf16_does(launches):
+    """The shapes that are listed for bf16 take the same kernels in fp16."""
+    calls = list(_calls("bf16"))
+    half = [[name, dict(args, dtype="fp16")] for name, args in calls]
+    assert [_kernels(a) for a in launches(*half)] == [_kernels(a) for a in launches(*calls)]
+
+
+def test_special_values_meet_operands_in_parts(launches):
+    """The shapes of the tests of infinities, tiny and huge values in fp32, forwards and backwards."""
+    layer, grad = launches(["linear", dict(m=2100, k=520, n=2050)], ["linear_grad", dict(m=2100, k=520, n=2050, act="silu")])
+    assert all("planes 3" in kernel for kernel in _products([layer]) | _products([grad]))

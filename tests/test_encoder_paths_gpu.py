@@ -4,10 +4,13 @@ Which kernels a shape takes is held by tests/test_encoder_launches.py, on the CP
 those of test_encoder_gpu.py.
 """
 
+import math
+
 import pytest
 
 import quiver_amd as quiver
-from test_encoder_gpu import TYPES, _gpu, _say
+from encoder_paths import GRAD, LINEAR, ORTHO
+from test_encoder_gpu import MUON, ROUND, TYPES, _check_linear, _check_linear_grad, _gpu, _randn, _say, _slope64
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +29,162 @@ def test_embed_grad_without_tokens(dtype, rows, dim):
         got = quiver.embed_grad(torch.empty((0, dim), dtype=TYPES[dtype], device=dev),
                                 torch.empty((0,), dtype=index, device=dev), rows)
         assert got.shape == (rows, dim) and not got.any()
+
+
+# ---- every tile, every way of reading, whole and in splits --------------------------------------
+
+
+def _each(shapes):
+    return [(dtype, *shape) for dtype in TYPES for shape in shapes["bf16" if dtype == "fp16" else dtype]]
+
+
+@pytest.mark.parametrize("dtype,m,k,n", _each(LINEAR))
+def test_linear_by_every_kernel(dtype, m, k, n):
+    g = torch.Generator().manual_seed(m + k + n)
+    _say("linear paths", dtype, m, k, n)
+    x, w = _randn(g, m, k, dtype=dtype), _randn(g, n, k, dtype=dtype, std=1 / math.sqrt(k))
+    _check_linear(dtype, x, w, _randn(g, n, dtype=dtype), "gelu", _randn(g, m, n, dtype=dtype))
+    _check_linear(dtype, x, w, None, "none", None)
+
+
+@pytest.mark.parametrize("dtype,m,k,n", _each(GRAD))
+def test_linear_grad_by_every_kernel(dtype, m, k, n):
+    g = torch.Generator().manual_seed(m + k + n)
+    _say("linear_grad paths", dtype, m, k, n)
+    x, w = _randn(g, m, k, dtype=dtype), _randn(g, n, k, dtype=dtype, std=1 / math.sqrt(k))
+    gr, pre = _randn(g, m, n, dtype=dtype), _randn(g, m, n, dtype=dtype, std=2.0)
+    _check_linear_grad(dtype, gr, x, w, pre, "gelu")
+    _check_linear_grad(dtype, gr, x, w, None, "none")
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_large_layers_of_strided_rows(dtype):
+    """Views with a stride, at and off 16-byte addresses, of a size that takes large tiles and fp32 parts."""
+    g = torch.Generator().manual_seed(12)
+    _say("large views", dtype)
+    m, k, n = 2100, 520, 2050
+    x, w = _randn(g, m, k + 24, dtype=dtype), _randn(g, n, k + 24, dtype=dtype, std=1 / math.sqrt(k))
+    gr, pre = _randn(g, m, n + 16, dtype=dtype), _randn(g, m, n + 16, dtype=dtype, std=2.0)
+    for at in (0, 8, 3):
+        s, t = slice(at, at + k), slice(at, at + n)
+        _check_linear(dtype, x[:, s], w[:, s], None, "silu", gr[:, t])
+        _check_linear_grad(dtype, gr[:, t], x[:, s], w[:, s], pre[:, t], "silu")
+
+
+def _ortho64_by_products(u, steps, co):
+    """The recurrence itself in 64 bits on the side with fewer rows, and the growth of an error (as _ortho64's, over
+    all singular values that occur: from 0 to the largest that the values of [0, 1] can reach)."""
+    a, b, c = co
+    x = u.double().reshape(-1, *u.shape[-2:])
+    tall = x.shape[1] > x.shape[2]
+    x = x.transpose(1, 2).contiguous() if tall else x
+    x = x / x.flatten(1).norm(dim=1)[:, None, None]
+    grow, top = 1.0, 1.0
+    for _ in range(steps):
+        t = torch.linspace(0, top, 500, dtype=torch.float64)
+        grow *= max(1.0, (a + 3 * b * t**2 + 5 * c * t**4).abs().max().item(), (a + b * t**2 + c * t**4).abs().max().item())
+        top = (a * t + b * t**3 + c * t**5).abs().max().item()
+        s = torch.bmm(x, x.transpose(1, 2).contiguous())
+        x = a * x + torch.bmm(b * s + c * torch.bmm(s, s), x)
+    return (x.transpose(1, 2) if tall else x).reshape(u.shape), grow
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("m,n,batch", ORTHO)
+def test_orthogonalize_by_every_kernel(dtype, m, n, batch):
+    g = torch.Generator().manual_seed(m + n + batch)
+    _say("orthogonalize paths", dtype, m, n, batch)
+    u = _randn(g, batch, m, n, dtype=dtype, std=1e-3)
+    side, depth = min(m, n), max(m, n)
+    for steps in (5, 2):
+        got = quiver.orthogonalize(u, steps=steps)
+        want, grow = _ortho64_by_products(u, steps, MUON)
+        bound = grow * (steps + 1) * 2 * math.sqrt(depth) * 2.0**-22 * math.sqrt(side)  # as in test_orthogonalize
+        err = (got.double() - want).flatten(-2).norm(dim=-1)
+        size = want.flatten(-2).norm(dim=-1)
+        assert bool((err <= bound + ROUND[dtype] * size).all()), (steps, err.max().item(), bound)
+        assert torch.equal(got, quiver.orthogonalize(u, steps=steps))
+
+
+# ---- fp32 operands in three parts ---------------------------------------------------------------
+
+PARTS = (2100, 520, 2050)  # forwards and backwards
+
+
+def _single_products(g):
+    """x, w with one non-zero value in each row of w: every result is one product."""
+    m, k, n = PARTS
+    x = 1.0 + torch.randint(0, 2**23, (m, k), generator=g).double() * 2.0**-23  # all 24 bits
+    w = torch.zeros((n, k), dtype=torch.float64)
+    w[torch.arange(n), torch.arange(n) * 7 % k] = 1.0 + torch.randint(0, 2**23, (n,), generator=g).double() * 2.0**-23
+    return x.float().to(_gpu()), w.float().to(_gpu())
+
+
+def test_parts_hold_24_bits():
+    """One product per result: what the parts leave out is below 2^-25 of it and its six terms are added with at most
+    2^-23 of the sum each, 2^-20 altogether. A third part left out would show: it is up to 2^-18 of a value."""
+    _say("parts", *PARTS)
+    g = torch.Generator().manual_seed(31)
+    x, w = _single_products(g)
+    want = x.double() @ w.double().t()
+    assert ((quiver.linear(x, w).double() - want).abs() <= 2.0**-20 * want.abs()).all()
+    # Backwards: one non-zero value per row of the gradient for grad_x, per column for grad_weight.
+    m, k, n = PARTS
+    gr = torch.zeros((m, n), device=_gpu())
+    gr[torch.arange(m), torch.randperm(n, generator=g)[torch.arange(m) % n]] = x[:, 0]
+    dx, dw, _ = quiver.linear_grad(gr, x, w + 1.0)
+    want = gr.double() @ (w + 1.0).double()
+    assert ((dx.double() - want).abs() <= 2.0**-20 * want.abs()).all()
+    # A column of the gradient holds one value, or two where n < m: their products do not cancel.
+    want = gr.double().t() @ x.double()
+    assert ((dw.double() - want).abs() <= 2.0**-20 * want.abs()).all()
+
+
+def test_parts_of_small_and_large_values():
+    """Rows and columns of very different size, and values whose first part would round up to infinity."""
+    _say("parts range")
+    m, k, n = PARTS
+    g = torch.Generator().manual_seed(8)
+    x = _randn(g, m, k, dtype="fp32") * torch.logspace(-15, 15, m, device=_gpu())[:, None]
+    w = _randn(g, n, k, dtype="fp32") * torch.logspace(-12, 12, k, device=_gpu())[None, :]
+    _check_linear("fp32", x, w, None, "none", None)
+    gr = _randn(g, m, n, dtype="fp32") * torch.logspace(-8, 8, n, device=_gpu())[None, :]
+    _check_linear_grad("fp32", gr, x, w, None, "none")
+    big, half = torch.zeros((m, k), device=_gpu()), torch.zeros((n, k), device=_gpu())
+    big[:, 3], half[:, 3] = 3.402e38, 0.5
+    assert torch.equal(quiver.linear(big, half), torch.full((m, n), 1.701e38, device=_gpu()))
+    gr = torch.zeros((m, n), device=_gpu())
+    gr[:, 5] = 3.402e38
+    dx, dw, _ = quiver.linear_grad(gr, torch.zeros((m, k), device=_gpu()).index_fill_(0, torch.tensor([9], device=_gpu()), 0.5), half)
+    assert torch.equal(dx[:, 3], torch.full((m,), 1.701e38, device=_gpu())) and not dx[:, :3].any() and not dx[:, 4:].any()
+    assert torch.equal(dw[5], torch.full((k,), 1.701e38, device=_gpu())) and not dw[:5].any() and not dw[6:].any()
+
+
+def _same_specials(got, want):
+    """NaN and infinities in the same places, of the same sign."""
+    want = want.to(got.dtype)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)]) and torch.equal(torch.isinf(got), torch.isinf(want))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_large_layers_of_not_finite_values(dtype):
+    """As test_linear_not_finite, at a size that takes parts in fp32, and backwards."""
+    _say("large not finite", dtype)
+    m, k, n = PARTS
+    g = torch.Generator().manual_seed(3)
+    x, w = _randn(g, m, k, dtype=dtype), torch.ones((n, k), dtype=TYPES[dtype], device=_gpu())
+    x[1, 5], x[2, 7], x[3, 0], x[m - 1, k - 1] = float("inf"), float("nan"), -float("inf"), float("inf")
+    w[9] = 0.0
+    w[9, 5] = 2.0
+    w[11, 3] = float("inf")
+    w[n - 1, k - 1] = -1.0
+    _same_specials(quiver.linear(x, w), x.double() @ w.double().t())
+    gr, pre = _randn(g, m, n, dtype=dtype), _randn(g, m, n, dtype=dtype)
+    gr[4, 6], gr[5, n - 1], gr[m - 1, 0] = float("inf"), float("nan"), -float("inf")
+    for act in ("none", "silu"):
+        dx, dw, db = quiver.linear_grad(gr, x, w, preactivation=pre, activation=act)
+        dz = gr.double() * _slope64(pre.double(), act)
+        _same_specials(dx, dz @ w.double())
+        _same_specials(dw, dz.t() @ x.double())
+        _same_specials(db, dz.sum(0))
