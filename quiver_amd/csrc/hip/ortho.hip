@@ -133,11 +133,11 @@ struct ResultEpilogue {
 template <class T>
 __global__ void __launch_bounds__(256) parts_to_result_kernel(const half_t* __restrict__ x, uint64_t ld, uint64_t plane,
                                                               uint32_t m, uint32_t n, T* __restrict__ out) {
-  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= static_cast<uint64_t>(m) * n) return;
-  const half_t* p = x + blockIdx.y * 2 * plane + i / n * ld + i % n;
-  out[static_cast<uint64_t>(blockIdx.y) * m * n + i] =
-      static_cast<T>((static_cast<float>(p[0]) + static_cast<float>(p[plane])) / kScale);
+  const uint64_t count = static_cast<uint64_t>(m) * n;
+  for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<uint64_t>(gridDim.x) * 256) {
+    const half_t* p = x + blockIdx.y * 2 * plane + i / n * ld + i % n;
+    out[blockIdx.y * count + i] = static_cast<T>((static_cast<float>(p[0]) + static_cast<float>(p[plane])) / kScale);
+  }
 }
 
 // ---- small matrices: one work-group does all steps ---------------------------------------------
@@ -566,7 +566,7 @@ void orthogonalize(const T* update, uint64_t batch, uint32_t m, uint32_t n, uint
                      update, m, n, norm, x[0], l.ldx, l.plane_x);
   QVH_HIP(hipGetLastError());
   if (steps == 0) {
-    hipLaunchKernelGGL((parts_to_result_kernel<T>), dim3(static_cast<unsigned>(ceil_div(static_cast<uint64_t>(m) * n, 256)), nb),
+    hipLaunchKernelGGL((parts_to_result_kernel<T>), dim3(static_cast<unsigned>(std::min<uint64_t>(ceil_div(static_cast<uint64_t>(m) * n, 256), 1u << 20)), nb),
                        dim3(256), 0, s, x[0], l.ldx, l.plane_x, m, n, out);
     QVH_HIP(hipGetLastError());
     return;

@@ -100,3 +100,12 @@ def test_special_values_meet_operands_in_parts(launches):
     """The shapes of the tests of infinities, tiny and huge values in fp32, forwards and backwards."""
     layer, grad = launches(["linear", dict(m=2100, k=520, n=2050)], ["linear_grad", dict(m=2100, k=520, n=2050, act="silu")])
     assert all("planes 3" in kernel for kernel in _products([layer]) | _products([grad]))
+
+
+# ---- sizes past one launch ----------------------------------------------------------------------
+
+
+def test_the_largest_matrix_is_orthogonalised(launches):
+    for steps in (0, 1):
+        answer, = launches(["orthogonalize", dict(m=65536, n=65536, steps=steps)])
+        assert _kernels(answer)
