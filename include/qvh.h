@@ -369,7 +369,8 @@ qvh_status qvh_embed_grad_device(const void* d_grad, uint64_t row_stride, const 
 /* A linear layer: z = x w^T + bias, out = act(z) + residual, with x [m][k], w [n][k], bias [n] (nullable),
  * residual [m][n] (nullable), out [m][n]; z is also stored to `preactivation` (nullable), which the
  * backward pass of an activation takes. out may be the residual's own buffer, and no other overlap is
- * allowed. m is below 2^31, k and n at most 2^20, strides at most 2^22. fp32 products run on fp32 matrix
+ * allowed. m is below 2^31, k and n at most 2^20, strides at most 2^22; a product whose tiles or operands go past
+ * one launch (2^32 threads: about 10^9 rows where n is below 64, more for wider results) is refused. fp32 products run on fp32 matrix
  * instructions, large ones as sums of three bf16 parts of each operand (24 bits; what is dropped is below
  * fp32's own rounding). */
 typedef struct qvh_linear_args {

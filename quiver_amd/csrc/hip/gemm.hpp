@@ -794,7 +794,7 @@ __global__ void __launch_bounds__(128) gemm_join_symmetric_kernel(GemmArgs g, Ep
 
 /// Tile shape and number of splits for a product; the same for the workspace's size and for the launch.
 struct GemmPlan {
-  int tile = 0;  // which of the kind's shapes
+  int tile = 0;  // which of the kind's shapes; -1: none whose tiles go into one launch
   uint32_t splits = 1;
   size_t partial_bytes = 0;
   double us = 0.0;  // the estimate that chose them
@@ -811,9 +811,7 @@ void launch_tile(GemmArgs g, const Epi& epi, hipStream_t s) {
   g.tiles_n = static_cast<uint32_t>(ceil_div(g.n, Shape::BN));
   const uint64_t tiles = g.symmetric ? static_cast<uint64_t>(g.tiles_m) * (g.tiles_m + 1) / 2
                                      : static_cast<uint64_t>(g.tiles_m) * g.tiles_n;
-  const uint64_t blocks = tiles * g.splits;
-  QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "the matrix product is too large");
-  const dim3 grid(static_cast<unsigned>(blocks), g.batches);
+  const dim3 grid(static_cast<unsigned>(tiles * g.splits), g.batches);  // gemm_plan: fits a launch
   if (g.splits > 1) {
     const uint64_t ld = ceil_div(g.n, 8) * 8;
     const PartialEpilogue pe{g.partial, ld, ld * g.m};

@@ -16,16 +16,16 @@ namespace qvh {
 // 37.1, 64-tiles 51.2; 1,024 x 4,096 x 16,384 as 256-tiles in four pieces 131, 128-tiles in one 181.
 GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, Kind kind, uint32_t batches, bool symmetric) {
   struct Cost {
-    uint64_t bm, bn, together;  // tile, and work-groups that a CU holds
+    uint64_t bm, bn, threads, together;  // tile, its work-group, and how many of those a CU holds
     double alone, shared, end;  // us per step: one work-group on a CU, each of several; prologue and epilogue
   };
   constexpr Cost kCosts[6][3] = {
-      {{64, 64, 4, 0.45, 0.22, 2.0}, {128, 128, 2, 0.70, 0.53, 4.0}, {256, 256, 1, 1.75, 1.75, 8.0}},
-      {{64, 64, 3, 0.40, 0.20, 2.0}, {128, 128, 2, 0.55, 0.45, 4.0}, {256, 128, 1, 0.95, 0.95, 6.0}},
-      {{64, 64, 3, 0.50, 0.35, 2.0}, {128, 128, 1, 0.95, 0.95, 4.0}, {256, 128, 1, 1.80, 1.80, 6.0}},
-      {{64, 64, 3, 0.70, 0.52, 2.0}, {128, 128, 2, 2.10, 2.00, 4.0}, {}},
-      {{64, 64, 4, 0.56, 0.35, 2.0}, {128, 128, 2, 1.05, 0.75, 4.0}, {}},
-      {{64, 64, 3, 0.90, 0.62, 2.0}, {128, 128, 2, 2.40, 2.10, 4.0}, {}}};
+      {{64, 64, 256, 4, 0.45, 0.22, 2.0}, {128, 128, 256, 2, 0.70, 0.53, 4.0}, {256, 256, 512, 1, 1.75, 1.75, 8.0}},
+      {{64, 64, 256, 3, 0.40, 0.20, 2.0}, {128, 128, 512, 2, 0.55, 0.45, 4.0}, {256, 128, 512, 1, 0.95, 0.95, 6.0}},
+      {{64, 64, 256, 3, 0.50, 0.35, 2.0}, {128, 128, 512, 1, 0.95, 0.95, 4.0}, {256, 128, 512, 1, 1.80, 1.80, 6.0}},
+      {{64, 64, 256, 3, 0.70, 0.52, 2.0}, {128, 128, 256, 2, 2.10, 2.00, 4.0}, {}},
+      {{64, 64, 256, 4, 0.56, 0.35, 2.0}, {128, 128, 256, 2, 1.05, 0.75, 4.0}, {}},
+      {{64, 64, 256, 3, 0.90, 0.62, 2.0}, {128, 128, 256, 2, 2.40, 2.10, 4.0}, {}}};
   constexpr uint32_t kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
   constexpr double kCus = 256.0;
   GemmPlan best;
@@ -38,6 +38,8 @@ GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, Kind kind, uint32_t batch
     const uint64_t tiles = (symmetric ? tm * (tm + 1) / 2 : tm * tn) * batches;
     for (const uint32_t splits : kSplits) {
       if (splits > 1 && steps < 2 * splits) break;
+      // What one launch has room for: the tiles, or the pieces that are joined.
+      if (tiles / batches * splits * c.threads >= kGridThreads || (splits > 1 && m * ceil_div(n, 8) >= kGridThreads)) break;
       const double groups = static_cast<double>(tiles) * splits;
       const double per_cu = std::ceil(groups / kCus);
       const double rounds = std::ceil(per_cu / static_cast<double>(c.together));
@@ -53,6 +55,11 @@ GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, Kind kind, uint32_t batch
       }
     }
   }
+  if (least < 0.0) {
+    best.tile = -1;
+    best.us = HUGE_VAL;
+    return best;
+  }
   best.us = least;
   if (best.splits > 1) best.partial_bytes = static_cast<size_t>(best.splits) * batches * m * (ceil_div(n, 8) * 8) * 4;
   return best;
@@ -64,6 +71,7 @@ constexpr uint64_t kMaxRows = uint64_t{1} << 31, kMaxStride = uint64_t{1} << 22;
 constexpr uint32_t kMaxWidth = 1u << 20;
 constexpr uint64_t kSumRows = 512;  // rows whose column sums one work-group makes
 constexpr int kPlanes = 3;         // bf16 parts of an fp32 value
+constexpr char kTooLarge[] = "the matrix product is too large";
 
 // ---- operand preparation ----------------------------------------------------------------------
 
@@ -349,7 +357,7 @@ Prepared copy_of(const Matrix& x, int dtype, Space& ws) {
   p.job.plane = p.job.ld * x.rows;
   p.job.dst = ws.take(p.job.plane * (dtype == QVH_FP32 ? kPlanes : 1) * 2);
   const uint64_t blocks = ceil_div(p.job.ld / 8 * x.rows, 256);
-  QVH_REQUIRE(blocks <= 0x3FFFFFFFu, "the matrix product is too large");
+  QVH_REQUIRE(blocks * 256 < kGridThreads, kTooLarge);
   p.job.blocks = static_cast<uint32_t>(blocks);
   p.op.base = p.job.dst;
   p.op.ld = p.job.ld;
@@ -375,7 +383,7 @@ void launch_prepare(int dtype, const Prepared& a, const Prepared& b, hipStream_t
   const PrepareArgs& second = a.copy && b.copy ? b.job : none;
   const uint64_t blocks = static_cast<uint64_t>(first.blocks) + second.blocks;
   if (blocks == 0) return;
-  QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "the matrix product is too large");
+  QVH_REQUIRE(blocks * 256 < kGridThreads, kTooLarge);
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     hipLaunchKernelGGL((prepare_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, first, second);
@@ -476,6 +484,7 @@ LinearRun plan_linear(const qvh_linear_args& a, void* ws) {
   }
   r.few = ceil_div(a.m, 64) <= 65535 && few_us(a.m, a.k, a.n, a.dtype) < r.plan.us + (copies ? copy_us(a.dtype, elements) : 0.0);
   if (r.few) return r;
+  QVH_REQUIRE(r.plan.tile >= 0, kTooLarge);
   r.x = copies && copy_x ? copy_of(x, a.dtype, sp) : as_it_is(x);
   r.w = copies && copy_w ? copy_of(w, a.dtype, sp) : as_it_is(w);
   r.partial = sp.take(r.plan.partial_bytes);
@@ -624,6 +633,7 @@ GradRun plan_grad(const qvh_linear_grad_args& a, void* ws) {
         prepared = copy_of(other, a.dtype, sp);
       }
     }
+    QVH_REQUIRE(plan.tile >= 0, kTooLarge);
     partial = sp.take(plan.partial_bytes);
   };
   if (of_x) product(w, fw, a.m, a.n, r.w, r.kind_x, r.plan_x, r.partial_x);
@@ -722,7 +732,7 @@ qvh_status qvh_linear_grad_device(const qvh_linear_grad_args* args, void* d_work
       const PrepareArgs& first = r.x.copy ? r.x.job : r.w.copy ? r.w.job : none;
       const PrepareArgs& second = r.x.copy && r.w.copy ? r.w.job : none;
       const uint64_t copies = static_cast<uint64_t>(first.blocks) + second.blocks;
-      QVH_REQUIRE(r.job.blocks + copies <= 0x7FFFFFFFu, "the matrix product is too large");
+      QVH_REQUIRE((r.job.blocks + copies) * 256 < kGridThreads, kTooLarge);
       with_dtype(a.dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const bool tall = r.one && a.m > 128;

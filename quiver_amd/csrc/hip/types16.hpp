@@ -42,6 +42,9 @@ struct Loose<T, 1> {
   T v[1];
 };
 
+/// Threads along an axis that a launch has to stay below.
+constexpr uint64_t kGridThreads = uint64_t{1} << 32;
+
 /// From so many bytes on, as much as the L2s hold together, what is read or written once goes past them.
 constexpr uint64_t kStreamed = uint64_t{32} << 20;
 

@@ -109,3 +109,12 @@ def test_the_largest_matrix_is_orthogonalised(launches):
     for steps in (0, 1):
         answer, = launches(["orthogonalize", dict(m=65536, n=65536, steps=steps)])
         assert _kernels(answer)
+
+
+@pytest.mark.parametrize("name,args", [("linear", dict(m=2**31 - 1, k=1, n=1, dtype="bf16")),
+                                       ("linear", dict(m=2**31 - 1, k=8, n=8, dtype="fp32")),
+                                       ("linear_grad", dict(m=2**31 - 1, k=2, n=2, dtype="bf16"))])
+def test_products_past_one_launch_are_refused(launches, name, args):
+    """With the status of a wrong argument and words for it, before anything runs."""
+    answer, = launches([name, args])
+    assert answer["status"] == -22 and "too large" in answer["error"] and not answer["launches"]
