@@ -77,11 +77,14 @@ void launch_embed(const void* table, uint64_t rows, uint32_t dim, uint64_t strid
     const uint64_t total = count * cpr;
     const auto go = [&](auto unroll) {
       constexpr int U = decltype(unroll)::value;
-      const uint64_t blocks = ceil_div(total, 256 * U);
-      QVH_REQUIRE(blocks <= 0x7FFFFFFFu, "qvh_embed_device: too many tokens");
-      hipLaunchKernelGGL((embed_kernel<T, V, I, U>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s,
-                         static_cast<const T*>(table), rows, stride, static_cast<const I*>(tokens), count, dim, cpr, magic,
-                         scale, static_cast<T*>(out));
+      const uint64_t most = kGridThreads / 2 * U / cpr;  // tokens of a launch
+      for (uint64_t t = 0; t < count; t += most) {
+        const uint64_t n = std::min(most, count - t);
+        hipLaunchKernelGGL((embed_kernel<T, V, I, U>), dim3(static_cast<unsigned>(ceil_div(n * cpr, 256 * U))), dim3(256), 0,
+                           s, static_cast<const T*>(table), rows, stride, static_cast<const I*>(tokens) + t, n, dim, cpr,
+                           magic, scale, static_cast<T*>(out) + t * dim);
+        QVH_HIP(hipGetLastError());
+      }
     };
     // Two pieces per thread where the device is full several times over; below, one. Both sides, one and two, with
     // the tables in HBM: 250,007 x 100 fp32 35.1 and 32.0 us, 60,000 x 1,024 bf16 40.3 and 36.0; 16,000 x 100
@@ -93,7 +96,6 @@ void launch_embed(const void* table, uint64_t rows, uint32_t dim, uint64_t strid
       go(std::integral_constant<int, 2>{});
     }
   });
-  QVH_HIP(hipGetLastError());
 }
 
 // ---- gradient of a small batch: rows look for their tokens ------------------------------------

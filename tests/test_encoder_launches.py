@@ -118,3 +118,13 @@ def test_products_past_one_launch_are_refused(launches, name, args):
     """With the status of a wrong argument and words for it, before anything runs."""
     answer, = launches([name, args])
     assert answer["status"] == -22 and "too large" in answer["error"] and not answer["launches"]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("dim,count", [(1024, 80_000_000), (25, 2**31 - 1), (64, 2**31 - 1), (32_768, 1_500_000)])
+def test_embed_of_very_many_tokens(launches, dim, count, dtype):
+    answer, = launches(["embed", dict(rows=1000, dim=dim, count=count, dtype=dtype)])
+    names = _kernels(answer)
+    width = 4 if dtype == "fp32" else 8
+    threads = sum(grid * block for _, grid, _, block, _, _ in answer["launches"])
+    assert set(names) == {"embed_kernel"} and 2 * threads >= count * -(-dim // width)

@@ -31,6 +31,23 @@ def test_embed_grad_without_tokens(dtype, rows, dim):
         assert got.shape == (rows, dim) and not got.any()
 
 
+def test_embed_of_more_than_one_launch():
+    """A result of 2^33 pieces and more."""
+    _say("embed of more than one launch")
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 200 << 30:
+        pytest.skip("needs 150 GB of GPU memory")
+    dim, count = 1024, 2**26 + 2_000_003
+    table = _randn(torch.Generator().manual_seed(1), 997, dim, dtype="bf16")
+    tok = torch.arange(count, device=_gpu(), dtype=torch.int32) % 997
+    got = quiver.embed(table, tok)
+    for at in (0, 2**25 - 5, 2**26 - 5, 2**26 + 1_000_000, count - 1000):
+        s = slice(at, at + 1000)
+        assert torch.equal(got[s], table[tok[s].long()])
+    del got
+    torch.cuda.empty_cache()
+
+
 # ---- every tile, every way of reading, whole and in splits --------------------------------------
 
 
