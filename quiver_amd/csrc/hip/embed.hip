@@ -378,7 +378,8 @@ __global__ void __launch_bounds__(kSortWaves * 64) scatter_kernel(
 // ---- sums over the sorted list ----------------------------------------------------------------
 
 constexpr uint32_t kMostEntries = 2048;  // sorted entries of a work-group's pieces
-constexpr uint32_t kZeroRows = 64;  // table rows that one work-group checks for having no token
+constexpr uint32_t kZeroRows = 64;  // table rows that one work-group checks at a time for having no token
+constexpr uint64_t kZeroBlocks = 1u << 22;  // work-groups that do so, at most
 
 struct SumArgs {
   const void* grad;
@@ -390,7 +391,7 @@ struct SumArgs {
   void* out;
   float* partial;  // [piece][2][dim]: the run that came from the piece before, the one that goes on
   uint32_t piece;  // sorted entries that one group of lanes adds
-  uint32_t pieces, sum_blocks, slabs;
+  uint32_t pieces, sum_blocks, zero_blocks, slabs;
   uint32_t cpr;
 };
 
@@ -423,22 +424,24 @@ __device__ __forceinline__ uint32_t wave_lower_bound(const uint32_t* keys, uint3
 /// Rows without a token become zero (work-groups past the sums').
 template <class T, int V>
 __device__ __forceinline__ void zero_rows(const SumArgs& a, uint32_t block, uint32_t* s_flag) {
-  const uint64_t r0 = static_cast<uint64_t>(block) * kZeroRows;
-  if (threadIdx.x < kZeroRows) {
-    const uint64_t r = r0 + threadIdx.x;
-    uint32_t touched = 1;
-    if (r < a.rows) {
-      const uint32_t i = lower_bound(a.keys, a.count, static_cast<uint32_t>(r));
-      touched = i < a.count && a.keys[i] == r ? 1u : 0u;
+  for (uint64_t r0 = static_cast<uint64_t>(block) * kZeroRows; r0 < a.rows; r0 += static_cast<uint64_t>(a.zero_blocks) * kZeroRows) {
+    if (threadIdx.x < kZeroRows) {
+      const uint64_t r = r0 + threadIdx.x;
+      uint32_t touched = 1;
+      if (r < a.rows) {
+        const uint32_t i = lower_bound(a.keys, a.count, static_cast<uint32_t>(r));
+        touched = i < a.count && a.keys[i] == r ? 1u : 0u;
+      }
+      s_flag[threadIdx.x] = touched;
     }
-    s_flag[threadIdx.x] = touched;
-  }
-  __syncthreads();
-  const float zero[V] = {};
-  T* out = static_cast<T*>(a.out) + r0 * a.dim;
-  for (uint32_t i = threadIdx.x; i < kZeroRows * a.cpr; i += 256) {
-    const uint32_t row = i / a.cpr, c = (i - row * a.cpr) * V;
-    if (!s_flag[row]) store_floats<T, V>(out + static_cast<uint64_t>(row) * a.dim + (c < a.dim - V ? c : a.dim - V), zero);
+    __syncthreads();
+    const float zero[V] = {};
+    T* out = static_cast<T*>(a.out) + r0 * a.dim;
+    for (uint32_t i = threadIdx.x; i < kZeroRows * a.cpr; i += 256) {
+      const uint32_t row = i / a.cpr, c = (i - row * a.cpr) * V;
+      if (!s_flag[row]) store_floats<T, V>(out + static_cast<uint64_t>(row) * a.dim + (c < a.dim - V ? c : a.dim - V), zero);
+    }
+    __syncthreads();  // the flags are read
   }
 }
 
@@ -704,7 +707,7 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
     a.piece = l.piece;
     a.pieces = static_cast<uint32_t>(ceil_div(count, l.piece));
     a.cpr = static_cast<uint32_t>(ceil_div(dim, V));
-    const uint32_t zero_blocks = static_cast<uint32_t>(ceil_div(rows, kZeroRows));
+    a.zero_blocks = static_cast<uint32_t>(std::min(ceil_div(rows, kZeroRows), kZeroBlocks));
     const auto sum = [&](auto group) {
       constexpr int G = decltype(group)::value;
       QVH_REQUIRE(256 / G * a.piece <= kMostEntries, "qvh_embed_grad_device: pieces past the work-group's memory");
@@ -715,7 +718,7 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
       // (26 MB) 44 and 47.
       const bool stream = count * dim * sizeof(T) >= kStreamed;
       const auto kernel = stream ? embed_grad_sum_kernel<T, V, G, true> : embed_grad_sum_kernel<T, V, G, false>;
-      hipLaunchKernelGGL(kernel, dim3(a.sum_blocks + zero_blocks, a.slabs), dim3(256), 0, s, a);
+      hipLaunchKernelGGL(kernel, dim3(a.sum_blocks + a.zero_blocks, a.slabs), dim3(256), 0, s, a);
     };
     if (a.cpr <= 8) {
       sum(std::integral_constant<int, 8>{});

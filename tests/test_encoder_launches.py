@@ -128,3 +128,10 @@ def test_embed_of_very_many_tokens(launches, dim, count, dtype):
     width = 4 if dtype == "fp32" else 8
     threads = sum(grid * block for _, grid, _, block, _, _ in answer["launches"])
     assert set(names) == {"embed_kernel"} and 2 * threads >= count * -(-dim // width)
+
+
+@pytest.mark.parametrize("rows,dim,count", [(2**30 + 70, 1, 10), (2**30 + 70, 1, 0), (2**32 - 2, 1, 5000), (2**31, 30, 100_000)])
+def test_embed_grad_of_very_many_rows(launches, rows, dim, count):
+    """Every row is cleared or written, in launches that the runtime takes."""
+    answer, = launches(["embed_grad", dict(rows=rows, dim=dim, count=count, dtype="bf16")])
+    assert "embed_grad_sum_kernel" in _kernels(answer)

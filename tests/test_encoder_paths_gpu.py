@@ -31,6 +31,19 @@ def test_embed_grad_without_tokens(dtype, rows, dim):
         assert got.shape == (rows, dim) and not got.any()
 
 
+@pytest.mark.parametrize("count", [0, 10])
+def test_embed_grad_of_more_than_2_30_rows(count):
+    """More rows than there are work-groups to clear them."""
+    _say("embed_grad of 2^30 rows", count)
+    rows = 2**30 + 70
+    out = quiver.embed_grad(torch.ones((count, 1), dtype=torch.bfloat16, device=_gpu()),
+                            torch.arange(count, device=_gpu()) * (rows // 10) + 69, rows)
+    named = torch.arange(count, device=_gpu()) * (rows // 10) + 69
+    assert bool((out[named] == 1).all())
+    out[named] = 0
+    assert not out.any()
+
+
 def test_embed_of_more_than_one_launch():
     """A result of 2^33 pieces and more."""
     _say("embed of more than one launch")
