@@ -336,7 +336,7 @@ qvh_status qvh_nearest_centroid(const float* x, uint64_t n, const float* centroi
  * The encoder in front of an index (no counterpart in the reference, whose callers bring finished
  * vectors): embedding lookup, linear layers, their gradients, and orthogonalised updates. All buffers
  * are device memory; every call enqueues on `stream` (NULL = the legacy null stream here) without
- * synchronizing and allocates nothing. Workspaces are the caller's: *_workspace gives the bytes (0:
+ * synchronizing, allocates nothing and leaves the thread's current device as it was. Workspaces are the caller's: *_workspace gives the bytes (0:
  * none needed, NULL may be passed), 16-byte aligned, in use until the call's work on the stream is
  * done. Element types are QVH_FP32, QVH_FP16 and QVH_BF16, the same for all of a call's matrices;
  * sums are fp32, rounded once where they are stored. Strides count elements between rows; elements of

@@ -62,6 +62,19 @@ int guarded(F&& f) noexcept {
 /// there is no gfx950 device.
 int current_device();
 
+/// Makes that device the thread's current one, and the thread's own again at the end: for calls that come
+/// between a caller's other GPU work, which may be on another device.
+class DeviceScope {
+ public:
+  DeviceScope();
+  ~DeviceScope();
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+
+ private:
+  int callers_ = -1;  // to go back to, where it is another one
+};
+
 /// Device allocation that honours the QVH_FAULT_ALLOC fault hook (see core.hip): the N-th
 /// allocation of the process fails with QVH_ENOMEM when QVH_FAULT_ALLOC=N is set.
 void* device_alloc(size_t bytes);

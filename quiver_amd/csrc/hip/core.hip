@@ -43,6 +43,17 @@ void check_device(int dev) {
   }
 }
 
+/// The device chosen by qvh_init, or 0, checked once.
+int chosen_device() {
+  std::lock_guard<std::mutex> lock(g_device_mu);
+  if (g_device < 0) g_device = 0;
+  if (!g_checked) {
+    check_device(g_device);
+    g_checked = true;
+  }
+  return g_device;
+}
+
 // simd::normalize (src/simd/dispatch.cc:119-135) of every row in place, eight lanes per row: the
 // group computes the row's dot product in the reference's order (exact_group8, bit for bit as
 // exact_dot), every lane then scales its share of the row by the same 1/sqrt(norm^2). A non-finite
@@ -122,14 +133,22 @@ thread_local PinnedWord t_finite;
 void set_last_error(const std::string& msg) { t_last_error = msg; }
 
 int current_device() {
-  std::lock_guard<std::mutex> lock(g_device_mu);
-  if (g_device < 0) g_device = 0;
-  if (!g_checked) {
-    check_device(g_device);
-    g_checked = true;
-  }
-  QVH_HIP(hipSetDevice(g_device));
-  return g_device;
+  const int device = chosen_device();
+  QVH_HIP(hipSetDevice(device));
+  return device;
+}
+
+DeviceScope::DeviceScope() {
+  const int device = chosen_device();
+  int now = device;
+  QVH_HIP(hipGetDevice(&now));
+  if (now == device) return;
+  QVH_HIP(hipSetDevice(device));
+  callers_ = now;
+}
+
+DeviceScope::~DeviceScope() {
+  if (callers_ >= 0) (void)hipSetDevice(callers_);
 }
 
 void* device_alloc(size_t bytes) {
@@ -188,7 +207,7 @@ qvh_status qvh_init(int device) {
 qvh_status qvh_get_device(int* device) {
   return qvh::guarded([&] {
     QVH_REQUIRE(device != nullptr, "qvh_get_device: null argument");
-    *device = qvh::current_device();
+    *device = qvh::chosen_device();
   });
 }
 

@@ -768,7 +768,7 @@ qvh_status qvh_embed_device(const void* d_table, uint64_t rows, uint32_t dim, ui
     QVH_REQUIRE(row_stride >= dim || rows <= 1, "qvh_embed_device: the row stride must be at least dim");
     if (count == 0) return;
     QVH_REQUIRE((d_table || rows == 0) && d_tokens && d_out, "qvh_embed_device: null buffer");
-    current_device();
+    const DeviceScope device;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     with_dtype(dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
@@ -807,7 +807,7 @@ qvh_status qvh_embed_grad_device(const void* d_grad, uint64_t row_stride, const 
                 "qvh_embed_grad_device: the workspace is too small");
     QVH_REQUIRE(reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0,
                 "qvh_embed_grad_device: the workspace must be 16-byte aligned");
-    current_device();
+    const DeviceScope device;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     with_dtype(dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;

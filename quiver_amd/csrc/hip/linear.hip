@@ -690,7 +690,7 @@ qvh_status qvh_linear_device(const qvh_linear_args* args, void* d_workspace, uin
     if (a.m == 0 || a.n == 0) return;
     const LinearRun r = plan_linear(a, d_workspace);
     check_workspace("qvh_linear_device", d_workspace, workspace_bytes, r.bytes);
-    current_device();
+    const DeviceScope device;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (r.few) {
       with_dtype(a.dtype, [&](auto* t) { launch_few<std::remove_pointer_t<decltype(t)>>(a, s); });
@@ -724,7 +724,7 @@ qvh_status qvh_linear_grad_device(const qvh_linear_grad_args* args, void* d_work
     const qvh_linear_grad_args& a = *args;
     const GradRun r = plan_grad(a, d_workspace);
     check_workspace("qvh_linear_grad_device", d_workspace, workspace_bytes, r.bytes);
-    current_device();
+    const DeviceScope device;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const bool products = a.k > 0 && (a.grad_x || a.grad_weight);
     if (r.slope && r.job.blocks > 0) {

@@ -636,7 +636,7 @@ qvh_status qvh_orthogonalize_device(const void* d_update, uint64_t batch, uint32
     const size_t need = ortho_layout(batch, m, n).total;
     QVH_REQUIRE(need == 0 || (d_workspace != nullptr && workspace_bytes >= need), w + ": the workspace is too small");
     QVH_REQUIRE(reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, w + ": the workspace must be 16-byte aligned");
-    current_device();
+    const DeviceScope device;
     with_dtype(dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       orthogonalize<T>(static_cast<const T*>(d_update), batch, m, n, steps, a, b, c, static_cast<T*>(d_out),

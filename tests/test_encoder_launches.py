@@ -135,3 +135,19 @@ def test_embed_grad_of_very_many_rows(launches, rows, dim, count):
     """Every row is cleared or written, in launches that the runtime takes."""
     answer, = launches(["embed_grad", dict(rows=rows, dim=dim, count=count, dtype="bf16")])
     assert "embed_grad_sum_kernel" in _kernels(answer)
+
+
+# ---- the caller's device ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("name,args", [
+    ("get_device", {}), ("embed", dict(rows=100, dim=64, count=10)), ("embed_grad", dict(rows=100, dim=64, count=9000)),
+    ("embed_grad", dict(rows=100, dim=64, count=10)), ("linear", dict(m=3, k=64, n=64)), ("linear", dict(m=3000, k=640, n=640)),
+    ("linear_grad", dict(m=300, k=64, n=64)), ("orthogonalize", dict(m=64, n=64)), ("orthogonalize", dict(m=640, n=640)),
+    ("linear", dict(m=2**31 - 1, k=64, n=64))])
+def test_the_callers_device_stays(launches, name, args):
+    """The kernels run on the library's device (0), and the caller's current one (1) is the same after the call, a refused
+    one too."""
+    answer, = launches([name, args])
+    assert answer["device"] == [1, 1]
+    assert all(launch[5] == 0 for launch in answer["launches"])
