@@ -9,8 +9,9 @@
 
 Tensors are float32, float16 or bfloat16, the same for all matrices of a call; sums are fp32 and
 results are rounded once. Calls run on torch's current stream, return without waiting, and give the
-same bits for the same inputs. Workspaces come from torch's allocator. Nothing here records an
-autograd graph: the gradients are calls of their own. Wrong arguments raise ``ValueError``
+same bits for the same inputs. Workspaces come from torch's allocator. ``embed`` and ``linear`` take part in
+torch's autograd where an input requires a gradient; results of ``embed_grad`` and ``linear_grad``, which
+are its backward passes, are constants to it. Wrong arguments raise ``ValueError``
 (``TypeError`` where something is not a tensor). Rows may be strided; any other layout is copied
 first. The reference has no counterpart: its callers bring finished vectors
 (python/quiver/__init__.py:166-251).
@@ -29,11 +30,13 @@ _torch = None
 _tensor = None
 _dtypes = {}
 _raw_stream = None
+_forward_ad = None
+_grad_enabled = None
 
 
 def _load_torch():
     """torch, once it is known to share this library's HIP runtime."""
-    global _torch, _tensor, _raw_stream
+    global _torch, _tensor, _raw_stream, _forward_ad, _grad_enabled
     if _torch is None:
         import torch
 
@@ -46,14 +49,41 @@ def _load_torch():
         # The current stream's handle alone; torch.cuda.current_stream makes an object of it, at 2 us a call.
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         _tensor = torch.Tensor
+        _forward_ad = torch.autograd.forward_ad
+        _grad_enabled = torch.is_grad_enabled
         _torch = torch
     return _torch
 
 
+def _differentiated(x, weight=None, bias=None, residual=None) -> bool:
+    """Whether autograd has to know of a call: an input requires a gradient, or carries a tangent."""
+    if _torch is None:
+        _load_torch()
+    try:
+        if (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)
+                or (residual is not None and residual.requires_grad)):
+            return _grad_enabled() or _forward_ad._current_level >= 0
+        if _forward_ad._current_level < 0:
+            return False
+        return any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in (x, weight, bias, residual))
+    except AttributeError:
+        return False  # not a tensor, which the call refuses
+
+
+def _node(name: str, *args):
+    from . import autograd
+
+    return getattr(autograd, name).apply(*args)
+
+
 def _check(name: str, x, device=None, dtype=None):
     """A floating device tensor, on `device` and of `dtype` where those are given."""
-    if dtype is not None and x.__class__ is _tensor and x.dtype is dtype and x.device == device:
-        return  # what nearly every call finds, in a third of the time
+    if x.__class__ is _tensor:  # what nearly every call finds, in a third of the time
+        if dtype is not None:
+            if x.dtype is dtype and x.device == device:
+                return
+        elif x.is_cuda and x.dtype in _dtypes and x.device.index == _quiver._device_index():
+            return
     torch = _load_torch()
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor in GPU memory")
@@ -122,6 +152,10 @@ def embed(table, tokens, scale: float = 1.0):
     A token outside the table gives a row of zeros: -1 is padding, and the label of an empty search
     result. Tokens are int32 or int64; dim is at most 32768.
     """
+    return _node("Embed", table, tokens, scale) if _differentiated(table) else _embed(table, tokens, scale)
+
+
+def _embed(table, tokens, scale):
     _check("table", table)
     if table.dim() != 2:
         raise ValueError(f"table must be [rows, dim], got shape {tuple(table.shape)}")
@@ -167,6 +201,12 @@ def linear(x, weight, bias=None, activation: Optional[str] = None, residual=None
     relu, gelu (with the error function) or silu. With keep_preactivation the sum in front of the
     activation, which ``linear_grad`` takes, comes back too: (result, preactivation).
     """
+    if _differentiated(x, weight, bias, residual):
+        return _node("Linear", x, weight, bias, residual, activation, keep_preactivation)
+    return _linear(x, weight, bias, activation, residual, keep_preactivation)
+
+
+def _linear(x, weight, bias, activation, residual, keep_preactivation):
     _check("x", x)
     device, dtype = x.device, x.dtype
     _check("weight", weight, device, dtype)
@@ -175,8 +215,8 @@ def linear(x, weight, bias=None, activation: Optional[str] = None, residual=None
     n, k = weight.shape
     act = _activation(activation)
     shape = x.shape[:-1] + (n,)
-    xr, xs = _rows(x, k)
-    wr, ws = _rows(weight, k)
+    xr, xs = (x, k) if x.is_contiguous() else _rows(x, k)
+    wr, ws = (weight, k) if weight.is_contiguous() else _rows(weight, k)
     br = rr = None
     rs = n
     if bias is not None:
@@ -209,6 +249,10 @@ def linear_grad(grad, x, weight, preactivation=None, activation: Optional[str] =
     preactivation is what ``linear`` kept; it is needed with an activation only. grad_bias is None without
     ``bias``, grad_x without ``inputs``. The residual's gradient is ``grad`` itself.
     """
+    return _linear_grad(grad, x, weight, preactivation, activation, bias, inputs, True)
+
+
+def _linear_grad(grad, x, weight, preactivation, activation, bias, inputs, weights):
     _check("grad", grad)
     device, dtype = grad.device, grad.dtype
     _check("x", x, device, dtype)
@@ -232,10 +276,11 @@ def linear_grad(grad, x, weight, preactivation=None, activation: Optional[str] =
     wr, ws = _rows(weight, k)
     m = grad.numel() // n if n else x.numel() // k if k else 0
     gx = x.new_empty(x.shape) if inputs else None
-    gw = weight.new_empty((n, k))
+    gw = weight.new_empty((n, k)) if weights else None
     gb = weight.new_empty((n,)) if bias else None
     args = (m, k, n, _dtypes[dtype], act, gr.data_ptr(), gs, 0 if pr is None else pr.data_ptr(), ps, xr.data_ptr(), xs,
-            wr.data_ptr(), ws, 0 if gx is None else gx.data_ptr(), k, gw.data_ptr(), k, 0 if gb is None else gb.data_ptr())
+            wr.data_ptr(), ws, 0 if gx is None else gx.data_ptr(), k, 0 if gw is None else gw.data_ptr(), k,
+            0 if gb is None else gb.data_ptr())
     stream = _stream(device)
     need = _quiver._linear_grad(*args, 0, 0, stream)
     if need:
@@ -250,8 +295,15 @@ def orthogonalize(update, steps: int = 5, coefficients: Sequence[float] = (3.444
     From ``X = G / |G|_F``, ``steps`` times ``X <- a X + (b A + c A A) X`` with ``A = X X^T`` (from the right
     where m > n): the singular vectors stay, every singular value s goes through a s + b s^3 + c s^5.
     The default coefficients bring all but tiny ones near 1 in five steps. A zero matrix stays zero.
-    Coefficients that let singular values grow without bound are refused.
+    Coefficients that let singular values grow without bound are refused. It makes an optimiser's steps
+    and has no derivative: a backward pass through it raises an error.
     """
+    if _differentiated(update):
+        return _node("Orthogonalize", update, steps, coefficients)
+    return _orthogonalize(update, steps, coefficients)
+
+
+def _orthogonalize(update, steps, coefficients):
     _check("update", update)
     if update.dim() < 2:
         raise ValueError(f"update must be [..., m, n], got shape {tuple(update.shape)}")
