@@ -101,6 +101,24 @@ __device__ __forceinline__ float normal_tail(float a, float z, float* e) {
   return p * t * *e;
 }
 
+/// exp(-z), z from -88 on, to its last bits: two to the power z log2(e) is rounded to, times what that leaves out of z.
+__device__ __forceinline__ float exp_minus(float z) {
+  const float t = z * -1.44269504f, e = __builtin_amdgcn_exp2f(t);
+  return fmaf(e, fmaf(t, 1.90465421e-9f, fmaf(t, -0.69314718f, -z)), e);  // ln 2 in two parts
+}
+
+/// 1 / (1 + exp(-z)), *other the same of -z. FINE: for fp32 results, to the last bits for every z (0 below -87.4, where it would be
+/// less than the smallest normal number). Four instructions more than the other form: 10,000 x 768 x 768 with SiLU 98.9 us for
+/// 98.1; expf and a division would make it 102. For 16-bit ones the hardware's exponential of z, whose error of |z| 2^-24 is far
+/// below their rounding.
+template <bool FINE>
+__device__ __forceinline__ float logistic(float z, float* other) {
+  const float e = FINE ? exp_minus(__builtin_amdgcn_fmed3f(z, -88.0f, 88.0f)) : __expf(-z);
+  const float s = __builtin_amdgcn_rcpf(1.0f + e);
+  *other = FINE ? e * s : 1.0f - s;
+  return s;
+}
+
 /// FINE: for fp32 results.
 template <bool FINE>
 __device__ __forceinline__ float activate(float z, int act) {
@@ -112,7 +130,10 @@ __device__ __forceinline__ float activate(float z, int act) {
     float e;
     return fmaf(-a, normal_tail(a, z, &e), fmaxf(z, 0.0f));
   }
-  if (act == QVH_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+  if (act == QVH_ACT_SILU) {
+    float other;
+    return z * logistic<FINE>(z, &other);
+  }
   return z;
 }
 
@@ -122,15 +143,16 @@ __device__ __forceinline__ float activate_slope(float z, int act) {
   if (act == QVH_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
   if (act == QVH_ACT_GELU) {
     if constexpr (FINE) {
-      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+      return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * exp_minus(fminf(0.5f * z * z, 120.0f)) * 0.39894228040143268f;
     }
     float e;
     const float tail = normal_tail(fabsf(z), z, &e);
     return fmaf(z * 0.39894228f, e, z > 0.0f ? 1.0f - tail : tail);
   }
   if (act == QVH_ACT_SILU) {
-    const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-z));
-    return s * (1.0f + z * (1.0f - s));
+    float other;
+    const float s = logistic<FINE>(z, &other);
+    return s * (1.0f + z * other);
   }
   return 1.0f;
 }

@@ -10,7 +10,7 @@ import pytest
 
 import quiver_amd as quiver
 from encoder_paths import GRAD, LINEAR, ORTHO
-from test_encoder_gpu import MUON, ROUND, TYPES, _check_linear, _check_linear_grad, _gpu, _randn, _say, _slope64
+from test_encoder_gpu import MUON, ROUND, TYPES, _check_linear, _check_linear_grad, _gpu, _randn, _say, _slope64, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -218,3 +218,49 @@ def test_large_layers_of_not_finite_values(dtype):
         _same_specials(dx, dz @ w.double())
         _same_specials(dw, dz.t() @ x.double())
         _same_specials(db, dz.sum(0))
+
+
+# ---- activations by themselves ------------------------------------------------------------------
+
+
+def _through(z, act):
+    """act(z) and its slope at z, by a layer and a gradient of one product with 1."""
+    one = torch.ones((1, 1), dtype=z.dtype, device=z.device)
+    y = quiver.linear(z[:, None], one, activation=act)
+    slope, _, _ = quiver.linear_grad(torch.ones_like(z)[:, None], z[:, None], one, preactivation=z[:, None], activation=act)
+    return y[:, 0].double(), slope[:, 0].double()
+
+
+@pytest.mark.parametrize("count", [40, 20_000])
+def test_fp32_silu_is_good_to_its_last_bits(count):
+    """The exponential, a sum, a quotient and a product: 8 roundings of 2^-24 at most, whatever the size of z, and 16 of the
+    slope's terms; below that the smallest normal number times z."""
+    _say("silu fp32", count)
+    z = torch.cat([torch.linspace(-100, 100, count - 8), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 700.0, -700.0, 3e38, -3e38])]).to(_gpu())
+    y, slope = _through(z, "silu")
+    zd = z.double()
+    s, q = torch.sigmoid(zd), torch.sigmoid(-zd)
+    tiny = (1 + zd.abs().clamp(max=1e3)) * 2.0**-126
+    _within(y, zd * s, (zd * s).abs() * 2.0**-21 + tiny)
+    _within(slope, s * (1 + zd * q), s * (1 + zd.abs() * q) * 2.0**-20 + tiny)
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu", "relu"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_activations_of_not_finite_values(dtype, act):
+    """What the formulas give: infinity and NaN go through; -infinity is 0 for ReLU and infinity times 0 for the others."""
+    _say("activations not finite", dtype, act)
+    z = torch.tensor([float("inf"), -float("inf"), float("nan")] * 20, dtype=TYPES[dtype], device=_gpu())
+    y, _ = _through(z, act)
+    assert bool((y[0::3] == float("inf")).all()) and bool(torch.isnan(y[2::3]).all())
+    assert bool((y[1::3] == 0).all()) if act == "relu" else bool(torch.isnan(y[1::3]).all())
+
+
+def test_fp32_gelu_slope():
+    """Phi to 2^-23; z phi(z) to 8 roundings and that of z^2 in the exponent, 2^-24 of it."""
+    _say("gelu slope fp32")
+    z = torch.linspace(-15, 15, 30_001).to(_gpu())
+    _, slope = _through(z, "gelu")
+    zd = z.double()
+    term = zd * torch.exp(-0.5 * zd * zd) / math.sqrt(2 * math.pi)
+    _within(slope, torch.special.ndtr(zd) + term, 2.0**-23 + term.abs() * (zd * zd + 8) * 2.0**-24)
