@@ -264,3 +264,21 @@ def test_fp32_gelu_slope():
     zd = z.double()
     term = zd * torch.exp(-0.5 * zd * zd) / math.sqrt(2 * math.pi)
     _within(slope, torch.special.ndtr(zd) + term, 2.0**-23 + term.abs() * (zd * zd + 8) * 2.0**-24)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_16_bit_gelu_is_rounded_once(dtype):
+    """Every number of the type from -9 to 9: half of the spacing of numbers at the result, and what the fp32 evaluation may
+    leave before that. It has 1.7e-8 from the fit of the normal tail, and 5 + 3 roundings of values below 0.6, so less
+    than 2^-23 for GELU; its slope has two such terms, and Phi's rounding: 2^-22."""
+    _say("gelu 16 bit", dtype)
+    z = torch.arange(-2**15, 2**15, dtype=torch.int32).to(torch.int16).view(TYPES[dtype])
+    z = z[torch.isfinite(z) & (z.abs() <= 9)].to(_gpu())
+    bits, least = (11, -24) if dtype == "fp16" else (8, -133)
+    half = lambda v: 0.5 * torch.exp2((torch.floor(torch.log2(v.abs().clamp(min=1e-300))) - bits + 1).clamp(min=least))  # noqa: E731
+    y, slope = _through(z, "gelu")
+    zd = z.double()
+    want = zd * torch.special.ndtr(zd)
+    assert ((y - want).abs() <= half(want.abs() + 2.0**-23) + 2.0**-23).all(), ((y - want).abs() - half(want)).max().item()
+    want = torch.special.ndtr(zd) + zd * torch.exp(-0.5 * zd * zd) / math.sqrt(2 * math.pi)
+    assert ((slope - want).abs() <= half(want.abs() + 2.0**-22) + 2.0**-22).all(), ((slope - want).abs() - half(want)).max().item()
