@@ -24,10 +24,10 @@ constexpr uint32_t kMaxDim = 32768;
 // ---- lookup -----------------------------------------------------------------------------------
 
 /// Piece c of a row is V elements (vector_width), cpr pieces a row; U pieces per thread, 256 apart, so that each
-/// thread has U independent row reads in flight. Bound by memory: 250,007 tokens of 100 fp32 (a fifth of them
+/// thread has U independent row reads in flight. PAST: the result is stored past the L2s. Bound by memory: 250,007 tokens of 100 fp32 (a fifth of them
 /// padding) in a table of 1.18 million rows 22 us, the 182 MB it moves at 8 TB/s, some of the rows from the
 /// caches; 24 tokens of 768 bf16 2.4 us, the launch.
-template <class T, int V, class I, int U>
+template <class T, int V, class I, int U, bool PAST>
 __global__ void __launch_bounds__(256) embed_kernel(const T* __restrict__ table, uint64_t rows, uint64_t stride,
                                                     const I* __restrict__ tokens, uint64_t count, uint32_t dim,
                                                     uint32_t cpr, uint32_t magic, float scale, T* __restrict__ out) {
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(256) embed_kernel(const T* __restrict__ table,
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (at[u] < total) store_floats<T, V, (U > 1)>(out + row[u] * dim + col[u], x[u]);
+    if (at[u] < total) store_floats<T, V, PAST>(out + row[u] * dim + col[u], x[u]);
   }
 }
 
@@ -75,12 +75,12 @@ void launch_embed(const void* table, uint64_t rows, uint32_t dim, uint64_t strid
     const uint32_t cpr = static_cast<uint32_t>(ceil_div(dim, V));
     const uint32_t magic = cpr == 1 ? 0u : static_cast<uint32_t>((uint64_t{1} << 32) / cpr + 1);
     const uint64_t total = count * cpr;
-    const auto go = [&](auto unroll) {
+    const auto go = [&](auto unroll, auto past) {
       constexpr int U = decltype(unroll)::value;
       const uint64_t most = kGridThreads / 2 * U / cpr;  // tokens of a launch
       for (uint64_t t = 0; t < count; t += most) {
         const uint64_t n = std::min(most, count - t);
-        hipLaunchKernelGGL((embed_kernel<T, V, I, U>), dim3(static_cast<unsigned>(ceil_div(n * cpr, 256 * U))), dim3(256), 0,
+        hipLaunchKernelGGL((embed_kernel<T, V, I, U, decltype(past)::value>), dim3(static_cast<unsigned>(ceil_div(n * cpr, 256 * U))), dim3(256), 0,
                            s, static_cast<const T*>(table), rows, stride, static_cast<const I*>(tokens) + t, n, dim, cpr,
                            magic, scale, static_cast<T*>(out) + t * dim);
         QVH_HIP(hipGetLastError());
@@ -88,13 +88,14 @@ void launch_embed(const void* table, uint64_t rows, uint32_t dim, uint64_t strid
     };
     // Two pieces per thread where the device is full several times over; below, one. Both sides, one and two, with
     // the tables in HBM: 250,007 x 100 fp32 35.1 and 32.0 us, 60,000 x 1,024 bf16 40.3 and 36.0; 16,000 x 100
-    // fp32 3.8 and 4.2. (Four: 33.1, 36.4, 4.8.) The result, of 32 MB or more then, is stored past the L2s: 250,007 x
-    // 1,024 bf16 162 us through them, 143 past; 250,007 x 100 fp32 31.9 and 32.7.
-    if (total < (1u << 21)) {
-      go(std::integral_constant<int, 1>{});
-    } else {
-      go(std::integral_constant<int, 2>{});
+    // fp32 3.8 and 4.2. (Four: 33.1, 36.4, 4.8.) A result that the L2s cannot hold is stored past them, in whole pieces of 16
+    // bytes: 250,007 x 1,024 bf16 162 us through them, 143 past; 250,007 x 100 fp32 31.9 and 32.7; a smaller one,
+    // 1,050,000 x 9 bf16, 11.2 either way.
+    if (total < (1u << 21)) return go(std::integral_constant<int, 1>{}, std::false_type{});
+    if constexpr (V * sizeof(T) == 16) {
+      if (count * dim * sizeof(T) >= kStreamed) return go(std::integral_constant<int, 2>{}, std::true_type{});
     }
+    go(std::integral_constant<int, 2>{}, std::false_type{});
   });
 }
 

@@ -25,7 +25,8 @@ void gemm_forms(Form form, const GemmArgs& g, const Epi& e, const GemmPlan& p, v
 }
 
 /// A layer of 16-bit elements with results of 32 MB or more, as much as the L2s hold together, stores them past those,
-/// whose lines the operands then keep; so large a result takes the largest tile. Both sides, kept and past:
+/// whose lines the operands then keep. Only the largest tile does, in one piece: so large a result takes it
+/// unless n or k is small, and then there is little of the operands to keep. Both sides, kept and past:
 /// 16,384 x 1,024 x 4,096 bf16, GELU, two results of 134 MB 182 and 174 us; three layers of 4,096 x 1,024 x 1,024,
 /// 8 MB each, in a row 19.5 and 20.6 us a layer. True where it has launched.
 template <class T>

@@ -84,13 +84,17 @@ def get_device(lib):
 
 
 def _short(mangled):
-    """The kernel's name; for a product also how its operands are read, its tile and its epilogue."""
+    """The kernel's name; for a product also how its operands are read, its tile and its epilogue, for a lookup its
+    pieces' elements, how many a thread has, and whether they are stored past the L2s."""
     name = re.search(r"([a-z][a-z_]*_kernel)", mangled).group(1)
     if name == "gemm_kernel":
         read = "".join("rk"[int(b)] for b in re.findall(r"Lb([01])E", mangled)[:2])  # by rows, by k
         tile = re.findall(r"Li(\d+)E", re.search(r"4TileI((?:Li\d+E)+)E", mangled).group(1))
         name += f" {read} {'x'.join(tile[:2])} depth {tile[4]} planes {tile[6]} loads {tile[7]} " + \
             re.search(r"\d([A-Z][a-z]+)Epilogue", mangled).group(1).lower()
+    if name == "embed_kernel":
+        elements, each = re.findall(r"Li(\d+)E", mangled)
+        name += f" {elements} x {each}" + (" past" if re.search(r"Lb1E", mangled) else "")
     return name
 
 
