@@ -656,13 +656,11 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
                            static_cast<uint32_t>(count), static_cast<uint32_t>(rows), dim, own, scale,
                            static_cast<T*>(out));
       };
-      if (ceil_div(dim, V) <= 16) {
-        go(std::integral_constant<int, 16>{});
-      } else if (ceil_div(dim, V) <= 32) {
-        go(std::integral_constant<int, 32>{});
-      } else {
-        go(std::integral_constant<int, 64>{});
+      if constexpr (V * sizeof(T) == 16) {  // narrower rows have one piece or two
+        if (ceil_div(dim, V) > 32) return go(std::integral_constant<int, 64>{});
+        if (ceil_div(dim, V) > 16) return go(std::integral_constant<int, 32>{});
       }
+      go(std::integral_constant<int, 16>{});
     });
     QVH_HIP(hipGetLastError());
     return;
@@ -717,19 +715,24 @@ void launch_embed_grad(const void* grad, uint64_t stride, const void* tokens, ui
       // Gradients that the L2s cannot hold are read past them, so that the partial sums stay for the join. Both sides,
       // through and past: 250,007 x 100 bf16 146 and 131 us a call, 262,144 x 1,024 193 and 184; 100,000 x 128
       // (26 MB) 44 and 47.
-      const bool stream = count * dim * sizeof(T) >= kStreamed;
-      const auto kernel = stream ? embed_grad_sum_kernel<T, V, G, true> : embed_grad_sum_kernel<T, V, G, false>;
-      hipLaunchKernelGGL(kernel, dim3(a.sum_blocks + a.zero_blocks, a.slabs), dim3(256), 0, s, a);
+      const dim3 grid(a.sum_blocks + a.zero_blocks, a.slabs);
+      if constexpr (V * sizeof(T) == 16) {
+        if (count * dim * sizeof(T) >= kStreamed) {
+          hipLaunchKernelGGL((embed_grad_sum_kernel<T, V, G, true>), grid, dim3(256), 0, s, a);
+          return;
+        }
+      }
+      hipLaunchKernelGGL((embed_grad_sum_kernel<T, V, G, false>), grid, dim3(256), 0, s, a);
     };
-    if (a.cpr <= 8) {
+    const auto any = [&] {
+      if constexpr (V * sizeof(T) == 16) {  // narrower rows have one piece or two
+        if (a.cpr > 32) return sum(std::integral_constant<int, 64>{});
+        if (a.cpr > 16) return sum(std::integral_constant<int, 32>{});
+        if (a.cpr > 8) return sum(std::integral_constant<int, 16>{});
+      }
       sum(std::integral_constant<int, 8>{});
-    } else if (a.cpr <= 16) {
-      sum(std::integral_constant<int, 16>{});
-    } else if (a.cpr <= 32) {
-      sum(std::integral_constant<int, 32>{});
-    } else {
-      sum(std::integral_constant<int, 64>{});
-    }
+    };
+    any();
     QVH_HIP(hipGetLastError());
     if (a.pieces > 1) {
       const unsigned blocks = static_cast<unsigned>(ceil_div(a.pieces, kJoinWaves));

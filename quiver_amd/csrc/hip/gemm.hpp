@@ -769,6 +769,12 @@ struct HasColumns<LinearEpilogue<T>> {
   static constexpr bool value = true;
 };
 
+/// Whether products with this epilogue may be symmetric ones.
+template <class Epi, class = void>
+struct MaySymmetric : std::false_type {};
+template <class Epi>
+struct MaySymmetric<Epi, std::void_t<decltype(Epi::kSymmetric)>> : std::true_type {};
+
 /// Adds the splits' partial sums and runs the epilogue. Four splits of 4,096 x 1,024: 67 MB from the last-level
 /// cache and 8 out in 13 us. Work-groups from `blocks` on add column sums.
 template <class Epi>
@@ -830,30 +836,37 @@ enum class Kind : int;
 /// `symmetric`: m = n, and only the tiles on and below the diagonal are computed.
 GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, Kind kind, uint32_t batches, bool symmetric);
 
-template <class T, bool AK, bool BK, class Shape, class Epi>
+/// SPLIT: whether the plan may split k.
+template <class T, bool AK, bool BK, class Shape, bool SPLIT = true, class Epi>
 void launch_tile(GemmArgs g, const Epi& epi, hipStream_t s) {
   g.tiles_m = static_cast<uint32_t>(ceil_div(g.m, Shape::BM));
   g.tiles_n = static_cast<uint32_t>(ceil_div(g.n, Shape::BN));
   const uint64_t tiles = g.symmetric ? static_cast<uint64_t>(g.tiles_m) * (g.tiles_m + 1) / 2
                                      : static_cast<uint64_t>(g.tiles_m) * g.tiles_n;
   const dim3 grid(static_cast<unsigned>(tiles * g.splits), g.batches);  // gemm_plan: fits a launch
-  if (g.splits > 1) {
-    const uint64_t ld = ceil_div(g.n, 8) * 8;
-    const PartialEpilogue pe{g.partial, ld, ld * g.m};
-    hipLaunchKernelGGL((gemm_kernel<T, AK, BK, Shape, PartialEpilogue>), grid, dim3(Shape::WM * Shape::WN * 64), 0, s, g, pe);
-    QVH_HIP(hipGetLastError());
-    if (g.symmetric) {
-      const uint32_t side = static_cast<uint32_t>(ceil_div(g.m, 32));
-      hipLaunchKernelGGL((gemm_join_symmetric_kernel<Epi>), dim3(side * (side + 1) / 2, g.batches), dim3(128), 0, s, g, epi);
-    } else {
+  if constexpr (SPLIT) {
+    if (g.splits > 1) {
+      const uint64_t ld = ceil_div(g.n, 8) * 8;
+      const PartialEpilogue pe{g.partial, ld, ld * g.m};
+      hipLaunchKernelGGL((gemm_kernel<T, AK, BK, Shape, PartialEpilogue>), grid, dim3(Shape::WM * Shape::WN * 64), 0, s, g, pe);
+      QVH_HIP(hipGetLastError());
+      if constexpr (MaySymmetric<Epi>::value) {
+        if (g.symmetric) {
+          const uint32_t side = static_cast<uint32_t>(ceil_div(g.m, 32));
+          hipLaunchKernelGGL((gemm_join_symmetric_kernel<Epi>), dim3(side * (side + 1) / 2, g.batches), dim3(128), 0, s, g, epi);
+          QVH_HIP(hipGetLastError());
+          return;
+        }
+      }
       const uint32_t join = static_cast<uint32_t>(ceil_div(ld / 8 * g.m, 256));
       uint32_t more = 0;
       if constexpr (HasColumns<Epi>::value) more = static_cast<uint32_t>(ceil_div(epi.columns.cols, 64));
       hipLaunchKernelGGL((gemm_join_kernel<Epi>), dim3(join + more, g.batches), dim3(256), 0, s, g, epi, join);
+      QVH_HIP(hipGetLastError());
+      return;
     }
-  } else {
-    hipLaunchKernelGGL((gemm_kernel<T, AK, BK, Shape, Epi>), grid, dim3(Shape::WM * Shape::WN * 64), 0, s, g, epi);
   }
+  hipLaunchKernelGGL((gemm_kernel<T, AK, BK, Shape, Epi>), grid, dim3(Shape::WM * Shape::WN * 64), 0, s, g, epi);
   QVH_HIP(hipGetLastError());
 }
 
@@ -880,7 +893,7 @@ template <>
 struct Shapes<Kind::kPlane2> {
   using S0 = Tile<64, 64, 2, 2, 64, 2, 2>;
   using S1 = Tile<128, 128, 2, 2, 32, 2, 2>;
-  using S2 = Tile<256, 128, 4, 2, 32, 3, 2>;
+  using S2 = void;
   using Alone = Tile<128, 128, 2, 4, 64, 2, 2>;
 };
 template <>
@@ -915,17 +928,18 @@ void launch_gemm(GemmArgs g, const Epi& epi, const GemmPlan& plan, void* partial
   g.partial = static_cast<float*>(partial);
   using S = Shapes<K>;
   if constexpr (!std::is_void_v<typename S::S2>) {
-    // A symmetric product's tiles are square.
-    if (plan.tile == 2 && (S::S2::BM == S::S2::BN || !g.symmetric)) return launch_tile<T, AK, BK, typename S::S2>(g, epi, s);
+    if (plan.tile == 2) return launch_tile<T, AK, BK, typename S::S2>(g, epi, s);
   }
+  // One operand by rows and one by k is P X (gemm_plan: neither its 64-tiles nor its deep ones are split).
+  constexpr bool kSplit = K != Kind::kPlane2 || AK == BK;
   if constexpr (K == Kind::kPlane2) {
     // The deep tile where every work-group has a CU to itself; past that two shallow ones on a CU hide each
     // other's waits (orthogonalisation of 1,024 x 4,096 393 us, 364 with it; six of 678 x 1,096 451, 482).
     const uint64_t groups = ceil_div(g.m, 128) * ceil_div(g.n, 128) * g.splits * g.batches;
-    if (plan.tile == 1 && groups <= 256) return launch_tile<T, AK, BK, typename S::Alone>(g, epi, s);
+    if (plan.tile == 1 && groups <= 256) return launch_tile<T, AK, BK, typename S::Alone, kSplit>(g, epi, s);
   }
   if (plan.tile >= 1) return launch_tile<T, AK, BK, typename S::S1>(g, epi, s);
-  launch_tile<T, AK, BK, typename S::S0>(g, epi, s);
+  launch_tile<T, AK, BK, typename S::S0, kSplit>(g, epi, s);
 }
 
 }  // namespace qvh

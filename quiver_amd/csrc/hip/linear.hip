@@ -21,7 +21,7 @@ GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, Kind kind, uint32_t batch
   };
   constexpr Cost kCosts[6][3] = {
       {{64, 64, 256, 4, 0.45, 0.22, 2.0}, {128, 128, 256, 2, 0.70, 0.53, 4.0}, {256, 256, 512, 1, 1.75, 1.75, 8.0}},
-      {{64, 64, 256, 3, 0.40, 0.20, 2.0}, {128, 128, 512, 2, 0.55, 0.45, 4.0}, {256, 128, 512, 1, 0.95, 0.95, 6.0}},
+      {{64, 64, 256, 3, 0.40, 0.20, 2.0}, {128, 128, 512, 2, 0.55, 0.45, 4.0}, {}},
       {{64, 64, 256, 3, 0.50, 0.35, 2.0}, {128, 128, 512, 1, 0.95, 0.95, 4.0}, {256, 128, 512, 1, 1.80, 1.80, 6.0}},
       {{64, 64, 256, 3, 0.70, 0.52, 2.0}, {128, 128, 256, 2, 2.10, 2.00, 4.0}, {}},
       {{64, 64, 256, 4, 0.56, 0.35, 2.0}, {128, 128, 256, 2, 1.05, 0.75, 4.0}, {}},
@@ -38,6 +38,9 @@ GemmPlan gemm_plan(uint64_t m, uint64_t n, uint64_t k, Kind kind, uint32_t batch
     const uint64_t tiles = (symmetric ? tm * (tm + 1) / 2 : tm * tn) * batches;
     for (const uint32_t splits : kSplits) {
       if (splits > 1 && steps < 2 * splits) break;
+      // P X of an orthogonalisation is split as shallow 128-tiles only (launch_gemm): where the others would gain by it,
+      // 64-tiles in one piece are faster still (300,000 shapes, none of them split otherwise without this line).
+      if (kind == Kind::kPlane2 && !symmetric && splits > 1 && (t == 0 || tiles * splits <= 256)) continue;
       // What one launch has room for: the tiles, or the pieces that are joined.
       if (tiles / batches * splits * c.threads >= kGridThreads || (splits > 1 && m * ceil_div(n, 8) >= kGridThreads)) break;
       const double groups = static_cast<double>(tiles) * splits;

@@ -33,7 +33,7 @@ template <class T>
 bool gemm_streamed(Form form, const GemmArgs& g, const LinearEpilogue<T>& e, const GemmPlan& p, hipStream_t s) {
   if (form != Form::kRowsRows || p.tile != 2 || p.splits != 1) return false;
   if (static_cast<uint64_t>(g.m) * g.n * sizeof(T) < kStreamed) return false;
-  launch_tile<T, false, false, Shapes<Kind::kPlane1>::S2>(g, StreamedEpilogue<T>{e}, s);
+  launch_tile<T, false, false, Shapes<Kind::kPlane1>::S2, false>(g, StreamedEpilogue<T>{e}, s);
   return true;
 }
 

@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(256) start_kernel(const T* __restrict__ g, uin
 
 /// Parts of scale * acc, or of a + b S + c scale * acc with S's parts given; zeros behind the last column.
 struct PartsEpilogue {
+  static constexpr bool kSymmetric = true;  // S and S S are
   half_t* out;
   const half_t* s;  // null: no polynomial
   uint64_t ld, plane;

@@ -99,6 +99,15 @@ void recorder_shape(int i, unsigned long long* out) {
   std::memcpy(out, v, sizeof(v));
 }
 void recorder_clear() { g_launches.clear(); }
+/// The name of the i-th kernel that the library holds, null behind the last.
+const char* recorder_kernel(int i) {
+  static std::vector<const char*> all = [] {
+    std::vector<const char*> v;
+    for (const auto& n : names()) v.push_back(n.second.c_str());
+    return v;
+  }();
+  return i < static_cast<int>(all.size()) ? all[i] : nullptr;
+}
 int recorder_device() { return g_device; }
 
 }  // extern "C"

@@ -2,7 +2,7 @@
 
     python tests/launches.py RECORDER < calls > launches
 
-Both are JSON. A call is [name, {argument: value}]; its answer is the status, the error's text, the workspace's
+Both are JSON: a list of answers, and in front of it the names of all product kernels that the library holds. A call is [name, {argument: value}]; its answer is the status, the error's text, the workspace's
 size, the current device afterwards, and the launches as [kernel, grid x, grid y, threads, LDS bytes, device].
 RECORDER is tests/cpp/launch_recorder.cc, compiled. Buffers are made-up addresses: nothing reads them.
 """
@@ -10,6 +10,7 @@ RECORDER is tests/cpp/launch_recorder.cc, compiled. Buffers are made-up addresse
 from __future__ import annotations
 
 import ctypes as C
+import itertools
 import json
 import os
 import re
@@ -101,6 +102,7 @@ def _short(mangled):
 def main():
     recorder = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)
     recorder.recorder_name.restype = C.c_char_p
+    recorder.recorder_kernel.restype = C.c_char_p
     lib = C.CDLL(LIB)
     lib.qvh_last_error.restype = C.c_char_p
     answers = []
@@ -115,7 +117,8 @@ def main():
             launches.append([_short(recorder.recorder_name(i).decode()), shape[0], shape[1], shape[2], shape[4], shape[5]])
         answers.append(dict(status=status, error=lib.qvh_last_error().decode() if status else "", workspace=need,
                             device=[before, recorder.recorder_device()], launches=launches))
-    json.dump(answers, sys.stdout)
+    held = itertools.takewhile(lambda name: name is not None, (recorder.recorder_kernel(i) for i in itertools.count()))
+    json.dump([sorted({_short(name.decode()) for name in held if b"11gemm_kernel" in name}), answers], sys.stdout)
 
 
 if __name__ == "__main__":

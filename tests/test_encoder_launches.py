@@ -16,7 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 
 @pytest.fixture(scope="module")
 def launches(tmp_path_factory):
-    """launches([name, arguments], ...): the answers to these calls, made in a process of their own."""
+    """launches([name, arguments], ...): the answers to these calls, made in a process of their own. launches.held: the
+    product kernels that the library holds."""
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     recorder = str(tmp_path_factory.mktemp("recorder") / "liblaunch_recorder.so")
     subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-w", "-D__HIP_PLATFORM_AMD__", f"-I{rocm}/include",
@@ -26,7 +27,8 @@ def launches(tmp_path_factory):
         p = subprocess.run([sys.executable, os.path.join(HERE, "launches.py"), recorder], input=json.dumps(calls),
                            capture_output=True, text=True)
         assert p.returncode == 0, p.stderr
-        return json.loads(p.stdout)
+        run.held, answers = json.loads(p.stdout)
+        return answers
 
     return run
 
@@ -87,6 +89,14 @@ def test_tested_orthogonalisations_take_every_product_kernel(launches):
     taken = _products(launches(*(["orthogonalize", dict(m=size(16384), n=size(16384), steps=2, batch=rng.choice([1, 1, 2, 6, 12, size(200)]))]
                                  for _ in range(6000))))
     assert taken <= tested, sorted(taken - tested)
+
+
+def test_every_product_kernel_is_taken_by_a_call(launches):
+    """Nothing is built that no call reaches."""
+    calls = [c for dtype in ("bf16", "fp32") for c in _calls(dtype)]
+    calls += [["orthogonalize", dict(m=m, n=n, batch=b, steps=2)] for m, n, b in ORTHO]
+    taken = _products(launches(*calls))
+    assert set(launches.held) == taken, sorted(set(launches.held) - taken)
 
 
 def test_fp16_goes_as_bf16_does(launches):
