@@ -340,7 +340,9 @@ qvh_status qvh_nearest_centroid(const float* x, uint64_t n, const float* centroi
  * none needed, NULL may be passed), 16-byte aligned, in use until the call's work on the stream is
  * done. Element types are QVH_FP32, QVH_FP16 and QVH_BF16, the same for all of a call's matrices;
  * sums are fp32, rounded once where they are stored. Strides count elements between rows; elements of
- * a row are contiguous. Every result depends on the inputs alone, bit for bit.
+ * a row are contiguous. A call repeats bit for bit: nothing depends on timing. Kernels, splits of long sums and fp32's
+ * way of multiplying are chosen by the whole call, though (shapes, batch, strides, alignment of the buffers, which results are
+ * asked for), and another choice gives other last bits.
  * ------------------------------------------------------------------------------------------ */
 #define QVH_FP32 0
 #define QVH_FP16 1
@@ -371,8 +373,8 @@ qvh_status qvh_embed_grad_device(const void* d_grad, uint64_t row_stride, const 
  * backward pass of an activation takes. out may be the residual's own buffer, and no other overlap is
  * allowed. m is below 2^31, k and n at most 2^20, strides at most 2^22; a product whose tiles or operands go past
  * one launch (2^32 threads: about 10^9 rows where n is below 64, more for wider results) is refused. fp32 products run on fp32 matrix
- * instructions, large ones as sums of three bf16 parts of each operand (24 bits; what is dropped is below
- * fp32's own rounding). */
+ * instructions, large ones as sums of three bf16 parts of each operand (24 bits of values from 2^-100 on, fewer of
+ * smaller ones, whose parts are subnormal; what is dropped is below fp32's own rounding). */
 typedef struct qvh_linear_args {
   uint64_t m;
   uint32_t k, n;
@@ -394,9 +396,10 @@ qvh_status qvh_linear_device(const qvh_linear_args* args, void* d_workspace, uin
 
 /* Gradients of that layer from out's gradient grad [m][n]: with dz = grad * act'(preactivation),
  * grad_x [m][k] = dz w, grad_weight [n][k] = dz^T x, grad_bias [n] = the sum of dz over m (each nullable;
- * the residual's gradient is grad itself). preactivation is required with an activation. For 16-bit types
- * dz enters the two products rounded to the type, as any operand of the matrix unit; grad_bias does not
- * use the rounded values. */
+ * the residual's gradient is grad itself). preactivation is required with an activation. For 16-bit types and an
+ * activation dz enters the two products rounded to the type, as any operand of the matrix unit: by up to 2^-9 of a bf16
+ * term, 2^-12 of an fp16 one (2^-25 where that is less than 2^-14, and infinity past 65,504; slopes reach 1.13). grad_bias
+ * does not use the rounded values. */
 typedef struct qvh_linear_grad_args {
   uint64_t m;
   uint32_t k, n;

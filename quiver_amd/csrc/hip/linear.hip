@@ -143,8 +143,10 @@ __global__ void __launch_bounds__(256) prepare_kernel(PrepareArgs a, PrepareArgs
 
 /// dz = grad * act'(z) (stored if asked for) and its column sums over this work-group's rows. A thread
 /// has eight columns; LY threads share them, each taking every LY-th row. Bound by memory: 16,384 x
-/// 4,096 bf16 with GELU 403 MB in 82 us, 4.9 TB/s. dz is written for 16-bit results in their type: it feeds
-/// the matrix unit, which takes no wider ones (an error of 2^-9 of each term, as the gradient itself has).
+/// 4,096 bf16 with GELU 403 MB in 82 us, 4.9 TB/s. dz is written for 16-bit results in their type, since it feeds the
+/// matrix unit, which takes no wider ones: a rounding of each term by 2^-9 (bf16; 2^-12 in fp16, 2^-25 absolute below
+/// 2^-14), no larger than the one that the gradient came with; 2.3e-3 of a bf16 gradient's size altogether, 1.7e-3 without
+/// it. A second part for the rest would double both products.
 struct SlopeArgs {
   const void* grad;
   const void* pre;

@@ -8,8 +8,10 @@
     >>> w -= lr * quiver.orthogonalize(momentum)                         # momentum follows dw
 
 Tensors are float32, float16 or bfloat16, the same for all matrices of a call; sums are fp32 and
-results are rounded once. Calls run on torch's current stream, return without waiting, and give the
-same bits for the same inputs. Workspaces come from torch's allocator. ``embed`` and ``linear`` take part in
+results are rounded once. (One thing in between is too: where ``linear_grad`` has an activation and 16-bit
+tensors, the gradient behind it is rounded to their type for the products.) Calls run on torch's current stream, return
+without waiting, and repeat bit for bit; other shapes, strides, alignments, batches or results asked for may
+change the last bits. Workspaces come from torch's allocator. ``embed`` and ``linear`` take part in
 torch's autograd where an input requires a gradient; results of ``embed_grad`` and ``linear_grad``, which
 are its backward passes, are constants to it. Wrong arguments raise ``ValueError``
 (``TypeError`` where something is not a tensor). Rows may be strided; any other layout is copied
@@ -247,7 +249,9 @@ def linear_grad(grad, x, weight, preactivation=None, activation: Optional[str] =
     """Gradients of ``linear`` from its result's gradient: (grad_x, grad_weight, grad_bias).
 
     preactivation is what ``linear`` kept; it is needed with an activation only. grad_bias is None without
-    ``bias``, grad_x without ``inputs``. The residual's gradient is ``grad`` itself.
+    ``bias``, grad_x without ``inputs``. The residual's gradient is ``grad`` itself. With an activation and 16-bit
+    tensors, ``grad * act'(preactivation)`` enters the products rounded to their type (grad_bias does not use
+    the rounded values); in float16 it is infinite past 65,504 and keeps multiples of 2^-24 only.
     """
     return _linear_grad(grad, x, weight, preactivation, activation, bias, inputs, True)
 

@@ -158,6 +158,8 @@ def test_parts_hold_24_bits():
     x, w = _single_products(g)
     want = x.double() @ w.double().t()
     assert ((quiver.linear(x, w).double() - want).abs() <= 2.0**-20 * want.abs()).all()
+    for size in (2.0**-100, 2.0**100):  # the range that the parts hold
+        assert ((quiver.linear(x * size, w / size).double() - want).abs() <= 2.0**-20 * want.abs()).all()
     # Backwards: one non-zero value per row of the gradient for grad_x, per column for grad_weight.
     m, k, n = PARTS
     gr = torch.zeros((m, n), device=_gpu())
