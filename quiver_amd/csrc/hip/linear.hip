@@ -412,10 +412,6 @@ void run_product(Form form, Kind kind, int dtype, GemmArgs g, const void* bias, 
     e.ld_out = ld_out;
     e.ld_keep = ld_keep;
     e.act = act;
-    e.direct = g;
-    e.a_by_k = form == Form::kKK;
-    e.b_by_k = form != Form::kRowsRows;
-    e.planes = kind == Kind::kPlane3 ? kPlanes : 0;
     if constexpr (std::is_same_v<T, float>) {
       gemm_fp32(form, kind, g, e, plan, partial, s);
     } else if constexpr (std::is_same_v<T, half_t>) {

@@ -284,3 +284,58 @@ def test_16_bit_gelu_is_rounded_once(dtype):
     assert ((y - want).abs() <= half(want.abs() + 2.0**-23) + 2.0**-23).all(), ((y - want).abs() - half(want)).max().item()
     want = torch.special.ndtr(zd) + zd * torch.exp(-0.5 * zd * zd) / math.sqrt(2 * math.pi)
     assert ((slope - want).abs() <= half(want.abs() + 2.0**-22) + 2.0**-22).all(), ((slope - want).abs() - half(want)).max().item()
+
+
+def test_parts_that_overflow():
+    """Finite values whose products are past fp32: their parts overflow both ways, the results are infinite on the side of the
+    true sum, and finite sums of them finite."""
+    _say("parts overflow")
+    m, k, n = PARTS
+    g = torch.Generator().manual_seed(14)
+    x, w = _randn(g, m, k, dtype="fp32"), _randn(g, n, k, dtype="fp32")
+    x[7] *= 1e30  # with w below: sums of 1e40 and more, of either sign
+    w[5] *= 1e10
+    x[9], w[3] = 0.0, 0.0
+    x[9, 100], x[9, 101], w[3, 100], w[3, 101] = 3.3e38, -3.3e38, 1.25e5, 1.25e5  # 4e43 - 4e43
+    x[11], w[1] = 0.0, 0.0
+    x[11, 33], w[1, 33] = 3.4e38, -3.3e5
+    want = x.double() @ w.double().t()
+    got = quiver.linear(x, w)
+    assert torch.equal(got[7, 5].double(), want[7, 5].sign() * math.inf) and abs(want[7, 5]) > 1e39
+    assert got[11, 1] == -math.inf
+    assert got[9, 3] == 0 or torch.isnan(got[9, 3])  # in fp32 arithmetic, infinity minus infinity
+    plain = torch.ones(m, dtype=torch.bool, device=_gpu()).index_fill_(0, torch.tensor([7, 9, 11], device=_gpu()), False)
+    others = torch.ones(n, dtype=torch.bool, device=_gpu()).index_fill_(0, torch.tensor([5, 3, 1], device=_gpu()), False)
+    keep = plain[:, None] & others[None, :]
+    bound = (x.double().abs() @ w.double().abs().t()) * (k + 8) * 2.0**-23
+    assert (((got.double() - want).abs() <= bound + want.abs() * 2.0**-24) | ~keep).all()
+
+
+def test_infinities_do_not_stall_a_large_layer():
+    """One in each row makes every result of parts NaN at first, to be made again. That may take a second product that waits for
+    every load, some twenty times as long as the first; a hundred times would be a loop over single elements."""
+    _say("infinities' time")
+    m, k, n = 4096, 1024, 1024
+    g = torch.Generator().manual_seed(13)
+    x, w, gr = _randn(g, m, k, dtype="fp32"), _randn(g, n, k, dtype="fp32"), _randn(g, m, n, dtype="fp32")
+
+    def ms(call):
+        best = math.inf
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            call()
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    layer, grad = lambda: quiver.linear(x, w), lambda: quiver.linear_grad(gr, x, w)  # noqa: E731
+    layer(), grad()
+    before = ms(layer), ms(grad)
+    x[torch.arange(m), torch.randint(0, k, (m,), generator=g)] = float("inf")
+    after = ms(layer), ms(grad)
+    print("ms without and with infinities:", before, after, flush=True)
+    _same_specials(layer(), x.double() @ w.double().t())
+    _same_specials(grad()[1], gr.double().t() @ x.double())
+    assert after[0] < 40 * before[0] and after[1] < 40 * before[1]
