@@ -111,8 +111,8 @@ __device__ __forceinline__ float exp_minus(float z) {
 }
 
 /// 1 / (1 + exp(-z)), *other the same of -z. FINE: for fp32 results, to the last bits for every z (0 below -87.4, where it would be
-/// less than the smallest normal number). Four instructions more than the other form: 10,000 x 768 x 768 with SiLU 98.9 us for
-/// 98.1; expf and a division would make it 102. For 16-bit ones the hardware's exponential of z, whose error of |z| 2^-24 is far
+/// less than the smallest normal number). Four instructions more than the other form, 0.8 us of the 92 of 10,000 x 768 x 768 with
+/// SiLU; expf and a division would take 4. For 16-bit ones the hardware's exponential of z, whose error of |z| 2^-24 is far
 /// below their rounding.
 template <bool FINE>
 __device__ __forceinline__ float logistic(float z, float* other) {

@@ -11,8 +11,8 @@
 // part of values around 1/1000 stays a normal number. fp32 products of the same matrices would run on
 // instructions sixteen times as slow, three bf16 parts take twice the products.
 //
-// 4,096 x 1,024 bf16, five steps, 395 us: per step S 24 us and 5 to join its three parts of k, S S 16 and 5, P X 29
-// (1,024 x 1,024 results of two parts are a third of a chip's tiles; the matrix instructions of P X are busy 35% of
+// 4,096 x 1,024 bf16, five steps, 354 to 372 us: per step S 24 us and 5 to join its three parts of k, S S 15 in one piece, P X 29
+// (1,024 x 1,024 results of two parts are a third of a chip's tiles; the matrix instructions of P X are busy 34% of
 // the time). Since S and S S are symmetric, only their lower tiles are computed.
 #include <algorithm>
 #include <cmath>
