@@ -24,9 +24,9 @@ constexpr uint32_t kMaxDim = 32768;
 // ---- lookup -----------------------------------------------------------------------------------
 
 /// Piece c of a row is V elements (vector_width), cpr pieces a row; U pieces per thread, 256 apart, so that each
-/// thread has U independent row reads in flight. PAST: the result is stored past the L2s. Bound by memory: 250,007 tokens of 100 fp32 (a fifth of them
-/// padding) in a table of 1.18 million rows 22 us, the 182 MB it moves at 8 TB/s, some of the rows from the
-/// caches; 24 tokens of 768 bf16 2.4 us, the launch.
+/// thread has U independent row reads in flight. PAST: the result is stored past the L2s. Bound by memory:
+/// 250,007 tokens of 100 fp32 (a fifth of them padding) in a table of 1.18 million rows 22 us, the 182 MB it
+/// moves at 8 TB/s, some of the rows from the caches; 24 tokens of 768 bf16 2.4 us, the launch.
 template <class T, int V, class I, int U, bool PAST>
 __global__ void __launch_bounds__(256) embed_kernel(const T* __restrict__ table, uint64_t rows, uint64_t stride,
                                                     const I* __restrict__ tokens, uint64_t count, uint32_t dim,

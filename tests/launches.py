@@ -2,9 +2,10 @@
 
     python tests/launches.py RECORDER < calls > launches
 
-Both are JSON: a list of answers, and in front of it the names of all product kernels that the library holds. A call is [name, {argument: value}]; its answer is the status, the error's text, the workspace's
-size, the current device afterwards, and the launches as [kernel, grid x, grid y, threads, LDS bytes, device].
-RECORDER is tests/cpp/launch_recorder.cc, compiled. Buffers are made-up addresses: nothing reads them.
+Both are JSON. A call is [name, {argument: value}]. Out come the names of all product kernels that the library
+holds, and an answer to each call: the status, the error's text, the workspace's size, the current device
+before and after, and the launches as [kernel, grid x, grid y, threads, LDS bytes, device]. RECORDER is
+tests/cpp/launch_recorder.cc, compiled. Buffers are made-up addresses: nothing reads them.
 """
 
 from __future__ import annotations

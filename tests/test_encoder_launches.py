@@ -86,7 +86,8 @@ def test_tested_orthogonalisations_take_every_product_kernel(launches):
     tested = _products(launches(*(["orthogonalize", dict(m=m, n=n, batch=b, steps=2)] for m, n, b in ORTHO)))
     rng = random.Random(4)
     size = lambda hi: int(round(math.exp(rng.uniform(0, math.log(hi)))))  # noqa: E731
-    taken = _products(launches(*(["orthogonalize", dict(m=size(16384), n=size(16384), steps=2, batch=rng.choice([1, 1, 2, 6, 12, size(200)]))]
+    batch = lambda: rng.choice([1, 1, 2, 6, 12, size(200)])  # noqa: E731
+    taken = _products(launches(*(["orthogonalize", dict(m=size(16384), n=size(16384), steps=2, batch=batch())]
                                  for _ in range(6000))))
     assert taken <= tested, sorted(taken - tested)
 
@@ -175,3 +176,10 @@ def test_embed_stores_large_results_past_the_caches(launches, dtype, dim, count,
     """By the result's bytes (32 MB), where its pieces are of 16 bytes."""
     answer, = launches(["embed", dict(rows=1000, dim=dim, count=count, dtype=dtype)])
     assert _kernels(answer) == ["embed_kernel " + kernel]
+
+
+def test_large_results_of_any_width_go_past_the_caches(launches):
+    """A layer's, where it takes the largest tile whole: also with rows that end anywhere."""
+    for n in (920, 917):
+        answer, = launches(["linear", dict(m=27437, k=200, n=n, dtype="bf16", act="gelu", bias=True, residual=True, keep=True)])
+        assert _kernels(answer) == ["gemm_kernel rr 256x256 depth 64 planes 1 loads 16 streamed"]
