@@ -352,6 +352,7 @@ qvh_status qvh_nearest_centroid(const float* x, uint64_t n, const float* centroi
 #define QVH_ACT_RELU 1
 #define QVH_ACT_GELU 2 /* z Phi(z), with the error function */
 #define QVH_ACT_SILU 3 /* z / (1 + exp(-z)) */
+#define QVH_ACT_SIGMOID 4 /* 1 / (1 + exp(-z)), of a gate */
 
 /* out[count][dim] = scale * table[token], rows of zeros for tokens outside [0, rows): -1 is padding (and
  * an empty slot of a search's labels). index_bytes is 4 (int32 tokens) or 8 (int64); dim is at most
@@ -432,6 +433,81 @@ qvh_status qvh_orthogonalize_workspace(uint64_t batch, uint32_t m, uint32_t n, u
 qvh_status qvh_orthogonalize_device(const void* d_update, uint64_t batch, uint32_t m, uint32_t n, int dtype,
                                     uint32_t steps, float a, float b, float c, void* d_out, void* d_workspace,
                                     uint64_t workspace_bytes, void* stream);
+
+/* The way from one block of an encoder to the next: with norm(t) = t / sqrt(mean(t^2) + eps) over a row,
+ *   r = x + scale * act(gate) * norm(y) * post_weight,   h = norm(r) * weight,
+ * x the residual stream, y the block's result, gate (nullable) a factor for each element with gate_activation none,
+ * silu or sigmoid, scale (nullable) one for each column. y may be null: then h = norm(x) * weight, and gate,
+ * post_weight, scale and r are null too. Matrices are [rows][dim] (r and h contiguous), vectors [dim]. h is made of
+ * r before its rounding. dim is at most 16384, rows below 2^31, strides at most 2^22. Squares are fp32: rows whose sum of
+ * squares passes 3.4e38 have a norm of zeros. No result overlaps another buffer of the call. */
+typedef struct qvh_block_norm_args {
+  uint64_t rows;
+  uint32_t dim;
+  int dtype, gate_activation;
+  float eps;
+  const void* x;
+  uint64_t x_stride;
+  const void* y;
+  uint64_t y_stride;
+  const void* gate;
+  uint64_t gate_stride;
+  const void* weight;
+  const void* post_weight;
+  const void* scale;
+  void* r;
+  void* h;
+} qvh_block_norm_args;
+qvh_status qvh_block_norm_device(const qvh_block_norm_args* args, void* stream);
+
+/* Its gradients from those of h (grad_h) and of r (grad_r, nullable): grad_x (also r's whole gradient), grad_y, grad_gate
+ * [rows][dim], contiguous, and grad_weight, grad_post, grad_scale [dim]. Each is nullable. r is what the forward pass
+ * gave, or x where there is no y. */
+typedef struct qvh_block_norm_grad_args {
+  uint64_t rows;
+  uint32_t dim;
+  int dtype, gate_activation;
+  float eps;
+  const void* grad_h;
+  uint64_t grad_h_stride;
+  const void* grad_r;
+  uint64_t grad_r_stride;
+  const void* r;
+  uint64_t r_stride;
+  const void* y;
+  uint64_t y_stride;
+  const void* gate;
+  uint64_t gate_stride;
+  const void* weight;
+  const void* post_weight;
+  const void* scale;
+  void* grad_x;
+  void* grad_y;
+  void* grad_gate;
+  void* grad_weight;
+  void* grad_post;
+  void* grad_scale;
+} qvh_block_norm_grad_args;
+qvh_status qvh_block_norm_grad_workspace(const qvh_block_norm_grad_args* args, uint64_t* bytes);
+qvh_status qvh_block_norm_grad_device(const qvh_block_norm_grad_args* args, void* d_workspace, uint64_t workspace_bytes,
+                                      void* stream);
+
+/* The norm over all gradients of a model, sqrt of the sum of their squares (fp64 sums, an fp32 result), and the gradients
+ * times min(1, max_norm / (norm + eps)). Each is `count` contiguous elements of its own type; out may be the gradient itself;
+ * results that overlap one another or another gradient are refused. Elements that are not finite make the norm so: an infinite one leaves zeros (NaN where the
+ * infinities were), NaN leaves NaN. The list is host memory, read before the call returns. At most 2^20 gradients
+ * of 2^40 elements, 2^44 in all. */
+typedef struct qvh_gradient {
+  const void* grad;
+  void* out; /* not of the norm alone */
+  uint64_t count;
+  int dtype;
+} qvh_gradient;
+qvh_status qvh_grad_norm_workspace(const qvh_gradient* grads, uint64_t count, uint64_t* bytes); /* of both calls */
+qvh_status qvh_grad_norm_device(const qvh_gradient* grads, uint64_t count, float* d_norm, void* d_workspace,
+                                uint64_t workspace_bytes, void* stream);
+qvh_status qvh_clip_grad_norm_device(const qvh_gradient* grads, uint64_t count, float max_norm, float eps,
+                                     float* d_norm /* nullable */, void* d_workspace, uint64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import torch
 
-from . import encoder
+from . import blocks, encoder
 
 
 class _Once(torch.autograd.Function):
@@ -72,6 +72,33 @@ class Linear(torch.autograd.Function):
             if grad is not None or grad_pre is not None:
                 gx, gw, gb = _once("linear", gradient, grad, grad_pre, x, weight, pre)
         return gx, gw, gb, grad if want_r else None, None, None
+
+
+class BlockNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, y, post_weight, gate, gate_activation, scale, eps):
+        result = blocks._block_norm(x, weight, y, post_weight, gate, gate_activation, scale, eps)
+        ctx.settings = gate_activation, eps
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x if y is None else result[0], weight, y, post_weight, gate, scale)
+        return result
+
+    @staticmethod
+    def backward(ctx, *grads):
+        grad_r, grad_h = grads if len(grads) == 2 else (None, grads[0])
+        if grad_r is None and grad_h is None:
+            return (None,) * 8
+        r, weight, y, post, gate, scale = ctx.saved_tensors
+        activation, eps = ctx.settings
+        need = ctx.needs_input_grad
+        wanted = need[0], need[1], need[2], need[3], need[4], need[6]
+
+        def gradient():
+            h = grad_h if grad_h is not None else torch.zeros_like(r)
+            return blocks._block_norm_grad(h, r, weight, grad_r, y, post, gate, activation, scale, eps, wanted)
+
+        gx, gw, gy, gp, gg, gs = _once("block_norm", gradient, grad_h, grad_r, r, weight, y, post, gate, scale)
+        return gx, gw, gy, gp, gg, None, gs, None
 
 
 class Orthogonalize(torch.autograd.Function):

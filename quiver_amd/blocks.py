@@ -1,0 +1,213 @@
+"""Blocks of an encoder, and their training step, on torch (ROCm) tensors in GPU memory.
+
+    >>> x, h = quiver.block_norm(x, w_in, y=y, post_weight=w_out, gate=g, gate_activation="silu", scale=s)
+    >>> norm = quiver.clip_grad_norm(grads, 1.0, out=grads)[1]           # in front of the optimiser's step
+
+They follow the rules of quiver_amd/encoder.py, whose layers go between them: types, streams, errors, strided rows,
+workspaces, results that repeat bit for bit, torch's autograd where an input requires a gradient.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Sequence, Tuple
+
+from . import _quiver
+from . import encoder as _encoder
+from .encoder import _check, _dtypes, _node, _rows, _stream, _workspace
+
+_GATES = {None: 0, "none": 0, "silu": 3, "sigmoid": 4}
+
+
+def _gate_activation(name) -> int:
+    try:
+        return _GATES[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"gate_activation must be none, silu or sigmoid, got {name!r}") from None
+
+
+def _differentiated(*tensors) -> bool:
+    return any(t is not None and _encoder._differentiated(t) for t in tensors)
+
+
+def _vector(name, v, dim, device, dtype):
+    _check(name, v, device, dtype)
+    if v.shape != (dim,):
+        raise ValueError(f"{name} must have shape ({dim},), got {tuple(v.shape)}")
+    return v if v.is_contiguous() else v.contiguous()
+
+
+def _matrix(name, m, shape, device, dtype):
+    _check(name, m, device, dtype)
+    if m.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(m.shape)}")
+    return _rows(m, shape[-1])
+
+
+def _pointer(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+# ---- norms around a block ---------------------------------------------------------------------
+
+
+def block_norm(x, weight, y=None, post_weight=None, gate=None, gate_activation: Optional[str] = None, scale=None, eps: float = 1e-6):
+    """From one block to the next: ``(r, h)`` with ``r = x + scale * act(gate) * norm(y) * post_weight`` and
+    ``h = norm(r) * weight``, where ``norm(t) = t / sqrt(mean(t^2) + eps)`` over the last dimension.
+
+    x [..., dim] is the residual stream, y of its shape the block's result, weight and post_weight [dim]. gate, a factor for
+    each element, has y's shape (gate_activation: none, silu or sigmoid), scale [dim] is one for each column; both may be
+    left out. Without y there is no block yet: ``h = norm(x) * weight`` alone. dim is at most 16384.
+    """
+    if _differentiated(x, weight, y, post_weight, gate, scale):
+        return _node("BlockNorm", x, weight, y, post_weight, gate, gate_activation, scale, eps)
+    return _block_norm(x, weight, y, post_weight, gate, gate_activation, scale, eps)
+
+
+def _block_arguments(x, weight, y, post_weight, gate, gate_activation, scale):
+    """What both passes check, as the calls take it: (tensors to hold, activation, arguments from y on)."""
+    _check("x", x)
+    device, dtype = x.device, x.dtype
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must be [..., dim], got shape {tuple(x.shape)}")
+    dim = x.shape[-1]
+    act = _gate_activation(gate_activation)
+    w = _vector("weight", weight, dim, device, dtype)
+    if y is None:
+        for name, t in (("post_weight", post_weight), ("gate", gate), ("scale", scale)):
+            if t is not None:
+                raise ValueError(f"{name} belongs to a block's result y")
+        return (w, None, None, None, None), act, (0, dim, 0, dim, w.data_ptr(), 0, 0)
+    yr, ys = _matrix("y", y, x.shape, device, dtype)
+    if post_weight is None:
+        raise ValueError("y needs post_weight")
+    pw = _vector("post_weight", post_weight, dim, device, dtype)
+    gr, gs = (None, dim) if gate is None else _matrix("gate", gate, x.shape, device, dtype)
+    sc = None if scale is None else _vector("scale", scale, dim, device, dtype)
+    return (w, yr, pw, gr, sc), act, (yr.data_ptr(), ys, _pointer(gr), gs, w.data_ptr(), pw.data_ptr(), _pointer(sc))
+
+
+def _block_norm(x, weight, y, post_weight, gate, gate_activation, scale, eps):
+    held, act, args = _block_arguments(x, weight, y, post_weight, gate, gate_activation, scale)
+    dim = x.shape[-1]
+    xr, xs = _rows(x, dim)
+    h = x.new_empty(x.shape)
+    r = None if y is None else x.new_empty(x.shape)
+    _quiver._block_norm(x.numel() // dim, dim, _dtypes[x.dtype], act, eps, xr.data_ptr(), xs, *args, _pointer(r), h.data_ptr(),
+                        _stream(x.device))
+    return h if y is None else (r, h)
+
+
+def block_norm_grad(grad_h, r, weight, grad_r=None, y=None, post_weight=None, gate=None, gate_activation: Optional[str] = None,
+                    scale=None, eps: float = 1e-6) -> Tuple:
+    """Gradients of ``block_norm`` from its results': (grad_x, grad_weight, grad_y, grad_post_weight, grad_gate, grad_scale).
+
+    r is what ``block_norm`` returned (x itself where there is no y), grad_r its gradient where it was used besides h. Gradients of
+    what the block does not have are None.
+    """
+    return _block_norm_grad(grad_h, r, weight, grad_r, y, post_weight, gate, gate_activation, scale, eps, (True,) * 6)
+
+
+def _block_norm_grad(grad_h, r, weight, grad_r, y, post_weight, gate, gate_activation, scale, eps, wanted):
+    held, act, args = _block_arguments(r, weight, y, post_weight, gate, gate_activation, scale)
+    device, dtype, dim = r.device, r.dtype, r.shape[-1]
+    rr, rs = _rows(r, dim)
+    gh, ghs = _matrix("grad_h", grad_h, r.shape, device, dtype)
+    gr, grs = (None, dim) if grad_r is None else _matrix("grad_r", grad_r, r.shape, device, dtype)
+    has = (True, True, y is not None, y is not None, gate is not None, scale is not None)
+    matrix = (True, False, True, False, True, False)
+    out = [r.new_empty(r.shape if m else (dim,)) if h and w else None for h, m, w in zip(has, matrix, wanted)]
+    gx, gw, gy, gp, gg, gs = out
+    args = (r.numel() // dim, dim, _dtypes[dtype], act, eps, gh.data_ptr(), ghs, _pointer(gr), grs, rr.data_ptr(), rs, *args,
+            _pointer(gx), _pointer(gy), _pointer(gg), _pointer(gw), _pointer(gp), _pointer(gs))
+    stream = _stream(device)
+    need = _quiver._block_norm_grad(*args, 0, 0, stream)
+    if need:
+        work = _workspace(need, device)
+        _quiver._block_norm_grad(*args, work.data_ptr(), need, stream)
+    return tuple(out)
+
+
+# ---- the gradients' norm ----------------------------------------------------------------------
+
+
+def _gradients(name, tensors):
+    """The tensors as contiguous ones, and lists of their addresses, elements and types."""
+    torch = _encoder._load_torch()
+    tensors = list(tensors)
+    held, pointers, counts, types = [], [], [], []
+    device = None
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be torch tensors in GPU memory")
+        if device is None:
+            _check(name, t)
+            device = t.device
+        elif t.device != device:
+            raise ValueError(f"{name}: one is on {t.device}, the others on {device}")
+        kind = _dtypes.get(t.dtype)
+        if kind is None:
+            raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+        if t.layout is not torch.strided:
+            raise ValueError(f"{name} must be dense tensors")
+        if not t.is_contiguous():
+            t = t.contiguous()
+        held.append(t)
+        pointers.append(t.data_ptr())
+        counts.append(t.numel())
+        types.append(kind)
+    return tensors, held, pointers, counts, types, device
+
+
+def _run_clip(pointers, outs, counts, types, max_norm, eps, device):
+    norm = _encoder._torch.empty((), dtype=_encoder._torch.float32, device=device)
+    args = (pointers, outs, counts, types, max_norm, eps, norm.data_ptr())
+    stream = _stream(device)
+    need = _quiver._clip_grad_norm(*args, 0, 0, stream)
+    if need:
+        work = _workspace(need, device)
+        _quiver._clip_grad_norm(*args, work.data_ptr(), need, stream)
+    return norm
+
+
+def _own_device():
+    return _encoder._load_torch().device("cuda", _quiver._device_index())
+
+
+def grad_norm(grads: Sequence):
+    """The norm over all of a list of tensors, ``sqrt`` of the sum of their squares, as a float32 tensor of no dimensions.
+
+    The tensors may be of different types and shapes; sums are fp64. The norm of no tensors is zero.
+    """
+    _, held, pointers, counts, types, device = _gradients("grads", grads)
+    return _run_clip(pointers, [], counts, types, 0.0, 0.0, device or _own_device())
+
+
+def clip_grad_norm(grads: Sequence, max_norm: float, out: Optional[Sequence] = None, eps: float = 1e-6) -> Tuple:
+    """Gradients scaled down to a limit of their common norm: (list of ``grad * min(1, max_norm / (norm + eps))``, norm).
+
+    grads are the tensors of a model, of any of the three types each. out takes the results where it is given: tensors of
+    the same shapes and types, or ``out=grads`` to scale them in place. norm is ``grad_norm`` of the gradients as they came
+    in, and stays on the device. One that is infinite leaves zeros (NaN in place of infinities), NaN leaves NaN. The results
+    are constants to autograd.
+    """
+    grads, held, pointers, counts, types, device = _gradients("grads", grads)
+    torch = _encoder._torch
+    if out is None:
+        results = [torch.empty_like(t, requires_grad=False, memory_format=torch.contiguous_format) for t in held]
+        outs = [t.data_ptr() for t in results]
+        return results, _run_clip(pointers, outs, counts, types, max_norm, eps, device or _own_device())
+    results, filled, outs, out_counts, out_types, _ = _gradients("out", out)
+    if len(results) != len(grads) or out_types != types or any(a.shape != b.shape for a, b in zip(results, grads)):
+        raise ValueError("out must hold a tensor of each gradient's shape and type")
+    if results and results[0].device != device:
+        raise ValueError(f"out is on {results[0].device}, the gradients on {device}")
+    # A result that is not contiguous is made aside; its gradient, where it is the same tensor, was copied already.
+    norm = _run_clip(pointers, outs, counts, types, max_norm, eps, device or _own_device())
+    with torch.no_grad():
+        for t, f in zip(results, filled):
+            if t is not f:
+                t.copy_(f)
+    written = [t for t, f in zip(results, filled) if t is f]
+    if written:
+        torch.autograd.graph.increment_version(written)
+    return results, norm

@@ -664,12 +664,6 @@ void check_grad(const char* who, const qvh_linear_grad_args* a) {
   QVH_REQUIRE(reinterpret_cast<uintptr_t>(a->grad_bias) % e == 0, w + ": grad_bias is not aligned to its element type");
 }
 
-void check_workspace(const char* who, const void* ws, uint64_t have, size_t need) {
-  const std::string w(who);
-  QVH_REQUIRE(need == 0 || (ws != nullptr && have >= need), w + ": the workspace is too small");
-  QVH_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 16 == 0, w + ": the workspace must be 16-byte aligned");
-}
-
 }  // namespace
 }  // namespace qvh
 

@@ -17,6 +17,12 @@ inline void require_dtype(const char* who, int dtype) {
               std::string(who) + ": dtype must be QVH_FP32, QVH_FP16 or QVH_BF16");
 }
 
+inline void check_workspace(const char* who, const void* ws, uint64_t have, size_t need) {
+  const std::string w(who);
+  QVH_REQUIRE(need == 0 || (ws != nullptr && have >= need), w + ": the workspace is too small");
+  QVH_REQUIRE(reinterpret_cast<uintptr_t>(ws) % 16 == 0, w + ": the workspace must be 16-byte aligned");
+}
+
 /// Calls f with a null pointer of the element type that `dtype` names.
 template <class F>
 void with_dtype(int dtype, F&& f) {

@@ -218,6 +218,52 @@ PYBIND11_MODULE(_quiver, m) {
     check(qvh_linear_grad_device(&a, ptr(work), work_bytes, ptr(stream)));
     return 0;
   });
+  m.def("_block_norm", [check, ptr](std::uint64_t rows, std::uint32_t dim, int dtype, int act, float eps, std::uintptr_t x,
+                                    std::uint64_t xs, std::uintptr_t y, std::uint64_t ys, std::uintptr_t gate,
+                                    std::uint64_t gs, std::uintptr_t weight, std::uintptr_t post, std::uintptr_t scale,
+                                    std::uintptr_t r, std::uintptr_t h, std::uintptr_t stream) {
+    const qvh_block_norm_args a{rows, dim, dtype, act, eps, ptr(x), xs, ptr(y), ys, ptr(gate), gs, ptr(weight), ptr(post), ptr(scale), ptr(r), ptr(h)};
+    check(qvh_block_norm_device(&a, ptr(stream)));
+  });
+  m.def("_block_norm_grad",
+        [check, ptr](std::uint64_t rows, std::uint32_t dim, int dtype, int act, float eps, std::uintptr_t gh, std::uint64_t ghs,
+                     std::uintptr_t gr, std::uint64_t grs, std::uintptr_t r, std::uint64_t rs, std::uintptr_t y,
+                     std::uint64_t ys, std::uintptr_t gate, std::uint64_t gs, std::uintptr_t weight, std::uintptr_t post,
+                     std::uintptr_t scale, std::uintptr_t gx, std::uintptr_t gy, std::uintptr_t gg, std::uintptr_t gw,
+                     std::uintptr_t gp, std::uintptr_t gsc, std::uintptr_t work, std::uint64_t work_bytes,
+                     std::uintptr_t stream) -> std::uint64_t {
+          const qvh_block_norm_grad_args a{rows, dim, dtype, act, eps, ptr(gh), ghs, ptr(gr), grs, ptr(r), rs, ptr(y), ys, ptr(gate), gs,
+                                           ptr(weight), ptr(post), ptr(scale), ptr(gx), ptr(gy), ptr(gg), ptr(gw), ptr(gp), ptr(gsc)};
+          if (work_bytes == 0) {
+            std::uint64_t need = 0;
+            check(qvh_block_norm_grad_workspace(&a, &need));
+            if (need > 0) return need;
+          }
+          check(qvh_block_norm_grad_device(&a, ptr(work), work_bytes, ptr(stream)));
+          return 0;
+        });
+  // Lists of addresses, results' addresses (empty: the norm alone), elements and types.
+  m.def("_clip_grad_norm",
+        [check, ptr](const std::vector<std::uintptr_t>& grads, const std::vector<std::uintptr_t>& outs,
+                     const std::vector<std::uint64_t>& counts, const std::vector<int>& dtypes, float max_norm, float eps,
+                     std::uintptr_t norm, std::uintptr_t work, std::uint64_t work_bytes, std::uintptr_t stream) -> std::uint64_t {
+          std::vector<qvh_gradient> list(grads.size());
+          for (std::size_t i = 0; i < grads.size(); ++i) {
+            list[i] = {ptr(grads[i]), outs.empty() ? nullptr : ptr(outs.at(i)), counts.at(i), dtypes.at(i)};
+          }
+          if (work_bytes == 0) {
+            std::uint64_t need = 0;
+            check(qvh_grad_norm_workspace(list.data(), list.size(), &need));
+            if (need > 0) return need;
+          }
+          float* d_norm = static_cast<float*>(ptr(norm));
+          if (outs.empty() && !grads.empty()) {
+            check(qvh_grad_norm_device(list.data(), list.size(), d_norm, ptr(work), work_bytes, ptr(stream)));
+          } else {
+            check(qvh_clip_grad_norm_device(list.data(), list.size(), max_norm, eps, d_norm, ptr(work), work_bytes, ptr(stream)));
+          }
+          return 0;
+        });
   m.def("_orthogonalize_workspace", [check](std::uint64_t batch, std::uint32_t m, std::uint32_t n) {
     std::uint64_t bytes = 0;
     check(qvh_orthogonalize_workspace(batch, m, n, &bytes));
