@@ -509,6 +509,56 @@ qvh_status qvh_grad_norm_device(const qvh_gradient* grads, uint64_t count, float
 qvh_status qvh_clip_grad_norm_device(const qvh_gradient* grads, uint64_t count, float max_norm, float eps,
                                      float* d_norm /* nullable */, void* d_workspace, uint64_t workspace_bytes, void* stream);
 
+/* Linear attention with a decay for each head, d = exp(log_decay[head]):
+ *   S_t = d S_{t-1} + k_t v_t^T,   out_t = scale S_t^T q_t     for the tokens t = 0 .. of a text, in order,
+ * from S_{-1} = state (fp32 [batch][heads][dk][dv], nullable: zeros) to state_out (nullable; may be the same buffer). q is
+ * [batch][tokens][heads][dk], k [..][kv_heads][dk], v [..][kv_heads][dv], each with element strides of text, token and head,
+ * out [batch][tokens][heads][dv], contiguous; heads / kv_heads neighbouring heads share keys and values, each with its own
+ * state. log_decay is fp32 [heads], at most 0 (-infinity: no memory); larger ones are taken as they are, and powers of them may
+ * overflow. lengths (nullable), index_bytes 4 or 8 each, [batch], are the texts' tokens, clamped to [0, tokens]:
+ * those behind them change no state and give zeros, whatever they hold. A token that is not finite changes results of its own
+ * and later tokens only. dk and dv are at most 256, batch * heads below 2^16, tokens below 2^31, strides below 2^40.
+ * Scores and the state enter 16-bit products rounded to their type once, each by up to 2^-9 of a bf16 term, 2^-12 of an fp16
+ * one; states themselves are fp32 throughout. */
+typedef struct qvh_attention_args {
+  uint64_t batch, tokens;
+  uint32_t heads, kv_heads, dk, dv;
+  int dtype;
+  float scale;
+  const void* q;
+  uint64_t q_stride[3];
+  const void* k;
+  uint64_t k_stride[3];
+  const void* v;
+  uint64_t v_stride[3];
+  const float* log_decay;
+  const void* lengths;
+  int index_bytes;
+  const float* state;
+  float* state_out;
+  void* out;
+} qvh_attention_args;
+qvh_status qvh_attention_workspace(const qvh_attention_args* args, uint64_t* bytes);
+qvh_status qvh_attention_device(const qvh_attention_args* args, void* d_workspace, uint64_t workspace_bytes, void* stream);
+
+/* Its gradients from out's (grad, with strides as q's) and the last state's (grad_state, nullable): grad_q, grad_k, grad_v,
+ * contiguous in the order of q, k and v, and grad_first, the first state's (fp32, nullable). forward holds what the forward pass
+ * was given; its out and state_out are not used. Shared heads' gradients are fp32 sums over the heads. log_decay is a
+ * constant. No result overlaps another buffer of the call. */
+typedef struct qvh_attention_grad_args {
+  qvh_attention_args forward;
+  const void* grad;
+  uint64_t grad_stride[3];
+  const float* grad_state;
+  void* grad_q;
+  void* grad_k;
+  void* grad_v;
+  float* grad_first;
+} qvh_attention_grad_args;
+qvh_status qvh_attention_grad_workspace(const qvh_attention_grad_args* args, uint64_t* bytes);
+qvh_status qvh_attention_grad_device(const qvh_attention_grad_args* args, void* d_workspace, uint64_t workspace_bytes,
+                                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -45,11 +45,12 @@ def _load_extension():
 _quiver = _load_extension()
 simd_isa = _quiver.simd_isa
 
-from .blocks import block_norm, block_norm_grad, clip_grad_norm, grad_norm  # noqa: E402
+from .blocks import (block_norm, block_norm_grad, clip_grad_norm, grad_norm, linear_attention,  # noqa: E402
+                     linear_attention_grad)
 from .encoder import embed, embed_grad, linear, linear_grad, orthogonalize  # noqa: E402
 
 __all__ = ["FlatIndex", "IvfPqIndex", "block_norm", "block_norm_grad", "clip_grad_norm", "embed", "embed_grad", "grad_norm",
-           "kmeans", "linear", "linear_grad", "orthogonalize", "simd_isa"]
+           "kmeans", "linear", "linear_attention", "linear_attention_grad", "linear_grad", "orthogonalize", "simd_isa"]
 __version__ = "0.1.0"
 
 ArrayLike = Union[np.ndarray, Iterable]

@@ -101,6 +101,29 @@ class BlockNorm(torch.autograd.Function):
         return gx, gw, gy, gp, gg, None, gs, None
 
 
+class LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, lengths, scale, keep_state):
+        result = blocks._linear_attention(q, k, v, log_decay, state, lengths, scale, keep_state)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
+        return result
+
+    @staticmethod
+    def backward(ctx, grad, grad_state=None):
+        if grad is None and grad_state is None:
+            return (None,) * 8
+        q, k, v, log_decay, state, lengths = ctx.saved_tensors
+
+        def gradient():
+            g = grad if grad is not None else q.new_zeros((*q.shape[:3], v.shape[3]))
+            return blocks.linear_attention_grad(g, q, k, v, log_decay, state, lengths, ctx.scale, grad_state)
+
+        gq, gk, gv, first = _once("linear_attention", gradient, grad, grad_state, q, k, v, state)
+        return gq, gk, gv, None, first, None, None, None
+
+
 class Orthogonalize(torch.autograd.Function):
     @staticmethod
     def forward(ctx, update, steps, coefficients):

@@ -1,6 +1,7 @@
 """Blocks of an encoder, and their training step, on torch (ROCm) tensors in GPU memory.
 
     >>> x, h = quiver.block_norm(x, w_in, y=y, post_weight=w_out, gate=g, gate_activation="silu", scale=s)
+    >>> o, state = quiver.linear_attention(q, k, v, log_decay, lengths=lengths, keep_state=True)
     >>> norm = quiver.clip_grad_norm(grads, 1.0, out=grads)[1]           # in front of the optimiser's step
 
 They follow the rules of quiver_amd/encoder.py, whose layers go between them: types, streams, errors, strided rows,
@@ -125,6 +126,139 @@ def _block_norm_grad(grad_h, r, weight, grad_r, y, post_weight, gate, gate_activ
         work = _workspace(need, device)
         _quiver._block_norm_grad(*args, work.data_ptr(), need, stream)
     return tuple(out)
+
+
+# ---- linear attention -------------------------------------------------------------------------
+
+
+def linear_attention(q, k, v, log_decay, state=None, lengths=None, scale: Optional[float] = None, keep_state: bool = False,
+                     state_out=None):
+    """Attention without a softmax: ``S_t = exp(log_decay) S_{t-1} + k_t v_t^T`` and ``out_t = scale * S_t^T q_t``, token by token.
+
+    q is [batch, tokens, heads, dk], k [batch, tokens, kv_heads, dk], v [batch, tokens, kv_heads, dv], out [batch, tokens, heads, dv];
+    kv_heads divides heads, and neighbouring heads share theirs. Views are read as they are where their last dimension is contiguous.
+    log_decay, float32 [heads] and at most 0, is a constant to autograd. scale is ``dk ** -0.5`` where it is left out.
+    lengths (int32 or int64 [batch], clamped to [0, tokens]): the tokens of each text in front of its padding, which changes no
+    state and gives zeros. dk and dv are at most 256.
+
+    A text can go on where it ended: state, float32 [batch, heads, dk, dv], is what it starts from (zeros where it is
+    left out), and with keep_state the last one comes back too: (out, state). state_out takes it where it is given, and may be
+    ``state`` itself, for texts that grow by a token at a time.
+    """
+    if _differentiated(q, k, v, state):
+        if state_out is not None:
+            raise ValueError("state_out is not for calls that autograd records")
+        return _node("LinearAttention", q, k, v, log_decay, state, lengths, scale, keep_state)
+    return _linear_attention(q, k, v, log_decay, state, lengths, scale, keep_state, state_out)
+
+
+def _heads(name, t, device, dtype):
+    """A [batch, tokens, heads, dim] tensor with contiguous rows of dim, and its strides."""
+    _check(name, t, device, dtype)
+    if t.dim() != 4:
+        raise ValueError(f"{name} must be [batch, tokens, heads, dim], got shape {tuple(t.shape)}")
+    s = t.stride()
+    if s[3] != 1 and t.shape[3] > 1:
+        t = t.contiguous()
+        s = t.stride()
+    return t, s[:3]
+
+
+def _state(name, t, shape, device):
+    if not isinstance(t, _encoder._tensor):
+        raise TypeError(f"{name} must be a torch tensor in GPU memory")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+    if t.dtype is not _encoder._torch.float32:
+        raise ValueError(f"{name} must be float32, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _attention_arguments(q, k, v, log_decay, state, lengths, scale):
+    """(tensors to hold, sizes, scale, strides, arguments from log_decay on, shape of a state)."""
+    _check("q", q)
+    device, dtype = q.device, q.dtype
+    q, qs = _heads("q", q, device, dtype)
+    k, ks = _heads("k", k, device, dtype)
+    v, vs = _heads("v", v, device, dtype)
+    batch, tokens, heads, dk = q.shape
+    kv_heads, dv = v.shape[2:]
+    if k.shape != (batch, tokens, kv_heads, dk) or v.shape[:2] != q.shape[:2] or kv_heads < 1 or heads % kv_heads:
+        raise ValueError("q must be [batch, tokens, heads, dk], k [batch, tokens, kv_heads, dk] and v [batch, tokens, kv_heads, dv] with "
+                         f"heads a multiple of kv_heads, got shapes {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    log_decay = _state("log_decay", log_decay, (heads,), device)
+    if state is not None:
+        state = _state("state", state, (batch, heads, dk, dv), device)
+    size = 0
+    if lengths is not None:
+        torch = _encoder._torch
+        if not isinstance(lengths, torch.Tensor):
+            raise TypeError("lengths must be a torch tensor in GPU memory")
+        if lengths.device != device:
+            raise ValueError(f"lengths are on {lengths.device}, the other tensors on {device}")
+        if lengths.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"lengths must be int32 or int64, got {lengths.dtype}")
+        if lengths.shape != (batch,):
+            raise ValueError(f"lengths must have shape ({batch},), got {tuple(lengths.shape)}")
+        lengths = lengths if lengths.is_contiguous() else lengths.contiguous()
+        size = lengths.element_size()
+    sizes = (batch, tokens, heads, kv_heads, dk, dv, _dtypes[dtype])
+    if scale is None:
+        scale = dk ** -0.5 if dk else 1.0
+    return ((q, k, v, log_decay, state, lengths), sizes, scale, (*qs, *ks, *vs),
+            (log_decay.data_ptr(), _pointer(lengths), size, _pointer(state)), (batch, heads, dk, dv))
+
+
+def _linear_attention(q, k, v, log_decay, state, lengths, scale, keep_state, state_out=None):
+    (q, k, v, *held), sizes, scale, strides, args, shape = _attention_arguments(q, k, v, log_decay, state, lengths, scale)
+    torch = _encoder._torch
+    device = q.device
+    out = q.new_empty((*q.shape[:3], sizes[5]))
+    last = filled = None
+    if state_out is not None:
+        last, filled = state_out, _state("state_out", state_out, shape, device)
+    elif keep_state:
+        last = filled = torch.empty(shape, dtype=torch.float32, device=device)
+    args = (sizes, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, *args, _pointer(filled), out.data_ptr())
+    stream = _stream(device)
+    need = _quiver._attention(*args, 0, 0, stream)
+    if need:
+        work = _workspace(need, device)
+        _quiver._attention(*args, work.data_ptr(), need, stream)
+    if state_out is not None:
+        if filled is not last:
+            last.copy_(filled)
+        else:
+            torch.autograd.graph.increment_version(last)
+    return out if last is None else (out, last)
+
+
+def linear_attention_grad(grad, q, k, v, log_decay, state=None, lengths=None, scale: Optional[float] = None, grad_state=None) -> Tuple:
+    """Gradients of ``linear_attention`` from its result's: (grad_q, grad_k, grad_v, grad_first).
+
+    grad_state is the last state's gradient where that was used. grad_first is the gradient of ``state``, None where the texts
+    started from zeros. Padding has gradients of zero.
+    """
+    (q, k, v, *held), sizes, scale, strides, args, shape = _attention_arguments(q, k, v, log_decay, state, lengths, scale)
+    device = q.device
+    grad, gs = _heads("grad", grad, device, q.dtype)
+    if grad.shape != (*q.shape[:3], sizes[5]):
+        raise ValueError(f"grad must have shape {(*q.shape[:3], sizes[5])}, got {tuple(grad.shape)}")
+    if grad_state is not None:
+        grad_state = _state("grad_state", grad_state, shape, device)
+    contiguous = _encoder._torch.contiguous_format
+    gq, gk, gv = (_encoder._torch.empty_like(t, memory_format=contiguous) for t in (q, k, v))
+    first = None if state is None else _encoder._torch.empty(shape, dtype=_encoder._torch.float32, device=device)
+    args = (sizes, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), (*strides, *gs), *args, grad.data_ptr(), _pointer(grad_state),
+            gq.data_ptr(), gk.data_ptr(), gv.data_ptr(), _pointer(first))
+    stream = _stream(device)
+    need = _quiver._attention_grad(*args, 0, 0, stream)
+    if need:
+        work = _workspace(need, device)
+        _quiver._attention_grad(*args, work.data_ptr(), need, stream)
+    return gq, gk, gv, first
 
 
 # ---- the gradients' norm ----------------------------------------------------------------------

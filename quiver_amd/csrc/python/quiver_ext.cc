@@ -8,6 +8,7 @@
 #include <link.h>
 
 #include <algorithm>
+#include <array>
 #include <cstring>
 #include <string>
 #include <utility>
@@ -240,6 +241,72 @@ PYBIND11_MODULE(_quiver, m) {
             if (need > 0) return need;
           }
           check(qvh_block_norm_grad_device(&a, ptr(work), work_bytes, ptr(stream)));
+          return 0;
+        });
+  // sizes: batch, tokens, heads, kv_heads, dk, dv, dtype; strides: three each of q, k and v (and of the result's gradient).
+  const auto attention_args = [ptr](const std::array<std::uint64_t, 7>& n, float scale, std::uintptr_t q, std::uintptr_t k,
+                                    std::uintptr_t v, const std::uint64_t* st, std::uintptr_t log_decay, std::uintptr_t lengths,
+                                    int index_bytes, std::uintptr_t state) {
+    qvh_attention_args a{};
+    a.batch = n[0];
+    a.tokens = n[1];
+    a.heads = static_cast<std::uint32_t>(n[2]);
+    a.kv_heads = static_cast<std::uint32_t>(n[3]);
+    a.dk = static_cast<std::uint32_t>(n[4]);
+    a.dv = static_cast<std::uint32_t>(n[5]);
+    a.dtype = static_cast<int>(n[6]);
+    a.scale = scale;
+    a.q = ptr(q);
+    a.k = ptr(k);
+    a.v = ptr(v);
+    std::copy(st, st + 3, a.q_stride);
+    std::copy(st + 3, st + 6, a.k_stride);
+    std::copy(st + 6, st + 9, a.v_stride);
+    a.log_decay = static_cast<const float*>(ptr(log_decay));
+    a.lengths = ptr(lengths);
+    a.index_bytes = index_bytes;
+    a.state = static_cast<const float*>(ptr(state));
+    return a;
+  };
+  m.def("_attention",
+        [check, ptr, attention_args](const std::array<std::uint64_t, 7>& sizes, float scale, std::uintptr_t q, std::uintptr_t k,
+                                     std::uintptr_t v, const std::array<std::uint64_t, 9>& strides, std::uintptr_t log_decay,
+                                     std::uintptr_t lengths, int index_bytes, std::uintptr_t state, std::uintptr_t state_out,
+                                     std::uintptr_t out, std::uintptr_t work, std::uint64_t work_bytes,
+                                     std::uintptr_t stream) -> std::uint64_t {
+          qvh_attention_args a = attention_args(sizes, scale, q, k, v, strides.data(), log_decay, lengths, index_bytes, state);
+          a.state_out = static_cast<float*>(ptr(state_out));
+          a.out = ptr(out);
+          if (work_bytes == 0) {
+            std::uint64_t need = 0;
+            check(qvh_attention_workspace(&a, &need));
+            if (need > 0) return need;
+          }
+          check(qvh_attention_device(&a, ptr(work), work_bytes, ptr(stream)));
+          return 0;
+        });
+  m.def("_attention_grad",
+        [check, ptr, attention_args](const std::array<std::uint64_t, 7>& sizes, float scale, std::uintptr_t q, std::uintptr_t k,
+                                     std::uintptr_t v, const std::array<std::uint64_t, 12>& strides, std::uintptr_t log_decay,
+                                     std::uintptr_t lengths, int index_bytes, std::uintptr_t state, std::uintptr_t grad,
+                                     std::uintptr_t grad_state, std::uintptr_t gq, std::uintptr_t gk, std::uintptr_t gv,
+                                     std::uintptr_t first, std::uintptr_t work, std::uint64_t work_bytes,
+                                     std::uintptr_t stream) -> std::uint64_t {
+          qvh_attention_grad_args a{};
+          a.forward = attention_args(sizes, scale, q, k, v, strides.data(), log_decay, lengths, index_bytes, state);
+          a.grad = ptr(grad);
+          std::copy(strides.begin() + 9, strides.end(), a.grad_stride);
+          a.grad_state = static_cast<const float*>(ptr(grad_state));
+          a.grad_q = ptr(gq);
+          a.grad_k = ptr(gk);
+          a.grad_v = ptr(gv);
+          a.grad_first = static_cast<float*>(ptr(first));
+          if (work_bytes == 0) {
+            std::uint64_t need = 0;
+            check(qvh_attention_grad_workspace(&a, &need));
+            if (need > 0) return need;
+          }
+          check(qvh_attention_grad_device(&a, ptr(work), work_bytes, ptr(stream)));
           return 0;
         });
   // Lists of addresses, results' addresses (empty: the norm alone), elements and types.
