@@ -14,15 +14,15 @@
 // behind a token and not ahead of it (AttentionPass::ahead), and ends as the first state's gradient.
 //
 // Work. A work-group of four waves has one head of one text and 64 columns of v. A wave has 16 rows of the chunk for
-// the scores and the result and a quarter of X for the update. Scores are computed transposed, K Q^T, so that a
+// the scores and the result and 16 columns of X for the update. Scores are computed transposed, K Q^T, so that a
 // lane's accumulators are four neighbouring s of one row: what the next product takes as its operand, without a way through
 // LDS. K, V and X's copy for the matrix unit lie in LDS, the next chunk's K, V and Q are loaded while this one is
 // computed. Where there are few heads, a text is cut into segments: a first pass makes the state that each leaves by itself, a
 // scan over the segments the states that they start from.
 //
 // Precision. 16-bit: scores and X are rounded to the type where the matrix unit takes them (for float16 behind a
-// power of two, so that neither overflows or vanishes), once each, like the result. The update multiplies k by its decay and
-// adds up in fp32 to its last bits: the weighed k as a sum of three bfloat16 parts (24 bits), a float16 v as two.
+// power of two, so that neither overflows or vanishes), once each, like the result. The update multiplies v by its decay and
+// adds up in fp32 to its last bits: the weighed v is a sum of three bfloat16 parts (24 bits) or two float16 ones (22).
 // fp32: fp32 matrix instructions throughout.
 #include <algorithm>
 #include <cmath>
@@ -202,10 +202,8 @@ __device__ __forceinline__ V only_finite(V v) {
 
 template <class T, int KD>
 struct AttentionShape {
-  static constexpr uint32_t kStride = KD + 16 / sizeof(T);            // of K and X in LDS: rows four banks apart
+  static constexpr uint32_t kStride = KD + 16 / sizeof(T);                 // of K and X in LDS: rows four banks apart
   static constexpr uint32_t kVStride = kCols + (sizeof(T) == 2 ? 16 : 4);  // of V, read by columns
-  static constexpr int kBlocks = KD / 64;                             // of 16 dk, a wave's
-  static constexpr int kSlices = KD / 32;                             // of 32 dk
 };
 
 /// One chunk's operands on their way from memory.
@@ -215,18 +213,59 @@ struct ChunkLoads {
   X8 k[KD / 32], v[2], q[STATES ? 1 : KD / 32];
 };
 
-template <class T, int KD, bool STATES>
+/// A tensor's rows of one head of one text in chunks of 64, from the text's start or its end.
+template <class T, bool WHOLE>
+struct ChunkRows {
+  const char* base;  // the chunk's first row in memory
+  int64_t step;      // bytes from row to row
+  bool reverse;
+  __device__ __forceinline__ ChunkRows(const TokenTensor& t, uint32_t text, uint32_t head, uint32_t col, bool back, uint64_t length, uint64_t first)
+      : step(static_cast<int64_t>(t.token * sizeof(T))), reverse(back) {
+    base = static_cast<const char*>(t.base) + (text * t.batch + head / t.share * t.head + col) * sizeof(T);
+    base += (back ? static_cast<int64_t>(length) - kRows - static_cast<int64_t>(first) : static_cast<int64_t>(first)) * step;
+  }
+  __device__ __forceinline__ void advance() { base += reverse ? -step * kRows : step * kRows; }
+
+  /// Where this thread's elements c .. of row r lie; past everything where there are none.
+  __device__ __forceinline__ uint32_t offset(uint32_t r, uint32_t c, uint32_t cols) const {
+    return c < cols ? (reverse ? kRows - 1 - r : r) * static_cast<uint32_t>(step) + c * sizeof(T) : 1u << 31;
+  }
+  /// The rows that are there as a buffer: loads outside of it give zeros, so nothing has to ask for the text's end.
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(uint32_t rows, uint32_t cols) const {
+    const char* p = base + (reverse ? (kRows - rows) * step : 0);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, static_cast<int>((rows - 1) * step + cols * sizeof(T)), 0x27000);
+  }
+  __device__ __forceinline__ uint32_t shift(uint32_t rows) const { return reverse ? (kRows - rows) * static_cast<uint32_t>(step) : 0; }
+
+  static __device__ __forceinline__ typename Op<T>::x8 take(__amdgpu_buffer_rsrc_t b, uint32_t offset) {
+    const u32x4_t lo = __builtin_amdgcn_raw_buffer_load_b128(b, static_cast<int>(offset), 0, 0);
+    if constexpr (sizeof(T) == 2) {
+      return __builtin_bit_cast(typename Op<T>::x8, lo);
+    } else {
+      const u32x4_t hi = __builtin_amdgcn_raw_buffer_load_b128(b, static_cast<int>(offset) + 16, 0, 0);
+      return join(__builtin_bit_cast(f32x4_t, lo), __builtin_bit_cast(f32x4_t, hi));
+    }
+  }
+  /// Eight elements from column c of row r, by ordinary loads, where rows are not whole pieces.
+  __device__ __forceinline__ typename Op<T>::x8 take(uint32_t r, uint32_t c, uint32_t cols, uint64_t rows) const {
+    const T* at = reinterpret_cast<const T*>(base + (reverse ? kRows - 1 - r : r) * step) + c;
+    return fetch8(at, r < rows && c < cols ? cols - c : 0u);
+  }
+};
+
+/// WHOLE: rows of q, k and v are whole pieces of eight elements, 16-byte aligned, 2^31 bytes a chunk at most.
+template <class T, int KD, bool STATES, bool WHOLE>
 __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) attention_kernel(AttentionPass a) {
   using Shape = AttentionShape<T, KD>;
   using X8 = typename Op<T>::x8;
   using X4 = typename Op<T>::x4;
   constexpr bool kHalf = std::is_same<T, half_t>::value;
   constexpr uint32_t kS = Shape::kStride, kVS = Shape::kVStride;
-  constexpr int NB = Shape::kBlocks, NK = Shape::kSlices;
+  constexpr int NX = KD / 16, NK = KD / 32;
   __shared__ __attribute__((aligned(16))) T s_k[kRows * kS];
   __shared__ __attribute__((aligned(16))) T s_v[kRows * kVS];
   __shared__ __attribute__((aligned(16))) T s_x[STATES ? 16 : kCols * kS];
-  __shared__ float s_most[4];
+  __shared__ __attribute__((aligned(16))) float s_unlift[kHalf ? kCols : 4];
   __shared__ uint32_t s_odd[4];
 
   // The column slices of one head, which read the same q and k, follow one another on one XCD.
@@ -239,29 +278,24 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
   const uint32_t text = bh / a.heads, head = bh % a.heads, col0 = index % slices * kCols;
   const uint64_t first = segment * a.segment;
   const uint64_t last = segment + 1 == a.segments ? a.tokens : first + a.segment;  // tokens of the segment end here
-  const uint64_t length = length_of(a, text);
+  const uint64_t length = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(length_of(a, text))));  // below 2^31
   const uint64_t stop = length < last ? length : last;
 
   const uint32_t lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
   const uint32_t w = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6)));
-  const uint32_t dk0 = w * (KD / 4);
 
   // Token p of the pass, from the text's start or its end; those past the end stay where they are.
   const auto token = [&](uint64_t p) { return a.reverse && p < length ? length - 1 - p : p; };
-  const auto left = [](uint32_t all_of_it, uint32_t from) { return all_of_it > from ? all_of_it - from : 0u; };
-  const auto tokens_of = [&](const TokenTensor& t) {
-    return static_cast<const T*>(t.base) + text * t.batch + head / t.share * t.head + (length > 0 ? token(0) * t.token : 0);
-  };
-  const auto step_of = [&](const TokenTensor& t) { return a.reverse ? -static_cast<int64_t>(t.token) : static_cast<int64_t>(t.token); };
-  const int64_t q_step = step_of(a.q), k_step = step_of(a.k), v_step = step_of(a.v);
-  // This thread's piece of the segment's first chunk; further ones are whole rows away.
+  // This thread's pieces of a chunk.
   constexpr uint32_t kPieces = KD / 8, kKRows = 256 / kPieces;
   const uint32_t k_row = threadIdx.x / kPieces, k_col = threadIdx.x % kPieces * 8;
-  const uint32_t v_row = threadIdx.x / 8, v_col = threadIdx.x % 8 * 8;
-  const T* k = tokens_of(a.k) + static_cast<int64_t>(first + k_row) * k_step + k_col;
-  const T* v = tokens_of(a.v) + static_cast<int64_t>(first + v_row) * v_step + col0 + v_col;
-  const T* q = STATES ? nullptr : tokens_of(a.q) + static_cast<int64_t>(first + 16 * w + l) * q_step + 8 * g;
-  const uint32_t k_left = left(a.dk, k_col), v_left = left(a.dv, col0 + v_col);
+  const uint32_t v_row = threadIdx.x / 8, v_col = threadIdx.x % 8 * 8, q_row = 16 * w + l;
+  const uint32_t v_cols = a.dv - col0;
+  using Rows = ChunkRows<T, WHOLE>;
+  Rows k_at(a.k, text, head, 0, a.reverse, length, first), v_at(a.v, text, head, col0, a.reverse, length, first);
+  Rows q_at(STATES ? a.k : a.q, text, head, 0, a.reverse, length, first);
+  const uint32_t k_off = WHOLE ? k_at.offset(k_row, k_col, a.dk) : 0, v_off = WHOLE ? v_at.offset(v_row, v_col, v_cols) : 0;
+  const uint32_t q_off = WHOLE ? q_at.offset(q_row, 8 * g, a.dk) : 0;
 
   const double log2d = log2_decay(a, head);
   const float lg = static_cast<float>(log2d);
@@ -270,22 +304,25 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
   power(log2d, kRows, &whole_high, &whole_low);
 
   // Factors of the scores, row 16 w + l against s = 16 b + 4 g + i: of the block on the diagonal, and of those before it
-  // d^(16 + l - 4 g - i) d^(16 (w - b - 1)). Of k in the update, s = 16 c + 4 g + i: d^(15 - 4 g - i) d^(n - ahead - 15 - 16 c).
+  // d^(16 + l - 4 g - i) d^(16 (w - b - 1)). Of v in the update, s = 16 c + 4 g + i: d^(15 - 4 g - i) d^(n - ahead - 15 - 16 c).
   const auto uniform = [](float f) { return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(__float_as_uint(f))))); };
-  float diagonal[4], before[4], within[4], far_factor = 0.0f, block_factor[3], weight_factor[4];
+  float diagonal[4], before[4], within[4], far_factor = 0.0f, block_factor[4], weight_factor[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int apart = static_cast<int>(l) - static_cast<int>(4 * g + i);
-    diagonal[i] = a.near_scale * decay(apart > 0 ? apart : 0);
+    diagonal[i] = apart >= 0 ? a.near_scale * decay(apart) : 0.0f;
     before[i] = a.near_scale * decay(16 + apart);
     within[i] = decay(15 - static_cast<int>(4 * g + i));
     weight_factor[i] = uniform(a.kv_scale * decay(49 - static_cast<int>(a.ahead) - 16 * i));
-    if (i < 3) block_factor[i] = uniform(decay(16 * i));
+    const int away = static_cast<int>(w) - i - 1;
+    block_factor[i] = uniform(away >= 0 ? decay(16 * away) : 0.0f);
   }
   if constexpr (!STATES) far_factor = a.far_scale * decay(static_cast<int>(16 * w + l + a.ahead));
 
-  // X: dk0 + 16 n + 4 g + i, column at place 16 j + l.
-  f32x4_t x[NB][4];
+  // X: dk 16 n + 4 g + i, this wave's column at place 16 w + l. float16: times 2^x_lift, by columns.
+  f32x4_t x[NX];
+  int x_lift = 0;
+  bool settled = false;  // X holds infinities or NaN, perhaps
   {
     const float* from = nullptr;
     uint64_t sk = a.dv, sv = 1;
@@ -296,121 +333,113 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
       sk = a.state_dk;
       sv = a.state_dv;
     }
+    const uint32_t c = col0 + column_at(16 * w + l);
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
+    for (int n = 0; n < NX; ++n) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t c = col0 + column_at(16 * j + l);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t r = dk0 + 16 * n + 4 * g + i;
-          x[n][j][i] = from && r < a.dk && c < a.dv ? from[r * sk + c * sv] : 0.0f;
-        }
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t r = 16 * n + 4 * g + i;
+        x[n][i] = from && r < a.dk && c < a.dv ? from[r * sk + c * sv] : 0.0f;
+        settled = settled || !is_finite(x[n][i]);
       }
     }
+    settled = __any(settled);
   }
 
   ChunkLoads<T, KD, STATES> next;
   const auto load = [&](uint64_t rows) {
+    if constexpr (WHOLE) {
+      const uint32_t n = rows < kRows ? static_cast<uint32_t>(rows) : kRows;
+      const auto k_rows = k_at.buffer(n, a.dk), v_rows = v_at.buffer(n, v_cols);
+      const uint32_t k0 = k_off - k_at.shift(n), v0 = v_off - v_at.shift(n);
+      const uint32_t k_next = a.reverse ? -kKRows * static_cast<uint32_t>(k_at.step) : kKRows * static_cast<uint32_t>(k_at.step);
+      const uint32_t v_next = a.reverse ? -32 * static_cast<uint32_t>(v_at.step) : 32 * static_cast<uint32_t>(v_at.step);
 #pragma unroll
-    for (int u = 0; u < KD / 32; ++u) next.k[u] = fetch8(k + u * kKRows * k_step, k_row + u * kKRows < rows ? k_left : 0u);
+      for (int u = 0; u < KD / 32; ++u) next.k[u] = Rows::take(k_rows, k0 + u * k_next);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) next.v[u] = fetch8(v + u * 32 * v_step, v_row + u * 32 < rows ? v_left : 0u);
-    k += kRows * k_step;
-    v += kRows * v_step;
-    if constexpr (!STATES) {
+      for (int u = 0; u < 2; ++u) next.v[u] = Rows::take(v_rows, v0 + u * v_next);
+      if constexpr (!STATES) {
+        const auto q_rows = q_at.buffer(n, a.dk);
+        const uint32_t q0 = q_off - q_at.shift(n);
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk) next.q[kk] = fetch8(q + 32 * kk, 16 * w + l < rows ? left(a.dk, 32 * kk + 8 * g) : 0u);
-      q += kRows * q_step;
+        for (int kk = 0; kk < NK; ++kk) next.q[kk] = Rows::take(q_rows, 32 * kk + 8 * g < a.dk ? q0 + 32 * kk * sizeof(T) : 1u << 31);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < KD / 32; ++u) next.k[u] = k_at.take(k_row + u * kKRows, k_col, a.dk, rows);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) next.v[u] = v_at.take(v_row + u * 32, v_col, v_cols, rows);
+      if constexpr (!STATES) {
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) next.q[kk] = q_at.take(q_row, 32 * kk + 8 * g, a.dk, rows);
+      }
     }
+    k_at.advance();
+    v_at.advance();
+    q_at.advance();
   };
 
+  const auto left = [](uint32_t all_of_it, uint32_t from) { return all_of_it <= from ? 0u : WHOLE ? 8u : all_of_it - from; };
   const auto store_row = [&](uint64_t t, const float (&lo)[8], const float (&hi)[8]) {
     const uint32_t c = col0 + 16 * g;
     const uint64_t at = ((text * a.tokens + t) * a.heads + head) * a.dv + c;
-    if (a.out_fp32) {
-      store8(static_cast<float*>(a.out) + at, lo, left(a.dv, c));
-      store8(static_cast<float*>(a.out) + at + 8, hi, left(a.dv, c + 8));
-    } else {
-      store8(static_cast<T*>(a.out) + at, lo, left(a.dv, c));
-      store8(static_cast<T*>(a.out) + at + 8, hi, left(a.dv, c + 8));
-    }
+    const auto put = [&](auto* out) {
+      if (left(a.dv, c)) store8(out + at, lo, left(a.dv, c));
+      if (left(a.dv, c + 8)) store8(out + at + 8, hi, left(a.dv, c + 8));
+    };
+    if (a.out_fp32) return put(static_cast<float*>(a.out));
+    put(static_cast<T*>(a.out));
   };
 
-  bool settled = false;  // X holds infinities or NaN, perhaps
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) settled = settled || !is_finite(x[n][j][i]);
-    }
-  }
-  settled = __any(settled);
   if (first < stop) load(stop - first);
-  int x_lift = 0;  // float16: X's copy is 2^x_lift as large
   for (uint64_t c0 = first; c0 < stop; c0 += kRows) {
     const uint32_t rows = stop - c0 < kRows ? static_cast<uint32_t>(stop - c0) : kRows;
-    if constexpr (kHalf && !STATES) {
+    int copy_lift = 0, x_size = 0;  // float16: of X's copy beside X, and the binary order of X's column
+    if constexpr (kHalf) {
       float most = 0.0f;
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
+      for (int n = 0; n < NX; ++n) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(x[n][j][i]));
-        }
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(x[n][i]));
       }
-#pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) most = fmaxf(most, __uint_as_float(lane_xor_u32(__float_as_uint(most), off)));
-      if (!is_finite(most)) {  // by what is finite, then
+      if (settled) {  // by what is finite, then
         most = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
+        for (int n = 0; n < NX; ++n) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) most = fmaxf(most, is_finite(x[n][j][i]) ? fabsf(x[n][j][i]) : 0.0f);
-          }
+          for (int i = 0; i < 4; ++i) most = fmaxf(most, is_finite(x[n][i]) ? fabsf(x[n][i]) : 0.0f);
         }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) most = fmaxf(most, __uint_as_float(lane_xor_u32(__float_as_uint(most), off)));
       }
-      if (lane == 0) s_most[w] = most;
-    }
-    __syncthreads();  // the last chunk's reads of LDS are done
-    if constexpr (kHalf && !STATES) {
-      x_lift = lift(fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3])), 14, 100);
-    }
-#pragma unroll
-    for (int u = 0; u < KD / 32; ++u) {
-      const uint32_t at = u * 256 + threadIdx.x, r = at / (KD / 8), c = at % (KD / 8) * 8;
-      *reinterpret_cast<X8*>(s_k + r * kS + c) = next.k[u];
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint32_t at = u * 256 + threadIdx.x, r = at / 8, c = at % 8 * 8;
-      *reinterpret_cast<X4*>(s_v + r * kVS + place(c)) = __builtin_shufflevector(next.v[u], next.v[u], 0, 1, 2, 3);
-      *reinterpret_cast<X4*>(s_v + r * kVS + place(c + 4)) = __builtin_shufflevector(next.v[u], next.v[u], 4, 5, 6, 7);
+      most = fmaxf(most, __shfl_xor(most, 16, 64));
+      most = fmaxf(most, __shfl_xor(most, 32, 64));
+      copy_lift = lift(most, 14, 120);
+      x_size = most > 0.0f && is_finite(most) ? ilogbf(most) : -120;
     }
     bool finite = true;
 #pragma unroll
-    for (int u = 0; u < KD / 32; ++u) finite = finite && all_finite<T>(next.k[u]);
+    for (int u = 0; u < KD / 32; ++u) finite = all_finite<T>(next.k[u]) && finite;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) finite = finite && all_finite<T>(next.v[u]);
+    for (int u = 0; u < 2; ++u) finite = all_finite<T>(next.v[u]) && finite;
     finite = !__any(!finite);
+    __syncthreads();  // the last chunk's reads of LDS are done
     if (lane == 0) s_odd[w] = !finite;
+    if (kHalf && !STATES && g == 0) s_unlift[16 * w + l] = ldexpf(1.0f, -(x_lift + copy_lift));
+#pragma unroll
+    for (int u = 0; u < KD / 32; ++u) *reinterpret_cast<X8*>(s_k + (k_row + u * kKRows) * kS + k_col) = next.k[u];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      T* at = s_v + (v_row + u * 32) * kVS;
+      *reinterpret_cast<X4*>(at + place(v_col)) = __builtin_shufflevector(next.v[u], next.v[u], 0, 1, 2, 3);
+      *reinterpret_cast<X4*>(at + place(v_col + 4)) = __builtin_shufflevector(next.v[u], next.v[u], 4, 5, 6, 7);
+    }
     X8 qf[STATES ? 1 : NK];
     if constexpr (!STATES) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
+      for (int n = 0; n < NX; ++n) {
+        X4 copy;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          X4 copy;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) copy[i] = static_cast<T>(kHalf ? ldexpf(x[n][j][i], x_lift) : x[n][j][i]);
-          *reinterpret_cast<X4*>(s_x + (16 * j + l) * kS + dk0 + 16 * n + 4 * g) = copy;
-        }
+        for (int i = 0; i < 4; ++i) copy[i] = static_cast<T>(kHalf ? ldexpf(x[n][i], copy_lift) : x[n][i]);
+        *reinterpret_cast<X4*>(s_x + (16 * w + l) * kS + 16 * n + 4 * g) = copy;
       }
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) qf[kk] = next.q[kk];
@@ -421,38 +450,33 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
     if (c0 + kRows < stop) load(stop - c0 - kRows);
 
     if constexpr (!STATES) {
-      // Scores of this wave's rows with the s up to them, decayed.
+      // Scores of this wave's rows, decayed, zeros where s comes later. (All four blocks for 16 bits: the wave with the most
+      // of them decides, and without branches their products follow one another closely.)
       float p[4][4];
+      f32x4_t acc[4]{};
 #pragma unroll
       for (uint32_t b = 0; b < 4; ++b) {
-        f32x4_t acc{};
-        if (b <= w) {
+        if (sizeof(T) == 4 && b > w) continue;
 #pragma unroll
-          for (int kk = 0; kk < NK; ++kk) {
-            acc = Op<T>::mma(*reinterpret_cast<const X8*>(s_k + (16 * b + l) * kS + 32 * kk + 8 * g), qf[kk], acc);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (b == w) {
-            p[b][i] = 4 * g + i <= l ? acc[i] * diagonal[i] : 0.0f;
-          } else {
-            const uint32_t away = w - b - 1;
-            p[b][i] = b < w ? acc[i] * (before[i] * (away == 0 ? 1.0f : away == 1 ? block_factor[1] : block_factor[2])) : 0.0f;
-          }
-        }
+        for (int kk = 0; kk < NK; ++kk) acc[b] = Op<T>::mma(*reinterpret_cast<const X8*>(s_k + (16 * b + l) * kS + 32 * kk + 8 * g), qf[kk], acc[b]);
       }
+      __builtin_amdgcn_sched_barrier(0);
       // What the state gives.
       f32x4_t o[4]{};
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          o[j] = Op<T>::mma(*reinterpret_cast<const X8*>(s_x + (16 * j + l) * kS + 32 * kk + 8 * g), qf[kk], o[j]);
+        for (int j = 0; j < 4; ++j) o[j] = Op<T>::mma(*reinterpret_cast<const X8*>(s_x + (16 * j + l) * kS + 32 * kk + 8 * g), qf[kk], o[j]);
+      }
+#pragma unroll
+      for (uint32_t b = 0; b < 4; ++b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float factor = b == w ? diagonal[i] : before[i] * block_factor[b];
+          p[b][i] = b < w || (b == w && 4 * g + i <= l) ? acc[b][i] * factor : 0.0f;
         }
       }
       int p_lift = 0;  // float16: this row's scores and sums are 2^p_lift as large
-      float factor = far_factor;
       if constexpr (kHalf) {
         float most = 0.0f;
 #pragma unroll
@@ -463,45 +487,36 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
         most = fmaxf(most, __shfl_xor(most, 16, 64));
         most = fmaxf(most, __shfl_xor(most, 32, 64));
         p_lift = lift(most, 13, 40);
+        const float factor = ldexpf(far_factor, p_lift);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
+          const f32x4_t unlift = *reinterpret_cast<const f32x4_t*>(s_unlift + 16 * b + 4 * g);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[b][i] = ldexpf(p[b][i], p_lift);
+          for (int i = 0; i < 4; ++i) {
+            p[b][i] = ldexpf(p[b][i], p_lift);
+            o[b][i] *= unlift[i] * factor;
+          }
         }
-        factor = ldexpf(far_factor, p_lift);
-      }
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[j][i] *= kHalf ? ldexpf(factor, -x_lift) : factor;
+        for (int j = 0; j < 4; ++j) o[j] *= far_factor;
       }
-      // The block on the diagonal has scores that the mask takes away, which are zeros here; against infinities and NaN of
-      // v they would still count. There those of v are left out and added by themselves.
+      __builtin_amdgcn_sched_barrier(0);
+      // Scores that the mask takes away are zeros; against infinities and NaN of v they would still count. There those of v
+      // are left out, and the ones that the mask lets through are added by themselves.
 #pragma unroll
       for (uint32_t m = 0; m < 2; ++m) {
-        if (2 * m > w) continue;
+        if (sizeof(T) == 4 && 2 * m > w) continue;
         X8 pb;
 #pragma unroll
         for (int e = 0; e < 8; ++e) pb[e] = static_cast<T>(p[2 * m + (e >> 2)][e & 3]);
-        X4 v0[4], v1[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          v0[j] = column4(s_v, kVS, 32 * m, 16 * j);
-          v1[j] = column4(s_v, kVS, 32 * m + 16, 16 * j);
-          if (2 * m + 1 > w) v1[j] = X4{};
+          X4 v0 = column4(s_v, kVS, 32 * m, 16 * j), v1 = column4(s_v, kVS, 32 * m + 16, 16 * j);
+          if (odd && 2 * m >= w) v0 = only_finite(v0);
+          if (odd && 2 * m + 1 >= w) v1 = only_finite(v1);
+          o[j] = Op<T>::mma(join(v0, v1), pb, o[j]);
         }
-        if (odd && w >> 1 == m) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (w & 1) {
-              v1[j] = only_finite(v1[j]);
-            } else {
-              v0[j] = only_finite(v0[j]);
-            }
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = Op<T>::mma(join(v0[j], v1[j]), pb, o[j]);
       }
       if (odd) {
         float own[4];  // the scores of the block on the diagonal
@@ -522,109 +537,122 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
           }
         }
       }
-      const uint32_t r = 16 * w + l;
-      if (c0 + r < last) {
+      if (c0 + q_row < last) {
         float lo[8], hi[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float y0 = o[e >> 2][e & 3], y1 = o[2 + (e >> 2)][e & 3];
-          lo[e] = r >= rows ? 0.0f : kHalf ? ldexpf(y0, -p_lift) : y0;
-          hi[e] = r >= rows ? 0.0f : kHalf ? ldexpf(y1, -p_lift) : y1;
+          lo[e] = q_row >= rows ? 0.0f : kHalf ? ldexpf(y0, -p_lift) : y0;
+          hi[e] = q_row >= rows ? 0.0f : kHalf ? ldexpf(y1, -p_lift) : y1;
         }
-        store_row(token(c0 + r), lo, hi);
+        store_row(token(c0 + q_row), lo, hi);
       }
     }
 
-    // X, this wave's quarter.
+    __builtin_amdgcn_sched_barrier(0);
+    // X: this wave's columns. v times its decay in fp32, as three bfloat16 parts or two float16 ones, against k as it is.
+    constexpr int kParts = sizeof(T) == 4 ? 1 : kHalf ? 2 : 3;
+    X8 part[2][kParts];
+    int new_lift = x_lift;
+    {
+      float y[2][8];
+#pragma unroll
+      for (uint32_t m = 0; m < 2; ++m) {
+        const X8 vf = join(column4(s_v, kVS, 32 * m, 16 * w), column4(s_v, kVS, 32 * m + 16, 16 * w));
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+          float weight = within[e & 3] * weight_factor[2 * m + (e >> 2)];
+          if (rows < kRows) {
+            const int after = static_cast<int>(rows - a.ahead) - static_cast<int>(32 * m + 16 * (e >> 2) + 4 * g + (e & 3));
+            weight = a.kv_scale * decay(after > 0 ? after : 0);
+          }
+          y[m][e] = static_cast<float>(vf[e]) * weight;
+        }
+      }
+      if constexpr (kHalf) {
+        // Behind a power of two by columns, as large as float16 and X's own size allow.
+        float most = 0.0f;
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) most = fmaxf(most, odd && !is_finite(y[m][e]) ? 0.0f : fabsf(y[m][e]));
+        }
+        most = fmaxf(most, __shfl_xor(most, 16, 64));
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        if (most > 0.0f) {
+          const int top = 14 - ilogbf(most), room = 100 - (x_size - x_lift);
+          new_lift = top < room ? top : room;
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[m][e] = ldexpf(y[m][e], new_lift);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float rest = y[m][e];
+#pragma unroll
+          for (int z = 0; z < kParts; ++z) {
+            part[m][z][e] = static_cast<T>(rest);
+            if (z + 1 < kParts) rest -= static_cast<float>(part[m][z][e]);
+          }
+        }
+        if (odd) {  // an infinity has no lower parts
+#pragma unroll
+          for (int z = 1; z < kParts; ++z) part[m][z] = only_finite(part[m][z]);
+        }
+      }
+    }
     float high = whole_high, low = whole_low;
-    if (rows < kRows) {
-      power(log2d, rows, &high, &low);
+    if (rows < kRows) power(log2d, rows, &high, &low);
+    if constexpr (kHalf) {
+      high = ldexpf(high, new_lift - x_lift);
+      low = ldexpf(low, new_lift - x_lift);
+      x_lift = new_lift;
     }
     // The decay's second float counts over many chunks; times an infinity it would be NaN.
+    if (settled) {
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
+      for (int n = 0; n < NX; ++n) x[n] *= high;
+    } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int n = 0; n < NX; ++n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[n][j][i] = settled ? x[n][j][i] * high : fmaf(x[n][j][i], high, x[n][j][i] * low);
+        for (int i = 0; i < 4; ++i) x[n][i] = fmaf(x[n][i], high, x[n][i] * low);
       }
     }
     settled = settled || odd;
 #pragma unroll
     for (uint32_t m = 0; m < 2; ++m) {
-      float weight[8];
 #pragma unroll
-      for (uint32_t e = 0; e < 8; ++e) {
-        if (rows == kRows) {
-          weight[e] = within[e & 3] * weight_factor[2 * m + (e >> 2)];
-        } else {
-          const int after = static_cast<int>(rows - a.ahead) - static_cast<int>(32 * m + 16 * (e >> 2) + 4 * g + (e & 3));
-          weight[e] = a.kv_scale * decay(after > 0 ? after : 0);
-        }
-      }
-      X8 vb[4];
+      for (int n0 = 0; n0 < NX; n0 += 4) {
+        X8 kf[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) vb[j] = join(column4(s_v, kVS, 32 * m, 16 * j), column4(s_v, kVS, 32 * m + 16, 16 * j));
+        for (int n = 0; n < 4; ++n) kf[n] = join(column4(s_k, kS, 32 * m, 16 * (n0 + n)), column4(s_k, kS, 32 * m + 16, 16 * (n0 + n)));
+        if (odd && kParts > 1) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const X8 kf = join(column4(s_k, kS, 32 * m, dk0 + 16 * n), column4(s_k, kS, 32 * m + 16, dk0 + 16 * n));
-        if constexpr (sizeof(T) == 4) {
-          f32x8_t weighed;
+          for (int n = 0; n < 4; ++n) {
+            const X8 lower = only_finite(kf[n]);  // zeros among v's lower parts are none of v's
 #pragma unroll
-          for (int e = 0; e < 8; ++e) weighed[e] = kf[e] * weight[e];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[n][j] = Op<float>::mma(weighed, vb[j], x[n][j]);
-        } else {
-          using B8 = Op<bhalf_t>::x8;
-          B8 part[3];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float rest = static_cast<float>(kf[e]) * weight[e];
-#pragma unroll
-            for (int z = 0; z < 3; ++z) {
-              part[z][e] = static_cast<bhalf_t>(rest);
-              rest -= static_cast<float>(part[z][e]);
-            }
+            for (int z = kParts - 1; z >= 0; --z) x[n0 + n] = Op<T>::mma(z ? lower : kf[n], part[m][z], x[n0 + n]);
           }
-          if (odd) {  // an infinity has no lower parts
-            part[1] = only_finite(part[1]);
-            part[2] = only_finite(part[2]);
-          }
+        } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (kHalf) {
-              B8 vh, vl;
+          for (int z = kParts - 1; z >= 0; --z) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const float value = static_cast<float>(vb[j][e]);
-                vh[e] = static_cast<bhalf_t>(value);
-                vl[e] = static_cast<bhalf_t>(value - static_cast<float>(vh[e]));
-              }
-              const B8 lower = odd ? only_finite(vh) : vh;  // lower parts of k may be zeros where k is none
-              if (odd) vl = only_finite(vl);
-              x[n][j] = Op<bhalf_t>::mma(part[2], lower, x[n][j]);
-              x[n][j] = Op<bhalf_t>::mma(part[1], vl, x[n][j]);
-              x[n][j] = Op<bhalf_t>::mma(odd ? only_finite(part[0]) : part[0], vl, x[n][j]);
-              x[n][j] = Op<bhalf_t>::mma(part[1], lower, x[n][j]);
-              x[n][j] = Op<bhalf_t>::mma(part[0], vh, x[n][j]);
-            } else {
-              const B8 lower = odd ? only_finite(vb[j]) : vb[j];
-              x[n][j] = Op<bhalf_t>::mma(part[2], lower, x[n][j]);
-              x[n][j] = Op<bhalf_t>::mma(part[1], lower, x[n][j]);
-              x[n][j] = Op<bhalf_t>::mma(part[0], vb[j], x[n][j]);
-            }
+            for (int n = 0; n < 4; ++n) x[n0 + n] = Op<T>::mma(kf[n], part[m][z], x[n0 + n]);
           }
         }
       }
     }
     if (odd && a.dk < KD) {  // rows that X does not have stay zeros
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
+      for (int n = 0; n < NX; ++n) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[n][j][i] = dk0 + 16 * n + 4 * g + i < a.dk ? x[n][j][i] : 0.0f;
-        }
+        for (int i = 0; i < 4; ++i) x[n][i] = 16 * n + 4 * g + i < a.dk ? x[n][i] : 0.0f;
       }
     }
   }
@@ -633,7 +661,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
     // Tokens past the text's end, in chunks of their own.
     const uint64_t done = first < stop ? first + (stop - first + kRows - 1) / kRows * kRows : first;
     const float zero[8] = {};
-    for (uint64_t t = done + 16 * w + l; t < last; t += kRows) store_row(t, zero, zero);
+    for (uint64_t t = done + q_row; t < last; t += kRows) store_row(t, zero, zero);
   }
   float* to = nullptr;
   uint64_t sk = a.dv, sv = 1;
@@ -645,16 +673,14 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
     sv = a.state_dv;
   }
   if (!to) return;
+  asm volatile("" : "+s"(sk), "+s"(sv));  // the addresses anew: kept over the loop, they took more registers than there are
+  const uint32_t c = col0 + column_at(16 * w + l);
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
+  for (int n = 0; n < NX; ++n) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t c = col0 + column_at(16 * j + l);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t r = dk0 + 16 * n + 4 * g + i;
-        if (r < a.dk && c < a.dv) to[r * sk + c * sv] = x[n][j][i];
-      }
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t r = 16 * n + 4 * g + i;
+      if (r < a.dk && c < a.dv) to[r * sk + c * sv] = kHalf ? ldexpf(x[n][i], -x_lift) : x[n][i];
     }
   }
 }
@@ -805,21 +831,33 @@ uint64_t state_bytes(const AttentionPass& a) {
   return a.segments > 1 ? static_cast<uint64_t>(a.segments) * a.batch * a.heads * a.dk * a.dv * sizeof(float) : 0;
 }
 
+/// Whether rows of a tensor are whole pieces (attention_kernel's WHOLE).
+bool whole_rows(const TokenTensor& t, uint32_t dim, size_t size) {
+  const uint64_t odd = reinterpret_cast<uintptr_t>(t.base) | t.batch * size | t.token * size | t.head * size;
+  return dim % 8 == 0 && odd % 16 == 0 && (t.token + dim) * size * kRows < (uint64_t{1} << 31);
+}
+
 template <class T>
 void launch_pass(const AttentionPass& a, hipStream_t s) {
+  const bool whole = whole_rows(a.q, a.dk, sizeof(T)) && whole_rows(a.k, a.dk, sizeof(T)) && whole_rows(a.v, a.dv, sizeof(T));
+  const auto with_rows = [&](auto&& f) { whole ? f(std::true_type{}) : f(std::false_type{}); };
   const uint64_t slices = ceil_div(a.dv, kCols), all = static_cast<uint64_t>(a.batch) * a.heads;
   with_depth(a.dk, [&](auto depth) {
     constexpr int KD = decltype(depth)::value;
     const auto grid = [&](uint64_t segments) { return dim3(static_cast<unsigned>(ceil_div(all * segments, 8) * 8 * slices)); };
     if (a.segments > 1) {
-      hipLaunchKernelGGL((attention_kernel<T, KD, true>), grid(a.segments - 1), dim3(256), 0, s, a);
-      QVH_HIP(hipGetLastError());
+      with_rows([&](auto rows) {
+        hipLaunchKernelGGL((attention_kernel<T, KD, true, decltype(rows)::value>), grid(a.segments - 1), dim3(256), 0, s, a);
+        QVH_HIP(hipGetLastError());
+      });
       hipLaunchKernelGGL(attention_scan_kernel, dim3(static_cast<unsigned>(ceil_div(static_cast<uint64_t>(a.dk) * a.dv, 256)), static_cast<unsigned>(all)),
                          dim3(256), 0, s, a);
       QVH_HIP(hipGetLastError());
     }
-    hipLaunchKernelGGL((attention_kernel<T, KD, false>), grid(a.segments), dim3(256), 0, s, a);
-    QVH_HIP(hipGetLastError());
+    with_rows([&](auto rows) {
+      hipLaunchKernelGGL((attention_kernel<T, KD, false, decltype(rows)::value>), grid(a.segments), dim3(256), 0, s, a);
+      QVH_HIP(hipGetLastError());
+    });
   });
 }
 
