@@ -33,8 +33,9 @@
 namespace qvh {
 namespace {
 
-constexpr uint32_t kRows = 64;   // of a chunk
-constexpr uint32_t kCols = 64;   // of v, a work-group's
+constexpr int kWaves = 4;                // of a work-group
+constexpr uint32_t kRows = 16 * kWaves;  // tokens of a chunk
+constexpr uint32_t kCols = 16 * kWaves;  // of v, a work-group's
 constexpr uint32_t kMaxHead = 256;
 
 /// Tokens of one tensor: element strides of text, token and head; `share` heads of the call to one of its own.
@@ -50,6 +51,8 @@ struct AttentionPass {
   TokenTensor q, k, v;
   void* out = nullptr;  // [batch][token][head][dv]
   bool out_fp32 = false;
+  bool exact = false;  // the state is a result
+  bool wide = false;   // fp32
   const float* log_decay = nullptr;
   const void* lengths = nullptr;
   int index_bytes = 0;
@@ -64,6 +67,17 @@ struct AttentionPass {
   uint64_t segment = 0;  // tokens
   float* states = nullptr;
 };
+
+/// The passes of one launch: the gradients' three, which have nothing to wait for in one another.
+struct AttentionPasses {
+  AttentionPass pass[3];
+};
+
+/// One of the launch's passes, where its arguments lie: a copy with a varying index would go to memory of its own.
+__device__ __forceinline__ const AttentionPass& pass_of(uint32_t i) {
+  typedef const __attribute__((address_space(4))) AttentionPass* Constant;
+  return *(const AttentionPass*)((Constant)__builtin_amdgcn_kernarg_segment_ptr() + i);
+}
 
 typedef float f32x8_t __attribute__((ext_vector_type(8)));
 
@@ -135,10 +149,10 @@ __device__ __forceinline__ auto join(V4 a, V4 b) {
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-/// Where column c of the work-group's 64 lies in LDS: the four columns 16 g + 4 j + i, i = 0 .. 3, at 16 j + 4 g + i, so that
-/// a lane's accumulators of blocks j = 0 .. 3 are 16 neighbours of a result's row.
-__device__ __forceinline__ uint32_t place(uint32_t c) { return 16 * (c >> 2 & 3) + 4 * (c >> 4) + (c & 3); }
-__device__ __forceinline__ uint32_t column_at(uint32_t p) { return 16 * (p >> 2 & 3) + 4 * (p >> 4) + (p & 3); }
+/// Where a column of v lies in LDS: columns 32 u + 8 g + 4 t + i, i = 0 .. 3, at 16 (2 u + t) + 4 g + i, so that a lane's accumulators
+/// of blocks 2 u and 2 u + 1 are eight neighbours of a result's row, and four lanes' are 32.
+__device__ __forceinline__ uint32_t place(uint32_t c) { return 32 * (c >> 5) + 16 * (c >> 2 & 1) + 4 * (c >> 3 & 3) + (c & 3); }
+__device__ __forceinline__ uint32_t column_at(uint32_t p) { return 32 * (p >> 5) + 8 * (p >> 2 & 3) + 4 * (p >> 4 & 1) + (p & 3); }
 
 __device__ __forceinline__ uint64_t length_of(const AttentionPass& a, uint32_t text) {
   if (!a.lengths) return a.tokens;
@@ -171,23 +185,24 @@ __device__ __forceinline__ bool is_finite(float v) { return fabsf(v) < __builtin
 /// Whether all eight are finite.
 template <class T>
 __device__ __forceinline__ bool all_finite(typename Op<T>::x8 v) {
+  // Zero times each: NaN for infinities and NaN.
+  float sum = 0.0f;
   if constexpr (sizeof(T) == 2) {
-    constexpr uint32_t kExponent = std::is_same<T, half_t>::value ? 0x7C007C00u : 0x7F807F80u;
-    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-    const u32x4_t bits = __builtin_bit_cast(u32x4_t, v) & kExponent;
-    u16x2 most{};
+    typedef T x2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t two = bits[i];  // a value: a bit cast of the element itself takes the first one's bits
-      most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, two));
+      const x2 two = {v[2 * i], v[2 * i + 1]};
+      if constexpr (std::is_same<T, half_t>::value) {
+        sum = __builtin_amdgcn_fdot2(two, x2{}, sum, false);
+      } else {
+        sum = __builtin_amdgcn_fdot2_f32_bf16(two, x2{}, sum, false);
+      }
     }
-    return most[0] < (kExponent & 0xFFFF) && most[1] < (kExponent & 0xFFFF);
   } else {
-    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum = fmaf(v[i], 0.0f, sum);
-    return sum == 0.0f;
   }
+  return sum == 0.0f;
 }
 
 /// Zeros for what is not finite.
@@ -200,80 +215,86 @@ __device__ __forceinline__ V only_finite(V v) {
   return v;
 }
 
-template <class T, int KD>
-struct AttentionShape {
-  static constexpr uint32_t kStride = KD + 16 / sizeof(T);                 // of K and X in LDS: rows four banks apart
-  static constexpr uint32_t kVStride = kCols + (sizeof(T) == 2 ? 16 : 4);  // of V, read by columns
-};
-
 /// One chunk's operands on their way from memory.
 template <class T, int KD, bool STATES>
 struct ChunkLoads {
   using X8 = typename Op<T>::x8;
-  X8 k[KD / 32], v[2], q[STATES ? 1 : KD / 32];
+  X8 k[KD / 32], v[kWaves / 2], q[STATES ? 1 : KD / 32];
 };
 
-/// A tensor's rows of one head of one text in chunks of 64, from the text's start or its end.
+/// A tensor's rows of one head of one text, `rows` of them from token `first` of the pass on, in chunks of 64. WHOLE: a buffer that
+/// holds them and no more; offsets of 32 bits run through it, forwards or back, and loads outside give zeros, so nothing has to
+/// ask for the text's end. Otherwise ordinary loads, element by element where a row ends inside a piece.
 template <class T, bool WHOLE>
 struct ChunkRows {
-  const char* base;  // the chunk's first row in memory
-  int64_t step;      // bytes from row to row
-  bool reverse;
-  __device__ __forceinline__ ChunkRows(const TokenTensor& t, uint32_t text, uint32_t head, uint32_t col, bool back, uint64_t length, uint64_t first)
-      : step(static_cast<int64_t>(t.token * sizeof(T))), reverse(back) {
+  using X8 = typename Op<T>::x8;
+  const char* base;  // the first row of the pass; or of the chunk
+  int64_t step;      // bytes from row to row of the pass
+  uint64_t left;     // rows from the chunk on
+  __amdgpu_buffer_rsrc_t buffer;
+  uint32_t cols;
+
+  __device__ __forceinline__ ChunkRows(const TokenTensor& t, uint32_t text, uint32_t head, uint32_t col, uint32_t dim, bool back, uint64_t length,
+                                       uint64_t first, uint64_t rows)
+      : step(static_cast<int64_t>(t.token * sizeof(T))), left(rows), cols(dim - col) {
     base = static_cast<const char*>(t.base) + (text * t.batch + head / t.share * t.head + col) * sizeof(T);
-    base += (back ? static_cast<int64_t>(length) - kRows - static_cast<int64_t>(first) : static_cast<int64_t>(first)) * step;
+    base += (back ? static_cast<int64_t>(length) - 1 - static_cast<int64_t>(first) : static_cast<int64_t>(first)) * step;
+    if (back) step = -step;
+    if constexpr (WHOLE) {
+      const char* low = back && rows > 0 ? base + static_cast<int64_t>(rows - 1) * step : base;
+      const int64_t bytes = rows > 0 ? static_cast<int64_t>(rows - 1) * (back ? -step : step) + static_cast<int64_t>(cols * sizeof(T)) : 0;
+      buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(low), 0, static_cast<int>(bytes), 0x27000);
+    }
   }
-  __device__ __forceinline__ void advance() { base += reverse ? -step * kRows : step * kRows; }
-
-  /// Where this thread's elements c .. of row r lie; past everything where there are none.
-  __device__ __forceinline__ uint32_t offset(uint32_t r, uint32_t c, uint32_t cols) const {
-    return c < cols ? (reverse ? kRows - 1 - r : r) * static_cast<uint32_t>(step) + c * sizeof(T) : 1u << 31;
+  /// Where column c of row r of the first chunk is; what lies in no row stays outside through all chunks (2^31 bytes at most).
+  __device__ __forceinline__ uint32_t offset(uint32_t r, uint32_t c) const {
+    const uint32_t s = static_cast<uint32_t>(step);
+    if (c >= cols) return step < 0 ? 0xFFFFFF00u : 1u << 31;
+    return (step < 0 ? -(static_cast<uint32_t>(left) - 1) * s : 0) + r * s + c * sizeof(T);
   }
-  /// The rows that are there as a buffer: loads outside of it give zeros, so nothing has to ask for the text's end.
-  __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(uint32_t rows, uint32_t cols) const {
-    const char* p = base + (reverse ? (kRows - rows) * step : 0);
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, static_cast<int>((rows - 1) * step + cols * sizeof(T)), 0x27000);
-  }
-  __device__ __forceinline__ uint32_t shift(uint32_t rows) const { return reverse ? (kRows - rows) * static_cast<uint32_t>(step) : 0; }
-
-  static __device__ __forceinline__ typename Op<T>::x8 take(__amdgpu_buffer_rsrc_t b, uint32_t offset) {
-    const u32x4_t lo = __builtin_amdgcn_raw_buffer_load_b128(b, static_cast<int>(offset), 0, 0);
+  __device__ __forceinline__ X8 take(uint32_t offset) const {
+    const u32x4_t lo = __builtin_amdgcn_raw_buffer_load_b128(buffer, static_cast<int>(offset), 0, 0);
     if constexpr (sizeof(T) == 2) {
-      return __builtin_bit_cast(typename Op<T>::x8, lo);
+      return __builtin_bit_cast(X8, lo);
     } else {
-      const u32x4_t hi = __builtin_amdgcn_raw_buffer_load_b128(b, static_cast<int>(offset) + 16, 0, 0);
+      const u32x4_t hi = __builtin_amdgcn_raw_buffer_load_b128(buffer, static_cast<int>(offset) + 16, 0, 0);
       return join(__builtin_bit_cast(f32x4_t, lo), __builtin_bit_cast(f32x4_t, hi));
     }
   }
-  /// Eight elements from column c of row r, by ordinary loads, where rows are not whole pieces.
-  __device__ __forceinline__ typename Op<T>::x8 take(uint32_t r, uint32_t c, uint32_t cols, uint64_t rows) const {
-    const T* at = reinterpret_cast<const T*>(base + (reverse ? kRows - 1 - r : r) * step) + c;
-    return fetch8(at, r < rows && c < cols ? cols - c : 0u);
+  /// Eight elements from column c of the chunk's row r.
+  __device__ __forceinline__ X8 take(uint32_t r, uint32_t c) const {
+    return fetch8(reinterpret_cast<const T*>(base + r * step) + c, r < left && c < cols ? cols - c : 0u);
+  }
+  __device__ __forceinline__ void advance() {
+    base += step * kRows;
+    left = left > kRows ? left - kRows : 0;
   }
 };
 
-/// WHOLE: rows of q, k and v are whole pieces of eight elements, 16-byte aligned, 2^31 bytes a chunk at most.
+/// WHOLE: rows of q, k and v are whole pieces of eight elements, 16-byte aligned, and a segment spans less than 2^31 bytes.
 template <class T, int KD, bool STATES, bool WHOLE>
-__global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) attention_kernel(AttentionPass a) {
-  using Shape = AttentionShape<T, KD>;
+__global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) attention_kernel(AttentionPasses) {
+  const AttentionPass& a = pass_of(blockIdx.y);
   using X8 = typename Op<T>::x8;
   using X4 = typename Op<T>::x4;
   constexpr bool kHalf = std::is_same<T, half_t>::value;
-  constexpr uint32_t kS = Shape::kStride, kVS = Shape::kVStride;
+  constexpr uint32_t kKS = KD + (sizeof(T) == 2 ? 16 : 4);    // of K, read by rows and by columns
+  constexpr uint32_t kS = KD + 16 / sizeof(T);                 // of X in LDS: rows four banks apart
+  constexpr uint32_t kVS = kCols + (sizeof(T) == 2 ? 16 : 4);  // of V, read by columns
   constexpr int NX = KD / 16, NK = KD / 32;
-  __shared__ __attribute__((aligned(16))) T s_k[kRows * kS];
+  __shared__ __attribute__((aligned(16))) T s_k[kRows * kKS];
   __shared__ __attribute__((aligned(16))) T s_v[kRows * kVS];
   __shared__ __attribute__((aligned(16))) T s_x[STATES ? 16 : kCols * kS];
   __shared__ __attribute__((aligned(16))) float s_unlift[kHalf ? kCols : 4];
-  __shared__ uint32_t s_odd[4];
+  __shared__ uint32_t s_odd[kWaves];
 
-  // The column slices of one head, which read the same q and k, follow one another on one XCD.
+  // Neighbouring heads go to one XCD: their rows are neighbours in memory, and a head's by itself, whole tokens apart, may all
+  // lie in one of the sixteen channels of an L2. The column slices of a head, which read the same q and k, follow one another.
   const uint32_t slices = (a.dv + kCols - 1) / kCols, index = blockIdx.x >> 3;
-  const uint32_t segments = STATES ? a.segments - 1 : a.segments;
-  const uint64_t item = static_cast<uint64_t>(index / slices) * 8 + (blockIdx.x & 7);
   const uint32_t all = a.batch * a.heads;
-  if (item >= static_cast<uint64_t>(all) * segments) return;
+  const uint64_t items = static_cast<uint64_t>(all) * (STATES ? a.segments - 1 : a.segments), share = (items + 7) / 8;
+  const uint64_t item = (blockIdx.x & 7) * share + index / slices;
+  if (index / slices >= share || item >= items) return;
   const uint32_t segment = static_cast<uint32_t>(item / all), bh = static_cast<uint32_t>(item % all);
   const uint32_t text = bh / a.heads, head = bh % a.heads, col0 = index % slices * kCols;
   const uint64_t first = segment * a.segment;
@@ -290,12 +311,11 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
   constexpr uint32_t kPieces = KD / 8, kKRows = 256 / kPieces;
   const uint32_t k_row = threadIdx.x / kPieces, k_col = threadIdx.x % kPieces * 8;
   const uint32_t v_row = threadIdx.x / 8, v_col = threadIdx.x % 8 * 8, q_row = 16 * w + l;
-  const uint32_t v_cols = a.dv - col0;
+  const uint64_t here = stop > first ? stop - first : 0;
   using Rows = ChunkRows<T, WHOLE>;
-  Rows k_at(a.k, text, head, 0, a.reverse, length, first), v_at(a.v, text, head, col0, a.reverse, length, first);
-  Rows q_at(STATES ? a.k : a.q, text, head, 0, a.reverse, length, first);
-  const uint32_t k_off = WHOLE ? k_at.offset(k_row, k_col, a.dk) : 0, v_off = WHOLE ? v_at.offset(v_row, v_col, v_cols) : 0;
-  const uint32_t q_off = WHOLE ? q_at.offset(q_row, 8 * g, a.dk) : 0;
+  Rows k_at(a.k, text, head, 0, a.dk, a.reverse, length, first, here), v_at(a.v, text, head, col0, a.dv, a.reverse, length, first, here);
+  Rows q_at(STATES ? a.k : a.q, text, head, 0, a.dk, a.reverse, length, first, here);
+  uint32_t k_off = k_at.offset(k_row, k_col), v_off = v_at.offset(v_row, v_col), q_off = q_at.offset(q_row, 8 * g);
 
   const double log2d = log2_decay(a, head);
   const float lg = static_cast<float>(log2d);
@@ -303,19 +323,18 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
   float whole_high, whole_low;
   power(log2d, kRows, &whole_high, &whole_low);
 
-  // Factors of the scores, row 16 w + l against s = 16 b + 4 g + i: of the block on the diagonal, and of those before it
-  // d^(16 + l - 4 g - i) d^(16 (w - b - 1)). Of v in the update, s = 16 c + 4 g + i: d^(15 - 4 g - i) d^(n - ahead - 15 - 16 c).
+  // Factors of the scores, row 16 w + l against s = 16 b + 4 g + i: of the block on the diagonal, of the one before it
+  // d^(16 + l - 4 g - i), and d^16 more of each further one. Of v in the update, s = 16 c + 4 g + i: of the last sixteen
+  // rows d^(15 - 4 g - i + 1 - ahead), and again d^16 more of those before.
   const auto uniform = [](float f) { return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(__float_as_uint(f))))); };
-  float diagonal[4], before[4], within[4], far_factor = 0.0f, block_factor[4], weight_factor[4];
+  float diagonal[4], before[4], within[4], far_factor = 0.0f;
+  const float sixteen = uniform(decay(16));
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int apart = static_cast<int>(l) - static_cast<int>(4 * g + i);
     diagonal[i] = apart >= 0 ? a.near_scale * decay(apart) : 0.0f;
     before[i] = a.near_scale * decay(16 + apart);
-    within[i] = decay(15 - static_cast<int>(4 * g + i));
-    weight_factor[i] = uniform(a.kv_scale * decay(49 - static_cast<int>(a.ahead) - 16 * i));
-    const int away = static_cast<int>(w) - i - 1;
-    block_factor[i] = uniform(away >= 0 ? decay(16 * away) : 0.0f);
+    within[i] = a.kv_scale * decay(16 - static_cast<int>(4 * g + i + a.ahead));
   }
   if constexpr (!STATES) far_factor = a.far_scale * decay(static_cast<int>(16 * w + l + a.ahead));
 
@@ -347,53 +366,66 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
   }
 
   ChunkLoads<T, KD, STATES> next;
-  const auto load = [&](uint64_t rows) {
-    if constexpr (WHOLE) {
-      const uint32_t n = rows < kRows ? static_cast<uint32_t>(rows) : kRows;
-      const auto k_rows = k_at.buffer(n, a.dk), v_rows = v_at.buffer(n, v_cols);
-      const uint32_t k0 = k_off - k_at.shift(n), v0 = v_off - v_at.shift(n);
-      const uint32_t k_next = a.reverse ? -kKRows * static_cast<uint32_t>(k_at.step) : kKRows * static_cast<uint32_t>(k_at.step);
-      const uint32_t v_next = a.reverse ? -32 * static_cast<uint32_t>(v_at.step) : 32 * static_cast<uint32_t>(v_at.step);
+  const auto load = [&] {
+    const uint32_t k_step = static_cast<uint32_t>(k_at.step), v_step = static_cast<uint32_t>(v_at.step), q_step = static_cast<uint32_t>(q_at.step);
 #pragma unroll
-      for (int u = 0; u < KD / 32; ++u) next.k[u] = Rows::take(k_rows, k0 + u * k_next);
+    for (int u = 0; u < KD / 32; ++u) next.k[u] = WHOLE ? k_at.take(k_off + u * kKRows * k_step) : k_at.take(k_row + u * kKRows, k_col);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) next.v[u] = Rows::take(v_rows, v0 + u * v_next);
-      if constexpr (!STATES) {
-        const auto q_rows = q_at.buffer(n, a.dk);
-        const uint32_t q0 = q_off - q_at.shift(n);
+    for (int u = 0; u < kWaves / 2; ++u) next.v[u] = WHOLE ? v_at.take(v_off + u * 32 * v_step) : v_at.take(v_row + u * 32, v_col);
+    if constexpr (!STATES) {
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) next.q[kk] = Rows::take(q_rows, 32 * kk + 8 * g < a.dk ? q0 + 32 * kk * sizeof(T) : 1u << 31);
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < KD / 32; ++u) next.k[u] = k_at.take(k_row + u * kKRows, k_col, a.dk, rows);
-#pragma unroll
-      for (int u = 0; u < 2; ++u) next.v[u] = v_at.take(v_row + u * 32, v_col, v_cols, rows);
-      if constexpr (!STATES) {
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk) next.q[kk] = q_at.take(q_row, 32 * kk + 8 * g, a.dk, rows);
+      for (int kk = 0; kk < NK; ++kk) {
+        // dk is KD but for heads of other sizes, whose last pieces may be none.
+        const bool none = a.dk < KD && 32 * kk + 8 * g >= a.dk;
+        if constexpr (WHOLE) {
+          next.q[kk] = q_at.take(none ? (1u << 31) | q_off : q_off + 32 * kk * static_cast<uint32_t>(sizeof(T)));
+        } else {
+          next.q[kk] = q_at.take(q_row, 32 * kk + 8 * g);
+        }
       }
     }
-    k_at.advance();
-    v_at.advance();
-    q_at.advance();
+    if constexpr (WHOLE) {
+      k_off += kRows * k_step;
+      v_off += kRows * v_step;
+      q_off += kRows * q_step;
+    } else {
+      k_at.advance();
+      v_at.advance();
+      q_at.advance();
+    }
   };
 
   const auto left = [](uint32_t all_of_it, uint32_t from) { return all_of_it <= from ? 0u : WHOLE ? 8u : all_of_it - from; };
-  const auto store_row = [&](uint64_t t, const float (&lo)[8], const float (&hi)[8]) {
-    const uint32_t c = col0 + 16 * g;
-    const uint64_t at = ((text * a.tokens + t) * a.heads + head) * a.dv + c;
+  const bool all_columns = col0 + kCols <= a.dv;
+  // This lane's columns of a result's row, by eights.
+  const auto store_row = [&](uint64_t t, auto&& eight) {
+    const uint64_t at = ((text * a.tokens + t) * a.heads + head) * a.dv;
     const auto put = [&](auto* out) {
-      if (left(a.dv, c)) store8(out + at, lo, left(a.dv, c));
-      if (left(a.dv, c + 8)) store8(out + at + 8, hi, left(a.dv, c + 8));
+#pragma unroll
+      for (int u = 0; u < kWaves / 2; ++u) {
+        const uint32_t c = col0 + 32 * u + 8 * g;
+        float v[8];
+        eight(u, v);
+        if (all_columns) {
+          store8(out + at + c, v, 8);
+        } else if (left(a.dv, c)) {
+          store8(out + at + c, v, left(a.dv, c));
+        }
+      }
     };
     if (a.out_fp32) return put(static_cast<float*>(a.out));
     put(static_cast<T*>(a.out));
   };
 
-  if (first < stop) load(stop - first);
+  if (first < stop) load();
   for (uint64_t c0 = first; c0 < stop; c0 += kRows) {
     const uint32_t rows = stop - c0 < kRows ? static_cast<uint32_t>(stop - c0) : kRows;
+    // Products of these and what the text's end asks for are made where they are used: kept over the loop they took
+    // more registers than there are.
+    uint32_t own_g = g, own_l = l, own_dk = a.dk;
+    asm volatile("" : "+v"(own_g), "+v"(own_l), "+s"(own_dk));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(within[i]), "+v"(before[i]));
     int copy_lift = 0, x_size = 0;  // float16: of X's copy beside X, and the binary order of X's column
     if constexpr (kHalf) {
       float most = 0.0f;
@@ -419,15 +451,15 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
 #pragma unroll
     for (int u = 0; u < KD / 32; ++u) finite = all_finite<T>(next.k[u]) && finite;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) finite = all_finite<T>(next.v[u]) && finite;
+    for (int u = 0; u < kWaves / 2; ++u) finite = all_finite<T>(next.v[u]) && finite;
     finite = !__any(!finite);
     __syncthreads();  // the last chunk's reads of LDS are done
     if (lane == 0) s_odd[w] = !finite;
     if (kHalf && !STATES && g == 0) s_unlift[16 * w + l] = ldexpf(1.0f, -(x_lift + copy_lift));
 #pragma unroll
-    for (int u = 0; u < KD / 32; ++u) *reinterpret_cast<X8*>(s_k + (k_row + u * kKRows) * kS + k_col) = next.k[u];
+    for (int u = 0; u < KD / 32; ++u) *reinterpret_cast<X8*>(s_k + (k_row + u * kKRows) * kKS + k_col) = next.k[u];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < kWaves / 2; ++u) {
       T* at = s_v + (v_row + u * 32) * kVS;
       *reinterpret_cast<X4*>(at + place(v_col)) = __builtin_shufflevector(next.v[u], next.v[u], 0, 1, 2, 3);
       *reinterpret_cast<X4*>(at + place(v_col + 4)) = __builtin_shufflevector(next.v[u], next.v[u], 4, 5, 6, 7);
@@ -446,213 +478,256 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
     }
     __syncthreads();
     // Infinities or NaN in k or v: what the plain products would spread is kept apart.
-    const bool odd = __builtin_amdgcn_readfirstlane(static_cast<int>(s_odd[0] | s_odd[1] | s_odd[2] | s_odd[3])) != 0;
-    if (c0 + kRows < stop) load(stop - c0 - kRows);
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) any |= s_odd[i];
+    const bool odd = __builtin_amdgcn_readfirstlane(static_cast<int>(any)) != 0;
+    if (c0 + kRows < stop) load();
 
-    if constexpr (!STATES) {
-      // Scores of this wave's rows, decayed, zeros where s comes later. (All four blocks for 16 bits: the wave with the most
-      // of them decides, and without branches their products follow one another closely.)
-      float p[4][4];
-      f32x4_t acc[4]{};
+    // Whole chunks of finite values have no questions to ask.
+    const auto results = [&](auto slow) {
+      constexpr bool kSlow = decltype(slow)::value;
+      if constexpr (!STATES) {
+        // Scores of this wave's rows, decayed, zeros where s comes later, two blocks at a time so that their products follow
+        // one another closely.
+        float p[kHalf ? kWaves : 1][4], own[4] = {};  // own: the scores of the block on the diagonal
+        X8 pb[kWaves / 2];
+        float away[4];
 #pragma unroll
-      for (uint32_t b = 0; b < 4; ++b) {
-        if (sizeof(T) == 4 && b > w) continue;
+        for (int i = 0; i < 4; ++i) away[i] = before[i];
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) acc[b] = Op<T>::mma(*reinterpret_cast<const X8*>(s_k + (16 * b + l) * kS + 32 * kk + 8 * g), qf[kk], acc[b]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      // What the state gives.
-      f32x4_t o[4]{};
+        for (int m = kWaves / 2 - 1; m >= 0; --m) {
+          f32x4_t acc[2]{};
+          if (sizeof(T) == 2 || 2 * m <= static_cast<int>(w)) {
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk) {
+            for (int kk = 0; kk < NK; ++kk) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = Op<T>::mma(*reinterpret_cast<const X8*>(s_x + (16 * j + l) * kS + 32 * kk + 8 * g), qf[kk], o[j]);
-      }
-#pragma unroll
-      for (uint32_t b = 0; b < 4; ++b) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float factor = b == w ? diagonal[i] : before[i] * block_factor[b];
-          p[b][i] = b < w || (b == w && 4 * g + i <= l) ? acc[b][i] * factor : 0.0f;
-        }
-      }
-      int p_lift = 0;  // float16: this row's scores and sums are 2^p_lift as large
-      if constexpr (kHalf) {
-        float most = 0.0f;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(p[b][i]));
-        }
-        most = fmaxf(most, __shfl_xor(most, 16, 64));
-        most = fmaxf(most, __shfl_xor(most, 32, 64));
-        p_lift = lift(most, 13, 40);
-        const float factor = ldexpf(far_factor, p_lift);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const f32x4_t unlift = *reinterpret_cast<const f32x4_t*>(s_unlift + 16 * b + 4 * g);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            p[b][i] = ldexpf(p[b][i], p_lift);
-            o[b][i] *= unlift[i] * factor;
+              for (int u = 0; u < 2; ++u) {
+                if (sizeof(T) == 4 && 2 * m + u > static_cast<int>(w)) continue;
+                acc[u] = Op<T>::mma(*reinterpret_cast<const X8*>(s_k + (32 * m + 16 * u + l) * kKS + 32 * kk + 8 * g), qf[kk], acc[u]);
+              }
+            }
           }
-        }
-      } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] *= far_factor;
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      // Scores that the mask takes away are zeros; against infinities and NaN of v they would still count. There those of v
-      // are left out, and the ones that the mask lets through are added by themselves.
-#pragma unroll
-      for (uint32_t m = 0; m < 2; ++m) {
-        if (sizeof(T) == 4 && 2 * m > w) continue;
-        X8 pb;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pb[e] = static_cast<T>(p[2 * m + (e >> 2)][e & 3]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          X4 v0 = column4(s_v, kVS, 32 * m, 16 * j), v1 = column4(s_v, kVS, 32 * m + 16, 16 * j);
-          if (odd && 2 * m >= w) v0 = only_finite(v0);
-          if (odd && 2 * m + 1 >= w) v1 = only_finite(v1);
-          o[j] = Op<T>::mma(join(v0, v1), pb, o[j]);
-        }
-      }
-      if (odd) {
-        float own[4];  // the scores of the block on the diagonal
-#pragma unroll
-        for (int i = 0; i < 4; ++i) own[i] = w == 0 ? p[0][i] : w == 1 ? p[1][i] : w == 2 ? p[2][i] : p[3][i];
-#pragma unroll 1
-        for (uint32_t s = 0; s < 16; ++s) {
-          const uint32_t i0 = s & 3;
-          const float mine = i0 == 0 ? own[0] : i0 == 1 ? own[1] : i0 == 2 ? own[2] : own[3];
-          const float score = __shfl(mine, static_cast<int>(l + 16 * (s >> 2)), 64);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int u = 1; u >= 0; --u) {
+            const int b = 2 * m + u, at = static_cast<int>(w);
+            float y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float value = static_cast<float>(s_v[(16 * w + s) * kVS + 16 * j + 4 * g + i]);
-              if (s <= l && !is_finite(value)) o[j][i] = fmaf(score, value, o[j][i]);
+              y[i] = acc[u][i] * (b < at ? away[i] : b == at ? diagonal[i] : 0.0f);
+              // Zeros where the mask is; but not times infinities and NaN.
+              if (kSlow && odd) y[i] = b < at || (b == at && 4 * own_g + i <= own_l) ? y[i] : 0.0f;
+              if (kSlow && b == at) own[i] = y[i];
+            }
+            if (b < at) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) away[i] *= sixteen;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if constexpr (kHalf) {
+                p[b][i] = y[i];
+              } else {
+                pb[m][4 * u + i] = static_cast<T>(y[i]);
+              }
             }
           }
         }
-      }
-      if (c0 + q_row < last) {
-        float lo[8], hi[8];
+        __builtin_amdgcn_sched_barrier(0);
+        // What the state gives.
+        f32x4_t o[kWaves]{};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y0 = o[e >> 2][e & 3], y1 = o[2 + (e >> 2)][e & 3];
-          lo[e] = q_row >= rows ? 0.0f : kHalf ? ldexpf(y0, -p_lift) : y0;
-          hi[e] = q_row >= rows ? 0.0f : kHalf ? ldexpf(y1, -p_lift) : y1;
+        for (int kk = 0; kk < NK; ++kk) {
+#pragma unroll
+          for (int j = 0; j < kWaves; ++j) o[j] = Op<T>::mma(*reinterpret_cast<const X8*>(s_x + (16 * j + l) * kS + 32 * kk + 8 * g), qf[kk], o[j]);
         }
-        store_row(token(c0 + q_row), lo, hi);
-      }
-    }
-
-    __builtin_amdgcn_sched_barrier(0);
-    // X: this wave's columns. v times its decay in fp32, as three bfloat16 parts or two float16 ones, against k as it is.
-    constexpr int kParts = sizeof(T) == 4 ? 1 : kHalf ? 2 : 3;
-    X8 part[2][kParts];
-    int new_lift = x_lift;
-    {
-      float y[2][8];
+        __builtin_amdgcn_sched_barrier(0);
+        int p_lift = 0;  // float16: this row's scores and sums are 2^p_lift as large
+        if constexpr (kHalf) {
+          float most = 0.0f;
 #pragma unroll
-      for (uint32_t m = 0; m < 2; ++m) {
+          for (int b = 0; b < kWaves; ++b) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(p[b][i]));
+          }
+          most = fmaxf(most, __shfl_xor(most, 16, 64));
+          most = fmaxf(most, __shfl_xor(most, 32, 64));
+          p_lift = lift(most, 13, 40);
+          const float factor = ldexpf(far_factor, p_lift);
+#pragma unroll
+          for (int b = 0; b < kWaves; ++b) {
+            const f32x4_t unlift = *reinterpret_cast<const f32x4_t*>(s_unlift + 16 * b + 4 * g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              pb[b >> 1][4 * (b & 1) + i] = static_cast<T>(ldexpf(p[b][i], p_lift));
+              o[b][i] *= unlift[i] * factor;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kWaves; ++j) o[j] *= far_factor;
+        }
+        // Scores that the mask takes away are zeros; against infinities and NaN of v they would still count. There those of v
+        // are left out, and the ones that the mask lets through are added by themselves.
+#pragma unroll
+        for (uint32_t m = 0; m < kWaves / 2; ++m) {
+          if (sizeof(T) == 4 && 2 * m > w) continue;
+#pragma unroll
+          for (int j = 0; j < kWaves; ++j) {
+            X4 v0 = column4(s_v, kVS, 32 * m, 16 * j), v1 = column4(s_v, kVS, 32 * m + 16, 16 * j);
+            if (kSlow && odd && 2 * m >= w) v0 = only_finite(v0);
+            if (kSlow && odd && 2 * m + 1 >= w) v1 = only_finite(v1);
+            o[j] = Op<T>::mma(join(v0, v1), pb[m], o[j]);
+          }
+        }
+        if (kSlow && odd) {
+          if constexpr (kHalf) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) own[i] = ldexpf(own[i], p_lift);
+          }
+#pragma unroll 1
+          for (uint32_t s = 0; s < 16; ++s) {
+            const uint32_t i0 = s & 3;
+            const float mine = i0 == 0 ? own[0] : i0 == 1 ? own[1] : i0 == 2 ? own[2] : own[3];
+            const float score = __shfl(mine, static_cast<int>(l + 16 * (s >> 2)), 64);
+#pragma unroll
+            for (int j = 0; j < kWaves; ++j) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float value = static_cast<float>(s_v[(16 * w + s) * kVS + 16 * j + 4 * g + i]);
+                if (s <= l && !is_finite(value)) o[j][i] = fmaf(score, value, o[j][i]);
+              }
+            }
+          }
+        }
+        if (!kSlow || c0 + q_row < last) {
+          store_row(token(c0 + q_row), [&](int u, float (&v)[8]) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float y = o[2 * u + (e >> 2)][e & 3];
+              v[e] = kSlow && q_row >= rows ? 0.0f : kHalf ? ldexpf(y, -p_lift) : y;
+            }
+          });
+        }
+      }
+
+    };
+    const auto update = [&](auto slow, auto exact) {
+      constexpr bool kSlow = decltype(slow)::value, kExact = decltype(exact)::value;
+      // X: this wave's columns. v times its decay in fp32, as three bfloat16 parts or two float16 ones, against k as it is. Where
+      // nobody asks for the state, whose copy has 8 bits or 11, two parts do, and a decay rounded to fp32.
+      constexpr int kParts = sizeof(T) == 4 ? 1 : kHalf || !kExact ? 2 : 3;
+      // m from the last to the first, `scale` from `within` on.
+      const auto weighed = [&](int m, float (&scale)[4], float (&y)[8]) {
         const X8 vf = join(column4(s_v, kVS, 32 * m, 16 * w), column4(s_v, kVS, 32 * m + 16, 16 * w));
 #pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) {
-          float weight = within[e & 3] * weight_factor[2 * m + (e >> 2)];
-          if (rows < kRows) {
-            const int after = static_cast<int>(rows - a.ahead) - static_cast<int>(32 * m + 16 * (e >> 2) + 4 * g + (e & 3));
-            weight = a.kv_scale * decay(after > 0 ? after : 0);
+        for (int u = 1; u >= 0; --u) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float weight = scale[i];
+            if (kSlow && rows < kRows) {
+              const int after = static_cast<int>(rows - a.ahead) - static_cast<int>(32 * m + 16 * u + 4 * own_g + i);
+              weight = a.kv_scale * decay(after > 0 ? after : 0);
+            }
+            y[4 * u + i] = static_cast<float>(vf[4 * u + i]) * weight;
+            scale[i] *= sixteen;
           }
-          y[m][e] = static_cast<float>(vf[e]) * weight;
         }
-      }
+      };
+      float high = whole_high, low = whole_low;
+      if (kSlow && rows < kRows) power(log2d, rows, &high, &low);
       if constexpr (kHalf) {
         // Behind a power of two by columns, as large as float16 and X's own size allow.
-        float most = 0.0f;
+        float most = 0.0f, scale[4] = {within[0], within[1], within[2], within[3]};
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
+        for (int m = kWaves / 2 - 1; m >= 0; --m) {
+          float y[8];
+          weighed(m, scale, y);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) most = fmaxf(most, odd && !is_finite(y[m][e]) ? 0.0f : fabsf(y[m][e]));
+          for (int e = 0; e < 8; ++e) most = fmaxf(most, kSlow && odd && !is_finite(y[e]) ? 0.0f : fabsf(y[e]));
         }
         most = fmaxf(most, __shfl_xor(most, 16, 64));
         most = fmaxf(most, __shfl_xor(most, 32, 64));
+        int new_lift = x_lift;
         if (most > 0.0f) {
           const int top = 14 - ilogbf(most), room = 100 - (x_size - x_lift);
           new_lift = top < room ? top : room;
         }
+        high = ldexpf(high, new_lift - x_lift);
+        low = ldexpf(low, new_lift - x_lift);
+        x_lift = new_lift;
+      }
+      // The decay's second float counts over many chunks; times an infinity it would be NaN.
+      if (!kExact || settled) {
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
+        for (int n = 0; n < NX; ++n) x[n] *= high;
+      } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[m][e] = ldexpf(y[m][e], new_lift);
+        for (int n = 0; n < NX; ++n) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[n][i] = fmaf(x[n][i], high, x[n][i] * low);
         }
       }
+      settled = settled || (kSlow && odd);
+      float scale[4] = {within[0], within[1], within[2], within[3]};
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
+      for (int m = kWaves / 2 - 1; m >= 0; --m) {
+        __builtin_amdgcn_sched_barrier(0);
+        X8 part[kParts];
+        float rest[8];
+        weighed(m, scale, rest);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float rest = y[m][e];
+          if constexpr (kHalf) rest[e] = ldexpf(rest[e], x_lift);
 #pragma unroll
           for (int z = 0; z < kParts; ++z) {
-            part[m][z][e] = static_cast<T>(rest);
-            if (z + 1 < kParts) rest -= static_cast<float>(part[m][z][e]);
+            part[z][e] = static_cast<T>(rest[e]);
+            if (z + 1 < kParts) rest[e] -= static_cast<float>(part[z][e]);
           }
         }
-        if (odd) {  // an infinity has no lower parts
+        if (kSlow && odd) {  // an infinity has no lower parts
 #pragma unroll
-          for (int z = 1; z < kParts; ++z) part[m][z] = only_finite(part[m][z]);
+          for (int z = 1; z < kParts; ++z) part[z] = only_finite(part[z]);
+        }
+#pragma unroll
+        for (int n0 = 0; n0 < NX; n0 += 4) {
+          X8 kf[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) kf[n] = join(column4(s_k, kKS, 32 * m, 16 * (n0 + n)), column4(s_k, kKS, 32 * m + 16, 16 * (n0 + n)));
+          if (kSlow && odd && kParts > 1) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const X8 lower = only_finite(kf[n]);  // zeros among v's lower parts are none of v's
+#pragma unroll
+              for (int z = kParts - 1; z >= 0; --z) x[n0 + n] = Op<T>::mma(z ? lower : kf[n], part[z], x[n0 + n]);
+            }
+          } else {
+#pragma unroll
+            for (int z = kParts - 1; z >= 0; --z) {
+#pragma unroll
+              for (int n = 0; n < 4; ++n) x[n0 + n] = Op<T>::mma(kf[n], part[z], x[n0 + n]);
+            }
+          }
         }
       }
-    }
-    float high = whole_high, low = whole_low;
-    if (rows < kRows) power(log2d, rows, &high, &low);
-    if constexpr (kHalf) {
-      high = ldexpf(high, new_lift - x_lift);
-      low = ldexpf(low, new_lift - x_lift);
-      x_lift = new_lift;
-    }
-    // The decay's second float counts over many chunks; times an infinity it would be NaN.
-    if (settled) {
+      if (kSlow && odd && own_dk < KD) {  // rows that X does not have stay zeros
 #pragma unroll
-      for (int n = 0; n < NX; ++n) x[n] *= high;
+        for (int n = 0; n < NX; ++n) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[n][i] = 16 * n + 4 * own_g + i < own_dk ? x[n][i] : 0.0f;
+        }
+      }
+    };
+    if (odd || rows < kRows) {
+      results(std::true_type{});
+      update(std::true_type{}, std::true_type{});
     } else {
-#pragma unroll
-      for (int n = 0; n < NX; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[n][i] = fmaf(x[n][i], high, x[n][i] * low);
-      }
-    }
-    settled = settled || odd;
-#pragma unroll
-    for (uint32_t m = 0; m < 2; ++m) {
-#pragma unroll
-      for (int n0 = 0; n0 < NX; n0 += 4) {
-        X8 kf[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) kf[n] = join(column4(s_k, kS, 32 * m, 16 * (n0 + n)), column4(s_k, kS, 32 * m + 16, 16 * (n0 + n)));
-        if (odd && kParts > 1) {
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const X8 lower = only_finite(kf[n]);  // zeros among v's lower parts are none of v's
-#pragma unroll
-            for (int z = kParts - 1; z >= 0; --z) x[n0 + n] = Op<T>::mma(z ? lower : kf[n], part[m][z], x[n0 + n]);
-          }
-        } else {
-#pragma unroll
-          for (int z = kParts - 1; z >= 0; --z) {
-#pragma unroll
-            for (int n = 0; n < 4; ++n) x[n0 + n] = Op<T>::mma(kf[n], part[m][z], x[n0 + n]);
-          }
-        }
-      }
-    }
-    if (odd && a.dk < KD) {  // rows that X does not have stay zeros
-#pragma unroll
-      for (int n = 0; n < NX; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[n][i] = 16 * n + 4 * g + i < a.dk ? x[n][i] : 0.0f;
+      results(std::false_type{});
+      __builtin_amdgcn_sched_barrier(0);
+      if (sizeof(T) == 4 || a.exact) {
+        update(std::false_type{}, std::true_type{});
+      } else {
+        update(std::false_type{}, std::false_type{});
       }
     }
   }
@@ -660,8 +735,12 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
   if constexpr (!STATES) {
     // Tokens past the text's end, in chunks of their own.
     const uint64_t done = first < stop ? first + (stop - first + kRows - 1) / kRows * kRows : first;
-    const float zero[8] = {};
-    for (uint64_t t = done + q_row; t < last; t += kRows) store_row(t, zero, zero);
+    for (uint64_t t = done + q_row; t < last; t += kRows) {
+      store_row(t, [](int, float (&v)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+      });
+    }
   }
   float* to = nullptr;
   uint64_t sk = a.dv, sv = 1;
@@ -673,20 +752,22 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
     sv = a.state_dv;
   }
   if (!to) return;
-  asm volatile("" : "+s"(sk), "+s"(sv));  // the addresses anew: kept over the loop, they took more registers than there are
+  uint32_t dk = a.dk;
+  asm volatile("" : "+s"(sk), "+s"(sv), "+s"(dk));  // the addresses anew: kept over the loop, they took more registers than there are
   const uint32_t c = col0 + column_at(16 * w + l);
 #pragma unroll
   for (int n = 0; n < NX; ++n) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t r = 16 * n + 4 * g + i;
-      if (r < a.dk && c < a.dv) to[r * sk + c * sv] = kHalf ? ldexpf(x[n][i], -x_lift) : x[n][i];
+      if (r < dk && c < a.dv) to[r * sk + c * sv] = kHalf ? ldexpf(x[n][i], -x_lift) : x[n][i];
     }
   }
 }
 
 /// From what each segment leaves by itself to what it starts from.
-__global__ void __launch_bounds__(256) attention_scan_kernel(AttentionPass a) {
+__global__ void __launch_bounds__(256) attention_scan_kernel(AttentionPasses) {
+  const AttentionPass& a = pass_of(blockIdx.z);
   const uint32_t all = a.batch * a.heads, bh = blockIdx.y;
   const uint32_t size = a.dk * a.dv, at = blockIdx.x * 256 + threadIdx.x;
   if (at >= size) return;
@@ -816,48 +897,65 @@ void with_depth(uint32_t dk, F&& f) {
   f(std::integral_constant<int, 256>{});
 }
 
-/// Segments of a pass, as many as it takes to fill the device, of eight chunks or more.
-void cut(AttentionPass& a) {
-  const uint64_t slices = ceil_div(a.dv, kCols), groups = static_cast<uint64_t>(a.batch) * a.heads * slices;
-  const uint64_t chunks = ceil_div(a.tokens, kRows);
-  uint64_t segments = groups >= 512 || groups == 0 ? 1 : 1024 / groups;
-  segments = std::max<uint64_t>(1, std::min(segments, chunks / 8));
-  const uint64_t each = ceil_div(std::max<uint64_t>(chunks, 1), segments);
+/// Segments of a pass that is launched with `together` - 1 others like it: enough to fill the device, with work-groups of four chunks
+/// or more, where there is less than a work-group for most CUs. (A CU holds two of them, or one of a deep or fp32 head.) The
+/// segments' states are a third to a half of the pass again. Both sides, us, one segment and more: 8 texts of 4,096 tokens, 16
+/// heads of 128 bf16 (256 work-groups) 202 and 223 in two; 4 texts, 8 heads of 256 (128) 345 and 269 in two; one of 32,768, 16
+/// heads of 128 (32) 1,400 and 235 in sixteen, 247 in 32; one of 4,096, 8 heads of 64 (8) 113 and 28 in sixteen.
+void cut(AttentionPass& a, uint32_t together) {
+  const uint64_t groups = ceil_div(a.dv, kCols) * a.batch * a.heads * together;
+  const uint64_t chunks = std::max<uint64_t>(ceil_div(a.tokens, kRows), 1);
+  const uint64_t at_once = a.dk <= (a.wide ? 64u : 128u) ? 512 : 256;
+  uint64_t segments = groups >= 192 || groups == 0 ? 1 : std::max<uint64_t>(1, at_once / groups);
+  segments = std::max<uint64_t>(1, std::min(segments, chunks / 4));
+  // Rows far apart: segments that a buffer of 2^31 bytes holds, with room for the chunks around, where that can be.
+  const uint64_t apart = std::max({a.q.token, a.k.token, a.v.token}) * 4, most = apart ? (uint64_t{1} << 31) / apart / kRows : chunks + 4;
+  if (most > 8) segments = std::max(segments, ceil_div(chunks, most - 4));
+  const uint64_t each = ceil_div(chunks, segments);
   a.segment = each * kRows;
-  a.segments = static_cast<uint32_t>(ceil_div(std::max<uint64_t>(chunks, 1), each));
+  a.segments = static_cast<uint32_t>(ceil_div(chunks, each));
 }
 
 uint64_t state_bytes(const AttentionPass& a) {
   return a.segments > 1 ? static_cast<uint64_t>(a.segments) * a.batch * a.heads * a.dk * a.dv * sizeof(float) : 0;
 }
 
-/// Whether rows of a tensor are whole pieces (attention_kernel's WHOLE).
-bool whole_rows(const TokenTensor& t, uint32_t dim, size_t size) {
+/// Whether rows of a tensor are whole pieces that lie apart, and a segment's fit a buffer (attention_kernel's WHOLE).
+bool whole_rows(const AttentionPass& a, const TokenTensor& t, uint32_t dim, size_t size) {
   const uint64_t odd = reinterpret_cast<uintptr_t>(t.base) | t.batch * size | t.token * size | t.head * size;
-  return dim % 8 == 0 && odd % 16 == 0 && (t.token + dim) * size * kRows < (uint64_t{1} << 31);
+  return dim % 8 == 0 && odd % 16 == 0 && t.token >= dim && (a.segment + 2 * kRows) * t.token * size < (uint64_t{1} << 31);
 }
 
+/// `count` passes of one shape: the same dk and dv (or their swap, within one depth), texts and heads.
 template <class T>
-void launch_pass(const AttentionPass& a, hipStream_t s) {
-  const bool whole = whole_rows(a.q, a.dk, sizeof(T)) && whole_rows(a.k, a.dk, sizeof(T)) && whole_rows(a.v, a.dv, sizeof(T));
-  const auto with_rows = [&](auto&& f) { whole ? f(std::true_type{}) : f(std::false_type{}); };
-  const uint64_t slices = ceil_div(a.dv, kCols), all = static_cast<uint64_t>(a.batch) * a.heads;
-  with_depth(a.dk, [&](auto depth) {
-    constexpr int KD = decltype(depth)::value;
-    const auto grid = [&](uint64_t segments) { return dim3(static_cast<unsigned>(ceil_div(all * segments, 8) * 8 * slices)); };
-    if (a.segments > 1) {
-      with_rows([&](auto rows) {
-        hipLaunchKernelGGL((attention_kernel<T, KD, true, decltype(rows)::value>), grid(a.segments - 1), dim3(256), 0, s, a);
+void launch_passes(const AttentionPasses& p, uint32_t count, hipStream_t s) {
+  bool whole = true;
+  uint32_t depth = 0, segments = 1;
+  uint64_t slices = 1, size = 0;
+  for (uint32_t i = 0; i < count; ++i) {
+    const AttentionPass& a = p.pass[i];
+    whole = whole && whole_rows(a, a.q, a.dk, sizeof(T)) && whole_rows(a, a.k, a.dk, sizeof(T)) && whole_rows(a, a.v, a.dv, sizeof(T));
+    depth = std::max(depth, a.dk);
+    segments = std::max(segments, a.segments);
+    slices = std::max(slices, ceil_div(a.dv, kCols));
+    size = std::max<uint64_t>(size, static_cast<uint64_t>(a.dk) * a.dv);
+  }
+  const uint64_t all = static_cast<uint64_t>(p.pass[0].batch) * p.pass[0].heads;
+  const auto grid = [&](uint64_t parts) { return dim3(static_cast<unsigned>(ceil_div(all * parts, 8) * 8 * slices), count); };
+  with_depth(depth, [&](auto kd) {
+    constexpr int KD = decltype(kd)::value;
+    const auto go = [&](auto rows) {
+      constexpr bool WHOLE = decltype(rows)::value;
+      if (segments > 1) {
+        hipLaunchKernelGGL((attention_kernel<T, KD, true, WHOLE>), grid(segments - 1), dim3(256), 0, s, p);
         QVH_HIP(hipGetLastError());
-      });
-      hipLaunchKernelGGL(attention_scan_kernel, dim3(static_cast<unsigned>(ceil_div(static_cast<uint64_t>(a.dk) * a.dv, 256)), static_cast<unsigned>(all)),
-                         dim3(256), 0, s, a);
+        hipLaunchKernelGGL(attention_scan_kernel, dim3(static_cast<unsigned>(ceil_div(size, 256)), static_cast<unsigned>(all), count), dim3(256), 0, s, p);
+        QVH_HIP(hipGetLastError());
+      }
+      hipLaunchKernelGGL((attention_kernel<T, KD, false, WHOLE>), grid(segments), dim3(256), 0, s, p);
       QVH_HIP(hipGetLastError());
-    }
-    with_rows([&](auto rows) {
-      hipLaunchKernelGGL((attention_kernel<T, KD, false, decltype(rows)::value>), grid(a.segments), dim3(256), 0, s, a);
-      QVH_HIP(hipGetLastError());
-    });
+    };
+    whole ? go(std::true_type{}) : go(std::false_type{});
   });
 }
 
@@ -904,6 +1002,7 @@ AttentionPass forward_pass(const qvh_attention_args& in) {
   a.heads = in.heads;
   a.dk = in.dk;
   a.dv = in.dv;
+  a.wide = in.dtype == QVH_FP32;
   const uint32_t share = in.heads / in.kv_heads;
   a.q = tensor_of(in.q, in.q_stride, 1);
   a.k = tensor_of(in.k, in.k_stride, share);
@@ -914,15 +1013,15 @@ AttentionPass forward_pass(const qvh_attention_args& in) {
   a.index_bytes = in.index_bytes;
   a.state = in.state;
   a.state_out = in.state_out;
+  a.exact = in.state_out != nullptr;
   a.state_dk = in.dv;
   a.state_dv = 1;
   a.near_scale = a.far_scale = in.scale;
-  cut(a);
+  cut(a, 1);
   return a;
 }
 
-/// The three passes of the gradients, and where their workspaces lie: the segments' states, one pass after another, and
-/// shared heads' gradients by themselves.
+/// The three passes of the gradients, and where their workspaces lie: the segments' states and shared heads' gradients.
 struct GradPasses {
   AttentionPass q, k, v;
   float *parts_k = nullptr, *parts_v = nullptr;
@@ -936,6 +1035,7 @@ GradPasses grad_passes(const qvh_attention_grad_args& in, void* workspace) {
   AttentionPass a = forward_pass(f);
   const TokenTensor q = a.q, k = a.k, v = a.v, o = tensor_of(in.grad, in.grad_stride, 1);
   a.state_out = nullptr;
+  a.exact = false;
   // dq: forwards, the state transposed.
   g.q = a;
   g.q.dk = f.dv;
@@ -946,7 +1046,6 @@ GradPasses grad_passes(const qvh_attention_grad_args& in, void* workspace) {
   g.q.out = in.grad_q;
   g.q.state_dk = 1;
   g.q.state_dv = f.dv;
-  cut(g.q);
   // dv: backwards from the last state's gradient to the first one's.
   a.reverse = true;
   a.ahead = 0;
@@ -959,7 +1058,7 @@ GradPasses grad_passes(const qvh_attention_grad_args& in, void* workspace) {
   g.v.k = q;
   g.v.v = o;
   g.v.state_out = in.grad_first;
-  cut(g.v);
+  g.v.exact = in.grad_first != nullptr;
   // dk: the same, transposed.
   g.k = a;
   g.k.dk = f.dv;
@@ -969,15 +1068,16 @@ GradPasses grad_passes(const qvh_attention_grad_args& in, void* workspace) {
   g.k.v = q;
   g.k.state_dk = 1;
   g.k.state_dv = f.dv;
-  cut(g.k);
   char* at = static_cast<char*>(workspace);
   const auto take = [&](uint64_t bytes) {
     char* p = at ? at + g.bytes : nullptr;
     g.bytes += ceil_div(bytes, 16) * 16;
     return reinterpret_cast<float*>(p);
   };
-  float* states = take(std::max({state_bytes(g.q), state_bytes(g.k), state_bytes(g.v)}));
-  g.q.states = g.k.states = g.v.states = states;
+  for (AttentionPass* p : {&g.q, &g.k, &g.v}) {
+    cut(*p, 3);
+    p->states = take(state_bytes(*p));
+  }
   const uint64_t rows = f.batch * f.tokens * f.heads;
   if (share > 1) {
     g.parts_k = take(rows * f.dk * sizeof(float));
@@ -1034,7 +1134,7 @@ qvh_status qvh_attention_device(const qvh_attention_args* args, void* d_workspac
     with_dtype(args->dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       if (few) return launch_step<T>(a, s);
-      launch_pass<T>(a, s);
+      launch_passes<T>(AttentionPasses{{a, {}, {}}}, 1, s);
     });
   });
 }
@@ -1060,9 +1160,7 @@ qvh_status qvh_attention_grad_device(const qvh_attention_grad_args* args, void* 
     const qvh_attention_args& f = args->forward;
     with_dtype(f.dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
-      launch_pass<T>(g.q, s);
-      launch_pass<T>(g.k, s);
-      launch_pass<T>(g.v, s);
+      launch_passes<T>(AttentionPasses{{g.q, g.k, g.v}}, 3, s);
       if (g.parts_k && f.tokens > 0) {
         const uint64_t rows = f.batch * f.tokens * f.kv_heads;
         const auto sum = [&](const float* parts, uint32_t dim, void* out) {
