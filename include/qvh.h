@@ -503,7 +503,7 @@ typedef struct qvh_gradient {
   uint64_t count;
   int dtype;
 } qvh_gradient;
-qvh_status qvh_grad_norm_workspace(const qvh_gradient* grads, uint64_t count, uint64_t* bytes); /* of both calls */
+qvh_status qvh_grad_norm_workspace(uint64_t count, uint64_t* bytes); /* of both calls, for so many gradients of any size */
 qvh_status qvh_grad_norm_device(const qvh_gradient* grads, uint64_t count, float* d_norm, void* d_workspace,
                                 uint64_t workspace_bytes, void* stream);
 qvh_status qvh_clip_grad_norm_device(const qvh_gradient* grads, uint64_t count, float max_norm, float eps,

@@ -27,7 +27,19 @@ def _gate_activation(name) -> int:
 
 
 def _differentiated(*tensors) -> bool:
-    return any(t is not None and _encoder._differentiated(t) for t in tensors)
+    """Whether autograd has to know of a call (as encoder._differentiated, of any number of inputs)."""
+    if _encoder._torch is None:
+        _encoder._load_torch()
+    forward = _encoder._forward_ad
+    try:
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return _encoder._grad_enabled() or forward._current_level >= 0
+        if forward._current_level < 0:
+            return False
+        return any(t is not None and forward.unpack_dual(t).tangent is not None for t in tensors)
+    except AttributeError:
+        return False  # not a tensor, which the call refuses
 
 
 def _vector(name, v, dim, device, dtype):
@@ -294,12 +306,9 @@ def _gradients(name, tensors):
 
 def _run_clip(pointers, outs, counts, types, max_norm, eps, device):
     norm = _encoder._torch.empty((), dtype=_encoder._torch.float32, device=device)
-    args = (pointers, outs, counts, types, max_norm, eps, norm.data_ptr())
-    stream = _stream(device)
-    need = _quiver._clip_grad_norm(*args, 0, 0, stream)
-    if need:
-        work = _workspace(need, device)
-        _quiver._clip_grad_norm(*args, work.data_ptr(), need, stream)
+    need = _quiver._clip_grad_norm_most(len(pointers))
+    work = _workspace(need, device)
+    _quiver._clip_grad_norm(pointers, outs, counts, types, max_norm, eps, norm.data_ptr(), work.data_ptr(), need, _stream(device))
     return norm
 
 

@@ -21,6 +21,8 @@ constexpr uint32_t kTable = 120;        // tensors of a launch: its arguments st
 constexpr uint32_t kChunk = 8192;       // elements: 256 threads, eight vectors of four or four of eight each
 constexpr uint32_t kClipGroups = 2048;  // eight work-groups a CU
 
+constexpr uint64_t kMostGradients = uint64_t{1} << 20;
+
 struct ClipTable {
   const void* in[kTable];
   void* out[kTable];
@@ -46,10 +48,11 @@ __device__ __forceinline__ uint32_t tensor_of(const ClipTable& t, uint32_t chunk
 }
 
 /// Calls f<T>(first element, how many) for a chunk.
-template <class F>
+template <bool BACK, class F>
 __device__ __forceinline__ void with_chunk(const ClipTable& t, uint32_t chunk, F&& f) {
-  const uint32_t i = tensor_of(t, chunk);
-  const uint64_t from = static_cast<uint64_t>(chunk - t.chunk[i]) * kChunk, left = t.size[i] - from;
+  const uint32_t i = tensor_of(t, chunk), at = chunk - t.chunk[i];
+  const uint64_t chunks = (t.size[i] + kChunk - 1) / kChunk;
+  const uint64_t from = (BACK ? chunks - 1 - at : at) * kChunk, left = t.size[i] - from;
   const uint32_t n = left < kChunk ? static_cast<uint32_t>(left) : kChunk;
   if (t.dtype[i] == QVH_FP32) return f(static_cast<const float*>(t.in[i]) + from, static_cast<float*>(t.out[i]) + from, n);
   if (t.dtype[i] == QVH_FP16) return f(static_cast<const half_t*>(t.in[i]) + from, static_cast<half_t*>(t.out[i]) + from, n);
@@ -98,7 +101,7 @@ __global__ void __launch_bounds__(256) clip_norm_kernel(ClipTable t, double* __r
   __shared__ double s_sum[4];
   double sum = 0.0;
   for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-    with_chunk(t, c, [&](auto* x, auto*, uint32_t n) { sum += squares(x, n); });
+    with_chunk<false>(t, c, [&](auto* x, auto*, uint32_t n) { sum += squares(x, n); });
   }
   sum = group_sum(sum, s_sum);
   if (threadIdx.x == 0) parts[blockIdx.x] = sum;
@@ -137,7 +140,7 @@ __device__ __forceinline__ double all_parts(const double* __restrict__ parts, ui
   return group_sum(sum, s);
 }
 
-/// The chunks from the last to the first: what the norm read last may still be in the last-level cache.
+/// From the last gradient to the first, and each backwards: what the norm read last may still be in the last-level cache.
 __global__ void __launch_bounds__(256) clip_scale_kernel(ClipTable t, const double* __restrict__ parts, uint32_t count,
                                                          float max_norm, float eps, float* __restrict__ norm) {
   __shared__ double s_sum[4];
@@ -148,7 +151,7 @@ __global__ void __launch_bounds__(256) clip_scale_kernel(ClipTable t, const doub
   const float first = ratio < 0x1p-100 ? 0x1p-64f : 1.0f;
   const float factor = ratio >= 1.0 ? 1.0f : static_cast<float>(ratio < 0x1p-100 ? ratio * 0x1p64 : ratio);  // NaN stays
   for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-    with_chunk(t, t.chunks - 1 - c, [&](auto* x, auto* out, uint32_t k) {
+    with_chunk<true>(t, c, [&](auto* x, auto* out, uint32_t k) {
       if (factor != 1.0f || x != out) scaled(x, out, k, first, factor);
     });
   }
@@ -193,7 +196,7 @@ void check_apart(const char* who, const qvh_gradient* g, uint64_t n) {
 void check_gradients(const char* who, const qvh_gradient* g, uint64_t n, bool results) {
   const std::string w(who);
   QVH_REQUIRE(n == 0 || g != nullptr, w + ": null list of gradients");
-  QVH_REQUIRE(n <= (uint64_t{1} << 20), w + ": at most 2^20 gradients");
+  QVH_REQUIRE(n <= kMostGradients, w + ": at most 2^20 gradients");
   uint64_t chunks = 0;
   for (uint64_t i = 0; i < n; ++i) {
     require_dtype(who, g[i].dtype);
@@ -204,9 +207,9 @@ void check_gradients(const char* who, const qvh_gradient* g, uint64_t n, bool re
   QVH_REQUIRE(chunks < (uint64_t{1} << 31), w + ": too many elements in all");
 }
 
-/// Calls f(table, work-groups, parts before it) for every launch.
+/// Calls f(table, work-groups, parts before it) for every launch; from the last gradient to the first where `back`.
 template <class F>
-uint32_t each_table(const qvh_gradient* g, uint64_t n, F&& f) {
+uint32_t each_table(const qvh_gradient* g, uint64_t n, bool back, F&& f) {
   uint64_t all = 0;
   for (uint64_t i = 0; i < n; ++i) all += chunks_of(g[i]);
   ClipTable t;
@@ -217,7 +220,8 @@ uint32_t each_table(const qvh_gradient* g, uint64_t n, F&& f) {
     parts += groups;
     t.tensors = t.chunks = 0;
   };
-  for (uint64_t i = 0; i < n; ++i) {
+  for (uint64_t at = 0; at < n; ++at) {
+    const uint64_t i = back ? n - 1 - at : at;
     if (g[i].count == 0) continue;
     const uint32_t k = t.tensors++;
     t.in[k] = g[i].grad;
@@ -233,11 +237,11 @@ uint32_t each_table(const qvh_gradient* g, uint64_t n, F&& f) {
 }
 
 uint32_t count_parts(const qvh_gradient* g, uint64_t n) {
-  return each_table(g, n, [](const ClipTable&, uint32_t, uint32_t) {});
+  return each_table(g, n, false, [](const ClipTable&, uint32_t, uint32_t) {});
 }
 
 void run_norm(const qvh_gradient* g, uint64_t n, double* parts, hipStream_t s) {
-  each_table(g, n, [&](const ClipTable& t, uint32_t groups, uint32_t before) {
+  each_table(g, n, false, [&](const ClipTable& t, uint32_t groups, uint32_t before) {
     hipLaunchKernelGGL(clip_norm_kernel, dim3(groups), dim3(256), 0, s, t, parts + before);
     QVH_HIP(hipGetLastError());
   });
@@ -248,11 +252,13 @@ void run_norm(const qvh_gradient* g, uint64_t n, double* parts, hipStream_t s) {
 
 extern "C" {
 
-qvh_status qvh_grad_norm_workspace(const qvh_gradient* grads, uint64_t count, uint64_t* bytes) {
+qvh_status qvh_grad_norm_workspace(uint64_t count, uint64_t* bytes) {
   return qvh::guarded([&] {
+    using namespace qvh;
     QVH_REQUIRE(bytes != nullptr, "qvh_grad_norm_workspace: null output");
-    qvh::check_gradients("qvh_grad_norm_workspace", grads, count, false);
-    *bytes = qvh::count_parts(grads, count) * sizeof(double);
+    QVH_REQUIRE(count <= kMostGradients, "qvh_grad_norm_workspace: at most 2^20 gradients");
+    // A launch rounds its share of the work-groups up.
+    *bytes = count == 0 ? 0 : (kClipGroups + ceil_div(count, kTable)) * sizeof(double);
   });
 }
 
@@ -295,7 +301,7 @@ qvh_status qvh_clip_grad_norm_device(const qvh_gradient* grads, uint64_t count, 
       return;
     }
     run_norm(grads, count, sums, s);
-    each_table(grads, count, [&](const ClipTable& t, uint32_t groups, uint32_t before) {
+    each_table(grads, count, true, [&](const ClipTable& t, uint32_t groups, uint32_t before) {
       hipLaunchKernelGGL(clip_scale_kernel, dim3(groups), dim3(256), 0, s, t, sums, parts, max_norm, eps, before == 0 ? d_norm : nullptr);
       QVH_HIP(hipGetLastError());
     });

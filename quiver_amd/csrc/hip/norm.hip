@@ -25,7 +25,6 @@ namespace qvh {
 namespace {
 
 constexpr uint32_t kMaxNorm = 16384;  // columns
-constexpr uint32_t kParts = 512;      // work-groups of a backward pass, at most
 
 struct NormArgs {
   uint64_t rows = 0;
@@ -53,11 +52,12 @@ __device__ __forceinline__ float row_sum(float v, uint32_t lanes, float* s) {
   if (W > 1 || lanes > 16) add(16);
   if (W > 1 || lanes > 32) add(32);
   if constexpr (W > 1) {
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    const uint32_t wave = threadIdx.x >> 6, first = wave / W * W;
+    if ((threadIdx.x & 63) == 0) s[wave] = v;
     __syncthreads();
-    v = s[0];
+    v = s[first];
 #pragma unroll
-    for (int w = 1; w < W; ++w) v += s[w];
+    for (int w = 1; w < W; ++w) v += s[first + w];
   }
   return v;
 }
@@ -191,12 +191,30 @@ __global__ void __launch_bounds__(W == 1 ? 256 : W * 64) norm_kernel(NormArgs a)
   }
 }
 
+/// The matrices' pieces of one row.
+template <class T, int V, int P, bool BLOCK, bool GATE>
+struct GradRow {
+  Loose<T, V> r[P], dh[P], dr[P], y[BLOCK ? P : 1], gate[GATE ? P : 1];
+  __device__ __forceinline__ void load(const NormArgs& a, uint64_t row, const Pieces<V, P>& k, bool valid) {
+    load_row<T, V, P>(a.x, row * a.x_stride, k, valid, r);
+    load_row<T, V, P>(a.grad_h, row * a.grad_h_stride, k, valid, dh);
+    if (a.grad_r) load_row<T, V, P>(a.grad_r, row * a.grad_r_stride, k, valid, dr);
+    if constexpr (BLOCK) load_row<T, V, P>(a.y, row * a.y_stride, k, valid, y);
+    if constexpr (GATE) load_row<T, V, P>(a.gate, row * a.gate_stride, k, valid, gate);
+  }
+};
+
+/// The threads of a backward work-group.
+constexpr int grad_threads(int W) { return W <= 4 ? 256 : W * 64; }
+
+/// A work-group has as many rows at a time as its waves make up; the next ones are loaded while these are computed.
 template <class T, int V, int W, int P, bool BLOCK, bool GATE>
-__global__ void __launch_bounds__(W == 1 ? 512 : W * 64) norm_grad_kernel(NormArgs a) {
-  __shared__ float s_sum[4][W];
+__global__ void __launch_bounds__(grad_threads(W)) norm_grad_kernel(NormArgs a) {
+  constexpr int kGroup = grad_threads(W), kWaves = kGroup / 64;
+  __shared__ float s_sum[4][kWaves];
   const uint32_t lanes = W == 1 ? a.lanes : W * 64;
   const uint32_t thread = threadIdx.x & (lanes - 1);
-  const uint64_t per_group = W == 1 ? 512 / lanes : 1;
+  const uint64_t per_group = kGroup / lanes;
   const Pieces<V, P> k(thread, lanes, a.dim);
   Loose<T, V> weight[P], post[P], scale[P];
   load_row<T, V, P>(a.weight, 0, k, true, weight);
@@ -205,32 +223,29 @@ __global__ void __launch_bounds__(W == 1 ? 512 : W * 64) norm_grad_kernel(NormAr
     if (a.scale) load_row<T, V, P>(a.scale, 0, k, true, scale);
   }
   float sums[BLOCK ? 3 : 1][P][V] = {};
-  const uint64_t lead = blockIdx.x * per_group + (W == 1 ? (threadIdx.x & ~63u) / lanes : 0);
-  const uint64_t own = W == 1 ? (threadIdx.x & 63) / lanes : 0;
-  for (uint64_t row0 = lead; row0 < a.rows; row0 += gridDim.x * per_group) {
-    const uint64_t row = row0 + own;
+  // The first row of the wave decides (of the work-group, where a row has several waves), so that it stays together.
+  const uint64_t in_wave = W == 1 ? (threadIdx.x & 63) / lanes : threadIdx.x / lanes;
+  const uint64_t step = gridDim.x * per_group;
+  uint64_t row0 = blockIdx.x * per_group + (W == 1 ? (threadIdx.x & ~63u) / lanes : 0);
+  GradRow<T, V, P, BLOCK, GATE> next;
+  if (row0 < a.rows) next.load(a, row0 + in_wave, k, row0 + in_wave < a.rows);
+  for (; row0 < a.rows; row0 += step) {
+    const uint64_t row = row0 + in_wave;
     const bool valid = row < a.rows;
-    Loose<T, V> r[P], dh[P], dr[P], y[P], gate[P];
-    load_row<T, V, P>(a.x, row * a.x_stride, k, valid, r);
-    load_row<T, V, P>(a.grad_h, row * a.grad_h_stride, k, valid, dh);
-    if (a.grad_r) load_row<T, V, P>(a.grad_r, row * a.grad_r_stride, k, valid, dr);
-    if constexpr (BLOCK) {
-      load_row<T, V, P>(a.y, row * a.y_stride, k, valid, y);
-      if constexpr (GATE) load_row<T, V, P>(a.gate, row * a.gate_stride, k, valid, gate);
-    }
+    const GradRow<T, V, P, BLOCK, GATE> now = next;
+    if (row0 + step < a.rows) next.load(a, row + step, k, row + step < a.rows);
     float rr = 0.0f, ar = 0.0f, yy = 0.0f;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const bool once = static_cast<uint32_t>(i) >= k.again[p] && k.on[p];
-        const float v = once ? static_cast<float>(r[p].v[i]) : 0.0f;
+        const float v = once ? static_cast<float>(now.r[p].v[i]) : 0.0f;
         rr = fmaf(v, v, rr);
-        // Lanes past the row hold zeros of dh; times a weight that they never loaded it would be anything.
-        const float g = once ? static_cast<float>(dh[p].v[i]) * static_cast<float>(weight[p].v[i]) : 0.0f;
+        const float g = once ? static_cast<float>(now.dh[p].v[i]) * static_cast<float>(weight[p].v[i]) : 0.0f;
         ar = fmaf(g, v, ar);
         if constexpr (BLOCK) {
-          const float w = once ? static_cast<float>(y[p].v[i]) : 0.0f;
+          const float w = once ? static_cast<float>(now.y[p].v[i]) : 0.0f;
           yy = fmaf(w, w, yy);
         }
       }
@@ -244,11 +259,11 @@ __global__ void __launch_bounds__(W == 1 ? 512 : W * 64) norm_grad_kernel(NormAr
     for (int p = 0; p < P; ++p) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float rn = static_cast<float>(r[p].v[i]) * inv, g = static_cast<float>(dh[p].v[i]);
+        const float rn = static_cast<float>(now.r[p].v[i]) * inv, g = static_cast<float>(now.dh[p].v[i]);
         // A row past the last adds nothing, whatever its factors (eps may be 0, and the row's norm with it).
         if (valid) sums[0][p][i] = fmaf(g, rn, sums[0][p][i]);
         dx[p][i] = inv * fmaf(-rn, along, g * static_cast<float>(weight[p].v[i]));
-        if (a.grad_r) dx[p][i] += static_cast<float>(dr[p].v[i]);
+        if (a.grad_r) dx[p][i] += static_cast<float>(now.dr[p].v[i]);
       }
     }
     if (a.grad_x) store_row<T, V, P>(a.grad_x, row * a.dim, k, valid, [&](int p, int i) { return dx[p][i]; });
@@ -261,13 +276,13 @@ __global__ void __launch_bounds__(W == 1 ? 512 : W * 64) norm_grad_kernel(NormAr
       for (int p = 0; p < P; ++p) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float yn = static_cast<float>(y[p].v[i]) * inv_y, w = static_cast<float>(post[p].v[i]);
+          const float yn = static_cast<float>(now.y[p].v[i]) * inv_y, w = static_cast<float>(post[p].v[i]);
           const float u = yn * w;
           float du = dx[p][i], opened = 1.0f;
           if (a.scale) du *= static_cast<float>(scale[p].v[i]);
           if constexpr (GATE) {
             float slope;
-            opened = open_gate(static_cast<float>(gate[p].v[i]), a.act, &slope);
+            opened = open_gate(static_cast<float>(now.gate[p].v[i]), a.act, &slope);
             dgate[p][i] = du * u * slope;
             du *= opened;
           }
@@ -285,7 +300,7 @@ __global__ void __launch_bounds__(W == 1 ? 512 : W * 64) norm_grad_kernel(NormAr
       const float along_y = row_sum<W>(by, lanes, s_sum[3]) * a.share;
       if (a.grad_y) {
         store_row<T, V, P>(a.grad_y, row * a.dim, k, valid, [&](int p, int i) {
-          return inv_y * fmaf(-(static_cast<float>(y[p].v[i]) * inv_y), along_y, dx[p][i]);
+          return inv_y * fmaf(-(static_cast<float>(now.y[p].v[i]) * inv_y), along_y, dx[p][i]);
         });
       }
     }
@@ -304,12 +319,14 @@ __global__ void __launch_bounds__(W == 1 ? 512 : W * 64) norm_grad_kernel(NormAr
       }
     }
   };
-  if constexpr (W > 1) {
+  if constexpr (W * 64 == kGroup) {
 #pragma unroll
     for (int which = 0; which < kVectors; ++which) put(which, sums[which]);
   } else {
-    __shared__ float s_col[8][64 * P * V + 4];
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    // Rows of one wave first, then of the work-group's waves.
+    constexpr int kRowGroups = kWaves / W;
+    __shared__ float s_col[kRowGroups][W * 64 * P * V + 4];
+    const uint32_t group = threadIdx.x / (W * 64), own = threadIdx.x & (W * 64 - 1);
 #pragma unroll
     for (int which = 0; which < kVectors; ++which) {
 #pragma unroll
@@ -320,7 +337,7 @@ __global__ void __launch_bounds__(W == 1 ? 512 : W * 64) norm_grad_kernel(NormAr
           if (lanes <= 8) v += __uint_as_float(lane_xor_u32(__float_as_uint(v), 8));
           if (lanes <= 16) v += __uint_as_float(lane_xor_u32(__float_as_uint(v), 16));
           if (lanes <= 32) v += __uint_as_float(lane_xor_u32(__float_as_uint(v), 32));
-          s_col[wave][(p * 64 + lane) * V + i] = v;
+          s_col[group][(p * W * 64 + own) * V + i] = v;
         }
       }
       __syncthreads();
@@ -332,7 +349,7 @@ __global__ void __launch_bounds__(W == 1 ? 512 : W * 64) norm_grad_kernel(NormAr
           for (int i = 0; i < V; ++i) {
             float v = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) v += s_col[w][(p * 64 + lane) * V + i];
+            for (int w = 0; w < kRowGroups; ++w) v += s_col[w][(p * W * 64 + own) * V + i];
             total[p][i] = v;
           }
         }
@@ -376,8 +393,10 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(NormSums a) {
   }
 }
 
-/// Calls f<V, W, P>() for rows of `dim` elements of T; `lanes` are a row's threads.
-template <class T, class F>
+/// Calls f<V, W, P>() for rows of `dim` elements of T; `lanes` are a row's threads. Forward a thread has two pieces before a row
+/// gets four waves, backward, where it has five matrices and three sums of each, one piece as long as waves reach:
+/// 16,384 x 1,024 bf16 113 us with two pieces of a wave and FIGURE with one of two.
+template <class T, bool BACK, class F>
 void with_shape(uint32_t dim, uint32_t* lanes, F&& f) {
   constexpr int V = 16 / sizeof(T);
   using std::integral_constant;
@@ -389,13 +408,20 @@ void with_shape(uint32_t dim, uint32_t* lanes, F&& f) {
   const integral_constant<int, 1> one;
   const integral_constant<int, 2> two;
   const integral_constant<int, 4> four;
+  const integral_constant<int, 8> eight;
   const integral_constant<int, 16> sixteen;
   if (dim < V) return go(one, one, one, 8u);
   const uint32_t pieces = static_cast<uint32_t>(ceil_div(dim, V));
   if (pieces <= 64) return go(v, one, one, pieces <= 8 ? 8u : pieces <= 16 ? 16u : pieces <= 32 ? 32u : 64u);
-  if (pieces <= 128) return go(v, one, two, 64u);
-  if (pieces <= 256) return go(v, four, one, 256u);
-  if (pieces <= 512) return go(v, four, two, 256u);
+  if constexpr (BACK) {
+    if (pieces <= 128) return go(v, two, one, 128u);
+    if (pieces <= 256) return go(v, four, one, 256u);
+    if (pieces <= 512) return go(v, eight, one, 512u);
+  } else {
+    if (pieces <= 128) return go(v, one, two, 64u);
+    if (pieces <= 256) return go(v, four, one, 256u);
+    if (pieces <= 512) return go(v, four, two, 256u);
+  }
   if (pieces <= 1024) return go(v, sixteen, one, 1024u);
   if (sizeof(T) == 2 || pieces <= 2048) return go(v, sixteen, two, 1024u);
   if constexpr (sizeof(T) == 4) go(v, sixteen, four, 1024u);
@@ -408,19 +434,18 @@ void with_parts(bool block, bool gate, F&& f) {
   f(std::true_type{}, std::true_type{});
 }
 
-/// Work-groups of a backward pass: as many parts of every vector's sums.
+/// Work-groups of a backward pass, two a CU or fewer: as many parts of every vector's sums.
 uint32_t grad_groups(uint64_t rows, uint32_t dim, int dtype) {
-  const uint32_t v = dtype == QVH_FP32 ? 4 : 8;
-  const uint32_t pieces = static_cast<uint32_t>(ceil_div(dim, v));
-  uint64_t at_once = 1;
-  if (dim < v) {
-    at_once = 64;
-  } else if (pieces <= 64) {
-    at_once = 512 / (pieces <= 8 ? 8u : pieces <= 16 ? 16u : pieces <= 32 ? 32u : 64u);
-  } else if (pieces <= 128) {
-    at_once = 8;
-  }
-  return static_cast<uint32_t>(std::min<uint64_t>(ceil_div(rows, at_once), pieces > 512 ? kParts / 2 : kParts));
+  uint64_t groups = 0;
+  uint32_t lanes = 0;
+  with_dtype(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    with_shape<T, true>(dim, &lanes, [&](auto, auto w, auto) {
+      constexpr int W = decltype(w)::value;
+      groups = std::min<uint64_t>(ceil_div(rows, grad_threads(W) / lanes), W <= 4 ? 512 : 256);
+    });
+  });
+  return static_cast<uint32_t>(groups);
 }
 
 uint64_t grad_bytes(const qvh_block_norm_grad_args& a) {
@@ -511,7 +536,7 @@ qvh_status qvh_block_norm_device(const qvh_block_norm_args* args, void* stream) 
     a.h = in.h;
     with_dtype(in.dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
-      with_shape<T>(in.dim, &a.lanes, [&](auto v, auto w, auto p) {
+      with_shape<T, false>(in.dim, &a.lanes, [&](auto v, auto w, auto p) {
         constexpr int V = decltype(v)::value, W = decltype(w)::value, P = decltype(p)::value;
         with_parts(in.y != nullptr, in.gate != nullptr, [&](auto block, auto gate) {
           const uint64_t groups = ceil_div(a.rows, W == 1 ? 256 / a.lanes : 1);
@@ -570,11 +595,11 @@ qvh_status qvh_block_norm_grad_device(const qvh_block_norm_grad_args* args, void
     with_dtype(in.dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       if (groups > 0) {
-        with_shape<T>(in.dim, &a.lanes, [&](auto v, auto w, auto p) {
+        with_shape<T, true>(in.dim, &a.lanes, [&](auto v, auto w, auto p) {
           constexpr int V = decltype(v)::value, W = decltype(w)::value, P = decltype(p)::value;
           with_parts(in.y != nullptr, in.gate != nullptr, [&](auto block, auto gate) {
             hipLaunchKernelGGL((norm_grad_kernel<T, V, W, P, decltype(block)::value, decltype(gate)::value>), dim3(groups),
-                               dim3(W == 1 ? 512 : W * 64), 0, s, a);
+                               dim3(grad_threads(W)), 0, s, a);
             QVH_HIP(hipGetLastError());
           });
         });

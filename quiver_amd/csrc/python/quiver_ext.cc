@@ -309,19 +309,19 @@ PYBIND11_MODULE(_quiver, m) {
           check(qvh_attention_grad_device(&a, ptr(work), work_bytes, ptr(stream)));
           return 0;
         });
+  m.def("_clip_grad_norm_most", [check](std::uint64_t count) {
+    std::uint64_t bytes = 0;
+    check(qvh_grad_norm_workspace(count, &bytes));
+    return bytes;
+  });
   // Lists of addresses, results' addresses (empty: the norm alone), elements and types.
   m.def("_clip_grad_norm",
         [check, ptr](const std::vector<std::uintptr_t>& grads, const std::vector<std::uintptr_t>& outs,
                      const std::vector<std::uint64_t>& counts, const std::vector<int>& dtypes, float max_norm, float eps,
-                     std::uintptr_t norm, std::uintptr_t work, std::uint64_t work_bytes, std::uintptr_t stream) -> std::uint64_t {
+                     std::uintptr_t norm, std::uintptr_t work, std::uint64_t work_bytes, std::uintptr_t stream) {
           std::vector<qvh_gradient> list(grads.size());
           for (std::size_t i = 0; i < grads.size(); ++i) {
             list[i] = {ptr(grads[i]), outs.empty() ? nullptr : ptr(outs.at(i)), counts.at(i), dtypes.at(i)};
-          }
-          if (work_bytes == 0) {
-            std::uint64_t need = 0;
-            check(qvh_grad_norm_workspace(list.data(), list.size(), &need));
-            if (need > 0) return need;
           }
           float* d_norm = static_cast<float*>(ptr(norm));
           if (outs.empty() && !grads.empty()) {
@@ -329,7 +329,6 @@ PYBIND11_MODULE(_quiver, m) {
           } else {
             check(qvh_clip_grad_norm_device(list.data(), list.size(), max_norm, eps, d_norm, ptr(work), work_bytes, ptr(stream)));
           }
-          return 0;
         });
   m.def("_orthogonalize_workspace", [check](std::uint64_t batch, std::uint32_t m, std::uint32_t n) {
     std::uint64_t bytes = 0;
