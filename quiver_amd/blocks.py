@@ -232,7 +232,7 @@ def _linear_attention(q, k, v, log_decay, state, lengths, scale, keep_state, sta
     if state_out is not None:
         last, filled = state_out, _state("state_out", state_out, shape, device)
     elif keep_state:
-        last = filled = torch.empty(shape, dtype=torch.float32, device=device)
+        last = filled = held[0].new_empty(shape)  # log_decay's type
     args = (sizes, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, *args, _pointer(filled), out.data_ptr())
     stream = _stream(device)
     need = _quiver._attention(*args, 0, 0, stream)

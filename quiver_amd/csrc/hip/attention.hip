@@ -66,6 +66,8 @@ struct AttentionPass {
   uint32_t segments = 1;
   uint64_t segment = 0;  // tokens
   float* states = nullptr;
+  /// Segments whose own state is made: the last one's too where a result follows from it.
+  __host__ __device__ uint32_t parts() const { return state_out ? segments : segments - 1; }
 };
 
 /// The passes of one launch: the gradients' three, which have nothing to wait for in one another.
@@ -288,17 +290,17 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
   __shared__ __attribute__((aligned(16))) float s_unlift[kHalf ? kCols : 4];
   __shared__ uint32_t s_odd[kWaves];
 
-  // Neighbouring heads go to one XCD: their rows are neighbours in memory, and a head's by itself, whole tokens apart, may all
-  // lie in one of the sixteen channels of an L2. The column slices of a head, which read the same q and k, follow one another.
+  // Neighbouring heads, whose rows are neighbours in memory, go to one XCD, and the column slices of a head, which read the same
+  // q and k, follow one another on it.
   const uint32_t slices = (a.dv + kCols - 1) / kCols, index = blockIdx.x >> 3;
   const uint32_t all = a.batch * a.heads;
-  const uint64_t items = static_cast<uint64_t>(all) * (STATES ? a.segments - 1 : a.segments), share = (items + 7) / 8;
+  const uint64_t items = static_cast<uint64_t>(all) * (STATES ? a.parts() : a.segments), share = (items + 7) / 8;
   const uint64_t item = (blockIdx.x & 7) * share + index / slices;
   if (index / slices >= share || item >= items) return;
   const uint32_t segment = static_cast<uint32_t>(item / all), bh = static_cast<uint32_t>(item % all);
   const uint32_t text = bh / a.heads, head = bh % a.heads, col0 = index % slices * kCols;
   const uint64_t first = segment * a.segment;
-  const uint64_t last = segment + 1 == a.segments ? a.tokens : first + a.segment;  // tokens of the segment end here
+  const uint64_t last = segment + 1 == a.segments ? a.tokens : first + a.segment;  // the segment's tokens end here
   const uint64_t length = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(length_of(a, text))));  // below 2^31
   const uint64_t stop = length < last ? length : last;
 
@@ -724,7 +726,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
     } else {
       results(std::false_type{});
       __builtin_amdgcn_sched_barrier(0);
-      if (sizeof(T) == 4 || a.exact) {
+      if (sizeof(T) == 4 || (a.exact && (STATES || a.segments == 1))) {
         update(std::false_type{}, std::true_type{});
       } else {
         update(std::false_type{}, std::false_type{});
@@ -746,7 +748,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
   uint64_t sk = a.dv, sv = 1;
   if constexpr (STATES) {
     to = a.states + (static_cast<uint64_t>(segment) * all + bh) * a.dk * a.dv;
-  } else if (a.state_out && segment + 1 == a.segments) {
+  } else if (a.state_out && a.segments == 1) {
     to = a.state_out + static_cast<uint64_t>(bh) * a.dk * a.dv;
     sk = a.state_dk;
     sv = a.state_dv;
@@ -765,7 +767,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
   }
 }
 
-/// From what each segment leaves by itself to what it starts from.
+/// From what each segment leaves by itself to what it starts from, and what the last one leaves.
 __global__ void __launch_bounds__(256) attention_scan_kernel(AttentionPasses) {
   const AttentionPass& a = pass_of(blockIdx.z);
   const uint32_t all = a.batch * a.heads, bh = blockIdx.y;
@@ -774,18 +776,20 @@ __global__ void __launch_bounds__(256) attention_scan_kernel(AttentionPasses) {
   const uint64_t length = length_of(a, bh / a.heads);
   const double log2d = log2_decay(a, bh % a.heads);
   float x = 0.0f;
-  if (a.state) x = a.state[static_cast<uint64_t>(bh) * size + static_cast<uint64_t>(at / a.dv) * a.state_dk + static_cast<uint64_t>(at % a.dv) * a.state_dv];
+  const uint64_t place_of_state = static_cast<uint64_t>(bh) * size + static_cast<uint64_t>(at / a.dv) * a.state_dk + static_cast<uint64_t>(at % a.dv) * a.state_dv;
+  if (a.state) x = a.state[place_of_state];
   float* s = a.states + static_cast<uint64_t>(bh) * size + at;
   const uint64_t step = static_cast<uint64_t>(all) * size;
   float high, low;
   power(log2d, a.segment, &high, &low);
   for (uint32_t i = 0; i < a.segments; ++i) {
-    const float own = i + 1 < a.segments ? s[i * step] : 0.0f;
+    const float own = i < a.parts() ? s[i * step] : 0.0f;
     s[i * step] = x;
     const uint64_t from = i * a.segment, n = length > from ? length - from : 0;
     if (n < a.segment) power(log2d, n, &high, &low);
     x = is_finite(x) ? fmaf(x, high, fmaf(x, low, own)) : fmaf(x, high, own);
   }
+  if (a.state_out) a.state_out[place_of_state] = x;
 }
 
 /// The gradients of the heads that share one: their sum, in order.
@@ -930,24 +934,26 @@ bool whole_rows(const AttentionPass& a, const TokenTensor& t, uint32_t dim, size
 template <class T>
 void launch_passes(const AttentionPasses& p, uint32_t count, hipStream_t s) {
   bool whole = true;
-  uint32_t depth = 0, segments = 1;
+  uint32_t depth = 0, segments = 1, parts = 0;
   uint64_t slices = 1, size = 0;
   for (uint32_t i = 0; i < count; ++i) {
     const AttentionPass& a = p.pass[i];
     whole = whole && whole_rows(a, a.q, a.dk, sizeof(T)) && whole_rows(a, a.k, a.dk, sizeof(T)) && whole_rows(a, a.v, a.dv, sizeof(T));
     depth = std::max(depth, a.dk);
     segments = std::max(segments, a.segments);
+    parts = std::max(parts, a.parts());
     slices = std::max(slices, ceil_div(a.dv, kCols));
     size = std::max<uint64_t>(size, static_cast<uint64_t>(a.dk) * a.dv);
   }
   const uint64_t all = static_cast<uint64_t>(p.pass[0].batch) * p.pass[0].heads;
-  const auto grid = [&](uint64_t parts) { return dim3(static_cast<unsigned>(ceil_div(all * parts, 8) * 8 * slices), count); };
+  QVH_REQUIRE(ceil_div(all * std::max(segments, parts), 8) * 8 * slices * 256 < kGridThreads, "linear attention: too many segments for one launch");
+  const auto grid = [&](uint64_t each) { return dim3(static_cast<unsigned>(ceil_div(all * each, 8) * 8 * slices), count); };
   with_depth(depth, [&](auto kd) {
     constexpr int KD = decltype(kd)::value;
     const auto go = [&](auto rows) {
       constexpr bool WHOLE = decltype(rows)::value;
       if (segments > 1) {
-        hipLaunchKernelGGL((attention_kernel<T, KD, true, WHOLE>), grid(segments - 1), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((attention_kernel<T, KD, true, WHOLE>), grid(parts), dim3(256), 0, s, p);
         QVH_HIP(hipGetLastError());
         hipLaunchKernelGGL(attention_scan_kernel, dim3(static_cast<unsigned>(ceil_div(size, 256)), static_cast<unsigned>(all), count), dim3(256), 0, s, p);
         QVH_HIP(hipGetLastError());

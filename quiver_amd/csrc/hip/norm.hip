@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(NormSums a) {
 
 /// Calls f<V, W, P>() for rows of `dim` elements of T; `lanes` are a row's threads. Forward a thread has two pieces before a row
 /// gets four waves, backward, where it has five matrices and three sums of each, one piece as long as waves reach:
-/// 16,384 x 1,024 bf16 113 us with two pieces of a wave and FIGURE with one of two.
+/// 16,384 x 1,024 bf16 113 us with two pieces of a wave and 59 with one of two.
 template <class T, bool BACK, class F>
 void with_shape(uint32_t dim, uint32_t* lanes, F&& f) {
   constexpr int V = 16 / sizeof(T);

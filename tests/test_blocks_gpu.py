@@ -380,3 +380,212 @@ def test_refusals():
         quiver.block_norm([1.0], w)
     with pytest.raises(TypeError):
         quiver.clip_grad_norm([f, None], 1.0)
+
+
+# ---- together, streams, graphs ----------------------------------------------------------------
+
+
+def _encoder_state(dtype, texts=5, tokens=70, seed=0):
+    """A causal encoder of one block: a table, the norms' and the layers' weights, gates and decays."""
+    g = torch.Generator().manual_seed(seed)
+    d, h = 48, 3
+    w = lambda n, k: _randn(g, n, k, dtype=dtype, std=k ** -0.5)  # noqa: E731
+    v = lambda mean, n=d: mean + _randn(g, n, dtype=dtype, std=0.1)  # noqa: E731
+    return dict(tok=torch.randint(-1, 300, (texts, tokens), generator=g).to(_gpu()), table=_randn(g, 300, d, dtype=dtype), w_in=v(1.0),
+                w_qkv=w(3 * d, d), decay=-torch.exp2(-torch.arange(1.0, h + 1.0)).to(_gpu()), w_gate=w(d, d), w_att=v(1.0), s_att=v(0.4),
+                w_mid=v(1.0), w_up=w(2 * d, d), b_up=v(0.0, 2 * d), w_down=w(d, 2 * d), w_out=v(1.0), s_out=v(0.4), w_end=v(1.0),
+                lengths=torch.randint(1, tokens + 1, (texts,), generator=g).to(_gpu()), grad=_randn(g, texts, tokens, d, dtype=dtype))
+
+
+def _step(s, limit=0.5):
+    """Forwards, backwards by hand and the clipped gradients: as a program without autograd runs them."""
+    b, t, d = s["grad"].shape
+    heads = lambda x: x.unflatten(-1, (3, -1))  # noqa: E731
+    x0 = quiver.embed(s["table"], s["tok"])
+    h0 = quiver.block_norm(x0, s["w_in"])
+    qkv = quiver.linear(h0, s["w_qkv"])
+    q, k, v = (heads(p) for p in qkv.split(d, -1))
+    o = quiver.linear_attention(q, k, v, s["decay"], lengths=s["lengths"])
+    gate = quiver.linear(h0, s["w_gate"])
+    y0 = o.flatten(2)
+    x1, h1 = quiver.block_norm(x0, s["w_mid"], y=y0, post_weight=s["w_att"], gate=gate, gate_activation="silu", scale=s["s_att"])
+    u, z = quiver.linear(h1, s["w_up"], bias=s["b_up"], activation="gelu", keep_preactivation=True)
+    y1 = quiver.linear(u, s["w_down"])
+    x2, h2 = quiver.block_norm(x1, s["w_end"], y=y1, post_weight=s["w_out"], scale=s["s_out"])
+
+    dx2, dw_end, dy1, dw_out, _, ds_out = quiver.block_norm_grad(s["grad"], x2, s["w_end"], y=y1, post_weight=s["w_out"], scale=s["s_out"])
+    du, dw_down, _ = quiver.linear_grad(dy1, u, s["w_down"], bias=False)
+    dh1, dw_up, db_up = quiver.linear_grad(du, h1, s["w_up"], preactivation=z, activation="gelu")
+    dx1, dw_mid, dy0, dw_att, dgate, ds_att = quiver.block_norm_grad(dh1, x1, s["w_mid"], grad_r=dx2, y=y0, post_weight=s["w_att"], gate=gate,
+                                                                     gate_activation="silu", scale=s["s_att"])
+    dh0, dw_gate, _ = quiver.linear_grad(dgate, h0, s["w_gate"], bias=False)
+    dq, dk, dv, _ = quiver.linear_attention_grad(heads(dy0), q, k, v, s["decay"], lengths=s["lengths"])
+    dqkv = torch.cat([p.flatten(2) for p in (dq, dk, dv)], -1)
+    dh0b, dw_qkv, _ = quiver.linear_grad(dqkv, h0, s["w_qkv"], bias=False)
+    dx0, dw_in = quiver.block_norm_grad(dh0 + dh0b, x0, s["w_in"])[:2]
+    dtable = quiver.embed_grad(dx0 + dx1, s["tok"], len(s["table"]))
+    grads = dict(table=dtable, w_in=dw_in, w_qkv=dw_qkv, w_gate=dw_gate, w_att=dw_att, s_att=ds_att, w_mid=dw_mid, w_up=dw_up, b_up=db_up,
+                 w_down=dw_down, w_out=dw_out, s_out=ds_out, w_end=dw_end)
+    clipped, norm = quiver.clip_grad_norm(list(grads.values()), limit)
+    return h2, grads, clipped, norm
+
+
+def _plain_encoder(s):
+    """The same encoder in elementary operations, for torch's autograd in 64 bits."""
+    def norm(x, w):
+        return x / torch.sqrt((x * x).mean(-1, keepdim=True) + 1e-6) * w
+
+    b, t, d = s["grad"].shape
+    named = s["tok"] >= 0
+    x0 = torch.where(named[..., None], s["table"][s["tok"].clamp(min=0)], torch.zeros((), dtype=torch.float64, device=named.device))
+    h0 = norm(x0, s["w_in"])
+    q, k, v = (p.unflatten(-1, (3, -1)).transpose(1, 2) for p in (h0 @ s["w_qkv"].t()).split(d, -1))
+    at = torch.arange(t, device=x0.device)
+    live = at[None, :] < s["lengths"][:, None]
+    apart = (at[:, None] - at[None, :]).clamp(min=0).double()
+    scores = (q @ k.transpose(2, 3).contiguous() * torch.exp(s["decay"].double()[:, None, None] * apart)).tril() * live[:, None, None, :]
+    o = (scores @ v.contiguous()).transpose(1, 2).flatten(2) * (d // 3) ** -0.5 * live[..., None]
+    x1 = x0 + s["s_att"] * torch.nn.functional.silu(h0 @ s["w_gate"].t()) * norm(o, s["w_att"])
+    u = torch.nn.functional.gelu(norm(x1, s["w_mid"]) @ s["w_up"].t() + s["b_up"])
+    x2 = x1 + s["s_out"] * norm(u @ s["w_down"].t(), s["w_out"])
+    return norm(x2, s["w_end"])
+
+
+def test_an_encoder_block_trains():
+    """One step of a whole block in fp32, by hand and under torch's autograd, against autograd in 64 bits."""
+    s = _encoder_state("fp32")
+    _say("encoder block")
+    h2, grads, clipped, norm = _step(s)
+    wide = {k: v.double().requires_grad_(k in grads) if v.is_floating_point() else v for k, v in s.items()}
+    out = _plain_encoder(wide)
+    names = list(grads)
+    want = torch.autograd.grad(out, [wide[k] for k in names], wide["grad"])
+    # About forty fp32 products, norms and sums of up to 350 terms follow one another, each off by 512 2^-24 of its size at the
+    # most and passed on by factors of a few: 2^-10 of a result's largest element covers them with room.
+    assert (h2.double() - out).abs().max() <= 2.0**-10 * out.abs().max()
+    for name, g, w in zip(names, grads.values(), want):
+        assert (g.double() - w).abs().max() <= 2.0**-10 * w.abs().max(), name
+    total = math.sqrt(sum((w ** 2).sum().item() for w in want))
+    assert abs(norm.item() - total) <= 2.0**-10 * total
+    leaves = {k: v.detach().clone().requires_grad_(k in grads) if v.is_floating_point() else v for k, v in s.items()}
+    d = 48
+    x0 = quiver.embed(leaves["table"], s["tok"])
+    h0 = quiver.block_norm(x0, leaves["w_in"])
+    q, k, v = (p.unflatten(-1, (3, -1)) for p in quiver.linear(h0, leaves["w_qkv"]).split(d, -1))
+    o = quiver.linear_attention(q, k, v, s["decay"], lengths=s["lengths"]).flatten(2)
+    x1, h1 = quiver.block_norm(x0, leaves["w_mid"], y=o, post_weight=leaves["w_att"], gate=quiver.linear(h0, leaves["w_gate"]),
+                               gate_activation="silu", scale=leaves["s_att"])
+    y1 = quiver.linear(quiver.linear(h1, leaves["w_up"], bias=leaves["b_up"], activation="gelu"), leaves["w_down"])
+    _, h2 = quiver.block_norm(x1, leaves["w_end"], y=y1, post_weight=leaves["w_out"], scale=leaves["s_out"])
+    got = torch.autograd.grad(h2, [leaves[k] for k in names], s["grad"])
+    for name, g, w in zip(names, got, want):
+        assert (g.double() - w).abs().max() <= 2.0**-10 * w.abs().max(), name
+
+
+def test_block_norm_under_backward():
+    g = torch.Generator().manual_seed(31)
+    _say("block_norm autograd")
+    x, w = _randn(g, 6, 40, dtype="fp32"), _randn(g, 40, dtype="fp32")
+    parts = _block(g, (6, 40), "fp32")
+    cr, ch = _randn(g, 6, 40, dtype="fp32"), _randn(g, 6, 40, dtype="fp32")
+    leaves = [t.clone().requires_grad_() for t in (x, w, parts["y"], parts["post_weight"], parts["gate"], parts["scale"])]
+    call = lambda x, w, y, p, gate, s: quiver.block_norm(x, w, y=y, post_weight=p, gate=gate, scale=s, gate_activation="sigmoid")  # noqa: E731
+    r, h = call(*leaves)
+    torch.autograd.backward([r, h], [cr, ch])
+    plain = quiver.block_norm_grad(ch, r.detach(), w, grad_r=cr, gate_activation="sigmoid", **parts)
+    assert all(torch.equal(t.grad, p) for t, p in zip(leaves, plain))
+    r, h = call(*leaves)
+    only = torch.autograd.grad(r, leaves[2], cr)[0]  # h unused, one input wanted
+    assert torch.equal(only, quiver.block_norm_grad(ch * 0, r.detach(), w, grad_r=cr, gate_activation="sigmoid", **parts)[2])
+    gate = leaves[4][:1].detach().requires_grad_()
+    r, h = call(*leaves[:4], gate.expand(6, 40), leaves[5])
+    shared = torch.autograd.grad(h, gate, ch)[0]
+    each = quiver.block_norm_grad(ch, r.detach(), w, gate_activation="sigmoid", **{**parts, "gate": gate.detach().expand(6, 40)})[4]
+    assert torch.allclose(shared, each.sum(0, keepdim=True), rtol=1e-5, atol=1e-6)
+    h = quiver.block_norm(leaves[0], leaves[1])
+    first = torch.autograd.grad(h.sum(), leaves[0], create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="differentiated twice"):
+        first.sum().backward()
+    with torch.no_grad():
+        assert not quiver.block_norm(leaves[0], leaves[1]).requires_grad
+
+
+def _flat(result):
+    return [t for part in result for t in (part.values() if isinstance(part, dict) else part if isinstance(part, list) else [part])]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_calls_follow_the_current_stream_and_repeat(dtype):
+    _say("blocks streams", dtype)
+    want = _flat(_step(_encoder_state(dtype)))
+    assert all(torch.equal(a, b) for a, b in zip(_flat(_step(_encoder_state(dtype))), want))
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        later = [t.clone() for t in _flat(_step(_encoder_state(dtype)))]
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(later, want))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("texts,tokens", [(3, 5), (2, 700)])
+def test_calls_in_graphs(dtype, texts, tokens):
+    """Two graphs captured from the same calls, replayed by turns on new inputs with eager work between the replays."""
+    _say("blocks graph", dtype, texts, tokens)
+    states = [_encoder_state(dtype, texts, tokens, seed) for seed in (0, 1)]
+    for s in states:
+        _step(s)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in states:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(_flat(_step(s)))
+    for seed in (2, 3, 4):
+        for i in (0, 1):
+            fresh = _encoder_state(dtype, texts, tokens, seed + 10 * i)
+            for name, t in fresh.items():
+                states[i][name].copy_(t)
+            want = _flat(_step(fresh))
+            torch.cuda.synchronize()
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], want)), (seed, i)
+
+
+def test_a_growing_text_in_a_graph():
+    """One token a replay, the state in place."""
+    dev = _gpu()
+    g = torch.Generator().manual_seed(41)
+    _say("attention graph")
+    q, k, v = (_randn(g, 2, 20, 4, 32, dtype="bf16") for _ in range(3))
+    decay = torch.tensor([-0.1, -0.2, -0.5, 0.0], device=dev)
+    now = [t[:, :1].clone() for t in (q, k, v)]
+    state = torch.zeros((2, 4, 32, 32), device=dev)
+    quiver.linear_attention(*now, decay, state=state, state_out=state)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = quiver.linear_attention(*now, decay, state=state, state_out=state)
+    state.zero_()
+    eager = torch.zeros_like(state)
+    for t in range(20):
+        for a, b in zip(now, (q, k, v)):
+            a.copy_(b[:, t:t + 1])
+        want, _ = quiver.linear_attention(q[:, t:t + 1], k[:, t:t + 1], v[:, t:t + 1], decay, state=eager, state_out=eager)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(state, eager)
+
+
+def test_allocates_nothing_of_its_own():
+    import ctypes as C
+
+    from qvh_ctypes import LIB
+
+    lib = C.CDLL(LIB)
+    count = C.c_uint64()
+    assert lib.qvh_device_allocations(C.byref(count)) == 0
+    before = count.value
+    _step(_encoder_state("bf16"))
+    assert lib.qvh_device_allocations(C.byref(count)) == 0 and count.value == before
