@@ -8,41 +8,8 @@ import ctypes as C
 import pytest
 
 import quiver_amd as quiver
+from block_launches import U3, AttentionArgs, AttentionGradArgs, Gradient, NormArgs, NormGradArgs
 from test_encoder import BUF, _refused, lib  # noqa: F401  (lib: the fixture)
-
-U3 = C.c_uint64 * 3
-
-
-class NormArgs(C.Structure):
-    _fields_ = [("rows", C.c_uint64), ("dim", C.c_uint32), ("dtype", C.c_int), ("gate_activation", C.c_int), ("eps", C.c_float),
-                ("x", C.c_void_p), ("x_stride", C.c_uint64), ("y", C.c_void_p), ("y_stride", C.c_uint64), ("gate", C.c_void_p),
-                ("gate_stride", C.c_uint64), ("weight", C.c_void_p), ("post_weight", C.c_void_p), ("scale", C.c_void_p),
-                ("r", C.c_void_p), ("h", C.c_void_p)]
-
-
-class NormGradArgs(C.Structure):
-    _fields_ = [("rows", C.c_uint64), ("dim", C.c_uint32), ("dtype", C.c_int), ("gate_activation", C.c_int), ("eps", C.c_float),
-                ("grad_h", C.c_void_p), ("grad_h_stride", C.c_uint64), ("grad_r", C.c_void_p), ("grad_r_stride", C.c_uint64),
-                ("r", C.c_void_p), ("r_stride", C.c_uint64), ("y", C.c_void_p), ("y_stride", C.c_uint64), ("gate", C.c_void_p),
-                ("gate_stride", C.c_uint64), ("weight", C.c_void_p), ("post_weight", C.c_void_p), ("scale", C.c_void_p),
-                ("grad_x", C.c_void_p), ("grad_y", C.c_void_p), ("grad_gate", C.c_void_p), ("grad_weight", C.c_void_p),
-                ("grad_post", C.c_void_p), ("grad_scale", C.c_void_p)]
-
-
-class AttentionArgs(C.Structure):
-    _fields_ = [("batch", C.c_uint64), ("tokens", C.c_uint64), ("heads", C.c_uint32), ("kv_heads", C.c_uint32), ("dk", C.c_uint32),
-                ("dv", C.c_uint32), ("dtype", C.c_int), ("scale", C.c_float), ("q", C.c_void_p), ("q_stride", U3), ("k", C.c_void_p),
-                ("k_stride", U3), ("v", C.c_void_p), ("v_stride", U3), ("log_decay", C.c_void_p), ("lengths", C.c_void_p),
-                ("index_bytes", C.c_int), ("state", C.c_void_p), ("state_out", C.c_void_p), ("out", C.c_void_p)]
-
-
-class AttentionGradArgs(C.Structure):
-    _fields_ = [("forward", AttentionArgs), ("grad", C.c_void_p), ("grad_stride", U3), ("grad_state", C.c_void_p), ("grad_q", C.c_void_p),
-                ("grad_k", C.c_void_p), ("grad_v", C.c_void_p), ("grad_first", C.c_void_p)]
-
-
-class Gradient(C.Structure):
-    _fields_ = [("grad", C.c_void_p), ("out", C.c_void_p), ("count", C.c_uint64), ("dtype", C.c_int)]
 
 
 def _norm(lib, **change):  # noqa: F811
