@@ -56,6 +56,13 @@ def _matrix(name, m, shape, device, dtype):
     return _rows(m, shape[-1])
 
 
+def _written(tensors):
+    """Tells autograd of tensors that a call has written to."""
+    tensors = [t for t in tensors if not t.is_inference()]
+    if tensors:
+        _encoder._torch.autograd.graph.increment_version(tensors)
+
+
 def _pointer(t) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -225,7 +232,6 @@ def _attention_arguments(q, k, v, log_decay, state, lengths, scale):
 
 def _linear_attention(q, k, v, log_decay, state, lengths, scale, keep_state, state_out=None):
     (q, k, v, *held), sizes, scale, strides, args, shape = _attention_arguments(q, k, v, log_decay, state, lengths, scale)
-    torch = _encoder._torch
     device = q.device
     out = q.new_empty((*q.shape[:3], sizes[5]))
     last = filled = None
@@ -243,7 +249,7 @@ def _linear_attention(q, k, v, log_decay, state, lengths, scale, keep_state, sta
         if filled is not last:
             last.copy_(filled)
         else:
-            torch.autograd.graph.increment_version(last)
+            _written([last])
     return out if last is None else (out, last)
 
 
@@ -350,7 +356,5 @@ def clip_grad_norm(grads: Sequence, max_norm: float, out: Optional[Sequence] = N
         for t, f in zip(results, filled):
             if t is not f:
                 t.copy_(f)
-    written = [t for t, f in zip(results, filled) if t is f]
-    if written:
-        torch.autograd.graph.increment_version(written)
+    _written([t for t, f in zip(results, filled) if t is f])
     return results, norm

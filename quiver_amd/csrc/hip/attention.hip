@@ -535,7 +535,6 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
             }
           }
         }
-        __builtin_amdgcn_sched_barrier(0);
         // What the state gives.
         f32x4_t o[kWaves]{};
 #pragma unroll
@@ -543,7 +542,6 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
 #pragma unroll
           for (int j = 0; j < kWaves; ++j) o[j] = Op<T>::mma(*reinterpret_cast<const X8*>(s_x + (16 * j + l) * kS + 32 * kk + 8 * g), qf[kk], o[j]);
         }
-        __builtin_amdgcn_sched_barrier(0);
         int p_lift = 0;  // float16: this row's scores and sums are 2^p_lift as large
         if constexpr (kHalf) {
           float most = 0.0f;
@@ -674,7 +672,6 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
       float scale[4] = {within[0], within[1], within[2], within[3]};
 #pragma unroll
       for (int m = kWaves / 2 - 1; m >= 0; --m) {
-        __builtin_amdgcn_sched_barrier(0);
         X8 part[kParts];
         float rest[8];
         weighed(m, scale, rest);
@@ -725,7 +722,6 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
       update(std::true_type{}, std::true_type{});
     } else {
       results(std::false_type{});
-      __builtin_amdgcn_sched_barrier(0);
       if (sizeof(T) == 4 || (a.exact && (STATES || a.segments == 1))) {
         update(std::false_type{}, std::true_type{});
       } else {
@@ -947,6 +943,7 @@ void launch_passes(const AttentionPasses& p, uint32_t count, hipStream_t s) {
   }
   const uint64_t all = static_cast<uint64_t>(p.pass[0].batch) * p.pass[0].heads;
   QVH_REQUIRE(ceil_div(all * std::max(segments, parts), 8) * 8 * slices * 256 < kGridThreads, "linear attention: too many segments for one launch");
+  QVH_REQUIRE(segments == 1 || all < (uint64_t{1} << 16), "linear attention: rows this far apart of so many texts and heads");
   const auto grid = [&](uint64_t each) { return dim3(static_cast<unsigned>(ceil_div(all * each, 8) * 8 * slices), count); };
   with_depth(depth, [&](auto kd) {
     constexpr int KD = decltype(kd)::value;
@@ -986,10 +983,14 @@ bool check_attention(const char* name, const qvh_attention_args& a) {
   QVH_REQUIRE(a.heads > 0 && a.kv_heads > 0 && a.heads % a.kv_heads == 0, who + ": heads must be a multiple of kv_heads");
   QVH_REQUIRE(a.dk > 0 && a.dk <= kMaxHead && a.dv > 0 && a.dv <= kMaxHead, who + ": dk and dv must be in [1, 256]");
   QVH_REQUIRE(a.batch < (uint64_t{1} << 31) && a.tokens < (uint64_t{1} << 31), who + ": batch and tokens must be below 2^31");
-  QVH_REQUIRE(a.batch * a.heads < (uint64_t{1} << 16), who + ": batch times heads must be below 2^16");
+  QVH_REQUIRE(a.batch * a.heads <= (uint64_t{1} << 21), who + ": batch times heads must be at most 2^21");
   QVH_REQUIRE(!a.lengths || a.index_bytes == 4 || a.index_bytes == 8, who + ": lengths must be int32 or int64");
   QVH_REQUIRE(std::isfinite(a.scale), who + ": scale must be finite");
   if (a.batch == 0) return false;
+  if (a.state && a.state_out && a.state != a.state_out) {
+    const uint64_t size = a.batch * a.heads * a.dk * a.dv;
+    QVH_REQUIRE(a.state + size <= a.state_out || a.state_out + size <= a.state, who + ": state_out overlaps a part of state");
+  }
   QVH_REQUIRE(a.log_decay != nullptr, who + ": null log_decay");
   if (a.tokens > 0) {
     check_tensor(who, "q", a.q, a.q_stride);

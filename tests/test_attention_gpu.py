@@ -398,6 +398,33 @@ def test_under_backward(dtype):
         assert not quiver.linear_attention(*leaves[:3], g_).requires_grad
 
 
+def test_more_heads_than_a_launch_has_rows():
+    """70,000 texts of one token, and of nine."""
+    g = torch.Generator().manual_seed(37)
+    _say("attention 70,000 texts")
+    for tokens in (1, 9):
+        q, k, v, g_, s = _inputs(g, "bf16", 70_000, tokens, 1, 1, 8, 8, state=True)
+        got, last = quiver.linear_attention(q, k, v, g_, state=s, keep_state=True)
+        part, end = quiver.linear_attention(q[-30:], k[-30:], v[-30:], g_, state=s[-30:], keep_state=True)
+        want, size = _forward_64(q[-30:], k[-30:], v[-30:], g_, s[-30:], None, 8 ** -0.5)[0]
+        _within(got[-30:], want, _bound(want, size, "bf16", 300))
+        assert torch.equal(got[-30:], part) or tokens > 8  # nine tokens of thirty texts may go by segments
+        assert torch.isfinite(got).all() and torch.isfinite(last).all()
+
+
+def test_under_inference_mode():
+    g = torch.Generator().manual_seed(43)
+    _say("attention inference mode")
+    q, k, v, g_, s = _inputs(g, "bf16", 1, 2, 2, 1, 16, 16, state=True)
+    want = quiver.linear_attention(q, k, v, g_, state=s, keep_state=True)
+    with torch.inference_mode():
+        state = s.clone()
+        got = quiver.linear_attention(q, k, v, g_, state=state, state_out=state)
+        assert got[1] is state and all(torch.equal(a, b) for a, b in zip(got, want))
+        grads = [torch.ones(9, device=_gpu())]
+        assert abs(quiver.clip_grad_norm(grads, 1.0, out=grads)[0][0][0].item() - 1 / 3) < 1e-6
+
+
 def test_refusals():
     dev = _gpu()
     _say("attention refusals")

@@ -61,8 +61,8 @@ def _attention_args(**change):
 FAR = U3(2**40, 128, 32)
 ATTENTION = [(dict(dtype=7), "dtype"), (dict(heads=0), "heads"), (dict(kv_heads=3), "heads"), (dict(kv_heads=0), "heads"), (dict(dk=0), "dk"),
              (dict(dk=257), "dk"), (dict(dv=257), "dv"), (dict(tokens=2**31), "below 2^31"), (dict(batch=2**31), "below 2^31"),
-             (dict(batch=2**14), "2^16"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(log_decay=None), "log_decay"),
-             (dict(lengths=BUF, index_bytes=2), "lengths"), (dict(q=None), "null q"), (dict(k=None), "null k"), (dict(v=None), "null v"),
+             (dict(batch=2**20), "2^21"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(log_decay=None), "log_decay"),
+             (dict(state=BUF, state_out=C.c_void_p((1 << 20) + 64)), "overlaps"), (dict(lengths=BUF, index_bytes=2), "lengths"), (dict(q=None), "null q"), (dict(k=None), "null k"), (dict(v=None), "null v"),
              (dict(q_stride=FAR), "q's strides"), (dict(v_stride=FAR), "v's strides")]
 
 
