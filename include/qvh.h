@@ -488,7 +488,8 @@ typedef struct qvh_block_norm_grad_args {
   void* grad_post;
   void* grad_scale;
 } qvh_block_norm_grad_args;
-qvh_status qvh_block_norm_grad_workspace(const qvh_block_norm_grad_args* args, uint64_t* bytes);
+/* block: whether there is a y. */
+qvh_status qvh_block_norm_grad_workspace(uint64_t rows, uint32_t dim, int dtype, int block, uint64_t* bytes);
 qvh_status qvh_block_norm_grad_device(const qvh_block_norm_grad_args* args, void* d_workspace, uint64_t workspace_bytes,
                                       void* stream);
 

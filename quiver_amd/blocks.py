@@ -43,17 +43,19 @@ def _differentiated(*tensors) -> bool:
 
 
 def _vector(name, v, dim, device, dtype):
-    _check(name, v, device, dtype)
+    if v.__class__ is not _encoder._tensor or v.dtype is not dtype or v.device != device:
+        _check(name, v, device, dtype)
     if v.shape != (dim,):
         raise ValueError(f"{name} must have shape ({dim},), got {tuple(v.shape)}")
     return v if v.is_contiguous() else v.contiguous()
 
 
 def _matrix(name, m, shape, device, dtype):
-    _check(name, m, device, dtype)
+    if m.__class__ is not _encoder._tensor or m.dtype is not dtype or m.device != device:
+        _check(name, m, device, dtype)
     if m.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(m.shape)}")
-    return _rows(m, shape[-1])
+    return (m, shape[-1]) if m.is_contiguous() else _rows(m, shape[-1])
 
 
 def _written(tensors):
@@ -137,13 +139,11 @@ def _block_norm_grad(grad_h, r, weight, grad_r, y, post_weight, gate, gate_activ
     matrix = (True, False, True, False, True, False)
     out = [r.new_empty(r.shape if m else (dim,)) if h and w else None for h, m, w in zip(has, matrix, wanted)]
     gx, gw, gy, gp, gg, gs = out
-    args = (r.numel() // dim, dim, _dtypes[dtype], act, eps, gh.data_ptr(), ghs, _pointer(gr), grs, rr.data_ptr(), rs, *args,
-            _pointer(gx), _pointer(gy), _pointer(gg), _pointer(gw), _pointer(gp), _pointer(gs))
-    stream = _stream(device)
-    need = _quiver._block_norm_grad(*args, 0, 0, stream)
-    if need:
-        work = _workspace(need, device)
-        _quiver._block_norm_grad(*args, work.data_ptr(), need, stream)
+    rows, kind = r.numel() // dim, _dtypes[dtype]
+    need = _quiver._block_norm_grad_workspace(rows, dim, kind, y is not None)
+    work = _workspace(need, device) if need else None
+    _quiver._block_norm_grad(rows, dim, kind, act, eps, gh.data_ptr(), ghs, _pointer(gr), grs, rr.data_ptr(), rs, *args, _pointer(gx),
+                             _pointer(gy), _pointer(gg), _pointer(gw), _pointer(gp), _pointer(gs), _pointer(work), need, _stream(device))
     return tuple(out)
 
 
@@ -173,7 +173,8 @@ def linear_attention(q, k, v, log_decay, state=None, lengths=None, scale: Option
 
 def _heads(name, t, device, dtype):
     """A [batch, tokens, heads, dim] tensor with contiguous rows of dim, and its strides."""
-    _check(name, t, device, dtype)
+    if t.__class__ is not _encoder._tensor or t.dtype is not dtype or t.device != device:
+        _check(name, t, device, dtype)
     if t.dim() != 4:
         raise ValueError(f"{name} must be [batch, tokens, heads, dim], got shape {tuple(t.shape)}")
     s = t.stride()

@@ -448,9 +448,8 @@ uint32_t grad_groups(uint64_t rows, uint32_t dim, int dtype) {
   return static_cast<uint32_t>(groups);
 }
 
-uint64_t grad_bytes(const qvh_block_norm_grad_args& a) {
-  if (!a.grad_weight && !a.grad_post && !a.grad_scale && a.rows == 0) return 0;
-  return static_cast<uint64_t>(a.y ? 3 : 1) * grad_groups(a.rows, a.dim, a.dtype) * ceil_div(a.dim, 8) * 8 * sizeof(float);
+uint64_t grad_bytes(uint64_t rows, uint32_t dim, int dtype, bool block) {
+  return (block ? 3 : 1) * ceil_div(dim, 8) * 8 * sizeof(float) * static_cast<uint64_t>(grad_groups(rows, dim, dtype));
 }
 
 void check_shape(const char* who, uint64_t rows, uint32_t dim, int dtype, int act, float eps) {
@@ -551,11 +550,11 @@ qvh_status qvh_block_norm_device(const qvh_block_norm_args* args, void* stream) 
   });
 }
 
-qvh_status qvh_block_norm_grad_workspace(const qvh_block_norm_grad_args* args, uint64_t* bytes) {
+qvh_status qvh_block_norm_grad_workspace(uint64_t rows, uint32_t dim, int dtype, int block, uint64_t* bytes) {
   return qvh::guarded([&] {
     QVH_REQUIRE(bytes != nullptr, "qvh_block_norm_grad_workspace: null output");
-    qvh::check_backward("qvh_block_norm_grad_workspace", args);
-    *bytes = qvh::grad_bytes(*args);
+    qvh::check_shape("qvh_block_norm_grad_workspace", rows, dim, dtype, QVH_ACT_NONE, 0.0f);
+    *bytes = qvh::grad_bytes(rows, dim, dtype, block != 0);
   });
 }
 
@@ -565,7 +564,7 @@ qvh_status qvh_block_norm_grad_device(const qvh_block_norm_grad_args* args, void
     using namespace qvh;
     check_backward("qvh_block_norm_grad_device", args);
     const qvh_block_norm_grad_args& in = *args;
-    check_workspace("qvh_block_norm_grad_device", d_workspace, workspace_bytes, grad_bytes(in));
+    check_workspace("qvh_block_norm_grad_device", d_workspace, workspace_bytes, grad_bytes(in.rows, in.dim, in.dtype, in.y != nullptr));
     const DeviceScope device;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     NormArgs a;

@@ -226,22 +226,21 @@ PYBIND11_MODULE(_quiver, m) {
     const qvh_block_norm_args a{rows, dim, dtype, act, eps, ptr(x), xs, ptr(y), ys, ptr(gate), gs, ptr(weight), ptr(post), ptr(scale), ptr(r), ptr(h)};
     check(qvh_block_norm_device(&a, ptr(stream)));
   });
+  m.def("_block_norm_grad_workspace", [check](std::uint64_t rows, std::uint32_t dim, int dtype, bool block) {
+    std::uint64_t bytes = 0;
+    check(qvh_block_norm_grad_workspace(rows, dim, dtype, block, &bytes));
+    return bytes;
+  });
   m.def("_block_norm_grad",
         [check, ptr](std::uint64_t rows, std::uint32_t dim, int dtype, int act, float eps, std::uintptr_t gh, std::uint64_t ghs,
                      std::uintptr_t gr, std::uint64_t grs, std::uintptr_t r, std::uint64_t rs, std::uintptr_t y,
                      std::uint64_t ys, std::uintptr_t gate, std::uint64_t gs, std::uintptr_t weight, std::uintptr_t post,
                      std::uintptr_t scale, std::uintptr_t gx, std::uintptr_t gy, std::uintptr_t gg, std::uintptr_t gw,
                      std::uintptr_t gp, std::uintptr_t gsc, std::uintptr_t work, std::uint64_t work_bytes,
-                     std::uintptr_t stream) -> std::uint64_t {
+                     std::uintptr_t stream) {
           const qvh_block_norm_grad_args a{rows, dim, dtype, act, eps, ptr(gh), ghs, ptr(gr), grs, ptr(r), rs, ptr(y), ys, ptr(gate), gs,
                                            ptr(weight), ptr(post), ptr(scale), ptr(gx), ptr(gy), ptr(gg), ptr(gw), ptr(gp), ptr(gsc)};
-          if (work_bytes == 0) {
-            std::uint64_t need = 0;
-            check(qvh_block_norm_grad_workspace(&a, &need));
-            if (need > 0) return need;
-          }
           check(qvh_block_norm_grad_device(&a, ptr(work), work_bytes, ptr(stream)));
-          return 0;
         });
   // sizes: batch, tokens, heads, kv_heads, dk, dv, dtype; strides: three each of q, k and v (and of the result's gradient).
   const auto attention_args = [ptr](const std::array<std::uint64_t, 7>& n, float scale, std::uintptr_t q, std::uintptr_t k,

@@ -68,7 +68,7 @@ def block_norm_grad(lib, rows, dim, dtype="bf16", block=True, gate=True):
                      r_stride=dim, y=p, y_stride=dim, gate=q, gate_stride=dim, weight=BUF, post_weight=p, grad_x=BUF, grad_y=p, grad_gate=q,
                      grad_weight=BUF, grad_post=p)
     need = C.c_uint64()
-    status = lib.qvh_block_norm_grad_workspace(C.byref(a), C.byref(need))
+    status = lib.qvh_block_norm_grad_workspace(C.c_uint64(rows), C.c_uint32(dim), TYPES[dtype], int(block), C.byref(need))
     return need.value, status or lib.qvh_block_norm_grad_device(C.byref(a), C.c_void_p(BUF if need.value else 0), need, None)
 
 
