@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int apart = static_cast<int>(l) - static_cast<int>(4 * g + i);
-    diagonal[i] = apart >= 0 ? a.near_scale * decay(apart) : 0.0f;
+    diagonal[i] = a.near_scale * decay(apart > 0 ? apart : 0);
     before[i] = a.near_scale * decay(16 + apart);
     within[i] = a.kv_scale * decay(16 - static_cast<int>(4 * g + i + a.ahead));
   }
@@ -514,16 +514,21 @@ __global__ void __launch_bounds__(256, (sizeof(T) == 2 && KD <= 128) ? 2 : 1) at
           for (int u = 1; u >= 0; --u) {
             const int b = 2 * m + u, at = static_cast<int>(w);
             float y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              y[i] = acc[u][i] * (b < at ? away[i] : b == at ? diagonal[i] : 0.0f);
-              // Zeros where the mask is; but not times infinities and NaN.
-              if (kSlow && odd) y[i] = b < at || (b == at && 4 * own_g + i <= own_l) ? y[i] : 0.0f;
-              if (kSlow && b == at) own[i] = y[i];
-            }
             if (b < at) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) away[i] *= sixteen;
+              for (int i = 0; i < 4; ++i) {
+                y[i] = acc[u][i] * away[i];
+                away[i] *= sixteen;
+              }
+            } else if (b == at) {  // a choice, not a factor of zero: scores behind the mask may be infinite
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                y[i] = 4 * own_g + i <= own_l ? acc[u][i] * diagonal[i] : 0.0f;
+                if (kSlow) own[i] = y[i];
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) y[i] = 0.0f;
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {

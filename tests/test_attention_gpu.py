@@ -237,6 +237,21 @@ def test_tokens_that_are_not_finite_change_later_ones_only(dtype, tokens):
                 assert torch.equal(got[0, others], clean[0][0, others]) and torch.equal(last, clean[1])
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_scores_past_fp32_range_stay_behind_the_mask(dtype):
+    """Finite tokens whose products with earlier queries are infinite change nothing before them."""
+    g = torch.Generator().manual_seed(47)
+    _say("attention masked overflow", dtype)
+    q, k, v, g_, _ = _inputs(g, dtype, 1, 80, 2, 2, 32, 32)
+    q *= 1e18
+    clean = quiver.linear_attention(q, k, v, g_)
+    for at in (1, 17, 63, 79):
+        bad = k.clone()
+        bad[0, at] = 3e38
+        got = quiver.linear_attention(q, bad, v, g_)
+        assert torch.equal(got[:, :at], clean[:, :at]) and torch.isfinite(got[:, :at]).all(), at
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("tokens", [4, 150, 1_200])
 def test_decays_from_nothing_to_everything(dtype, tokens):
