@@ -20,6 +20,15 @@
 // computed. Where there are few heads, a text is cut into segments: a first pass makes the state that each leaves by itself, a
 // scan over the segments the states that they start from.
 //
+// What bounds it. 8 texts of 4,096 tokens, 16 heads of 128 bf16 (537 MB, 106 us at a copy's rate): 148 us a pass where every CU
+// has two work-groups (512 of them), 3.6 TB/s, 195 to 202 with one (256); backwards, three passes in one launch, 470 to 520. A wave has
+// 72 matrix instructions (1,150 cycles) and 360 others (1,450) a chunk and waits for the rest of its 5,700: for LDS behind the
+// two barriers, for one product's result in the next. LDS moves data 35% of the time. Three work-groups a CU would need
+// 168 registers a wave and keep the rest in memory (596 us a pass); eight waves with 128 columns and tokens, which load q
+// and k once, took as long and left half of the CUs empty at 128 heads. fp32: 8 texts of 1,000 tokens, 12 heads of 64, 49 us and 18 for the
+// segments' states: the fp32 matrix unit, which needs 22 of them. One token for each of 256 texts, 16 heads of 128: 105 us, the
+// states' 537 MB at 5.1 TB/s.
+//
 // Precision. 16-bit: scores and X are rounded to the type where the matrix unit takes them (for float16 behind a
 // power of two, so that neither overflows or vanishes), once each, like the result. The update multiplies v by its decay and
 // adds up in fp32 to its last bits: the weighed v is a sum of three bfloat16 parts (24 bits) or two float16 ones (22).
@@ -893,7 +902,9 @@ __global__ void __launch_bounds__(256) attention_step_kernel(AttentionPass a) {
 
 // ---- plans ------------------------------------------------------------------------------------
 
-constexpr uint64_t kFewTokens = 8;  // the recurrence itself, up to here
+/// The recurrence itself up to here, by chunks above. Both sides, us: one text, 16 heads of 64 bf16, two tokens 5.7 and 8.2, four 7.9
+/// and 8.2, eight 12.5 and 8.3; 64 texts, 16 heads of 128, two 32 and 54, four 43 and 54, eight 65 and 54.
+constexpr uint64_t kFewTokens = 4;
 
 template <class F>
 void with_depth(uint32_t dk, F&& f) {
@@ -925,7 +936,8 @@ uint64_t state_bytes(const AttentionPass& a) {
   return a.segments > 1 ? static_cast<uint64_t>(a.segments) * a.batch * a.heads * a.dk * a.dv * sizeof(float) : 0;
 }
 
-/// Whether rows of a tensor are whole pieces that lie apart, and a segment's fit a buffer (attention_kernel's WHOLE).
+/// Whether rows of a tensor are whole pieces that lie apart, and a segment's fit a buffer (attention_kernel's WHOLE). The other way costs
+/// half as much again: 8 texts of 4,096 tokens, 16 heads of 128 bf16 at whole pieces 222 us, one element further 355.
 bool whole_rows(const AttentionPass& a, const TokenTensor& t, uint32_t dim, size_t size) {
   const uint64_t odd = reinterpret_cast<uintptr_t>(t.base) | t.batch * size | t.token * size | t.head * size;
   return dim % 8 == 0 && odd % 16 == 0 && t.token >= dim && (a.segment + 2 * kRows) * t.token * size < (uint64_t{1} << 31);

@@ -13,8 +13,9 @@
 //
 // A row stays in registers from its load to its last store, so every matrix is read or written once, and the vectors
 // are loaded once per work-group, which takes many rows. Memory bounds it: forward five matrices, backward eight.
-// Rows of up to 128 pieces of 16 bytes belong to a wave or a part of one (8, 16 or 32 lanes, so that short rows leave few
-// lanes idle) and need no barrier; longer ones to a work-group of four or sixteen waves. The columns' sums of the
+// Rows of up to 64 pieces of 16 bytes belong to a wave or a part of one (8, 16 or 32 lanes, so that short rows leave few
+// lanes idle) and need no barrier; longer ones to two, four, eight or sixteen waves. 16,384 x 1,024 bf16 with a gate and a
+// scale: forward 30 us, 168 MB at 5.6 TB/s; backward 55 and 4.7 for the sums, 268 MB at 4.5; 24 x 768 forward 4.2, the launch. The columns' sums of the
 // backward pass stay in registers too, over all rows of a work-group, and a second launch adds the work-groups' parts
 // up in order: no atomics, the same bits each time.
 #include <algorithm>
@@ -393,10 +394,11 @@ __global__ void __launch_bounds__(1024) norm_sums_kernel(NormSums a) {
   }
 }
 
-/// Calls f<V, W, P>() for rows of `dim` elements of T; `lanes` are a row's threads. Forward a thread has two pieces before a row
-/// gets four waves, backward, where it has five matrices and three sums of each, one piece as long as waves reach:
-/// 16,384 x 1,024 bf16 113 us with two pieces of a wave and 59 with one of two.
-template <class T, bool BACK, class F>
+/// Calls f<V, W, P>() for rows of `dim` elements of T; `lanes` are a row's threads: one piece each as long as sixteen waves reach
+/// (two pieces of a wave: 16,384 x 1,024 bf16 forward 30.5 us, backward 113; one of two waves 30.0 and 59), and as few lanes
+/// of a wave as hold the row (10,007 x 100 fp32 on 32 lanes 5.2 us forward and 14.1 backward, on 64 6.7 and 17.4; 100,000 x 64
+/// bf16 on 8 lanes 10.1, on 64 39.9).
+template <class T, class F>
 void with_shape(uint32_t dim, uint32_t* lanes, F&& f) {
   constexpr int V = 16 / sizeof(T);
   using std::integral_constant;
@@ -413,15 +415,9 @@ void with_shape(uint32_t dim, uint32_t* lanes, F&& f) {
   if (dim < V) return go(one, one, one, 8u);
   const uint32_t pieces = static_cast<uint32_t>(ceil_div(dim, V));
   if (pieces <= 64) return go(v, one, one, pieces <= 8 ? 8u : pieces <= 16 ? 16u : pieces <= 32 ? 32u : 64u);
-  if constexpr (BACK) {
-    if (pieces <= 128) return go(v, two, one, 128u);
-    if (pieces <= 256) return go(v, four, one, 256u);
-    if (pieces <= 512) return go(v, eight, one, 512u);
-  } else {
-    if (pieces <= 128) return go(v, one, two, 64u);
-    if (pieces <= 256) return go(v, four, one, 256u);
-    if (pieces <= 512) return go(v, four, two, 256u);
-  }
+  if (pieces <= 128) return go(v, two, one, 128u);
+  if (pieces <= 256) return go(v, four, one, 256u);
+  if (pieces <= 512) return go(v, eight, one, 512u);
   if (pieces <= 1024) return go(v, sixteen, one, 1024u);
   if (sizeof(T) == 2 || pieces <= 2048) return go(v, sixteen, two, 1024u);
   if constexpr (sizeof(T) == 4) go(v, sixteen, four, 1024u);
@@ -434,13 +430,14 @@ void with_parts(bool block, bool gate, F&& f) {
   f(std::true_type{}, std::true_type{});
 }
 
-/// Work-groups of a backward pass, two a CU or fewer: as many parts of every vector's sums.
+/// Work-groups of a backward pass, two a CU or fewer, as its registers allow (16,384 x 1,024 bf16: 512 of them 55 us, 768 63): as
+/// many parts of every vector's sums.
 uint32_t grad_groups(uint64_t rows, uint32_t dim, int dtype) {
   uint64_t groups = 0;
   uint32_t lanes = 0;
   with_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    with_shape<T, true>(dim, &lanes, [&](auto, auto w, auto) {
+    with_shape<T>(dim, &lanes, [&](auto, auto w, auto) {
       constexpr int W = decltype(w)::value;
       groups = std::min<uint64_t>(ceil_div(rows, grad_threads(W) / lanes), W <= 4 ? 512 : 256);
     });
@@ -535,7 +532,7 @@ qvh_status qvh_block_norm_device(const qvh_block_norm_args* args, void* stream) 
     a.h = in.h;
     with_dtype(in.dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
-      with_shape<T, false>(in.dim, &a.lanes, [&](auto v, auto w, auto p) {
+      with_shape<T>(in.dim, &a.lanes, [&](auto v, auto w, auto p) {
         constexpr int V = decltype(v)::value, W = decltype(w)::value, P = decltype(p)::value;
         with_parts(in.y != nullptr, in.gate != nullptr, [&](auto block, auto gate) {
           const uint64_t groups = ceil_div(a.rows, W == 1 ? 256 / a.lanes : 1);
@@ -594,7 +591,7 @@ qvh_status qvh_block_norm_grad_device(const qvh_block_norm_grad_args* args, void
     with_dtype(in.dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       if (groups > 0) {
-        with_shape<T, true>(in.dim, &a.lanes, [&](auto v, auto w, auto p) {
+        with_shape<T>(in.dim, &a.lanes, [&](auto v, auto w, auto p) {
           constexpr int V = decltype(v)::value, W = decltype(w)::value, P = decltype(p)::value;
           with_parts(in.y != nullptr, in.gate != nullptr, [&](auto block, auto gate) {
             hipLaunchKernelGGL((norm_grad_kernel<T, V, W, P, decltype(block)::value, decltype(gate)::value>), dim3(groups),
