@@ -19,7 +19,9 @@ there is no CPU fallback: without a gfx950 device, adding or searching raises ``
 
 In front of an index, ``embed``, ``linear`` and their gradients ``embed_grad``, ``linear_grad``, and
 ``orthogonalize`` make and train the vectors on torch tensors (quiver_amd/encoder.py;
-examples/encoder_search.py trains a small text encoder, indexes its vectors and searches them).
+examples/encoder_search.py trains a small text encoder, indexes its vectors and searches them). ``block_norm``,
+``linear_attention``, their gradients, ``grad_norm`` and ``clip_grad_norm`` make blocks of such layers, which
+let a text's tokens see one another, and bound their training steps (quiver_amd/blocks.py).
 """
 
 from __future__ import annotations
