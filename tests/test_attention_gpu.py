@@ -176,7 +176,7 @@ def test_many_texts_fill_the_device(dtype):
 
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("index", [torch.int32, torch.int64])
-@pytest.mark.parametrize("tokens", [5, 70, 300])
+@pytest.mark.parametrize("tokens", [4, 5, 70, 300])
 def test_padding(dtype, index, tokens):
     """What lies behind a text's end counts for nothing, NaN and infinities too; lengths past either end are clamped."""
     g = torch.Generator().manual_seed(tokens)
@@ -200,7 +200,7 @@ def test_padding(dtype, index, tokens):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("tokens", [6, 90])
+@pytest.mark.parametrize("tokens", [4, 6, 90])
 def test_tokens_that_are_not_finite_change_later_ones_only(dtype, tokens):
     g = torch.Generator().manual_seed(tokens + 1)
     _say("attention special", dtype, tokens)
@@ -362,7 +362,7 @@ def test_past_32_bit_offsets():
         assert torch.equal(quiver.linear_attention(t["q"], t["k"], t["v"], g_), want)
 
 
-@pytest.mark.parametrize("tokens", [5, 100])
+@pytest.mark.parametrize("tokens", [4, 5, 100])
 def test_grad_against_differences(tokens):
     """A step along a direction changes the loss by the gradient's part along it (fp32, central differences)."""
     g = torch.Generator().manual_seed(23)
