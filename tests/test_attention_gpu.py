@@ -165,6 +165,51 @@ def test_long_texts_in_segments(dtype, tokens, shape):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+def test_segments_with_padding_and_the_state_in_place(dtype):
+    """Texts that end in any segment, on its ends and before the first; decays of everything and nothing; junk behind the ends."""
+    g = torch.Generator().manual_seed(53)
+    _say("attention segments", dtype)
+    tokens, ends = 1_100, [1_100, 0, 1, 320, 640, 641, 900]
+    q, k, v, _, s = _inputs(g, dtype, 7, tokens, 4, 2, 24, 40, state=True)
+    decay = torch.tensor([-0.01, 0.0, float("-inf"), -3.0], device=_gpu())
+    lengths = torch.tensor(ends, device=_gpu())
+    clean = _check(q, k, v, decay, s, lengths=lengths)
+    assert torch.equal(clean[1][1], s[1])
+    _check_grad(g, q, k, v, decay, s, lengths=lengths, grad_state=s)
+    behind = torch.arange(tokens, device=_gpu())[None] >= lengths[:, None]
+    for t in (q, k, v):
+        t[behind] = float("nan")
+    held = s.clone()
+    got = quiver.linear_attention(q, k, v, decay, state=held, lengths=lengths, state_out=held)
+    assert got[1] is held and all(torch.equal(a, b) for a, b in zip(got, clean))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("at", [0, 300, 1_099])
+def test_tokens_that_are_not_finite_in_segments(dtype, at):
+    g = torch.Generator().manual_seed(59)
+    _say("attention special segments", dtype, at)
+    q, k, v, g_, s = _inputs(g, dtype, 1, 1_100, 2, 2, 64, 48, state=True)
+    clean = quiver.linear_attention(q, k, v, g_, state=s, keep_state=True)
+    want, size = _forward_64(q, k, v, g_, s, None, 0.125)[0]
+    off = _bound(want, size, dtype, 64 + 1_100 + 256)
+    others = [c for c in range(48) if c != 17]
+    for junk in (float("inf"), float("-inf"), float("nan")):
+        bad = v.clone()
+        bad[0, at, 1, 17] = junk
+        got, last = quiver.linear_attention(q, k, bad, g_, state=s, keep_state=True)
+        assert torch.equal(got[:, :at], clean[0][:, :at]) and torch.equal(got[:, :, 0], clean[0][:, :, 0])
+        _within(got[:, :, 1][:, :, others], want[:, :, 1][:, :, others], off[:, :, 1][:, :, others], "other columns")
+        assert not torch.isfinite(got[0, at:, 1, 17]).any() and not torch.isfinite(last[0, 1, :, 17]).any()
+        assert torch.isfinite(last[0, 1][:, others]).all()
+        bad = k.clone()
+        bad[0, at, 1, 5] = junk
+        got, last = quiver.linear_attention(q, bad, v, g_, state=s, keep_state=True)
+        assert torch.equal(got[:, :at], clean[0][:, :at]) and torch.equal(got[:, :, 0], clean[0][:, :, 0])
+        assert not torch.isfinite(last[0, 1, 5]).any() and torch.isfinite(last[0, 1][[i for i in range(64) if i != 5]]).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_many_texts_fill_the_device(dtype):
     g = torch.Generator().manual_seed(11)
     _say("attention many", dtype)
