@@ -75,7 +75,7 @@ struct AttentionPass {
   uint32_t segments = 1;
   uint64_t segment = 0;  // tokens
   float* states = nullptr;
-  /// Segments whose own state is made: the last one's too where a result follows from it.
+  /// Segments whose own state is made, of a text that is cut: the last one's too where a result follows from it.
   __host__ __device__ uint32_t parts() const { return state_out ? segments : segments - 1; }
 };
 
@@ -943,9 +943,12 @@ bool whole_rows(const AttentionPass& a, const TokenTensor& t, uint32_t dim, size
   return dim % 8 == 0 && odd % 16 == 0 && t.token >= dim && (a.segment + 2 * kRows) * t.token * size < (uint64_t{1} << 31);
 }
 
-/// `count` passes of one shape: the same dk and dv (or their swap, within one depth), texts and heads.
+/// `count` passes of one shape: the same dk and dv (or their swap, within one depth), texts and heads. Each is cut by itself, so some
+/// may be whole texts: those have no states in the workspace, and are not among the passes that make them.
 template <class T>
 void launch_passes(const AttentionPasses& p, uint32_t count, hipStream_t s) {
+  AttentionPasses cut_ones;
+  uint32_t cut_count = 0;
   bool whole = true;
   uint32_t depth = 0, segments = 1, parts = 0;
   uint64_t slices = 1, size = 0;
@@ -954,25 +957,30 @@ void launch_passes(const AttentionPasses& p, uint32_t count, hipStream_t s) {
     whole = whole && whole_rows(a, a.q, a.dk, sizeof(T)) && whole_rows(a, a.k, a.dk, sizeof(T)) && whole_rows(a, a.v, a.dv, sizeof(T));
     depth = std::max(depth, a.dk);
     segments = std::max(segments, a.segments);
-    parts = std::max(parts, a.parts());
+    if (a.segments > 1) {
+      QVH_REQUIRE(a.states != nullptr, "linear attention: a text in segments without their states");
+      parts = std::max(parts, a.parts());
+      cut_ones.pass[cut_count++] = a;
+    }
     slices = std::max(slices, ceil_div(a.dv, kCols));
     size = std::max<uint64_t>(size, static_cast<uint64_t>(a.dk) * a.dv);
   }
   const uint64_t all = static_cast<uint64_t>(p.pass[0].batch) * p.pass[0].heads;
-  QVH_REQUIRE(ceil_div(all * std::max(segments, parts), 8) * 8 * slices * 256 < kGridThreads, "linear attention: too many segments for one launch");
+  QVH_REQUIRE(ceil_div(all * segments, 8) * 8 * slices * 256 < kGridThreads, "linear attention: too many segments for one launch");
   QVH_REQUIRE(segments == 1 || all < (uint64_t{1} << 16), "linear attention: rows this far apart of so many texts and heads");
-  const auto grid = [&](uint64_t each) { return dim3(static_cast<unsigned>(ceil_div(all * each, 8) * 8 * slices), count); };
+  const auto grid = [&](uint64_t each, uint32_t passes) { return dim3(static_cast<unsigned>(ceil_div(all * each, 8) * 8 * slices), passes); };
   with_depth(depth, [&](auto kd) {
     constexpr int KD = decltype(kd)::value;
     const auto go = [&](auto rows) {
       constexpr bool WHOLE = decltype(rows)::value;
-      if (segments > 1) {
-        hipLaunchKernelGGL((attention_kernel<T, KD, true, WHOLE>), grid(parts), dim3(256), 0, s, p);
+      if (cut_count > 0) {
+        hipLaunchKernelGGL((attention_kernel<T, KD, true, WHOLE>), grid(parts, cut_count), dim3(256), 0, s, cut_ones);
         QVH_HIP(hipGetLastError());
-        hipLaunchKernelGGL(attention_scan_kernel, dim3(static_cast<unsigned>(ceil_div(size, 256)), static_cast<unsigned>(all), count), dim3(256), 0, s, p);
+        hipLaunchKernelGGL(attention_scan_kernel, dim3(static_cast<unsigned>(ceil_div(size, 256)), static_cast<unsigned>(all), cut_count), dim3(256), 0,
+                           s, cut_ones);
         QVH_HIP(hipGetLastError());
       }
-      hipLaunchKernelGGL((attention_kernel<T, KD, false, WHOLE>), grid(segments), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((attention_kernel<T, KD, false, WHOLE>), grid(segments, count), dim3(256), 0, s, p);
       QVH_HIP(hipGetLastError());
     };
     whole ? go(std::true_type{}) : go(std::false_type{});
@@ -1100,7 +1108,8 @@ GradPasses grad_passes(const qvh_attention_grad_args& in, void* workspace) {
   };
   for (AttentionPass* p : {&g.q, &g.k, &g.v}) {
     cut(*p, 3);
-    p->states = take(state_bytes(*p));
+    const uint64_t bytes = state_bytes(*p);
+    p->states = bytes > 0 ? take(bytes) : nullptr;
   }
   const uint64_t rows = f.batch * f.tokens * f.heads;
   if (share > 1) {

@@ -16,6 +16,7 @@ struct Launch {
   dim3 grid, block;
   size_t lds;
   int device;
+  std::vector<char> argument;  // its first one, where recorder_keep asked for it
 };
 
 std::unordered_map<const void*, std::string>& names() {
@@ -25,6 +26,8 @@ std::unordered_map<const void*, std::string>& names() {
 std::vector<Launch> g_launches;
 int g_device = 1;  // not the library's, which is 0
 hipError_t g_error = hipSuccess;
+std::string g_kept;
+size_t g_kept_bytes = 0;
 struct Config {
   dim3 grid, block;
   size_t lds;
@@ -81,13 +84,17 @@ hipError_t hipGetLastError() {
 }
 
 /// Refuses what the runtime refuses: an empty grid, or 2^32 threads and more along an axis.
-hipError_t hipLaunchKernel(const void* f, dim3 grid, dim3 block, void**, size_t lds, hipStream_t) {
+hipError_t hipLaunchKernel(const void* f, dim3 grid, dim3 block, void** args, size_t lds, hipStream_t) {
   const unsigned g[3] = {grid.x, grid.y, grid.z}, b[3] = {block.x, block.y, block.z};
   for (int i = 0; i < 3; ++i) {
     const unsigned long long threads = static_cast<unsigned long long>(g[i]) * b[i];
     if (threads == 0 || threads >= 1ull << 32) return g_error = hipErrorInvalidConfiguration;
   }
-  g_launches.push_back({names()[f], grid, block, lds, g_device});
+  g_launches.push_back({names()[f], grid, block, lds, g_device, {}});
+  if (g_kept_bytes > 0 && names()[f].find(g_kept) != std::string::npos) {
+    const char* p = static_cast<const char*>(args[0]);
+    g_launches.back().argument.assign(p, p + g_kept_bytes);
+  }
   return hipSuccess;
 }
 
@@ -98,6 +105,13 @@ void recorder_shape(int i, unsigned long long* out) {
   const unsigned long long v[7] = {l.grid.x, l.grid.y, l.block.x, l.grid.z, l.lds, static_cast<unsigned long long>(l.device), 0};
   std::memcpy(out, v, sizeof(v));
 }
+/// From now on, kernels whose name holds `part` leave the bytes of their first argument, of which there are so many.
+void recorder_keep(const char* part, size_t bytes) {
+  g_kept = part;
+  g_kept_bytes = bytes;
+}
+/// They, or null.
+const void* recorder_argument(int i) { return g_launches[i].argument.empty() ? nullptr : g_launches[i].argument.data(); }
 void recorder_clear() { g_launches.clear(); }
 /// The name of the i-th kernel that the library holds, null behind the last.
 const char* recorder_kernel(int i) {

@@ -165,6 +165,34 @@ def test_long_texts_in_segments(dtype, tokens, shape):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("heads,kv_heads", [(8, 8), (12, 6)])
+@pytest.mark.parametrize("dk,dv", [(64, 128), (128, 64), (64, 256)])
+def test_gradients_of_which_some_go_in_segments(dtype, heads, kv_heads, dk, dv, monkeypatch):
+    """The three passes have dk columns or dv of them, and are cut or not by their number: nothing is written behind the workspace."""
+    from quiver_amd import blocks
+
+    g = torch.Generator().manual_seed(dk + dv + heads)
+    _say("attention_grad segments of some", dtype, heads, dk, dv)
+    held = []
+
+    def workspace(nbytes, device):
+        held.append((nbytes, torch.full((nbytes + (8 << 20),), 0xA5, dtype=torch.uint8, device=device)))
+        return held[-1][1][:nbytes]
+
+    monkeypatch.setattr(blocks, "_workspace", workspace)
+    inputs = _inputs(g, dtype, 4, 1_100, heads, kv_heads, dk, dv, state=True)
+    lengths = torch.tensor([1_100, 0, 321, 1_024], device=_gpu())
+    end = torch.randn(4, heads, dk, dv, generator=g).to(_gpu())
+    _check_grad(g, *inputs[:4], None)
+    _check_grad(g, *inputs, grad_state=end)
+    _check_grad(g, *inputs, lengths=lengths, grad_state=end)
+    grad = _randn(g, 4, 1_100, heads, dv, dtype=dtype)
+    calls = [quiver.linear_attention_grad(grad, *inputs[:4], state=inputs[4], grad_state=end) for _ in range(3)]
+    assert all(torch.equal(a, b) for c in calls[1:] for a, b in zip(c, calls[0]))
+    assert len(held) == 6 and all((t[n:] == 0xA5).all() for n, t in held)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_segments_with_padding_and_the_state_in_place(dtype):
     """Texts that end in any segment, on its ends and before the first; decays of everything and nothing; junk behind the ends."""
     g = torch.Generator().manual_seed(53)
