@@ -518,8 +518,7 @@ qvh_status qvh_clip_grad_norm_device(const qvh_gradient* grads, uint64_t count, 
  * state. log_decay is fp32 [heads], at most 0 (-infinity: no memory); larger ones are taken as they are, and powers of them may
  * overflow. lengths (nullable), index_bytes 4 or 8 each, [batch], are the texts' tokens, clamped to [0, tokens]:
  * those behind them change no state and give zeros, whatever they hold. A token that is not finite changes results of its own
- * and later tokens only. dk and dv are at most 256, batch * heads at most 2^21 (below 2^16
- * where tokens lie 4 MB apart or more and a text has to be cut), tokens below 2^31, strides below 2^40.
+ * and later tokens only. dk and dv are at most 256, batch * heads at most 2^21, tokens below 2^31, strides below 2^40.
  * Scores and the state enter 16-bit products rounded to their type once, each by up to 2^-9 of a bf16 term, 2^-12 of an fp16
  * one; states themselves are fp32 throughout. */
 typedef struct qvh_attention_args {

@@ -913,6 +913,11 @@ void with_depth(uint32_t dk, F&& f) {
   f(std::integral_constant<int, 256>{});
 }
 
+/// Whether launches take so many segments of `all` texts and heads.
+bool fits(uint64_t all, uint64_t segments, uint64_t slices) {
+  return segments == 1 || (all < (uint64_t{1} << 16) && ceil_div(all * segments, 8) * 8 * slices * 256 < kGridThreads);
+}
+
 /// Segments of a pass that is launched with `together` - 1 others like it: enough to fill the device, with work-groups of four chunks
 /// or more, where there is less than a work-group for most CUs. (A CU holds two of them, or one of a deep or fp32 head.) The
 /// segments' states are a third to a half of the pass again. Both sides, us, one segment and more: 8 texts of 4,096 tokens, 16
@@ -924,9 +929,13 @@ void cut(AttentionPass& a, uint32_t together) {
   const uint64_t at_once = a.dk <= (a.wide ? 64u : 128u) ? 512 : 256;
   uint64_t segments = groups >= 192 || groups == 0 ? 1 : std::max<uint64_t>(1, at_once / groups);
   segments = std::max<uint64_t>(1, std::min(segments, chunks / 4));
-  // Rows far apart: segments that a buffer of 2^31 bytes holds, with room for the chunks around, where that can be.
+  // Rows far apart: segments that a buffer of 2^31 bytes holds, with room for the chunks around, where that can be and the launches have
+  // room for as many; else whole texts by ordinary loads.
   const uint64_t apart = std::max({a.q.token, a.k.token, a.v.token}) * 4, most = apart ? (uint64_t{1} << 31) / apart / kRows : chunks + 4;
-  if (most > 8) segments = std::max(segments, ceil_div(chunks, most - 4));
+  const uint64_t all = static_cast<uint64_t>(a.batch) * a.heads;
+  if (most > 8 && fits(all, ceil_div(chunks, most - 4), ceil_div(std::max(a.dk, a.dv), kCols))) {
+    segments = std::max(segments, ceil_div(chunks, most - 4));
+  }
   const uint64_t each = ceil_div(chunks, segments);
   a.segment = each * kRows;
   a.segments = static_cast<uint32_t>(ceil_div(chunks, each));
@@ -966,8 +975,7 @@ void launch_passes(const AttentionPasses& p, uint32_t count, hipStream_t s) {
     size = std::max<uint64_t>(size, static_cast<uint64_t>(a.dk) * a.dv);
   }
   const uint64_t all = static_cast<uint64_t>(p.pass[0].batch) * p.pass[0].heads;
-  QVH_REQUIRE(ceil_div(all * segments, 8) * 8 * slices * 256 < kGridThreads, "linear attention: too many segments for one launch");
-  QVH_REQUIRE(segments == 1 || all < (uint64_t{1} << 16), "linear attention: rows this far apart of so many texts and heads");
+  QVH_REQUIRE(fits(all, segments, slices), "linear attention: too many segments for one launch");
   const auto grid = [&](uint64_t each, uint32_t passes) { return dim3(static_cast<unsigned>(ceil_div(all * each, 8) * 8 * slices), passes); };
   with_depth(depth, [&](auto kd) {
     constexpr int KD = decltype(kd)::value;

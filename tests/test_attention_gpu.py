@@ -500,6 +500,24 @@ def test_more_heads_than_a_launch_has_rows():
         assert torch.isfinite(got).all() and torch.isfinite(last).all()
 
 
+def test_many_texts_next_to_one_another_within_a_token():
+    """65,536 texts whose tokens lie 1 MB apart, longer than a buffer of 2^31 bytes: more than a launch cuts."""
+    dev = _gpu()
+    _say("attention 65,536 texts by token")
+    g = torch.Generator(device=dev).manual_seed(61)
+    q, k, v = (torch.randn((2_100, 65_536, 1, 8), generator=g, device=dev, dtype=torch.bfloat16).transpose(0, 1) for _ in range(3))
+    decay = torch.tensor([-0.01], device=dev)
+    got, last = quiver.linear_attention(q, k, v, decay, keep_state=True)
+    grads = quiver.linear_attention_grad(v, q, k, v, decay)
+    for some in (slice(0, 15), slice(-15, None)):
+        few = [t[some].contiguous() for t in (q, k, v)]
+        want, end = _forward_64(*few, decay, None, None, 8 ** -0.5)
+        _within(got[some], want[0], _bound(want[0], want[1], "bf16", 8 + 2_100 + 256))
+        _within(last[some], end[0], end[1] * (8 + 2_100 + 256) * 2.0**-23)
+        for a, (b, size) in zip(grads[:3], _grad_64(few[2], *few, decay, None, None, 8 ** -0.5, None)):
+            _within(a[some], b, _bound(b, size, "bf16", 8 + 8 + 2_100 + 257))
+
+
 def test_under_inference_mode():
     g = torch.Generator().manual_seed(43)
     _say("attention inference mode")

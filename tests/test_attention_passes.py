@@ -83,3 +83,15 @@ def test_states_where_one_tensors_rows_lie_far_apart(passes, dtype):
         _check(call, answer)
         cuts.append(_cuts(answer))
     assert any(len(c) > 1 and 1 in c for c in cuts)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("batch,tokens,heads,dk,dv", [(65_536, 1_000, 1, 8, 8), (2**19, 70, 4, 1, 1), (65_535, 250_000, 1, 8, 8),
+                                                      (2**21, 2_000, 1, 16, 16), (16_000, 16_000, 4, 8, 200)])
+def test_many_texts_whose_rows_lie_far_apart_are_taken(passes, dtype, batch, tokens, heads, dk, dv):
+    """Texts next to one another within a token, so many that no launch holds their segments: whole texts, by ordinary loads where no buffer holds one."""
+    shape = dict(batch=batch, tokens=tokens, heads=heads, kv_heads=heads, dk=dk, dv=dv, dtype=dtype, state=True, by_token=True)
+    for call, answer in passes([["attention", shape], ["attention_grad", shape]]):
+        _check(call, answer)
+        (kernel, _), = answer["launches"]
+        assert kernel.startswith("attention_kernel") and kernel.endswith(" 0") or tokens == 1_000, call
