@@ -156,7 +156,8 @@ def linear_attention(q, k, v, log_decay, state=None, lengths=None, scale: Option
 
     q is [batch, tokens, heads, dk], k [batch, tokens, kv_heads, dk], v [batch, tokens, kv_heads, dv], out [batch, tokens, heads, dv];
     kv_heads divides heads, and neighbouring heads share theirs. Views are read as they are where their last dimension is contiguous.
-    log_decay, float32 [heads] and at most 0, is a constant to autograd. scale is ``dk ** -0.5`` where it is left out.
+    log_decay, float32 [heads] and at most 0, is a constant: one that requires a gradient is refused where autograd records, and
+    is passed detached. scale is ``dk ** -0.5`` where it is left out.
     lengths (int32 or int64 [batch], clamped to [0, tokens]): the tokens of each text in front of its padding, which changes no
     state and gives zeros. dk and dv are at most 256.
 
@@ -164,7 +165,9 @@ def linear_attention(q, k, v, log_decay, state=None, lengths=None, scale: Option
     left out), and with keep_state the last one comes back too: (out, state). state_out takes it where it is given, and may be
     ``state`` itself, for texts that grow by a token at a time.
     """
-    if _differentiated(q, k, v, state):
+    if _differentiated(q, k, v, state, log_decay):
+        if _differentiated(log_decay):
+            raise ValueError("log_decay is a constant and would get no gradient: pass it detached")
         if state_out is not None:
             raise ValueError("state_out is not for calls that autograd records")
         return _node("LinearAttention", q, k, v, log_decay, state, lengths, scale, keep_state)

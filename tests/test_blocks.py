@@ -147,3 +147,31 @@ def test_python_calls_want_device_tensors():
     for call in (lambda: quiver.block_norm(1.0, f), lambda: quiver.linear_attention(None, q, q, f), lambda: quiver.grad_norm([1.0])):
         with pytest.raises(TypeError):
             call()
+
+
+def test_a_decay_that_wants_a_gradient_is_refused():
+    """It would get none, without a word. Refused ahead of all else, so that CPU tensors do."""
+    torch = pytest.importorskip("torch")
+    q = torch.zeros(1, 2, 1, 8)
+    decay = torch.zeros(1, requires_grad=True)
+    for inputs in ((q, q, q), (q.clone().requires_grad_(), q, q)):
+        with pytest.raises(ValueError, match="log_decay is a constant"):
+            quiver.linear_attention(*inputs, decay)
+        with pytest.raises(ValueError, match="log_decay is a constant"):
+            quiver.linear_attention(*inputs, decay * 2, keep_state=True)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(torch.zeros(1), torch.ones(1))
+        with pytest.raises(ValueError, match="log_decay is a constant"):
+            quiver.linear_attention(q, q, q, dual)
+
+
+def test_a_decay_is_taken_detached_or_without_autograd():
+    torch = pytest.importorskip("torch")
+    if torch.cuda.device_count() > 0:
+        pytest.skip("the library would take the tensors to a device")
+    q = torch.zeros(1, 2, 1, 8)
+    decay = torch.zeros(1, requires_grad=True)
+    with pytest.raises(ValueError, match="GPU memory"):
+        quiver.linear_attention(q, q, q, decay.detach())
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU memory"):
+        quiver.linear_attention(q, q, q, decay)
