@@ -494,10 +494,10 @@ qvh_status qvh_block_norm_grad_device(const qvh_block_norm_grad_args* args, void
                                       void* stream);
 
 /* The norm over all gradients of a model, sqrt of the sum of their squares (fp64 sums, an fp32 result), and the gradients
- * times min(1, max_norm / (norm + eps)). Each is `count` contiguous elements of its own type; out may be the gradient itself;
- * results that overlap one another or another gradient are refused. Elements that are not finite make the norm so: an infinite one leaves zeros (NaN where the
- * infinities were), NaN leaves NaN. The list is host memory, read before the call returns. At most 2^20 gradients
- * of 2^40 elements, 2^44 in all. */
+ * times min(1, max_norm / (norm + eps)), or as they are where norm + eps is 0. Each is `count` contiguous elements of its own
+ * type; out may be the gradient itself; results that overlap one another or another gradient are refused. Elements that are
+ * not finite make the norm so: an infinite one leaves zeros (NaN where the infinities were), NaN leaves NaN. The list is host
+ * memory, read before the call returns. At most 2^20 gradients of 2^40 elements, 2^44 in all. */
 typedef struct qvh_gradient {
   const void* grad;
   void* out; /* not of the norm alone */

@@ -340,8 +340,8 @@ def clip_grad_norm(grads: Sequence, max_norm: float, out: Optional[Sequence] = N
 
     grads are the tensors of a model, of any of the three types each. out takes the results where it is given: tensors of
     the same shapes and types, or ``out=grads`` to scale them in place. norm is ``grad_norm`` of the gradients as they came
-    in, and stays on the device. One that is infinite leaves zeros (NaN in place of infinities), NaN leaves NaN. The results
-    are constants to autograd.
+    in, and stays on the device. One that is infinite leaves zeros (NaN in place of infinities), NaN leaves NaN; gradients
+    of zeros stay, with an eps of 0 too. The results are constants to autograd.
     """
     grads, held, pointers, counts, types, device = _gradients("grads", grads)
     torch = _encoder._torch

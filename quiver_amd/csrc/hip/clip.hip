@@ -150,7 +150,8 @@ __global__ void __launch_bounds__(256) clip_scale_kernel(ClipTable t, const doub
   __shared__ double s_sum[4];
   const double n = sqrt(all_parts(parts, count, s_sum));
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
-  const double ratio = static_cast<double>(max_norm) / (n + static_cast<double>(eps));
+  const double over = n + static_cast<double>(eps);
+  const double ratio = over == 0.0 ? 1.0 : static_cast<double>(max_norm) / over;  // zeros stay
   // In two steps where fp32 has too few bits for it (norms past 1e30): a power of two, which is exact, and the rest.
   const float first = ratio < 0x1p-100 ? 0x1p-64f : 1.0f;
   const float factor = ratio >= 1.0 ? 1.0f : static_cast<float>(ratio < 0x1p-100 ? ratio * 0x1p64 : ratio);  // NaN stays

@@ -332,6 +332,23 @@ def test_clip_grad_norm_special():
         assert torch.equal(copy[~touched], base[~touched])
 
 
+def test_clip_grad_norm_of_zeros_where_nothing_is_added():
+    """A norm of 0 and an eps of 0 leave the gradients as they are, whatever the limit; other norms follow the formula."""
+    dev = _gpu()
+    _say("clip_grad_norm zeros")
+    zeros = [torch.zeros(9, device=dev), torch.full((3, 5), -0.0, device=dev, dtype=torch.bfloat16), torch.zeros(0, device=dev)]
+    for limit in (0.0, 1.0):
+        held = [t.clone() for t in zeros]
+        for out in (None, held):
+            clipped, norm = quiver.clip_grad_norm(zeros if out is None else held, limit, out=out, eps=0.0)
+            assert norm.item() == 0 and all(torch.equal(a, b) for a, b in zip(clipped, zeros))
+    one = torch.ones(4, device=dev)
+    assert not quiver.clip_grad_norm([one], 0.0, eps=0.0)[0][0].any()
+    assert torch.equal(quiver.clip_grad_norm([one], 1.0, eps=0.0)[0][0], one * 0.5)
+    one[2] = float("nan")
+    assert torch.isnan(quiver.clip_grad_norm([one], 0.0, eps=0.0)[0][0]).all()
+
+
 def test_clip_grad_norm_in_place_is_seen_by_autograd():
     dev = _gpu()
     x = torch.ones(4, device=dev, requires_grad=True)
