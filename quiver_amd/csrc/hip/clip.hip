@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(256) clip_norm_kernel(ClipTable t, double* __r
 }
 
 template <class T, bool PAST>
-__device__ __forceinline__ void scaled(const T* x, T* out, uint32_t n, float first, float factor) {
+__device__ __forceinline__ void scaled(const T* x, T* out, uint32_t n, float factor, int power) {
   constexpr uint32_t V = 16 / sizeof(T), kEach = kChunk / (256 * V);
   if (n == kChunk) {
     float v[kEach][V];
@@ -118,7 +118,7 @@ __device__ __forceinline__ void scaled(const T* x, T* out, uint32_t n, float fir
 #pragma unroll
     for (uint32_t u = 0; u < kEach; ++u) {
 #pragma unroll
-      for (uint32_t e = 0; e < V; ++e) v[u][e] = v[u][e] * first * factor;
+      for (uint32_t e = 0; e < V; ++e) v[u][e] = ldexpf(v[u][e] * factor, power);
       store_floats<T, V, PAST>(out + (u * 256 + threadIdx.x) * V, v[u]);
     }
     return;
@@ -128,10 +128,10 @@ __device__ __forceinline__ void scaled(const T* x, T* out, uint32_t n, float fir
     float v[V];
     load_floats<T, V>(x + i, v);
 #pragma unroll
-    for (uint32_t e = 0; e < V; ++e) v[e] = v[e] * first * factor;
+    for (uint32_t e = 0; e < V; ++e) v[e] = ldexpf(v[e] * factor, power);
     store_floats<T, V>(out + i, v);
   }
-  for (; i < n; ++i) out[i] = static_cast<T>(static_cast<float>(x[i]) * first * factor);
+  for (; i < n; ++i) out[i] = static_cast<T>(ldexpf(static_cast<float>(x[i]) * factor, power));
 }
 
 /// All parts added up, in every thread, the same bits in every work-group.
@@ -152,12 +152,12 @@ __global__ void __launch_bounds__(256) clip_scale_kernel(ClipTable t, const doub
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = static_cast<float>(n);
   const double over = n + static_cast<double>(eps);
   const double ratio = over == 0.0 ? 1.0 : static_cast<double>(max_norm) / over;  // zeros stay
-  // In two steps where fp32 has too few bits for it (norms past 1e30): a power of two, which is exact, and the rest.
-  const float first = ratio < 0x1p-100 ? 0x1p-64f : 1.0f;
-  const float factor = ratio >= 1.0 ? 1.0f : static_cast<float>(ratio < 0x1p-100 ? ratio * 0x1p64 : ratio);  // NaN stays
+  // Factors near the end of fp32's range and past it, which it would round or lose, as one in [0.5, 1) and a power of two.
+  int power = 0;
+  const float factor = ratio >= 1.0 ? 1.0f : static_cast<float>(ratio < 0x1p-100 ? frexp(ratio, &power) : ratio);  // NaN stays
   for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
     with_chunk<true>(t, c, [&](auto* x, auto* out, uint32_t k) {
-      if (factor != 1.0f || x != out) scaled<std::remove_pointer_t<decltype(out)>, PAST>(x, out, k, first, factor);
+      if (factor != 1.0f || power != 0 || x != out) scaled<std::remove_pointer_t<decltype(out)>, PAST>(x, out, k, factor, power);
     });
   }
 }

@@ -349,6 +349,22 @@ def test_clip_grad_norm_of_zeros_where_nothing_is_added():
     assert torch.isnan(quiver.clip_grad_norm([one], 0.0, eps=0.0)[0][0]).all()
 
 
+@pytest.mark.parametrize("limit", [1e-10, 1e-20, 1e-30, 2.0**-110, 2.0**-126, 2.0**-140, 0.0])
+def test_clip_grad_norm_to_limits_far_below_the_norm(limit):
+    """Factors that fp32 cannot hold, of gradients as large as it can: results that it holds come out as they are."""
+    dev = _gpu()
+    _say("clip_grad_norm far", limit)
+    for types in (("fp32",), ("bf16",), ("fp32", "bf16")):
+        values = torch.tensor([3e38, -1e38, 2.0**100, 1.0, 0.0, 2.0**-140], dtype=torch.float64)
+        grads = [values.to(TYPES[t]).repeat(2_000).to(dev) for t in types]  # more than a chunk of a work-group's, and a rest
+        norm = math.sqrt(sum((x.double() ** 2).sum().item() for x in grads))
+        clipped, _ = quiver.clip_grad_norm(grads, limit)
+        for a, x, t in zip(clipped, grads, types):
+            want = x.double() * (limit / (norm + 1e-6))
+            # The factor, a product and what is left of the fp32 range: half a step each; the limit itself is fp32.
+            _within(a, want, want.abs() * (ROUND[t] + 3 * E) + TINY[t] + 2.0**-149)
+
+
 def test_clip_grad_norm_in_place_is_seen_by_autograd():
     dev = _gpu()
     x = torch.ones(4, device=dev, requires_grad=True)
