@@ -65,6 +65,12 @@ def _written(tensors):
         _encoder._torch.autograd.graph.increment_version(tensors)
 
 
+def _own_elements(name, t):
+    """Refuses a result that could not take what is made aside of it, before anything is written."""
+    if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        raise ValueError(f"{name} has elements that share memory")
+
+
 def _pointer(t) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -241,6 +247,8 @@ def _linear_attention(q, k, v, log_decay, state, lengths, scale, keep_state, sta
     last = filled = None
     if state_out is not None:
         last, filled = state_out, _state("state_out", state_out, shape, device)
+        if filled is not last:
+            _own_elements("state_out", last)
     elif keep_state:
         last = filled = held[0].new_empty(shape)  # log_decay's type
     args = (sizes, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, *args, _pointer(filled), out.data_ptr())
@@ -355,10 +363,12 @@ def clip_grad_norm(grads: Sequence, max_norm: float, out: Optional[Sequence] = N
     if results and results[0].device != device:
         raise ValueError(f"out is on {results[0].device}, the gradients on {device}")
     # A result that is not contiguous is made aside; its gradient, where it is the same tensor, was copied already.
+    aside = [(t, f) for t, f in zip(results, filled) if t is not f]
+    for t, _ in aside:
+        _own_elements("out", t)
     norm = _run_clip(pointers, outs, counts, types, max_norm, eps, device or _own_device())
     with torch.no_grad():
-        for t, f in zip(results, filled):
-            if t is not f:
-                t.copy_(f)
-    _written([t for t, f in zip(results, filled) if t is f])
+        for t, f in aside:
+            t.copy_(f)
+    _written([t for t, f in zip(results, filled) if t is f] if aside else results)
     return results, norm

@@ -365,6 +365,23 @@ def test_clip_grad_norm_to_limits_far_below_the_norm(limit):
             _within(a, want, want.abs() * (ROUND[t] + 3 * E) + TINY[t] + 2.0**-149)
 
 
+def test_results_whose_elements_share_memory_are_refused_ahead_of_all_else():
+    """A gradient that torch expanded has one element in many places: nothing of the list is scaled in place by halves."""
+    dev = _gpu()
+    _say("shared elements")
+    whole, shared = torch.full((40,), 3.0, device=dev), torch.full((1, 8), 2.0, device=dev).expand(5, 8)
+    with pytest.raises(ValueError, match="share memory"):
+        quiver.clip_grad_norm([whole, shared], 1.0, out=[whole, shared])
+    assert (whole == 3.0).all() and (shared == 2.0).all()
+    clipped, norm = quiver.clip_grad_norm([whole, shared], 1.0)  # as inputs they are taken
+    assert abs(norm.item() - math.sqrt(360 + 160)) <= 1e-4 and clipped[1].shape == (5, 8)
+    q = torch.ones((2, 3, 4, 8), device=dev)
+    state = torch.zeros((1, 4, 8, 8), device=dev).expand(2, 4, 8, 8)
+    with pytest.raises(ValueError, match="share memory"):
+        quiver.linear_attention(q, q, q, torch.zeros(4, device=dev), state=state, state_out=state)
+    assert not state.any()
+
+
 def test_clip_grad_norm_in_place_is_seen_by_autograd():
     dev = _gpu()
     x = torch.ones(4, device=dev, requires_grad=True)
