@@ -18,6 +18,13 @@
 // scale: forward 30 us, 168 MB at 5.6 TB/s; backward 55 and 4.7 for the sums, 268 MB at 4.5; 24 x 768 forward 4.2, the launch. The columns' sums of the
 // backward pass stay in registers too, over all rows of a work-group, and a second launch adds the work-groups' parts
 // up in order: no atomics, the same bits each time.
+//
+// Backward rows past 4,096 columns do not fit: sixteen waves leave a thread 128 registers, and with a block a row, the next one, three
+// vectors and three sums take more, so that parts of them lie in scratch memory, by the compiler's report 61 to 77 registers of
+// 16-bit rows up to 8,192 columns and 264 to 279 past them, 100 to 180 and 457 to 639 of fp32 ones. That bounds them: 16.8 million
+// elements with a gate and a scale, calls in a row, 4,096 columns bf16 63 us and fp32 110, 5,000 237 and 403, 8,192 166 and 296, 16,384
+// 469 and 676. Without a block only the widest do (10 to 17, fp32 129): 27, 29, 27, 36 us and 43, 45, 46, 127. Forward rows
+// fit but for fp32 past 8,192 with a gate (25): 30, 45, 35, 39 us and 61, 72, 70, 90.
 #include <algorithm>
 
 #include "gemm.hpp"
@@ -430,8 +437,9 @@ void with_parts(bool block, bool gate, F&& f) {
   f(std::true_type{}, std::true_type{});
 }
 
-/// Work-groups of a backward pass, two a CU or fewer, as its registers allow (16,384 x 1,024 bf16: 512 of them 55 us, 768 63): as
-/// many parts of every vector's sums.
+/// Work-groups of a backward pass, two a CU or fewer: as many parts of every vector's sums. Measured where a thread has 182 registers
+/// (16,384 x 1,024 bf16 with a gate: 512 of them 55 us, 768 63). fp32 rows take 122 at most and would leave room for four a CU; for
+/// them more were not measured (10,007 x 100 fp32 takes 11.4 us of 6.3 by its bytes, its last round of rows less than half full).
 uint32_t grad_groups(uint64_t rows, uint32_t dim, int dtype) {
   uint64_t groups = 0;
   uint32_t lanes = 0;
